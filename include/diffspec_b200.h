@@ -552,6 +552,107 @@ int dsb_assign_request_slots(int64_t *slot_keys, int32_t num_slots,
 int dsb_rows_to_slots(const int32_t *active_slots, int32_t num_active, const int32_t *rows,
                       int32_t n, int32_t *slots, int32_t *error_flag, void *stream);
 
+/* RMSNorm of every query and key head, and RoPE, in one pass (fp32, each
+ * value rounded once when stored):
+ *   y = x * rsqrt(mean(x^2) + eps) * weight over each head of head_dim
+ *   out = y rotated at positions[t] + position_offset over its first
+ *         rotary_dim elements (NeoX halves, or pairs when !is_neox)
+ * query_out may be query (equal strides).  key_out / value_out are contiguous
+ * [tokens, num_kv_heads, head_dim] rows.  raw_key / raw_value (nullable, both
+ * or neither) also receive the normed keys before the rotation, and the
+ * values, at [slots[t], abs_positions[t]] of [num_slots, max_model_len,
+ * num_kv_heads, head_dim]; a negative slot is padding, a slot or position
+ * outside is flagged and skipped.  A position outside the cos_sin table is
+ * flagged (DSB_FLAG_POSITION) and its rows are normed but not rotated. */
+int dsb_qk_norm_rope(
+    const void *query, int64_t query_row_stride, void *query_out, int64_t query_out_row_stride,
+    int32_t num_query_heads, const void *key, int64_t key_row_stride, void *key_out,
+    const void *value, int64_t value_row_stride, void *value_out, int32_t num_kv_heads,
+    int32_t head_dim, int32_t rotary_dim, int32_t is_neox, const void *q_weight,
+    const void *k_weight, float eps, const int32_t *positions, int32_t position_offset,
+    int32_t tokens, const void *cos_sin, int64_t cos_sin_row_stride, int32_t rotary_rows,
+    int32_t cos_sin_dtype, int32_t dtype, void *raw_key, void *raw_value, const int32_t *slots,
+    const int64_t *abs_positions, int32_t num_slots, int64_t max_model_len, int32_t *error_flag,
+    void *stream);
+
+/* The same norms and rotation for the target's step: rotated keys and the
+ * values go to the paged caches, at the page that block-table row
+ * table_rows[t] (nullable: row t) has for positions[t].  A negative table row
+ * is padding (its queries are processed); a bad row, position or page is
+ * flagged and its K/V skipped. */
+int dsb_qk_norm_rope_paged(
+    const void *query, int64_t query_row_stride, void *query_out, int64_t query_out_row_stride,
+    int32_t num_query_heads, const void *key, int64_t key_row_stride, const void *value,
+    int64_t value_row_stride, int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+    int32_t is_neox, const void *q_weight, const void *k_weight, float eps,
+    const int32_t *positions, int32_t tokens, const void *cos_sin, int64_t cos_sin_row_stride,
+    int32_t rotary_rows, int32_t cos_sin_dtype, int32_t dtype, void *key_cache, void *value_cache,
+    int64_t num_blocks, int32_t block_size, const int32_t *block_table, int64_t block_table_stride,
+    int64_t block_table_rows, int64_t block_table_cols, const int32_t *table_rows,
+    int32_t *error_flag, void *stream);
+
+/* dsb_paged_decode_attention_lse for rows that share a prefix: rows
+ * [group_starts[i], group_starts[i + 1]) (num_groups + 1 entries, ascending;
+ * null: one group of every row) hold the same tokens at positions
+ * [0, prefix_lens[i]), which are read once for the group, through its first
+ * row's table; the tokens behind it, up to seq_lens[r], through the row's
+ * own.  max_prefix_len sizes the split of the prefix; a row with more than
+ * max_suffix_len tokens behind it is flagged (DSB_FLAG_POSITION) and cut.
+ * Any group of up to 16 query heads per kv head, head_dim 128. */
+int64_t dsb_shared_prefix_scratch_floats(int32_t query_rows, int32_t num_query_heads,
+                                         int32_t num_kv_heads, int32_t num_groups,
+                                         int32_t block_size, int32_t max_prefix_len,
+                                         int32_t max_suffix_len);
+int dsb_shared_prefix_attention_lse(
+    const void *query, int32_t query_rows, int32_t num_query_heads, int32_t num_kv_heads,
+    int32_t head_dim, const void *key_cache, const void *value_cache, int64_t num_blocks,
+    int32_t block_size, const int32_t *block_table, int64_t block_table_stride,
+    int64_t block_table_rows, int64_t block_table_cols, const int32_t *seq_lens,
+    const int32_t *table_rows, const int32_t *prefix_lens, const int32_t *group_starts,
+    int32_t num_groups, int32_t max_prefix_len, int32_t max_suffix_len, float scale,
+    int32_t dtype, void *out, float *lse, float *scratch, int64_t scratch_floats,
+    int32_t *error_flag, void *stream);
+
+/* Pages of a paged cache.  State, changed in place: ref_counts [num_pages]
+ * (rows that hold the page, 0: free), block_tables [table_rows, table_cols]
+ * (row stride table_stride; -1: none) and held [table_rows] (pages each row
+ * holds, its first entries).  Pages are handed out lowest id first, rows in
+ * call order.  status [2]: rows of the call left without pages, free pages
+ * after it.  At most 4096 rows a call.
+ *
+ * resize: row rows[i] gets the pages of lens[i] tokens.  Surplus pages go
+ * back first; the first row that does not fit and the later ones that need
+ * pages keep what they had (status[0] counts them).  Rows outside the table
+ * or named again, and lengths beyond it, are flagged and left alone. */
+int dsb_resize_requests(int32_t *ref_counts, int64_t num_pages, int32_t *block_tables,
+                        int64_t table_rows, int64_t table_stride, int64_t table_cols,
+                        int32_t *held, const int32_t *rows, const int32_t *lens, int32_t n,
+                        int32_t block_size, int32_t *status, int32_t *error_flag, void *stream);
+/* fork: the empty row children[i] starts with the first lens[i] tokens of row
+ * parents[i]: whole pages shared, the started page's tokens copied into a
+ * page of its own in each of the caches ([num_pages, block_size] tokens of
+ * token_bytes, a multiple of 16; `caches` is a host array). */
+int64_t dsb_fork_scratch_ints(int32_t n);
+int dsb_fork_requests(int32_t *ref_counts, int64_t num_pages, int32_t *block_tables,
+                      int64_t table_rows, int64_t table_stride, int64_t table_cols, int32_t *held,
+                      const int32_t *parents, const int32_t *children, const int32_t *lens,
+                      int32_t n, int32_t block_size, void *const *caches, int32_t num_caches,
+                      int64_t token_bytes, int32_t *status, int32_t *scratch, int64_t scratch_ints,
+                      int32_t *error_flag, void *stream);
+/* compact: with m live pages, the k-th live page of id >= m moves to the k-th
+ * free page below m, in the caches, the counts and every row's table. */
+int64_t dsb_compact_scratch_ints(int64_t num_pages);
+int dsb_compact_pages(int32_t *ref_counts, int64_t num_pages, int32_t *block_tables,
+                      int64_t table_rows, int64_t table_stride, int64_t table_cols, int32_t *held,
+                      int32_t block_size, void *const *caches, int32_t num_caches,
+                      int64_t token_bytes, int32_t *status, int32_t *scratch, int64_t scratch_ints,
+                      int32_t *error_flag, void *stream);
+/* copy: page src[i] -> page dst[i] of every cache (page_bytes a multiple of
+ * 16); pairs with a negative page are skipped, pages outside flagged. */
+int dsb_copy_pages(void *const *caches, int32_t num_caches, int64_t num_pages, int64_t page_bytes,
+                   const int32_t *src, const int32_t *dst, int32_t n, int32_t *error_flag,
+                   void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -603,3 +603,114 @@ def rope_qk(query, kv, positions, cos_sin, num_kv_heads, dtype="bf16"):
         q[t] = round_to(rope_rotate(q[t], row, d, True), dtype)
         k[t] = round_to(rope_rotate(k[t], row, d, True), dtype)
     return q.reshape(t_n, -1), k, v
+
+
+# ------------------------------------------- serving around a shared prompt
+# Not in the reference: per-head query/key norms with the rotation, and pages
+# shared by forked requests, restated plainly (fp64, loops).
+def qk_norm_rope(heads, weight, eps, cos_sin_rows, rotary_dim, is_neox_style=True):
+    """``heads [T, H, D]`` normed per head (``x / sqrt(mean(x^2) + eps) *
+    weight``) and rotated by each token's ``[cos | sin]`` row; fp64, nothing
+    rounded.  Returns (normed, rotated)."""
+    x = np.asarray(heads, dtype=np.float64)
+    y = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * np.asarray(weight, dtype=np.float64)
+    out = y.copy()
+    half = rotary_dim // 2
+    for i in range(half):
+        a, b = (i, i + half) if is_neox_style else (2 * i, 2 * i + 1)
+        c = np.asarray(cos_sin_rows, dtype=np.float64)[:, None, i]
+        s = np.asarray(cos_sin_rows, dtype=np.float64)[:, None, half + i]
+        out[..., a] = y[..., a] * c - y[..., b] * s
+        out[..., b] = y[..., b] * c + y[..., a] * s
+    return y, out
+
+
+class PagePool:
+    """Pages of a cache held by table rows: the lowest free page first, rows
+    in call order.  ``data[page]`` stands for the page's tokens."""
+
+    def __init__(self, pages, rows, cols, block_size):
+        self.refs = [0] * pages
+        self.tables = [[-1] * cols for _ in range(rows)]
+        self.held = [0] * rows
+        self.bs, self.cols = block_size, cols
+        self.flags = set()
+        self.lacking = 0
+
+    def free(self):
+        return [p for p, n in enumerate(self.refs) if n == 0]
+
+    def resize(self, rows, lens):
+        self.lacking = 0
+        todo, seen = [], set()
+        for r, n in zip(rows, lens):
+            if not 0 <= r < len(self.tables) or r in seen:
+                self.flags.add("slot")
+                continue
+            seen.add(r)
+            need = -(-n // self.bs)
+            if n < 0 or need > self.cols:
+                self.flags.add("position")
+                continue
+            todo.append((r, need))
+        for r, need in todo:
+            for j in range(need, self.held[r]):
+                self.refs[self.tables[r][j]] -= 1
+                self.tables[r][j] = -1
+            self.held[r] = min(self.held[r], need)
+        free, full = self.free(), False
+        for r, need in todo:
+            k = need - self.held[r]
+            if k <= 0:
+                continue
+            full = full or k > len(free)
+            if full:
+                self.lacking += 1
+                continue
+            for j in range(k):
+                page = free.pop(0)
+                self.refs[page] = 1
+                self.tables[r][self.held[r] + j] = page
+            self.held[r] = need
+
+    def fork(self, parents, children, lens):
+        """Returns the copies made: (source page, target page, tokens)."""
+        self.lacking = 0
+        todo, seen = [], set()
+        for up, c, n in zip(parents, children, lens):
+            rows = range(len(self.tables))
+            if up not in rows or c not in rows or c in seen or self.held[c]:
+                self.flags.add("slot")
+            elif n < 0 or n > self.held[up] * self.bs:
+                self.flags.add("position")
+            else:
+                todo.append((up, c, n // self.bs, n % self.bs))
+            seen.add(c)
+        free, copies = self.free(), []
+        for up, c, full, rest in todo:
+            if rest and not free:
+                self.lacking += 1
+                continue
+            for j in range(full):
+                self.tables[c][j] = self.tables[up][j]
+                self.refs[self.tables[up][j]] += 1
+            if rest:
+                page = free.pop(0)
+                self.refs[page] = 1
+                self.tables[c][full] = page
+                copies.append((self.tables[up][full], page, rest))
+            self.held[c] = full + (rest > 0)
+        return copies
+
+    def compact(self):
+        """Returns the moves made: (source page, target page)."""
+        live = sum(n > 0 for n in self.refs)
+        moved = [p for p, n in enumerate(self.refs) if n and p >= live]
+        holes = [p for p, n in enumerate(self.refs) if not n and p < live]
+        name = dict(zip(moved, holes))
+        for s, t in name.items():
+            self.refs[t], self.refs[s] = self.refs[s], 0
+        for r, row in enumerate(self.tables):
+            for j in range(self.held[r]):
+                row[j] = name.get(row[j], row[j])
+        return list(name.items())

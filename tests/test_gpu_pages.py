@@ -1,0 +1,222 @@
+"""Pages of a paged cache on the device (pages.resize_requests, fork_requests,
+compact_pages, copy_pages) against the oracle's plain pool: tables, reference
+counts, pages held, the status words and the cache contents, all exact."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+from oracle import diffspec_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+
+class _Pool:
+    """The device state beside the oracle's, with caches whose values say
+    where they were written."""
+
+    def __init__(self, dsb, cuda, pages, rows, cols, bs, layers=1, hk=2, d=8, dtype=torch.bfloat16,
+                 wide=0):
+        self.dsb, self.cuda, self.bs = dsb, cuda, bs
+        self.ref = O.PagePool(pages, rows, cols, bs)
+        ints = dict(dtype=torch.int32, device=cuda)
+        self.refs = torch.zeros(pages, **ints)
+        self.tables = torch.full((rows, cols + wide), -1, **ints)[:, :cols]
+        self.held = torch.zeros(rows, **ints)
+        g = torch.Generator(device=cuda).manual_seed(pages)
+        self.caches = [torch.randn((pages, bs, hk, d), generator=g, device=cuda).to(dtype)
+                       for _ in range(2 * layers)]
+        self.copy = [c.clone() for c in self.caches]
+
+    def ints(self, x):
+        return torch.tensor(x, dtype=torch.int32, device=self.cuda)
+
+    @property
+    def state(self):
+        return self.refs, self.tables, self.held
+
+    def resize(self, rows, lens):
+        st = self.dsb.pages.resize_requests(*self.state, self.ints(rows), self.ints(lens),
+                                            block_size=self.bs)
+        self.ref.resize(rows, lens)
+        self.check(st)
+
+    def fork(self, parents, children, lens):
+        st = self.dsb.pages.fork_requests(*self.state, self.ints(parents), self.ints(children),
+                                          self.ints(lens), self.caches)
+        for s, t, n in self.ref.fork(parents, children, lens):
+            for c in self.copy:
+                c[t, :n] = c[s, :n]
+        self.check(st)
+
+    def compact(self):
+        st = self.dsb.pages.compact_pages(*self.state, self.caches)
+        self.ref.lacking = 0
+        moves = self.ref.compact()
+        if moves:
+            s, t = (torch.tensor(x, device=self.cuda) for x in zip(*moves))
+            for c in self.copy:
+                c[t] = c[s]
+        self.check(st)
+
+    def check(self, status):
+        assert status.tolist() == [self.ref.lacking, len(self.ref.free())]
+        assert self.refs.tolist() == self.ref.refs
+        assert self.held.tolist() == self.ref.held
+        assert self.tables.tolist() == self.ref.tables
+        for a, b in zip(self.caches, self.copy):
+            assert torch.equal(a, b)
+        want = set()
+        for name, bit in (("slot", 1), ("position", 2)):
+            if name in self.ref.flags:
+                want.add(bit)
+        self.ref.flags.clear()
+        assert self.dsb._lib.read_and_clear_error_flag(self.cuda) == sum(want)
+
+
+@pytest.mark.parametrize("pages,rows,cols,bs,layers,dtype", [
+    (64, 8, 10, 16, 1, torch.bfloat16),
+    (40, 12, 9, 1, 2, torch.float16),      # one token a page
+    (3000, 40, 100, 5, 1, torch.float32),  # several passes over the pool, odd pages
+    (1, 2, 1, 16, 1, torch.bfloat16),      # a single page
+    (9000, 16, 700, 8, 3, torch.bfloat16),
+])
+def test_random_histories(dsb, cuda, pages, rows, cols, bs, layers, dtype):
+    rng = random.Random(pages)
+    p = _Pool(dsb, cuda, pages, rows, cols, bs, layers, dtype=dtype, wide=3)
+    longest = cols * bs
+    for step in range(60):
+        what = rng.random()
+        if what < 0.5:
+            n = rng.randint(0, rows)
+            who = rng.sample(range(rows), n)
+            p.resize(who, [rng.choice([0, 1, rng.randint(0, longest), rng.randint(0, bs)])
+                           for _ in who])
+        elif what < 0.85:
+            empty = [r for r in range(rows) if not p.ref.held[r]]
+            full = [r for r in range(rows) if p.ref.held[r]] or [0]
+            kids = rng.sample(empty, rng.randint(0, len(empty)))
+            ups = [rng.choice(full) for _ in kids]
+            p.fork(ups, kids, [rng.randint(0, p.ref.held[u] * bs) for u in ups])
+        else:
+            p.compact()
+
+
+def test_a_batch_forked_from_one_prompt_and_freed(dsb, cuda):
+    p = _Pool(dsb, cuda, 600, 66, 200, 16, layers=2)
+    p.resize([0], [2999])
+    p.fork([0] * 64, list(range(65, 1, -1)), [2999] * 64)
+    assert int(p.refs.max()) == 65
+    p.resize(list(range(2, 66)), [3000 + r for r in range(64)])  # each writes on
+    p.resize([0], [0])  # the parent leaves, its pages stay
+    assert int(p.refs.max()) == 64
+    p.resize(list(range(2, 66)), [0] * 64)
+    assert int(p.refs.sum()) == 0
+
+
+def test_exhaustion(dsb, cuda):
+    """Rows in order until the first that does not fit; a smaller one behind
+    it waits too; what is let go in the call can be given in it."""
+    p = _Pool(dsb, cuda, 10, 6, 10, 4)
+    p.resize([0, 1, 2, 3], [16, 12, 16, 4])  # 4 + 3 fit; 4 do not, nor does the 1 behind
+    assert p.ref.lacking == 2
+    p.resize([2, 0], [16, 0])
+    assert p.ref.lacking == 0
+    p.fork([1] * 4, [3, 4, 5, 0], [9, 8, 9, 9])  # three started pages, three free ones
+    assert p.ref.lacking == 0 and not p.ref.free()
+    p.resize([3, 4, 5, 0], [0] * 4)
+    p.resize([5], [8])
+    p.fork([1, 1, 1], [3, 4, 0], [9, 11, 8])  # one page left: the second finds none
+    assert p.ref.lacking == 1 and p.ref.held[:5] == [2, 3, 4, 3, 0]
+
+
+def test_compact_full_empty_and_settled_pools(dsb, cuda):
+    p = _Pool(dsb, cuda, 50, 4, 50, 2)
+    p.compact()  # nothing live
+    p.resize([0, 1], [60, 40])
+    p.compact()  # nothing free
+    p.resize([0], [0])
+    p.compact()  # all live pages move
+    p.compact()  # settled
+    p.fork([1], [2], [39])
+    p.resize([1], [0])
+    p.compact()
+
+
+def test_bad_rows_are_flagged_and_left_alone(dsb, cuda):
+    p = _Pool(dsb, cuda, 30, 5, 6, 4)
+    p.resize([0, 0, 1, 7, -1, 2], [8, 24, 99, 4, 4, -1])  # twice, too long, outside, negative
+    p.fork([0, 0, 0, 9, 0, 0], [1, 1, 0, 2, 8, 3], [5, 5, 5, 1, 1, 9])
+    p.fork([4, 3], [3, 4], [0, 0])  # of nothing
+    assert p.ref.held == [2, 2, 0, 0, 0]
+
+
+def test_bad_pages_are_flagged(dsb, cuda):
+    """Entries that are no page, and a page let go twice."""
+    p = _Pool(dsb, cuda, 8, 4, 4, 4)
+    take = lambda: dsb._lib.read_and_clear_error_flag(cuda)  # noqa: E731
+    p.resize([0, 1], [16, 8])
+    p.tables[0, 1] = 99
+    p.tables[0, 2] = p.tables[0, 3]
+    st = dsb.pages.resize_requests(*p.state, p.ints([0]), p.ints([0]), block_size=4)
+    assert take() == 4 and st.tolist() == [0, 4]
+    assert p.refs.tolist()[:4] == [0, 1, 1, 0]
+    p.tables[1, 1] = -1
+    dsb.pages.fork_requests(*p.state, p.ints([1, 1]), p.ints([2, 3]), p.ints([7, 3]), p.caches)
+    assert take() == 4 and p.held.tolist() == [0, 2, 0, 1]
+    p.tables[1, 1] = 77
+    dsb.pages.compact_pages(*p.state, p.caches)
+    assert take() == 4 and int(p.tables[1, 1]) == 77
+
+
+def test_copy_pages(dsb, cuda):
+    g = torch.Generator(device=cuda).manual_seed(0)
+    for layers, bs, hk, d, n in ((1, 16, 4, 128, 13), (3, 1, 1, 8, 500), (70, 2, 1, 8, 3)):
+        pages = 3 * n + 5
+        caches = [torch.randn((pages, bs, hk, d), generator=g, device=cuda).bfloat16()
+                  for _ in range(2 * layers)]
+        want = [c.clone() for c in caches]
+        perm = torch.randperm(pages, generator=g, device=cuda)
+        src, dst = perm[:n].int(), perm[n:2 * n].int()
+        for c in want:
+            c[dst.long()[1:]] = c[src.long()[1:]]
+        src[0] = -1
+        dsb.pages.copy_pages(caches, src, dst)
+        assert all(torch.equal(a, b) for a, b in zip(caches, want))
+        assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+        dst[1] = pages
+        dsb.pages.copy_pages(caches, src[:2], dst[:2])
+        assert dsb._lib.read_and_clear_error_flag(cuda) == 4
+        assert all(torch.equal(a, b) for a, b in zip(caches, want))
+        dsb.pages.copy_pages(caches, src[:0], dst[:0])
+
+
+def test_captured(dsb, cuda):
+    """A step of freeing, forking and compacting replayed from a graph does
+    what the calls did."""
+    a, b = (_Pool(dsb, cuda, 100, 10, 20, 16) for _ in range(2))
+    kids, ups = a.ints([3, 4, 5]), a.ints([0, 1, 0])
+    none, lens = a.ints([0, 0, 0]), a.ints([37, 64, 40])
+
+    def step(p):
+        dsb.pages.resize_requests(*p.state, kids, none, block_size=16)
+        dsb.pages.fork_requests(*p.state, ups, kids, lens, p.caches)
+        return dsb.pages.compact_pages(*p.state, p.caches)
+
+    for p in (a, b):
+        p.resize([0, 1], [100, 64])
+        step(p)  # (and loads the kernels)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(b)
+    for _ in range(3):
+        step(a)
+        graph.replay()
+    torch.cuda.synchronize()
+    for x, y in zip((*a.state, *a.caches), (*b.state, *b.caches)):
+        assert torch.equal(x, y)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0

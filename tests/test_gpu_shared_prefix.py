@@ -1,0 +1,290 @@
+"""Attention of requests that share a prefix, with the softmax LSE
+(kernels.shared_prefix_attention_lse), against a plain fp64 form that gives
+every row its own full sequence.
+
+Tolerances, from the arithmetic (u = 2^-24): a logit sums 128 products in
+fp32, off by at most dS = 128 u scale max(sum |q k|); the weights carry 16
+bits (two 16-bit terms, 2^-17 relative) and sum over L tokens in fp32; the
+exponential is good to 2^-22.  So an output is off by at most
+(2 dS + 2^-17 + 2^-22 + (L / 32 + 256) u) max|v| before its rounding (half a
+step), where partial sums of 32 or more lanes and splits bound the chain of
+additions, and the LSE by dS + 2^-22 + (L / 32 + 256) u + 2 u |lse|."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+_T = {"bf16": torch.bfloat16, "f16": torch.float16}
+_D = 128
+
+
+def _case(cuda, groups, hq, hk, page, dtype, seed, scale_q=2.0):
+    """groups: [(prefix, [request lengths], span), ...].  Shared whole pages,
+    the started one copied for each request; rows in group order."""
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    tables, seq, trow, starts, prefix = [], [], [], [0], []
+    used, reqs = 0, 0
+    cols = max(max(1, -(-max(p, max(lens)) // page)) for p, lens, _ in groups)
+    copies = []
+    for p, lens, span in groups:
+        shared = list(range(used, used + p // page))
+        used += p // page
+        first = None
+        for n in lens:
+            n_pages = -(-max(n, p) // page)
+            own = list(range(used, used + n_pages - len(shared)))
+            used += len(own)
+            tables.append(shared + own + [-1] * (cols - n_pages))
+            if p % page:
+                if first is None:
+                    first = own[0]
+                copies.append((first, own[0], p % page))
+            for j in range(span):
+                seq.append(max(0, n - (span - 1 - j)))
+                trow.append(reqs)
+            reqs += 1
+        starts.append(len(seq))
+        prefix.append(p)
+    total = used + 3
+    perm = torch.randperm(total, generator=g, device=cuda)
+    table = torch.tensor(tables, device=cuda)
+    table = torch.where(table >= 0, perm[table.clamp(min=0)], table).int()
+    key, value = (torch.randn((total, page, hk, _D), generator=g, device=cuda).to(_T[dtype])
+                  for _ in range(2))
+    for s, t, n in copies:
+        for c in (key, value):
+            c[perm[t], :n] = c[perm[s], :n].clone()
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    query = (torch.randn((len(seq), hq, _D), generator=g, device=cuda) * scale_q).to(_T[dtype])
+    return dict(query=query, key=key, value=value, table=table, seq=ints(seq), trow=ints(trow),
+                starts=ints(starts), prefix=ints(prefix), max_prefix=max(prefix),
+                max_suffix=max(max(0, s - p) for s, p in zip(
+                    seq, [prefix[i] for i in range(len(groups)) for _ in range(starts[i + 1] - starts[i])])))
+
+
+def _run(dsb, c, **kw):
+    kw = {**dict(max_prefix_len=c["max_prefix"], max_suffix_len=c["max_suffix"],
+                 group_starts=c["starts"], table_rows=c["trow"], scale=_D ** -0.5), **kw}
+    return dsb.kernels.shared_prefix_attention_lse(c["query"], c["key"], c["value"], c["table"],
+                                                   c["seq"], c["prefix"], **kw)
+
+
+def _check(c, out, lse, seq=None, scale=_D ** -0.5):
+    seq = c["seq"].tolist() if seq is None else seq
+    hk, page = c["key"].shape[2], c["key"].shape[1]
+    rows, hq, _ = c["query"].shape
+    u = 2.0 ** -24
+    step = torch.finfo(c["query"].dtype).eps / 2
+    tiny = torch.finfo(c["query"].dtype).smallest_normal * step
+    for r in range(rows):
+        if seq[r] <= 0:
+            assert (out[r] == 0).all() and torch.isneginf(lse[r]).all(), r
+            continue
+        entry = c["table"][c["trow"][r].long(), : -(-seq[r] // page)].long()
+        k = c["key"][entry].reshape(-1, hk, _D)[: seq[r]].double()
+        v = c["value"][entry].reshape(-1, hk, _D)[: seq[r]].double()
+        q = c["query"][r].double().view(hk, hq // hk, _D)
+        s = torch.einsum("kgd,tkd->kgt", q, k) * scale
+        ref_lse = torch.logsumexp(s, -1).reshape(hq)
+        ref = torch.einsum("kgt,tkd->kgd", torch.softmax(s, -1), v).reshape(hq, _D)
+        ds = 128 * u * scale * float(torch.einsum("kgd,tkd->kgt", q.abs(), k.abs()).max())
+        chain = (seq[r] / 32 + 256) * u
+        e = (2 * ds + 2.0 ** -17 + 2.0 ** -22 + chain) * float(v.abs().max())
+        off = (out[r].double() - ref).abs()
+        tol = step * (ref.abs() + e) + e + tiny
+        assert bool((off <= tol).all()), (r, float((off / tol).max()))
+        tol = ds + 2.0 ** -22 + chain + 2 * u * ref_lse.abs()
+        off = (lse[r].double() - ref_lse).abs()
+        assert bool((off <= tol).all()), (r, float((off / tol).max()))
+
+
+CASES = {
+    "one row": ([(40, [41], 1)], 8, 1, 16, "bf16"),
+    "two short": ([(500, [503, 537], 1)], 8, 1, 16, "bf16"),
+    "no prefix": ([(0, [33, 1, 200], 1)], 32, 4, 16, "bf16"),
+    "prefix alone": ([(256, [256, 256, 256], 1)], 32, 4, 16, "f16"),
+    "prefix of one token": ([(1, [1, 2, 70], 1)], 4, 2, 16, "bf16"),
+    "sixteen samples": ([(1000, [1001 + 13 * i for i in range(16)], 1)], 32, 4, 16, "bf16"),
+    "verify spans": ([(777, [790, 800, 1200], 5)], 32, 4, 16, "f16"),
+    "verify spans over two tiles": ([(650, [660 + i for i in range(5)], 5)], 64, 8, 32, "bf16"),
+    "many rows": ([(384, [400 + i for i in range(70)], 1)], 64, 8, 16, "bf16"),
+    "three groups": ([(130, [140, 131], 1), (0, [50], 1), (513, [600, 514, 700, 513], 1)],
+                     8, 2, 16, "f16"),
+    "groups of many rows": ([(300, [310 + i for i in range(20)], 3), (260, [270] * 11, 2)],
+                            32, 4, 16, "bf16"),
+    "rows shorter than the prefix": ([(300, [300, 120, 0, 310, 1], 1)], 16, 2, 16, "bf16"),
+    "empty rows": ([(64, [0, 0], 1), (40, [0, 60], 1)], 8, 1, 16, "bf16"),
+    "one head each": ([(200, [210, 260], 1)], 8, 8, 16, "f16"),
+    "sixteen heads a group": ([(200, [210, 260, 201], 2)], 32, 2, 16, "bf16"),
+    "heads off the powers of two": ([(333, [340, 400, 334], 1)], 12, 2, 16, "bf16"),
+    "five heads a group": ([(150, [160, 151], 3)], 15, 3, 8, "f16"),
+    "pages of 8": ([(203, [210, 280], 1)], 8, 1, 8, "bf16"),
+    "pages of 24": ([(500, [510, 600, 501], 1)], 8, 2, 24, "f16"),
+    "pages of 128": ([(1000, [1010, 1300], 1)], 8, 2, 128, "bf16"),
+    "pages of 256": ([(700, [710, 1300], 1)], 8, 2, 256, "f16"),
+    "pages of 5": ([(203, [210, 280], 1)], 8, 1, 5, "bf16"),
+    "pages of one": ([(97, [100, 98], 1)], 8, 2, 1, "f16"),
+    "long": ([(20000, [20100, 22000, 20001], 1)], 32, 4, 16, "bf16"),
+    "long, one row's tail": ([(131, [9000, 132], 1)], 8, 1, 16, "bf16"),
+}
+
+
+@pytest.mark.parametrize("name", list(CASES))
+def test_matches_fp64(dsb, cuda, name):
+    groups, hq, hk, page, dtype = CASES[name]
+    c = _case(cuda, groups, hq, hk, page, dtype, seed=len(name))
+    out, lse = _run(dsb, c)
+    torch.cuda.synchronize()
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+    _check(c, out, lse)
+    # the bounds are bounds: larger ones give the same answer to rounding
+    out2, lse2 = _run(dsb, c, max_prefix_len=4 * c["max_prefix"] + 999,
+                      max_suffix_len=3 * c["max_suffix"] + 700)
+    _check(c, out2, lse2)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+    # run again: the same bits
+    again, lse3 = _run(dsb, c)
+    assert torch.equal(out, again) and torch.equal(lse, lse3)
+
+
+def test_defaults_and_outputs(dsb, cuda):
+    """One group without group_starts, rows on their own table rows, outputs
+    and 64-bit indices of the caller's."""
+    c = _case(cuda, [(100, [120, 101, 133], 1)], 8, 2, 16, "bf16", 3)
+    out, lse = torch.empty_like(c["query"]), torch.empty((3, 8), device=cuda)
+    got = dsb.kernels.shared_prefix_attention_lse(
+        c["query"], c["key"], c["value"], c["table"].long(), c["seq"].long(), c["prefix"].long(),
+        scale=0.3, max_prefix_len=100, max_suffix_len=33, out=out, lse=lse)
+    assert got[0] is out and got[1] is lse
+    _check(c, out, lse, scale=0.3)
+    none = dsb.kernels.shared_prefix_attention_lse(
+        c["query"][:0], c["key"], c["value"], c["table"], c["seq"], c["prefix"], scale=0.3,
+        max_prefix_len=100, max_suffix_len=33)
+    assert none[0].shape == (0, 8, _D)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+def test_what_lies_behind_the_sequences_is_not_read(dsb, cuda):
+    """NaN and infinities in the pages behind every length, and in free pages,
+    leave the results alone."""
+    for page, dtype in ((16, "bf16"), (128, "f16"), (5, "bf16")):
+        c = _case(cuda, [(203, [203, 230, 204], 1), (70, [71, 90], 2)], 16, 2, page, dtype, 4)
+        seen = torch.zeros(c["key"].shape[:2], dtype=torch.bool, device=cuda)
+        for r in range(c["seq"].numel()):
+            t = torch.arange(int(c["seq"][r]), device=cuda)
+            seen[c["table"][c["trow"][r].long(), t // page].long(), t % page] = True
+        for cache, bad in ((c["key"], float("nan")), (c["value"], float("inf"))):
+            cache[~seen] = bad
+        out, lse = _run(dsb, c)
+        _check(c, out, lse)
+        c["value"][~seen] = float("nan")
+        out, lse = _run(dsb, c)
+        _check(c, out, lse)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_sharp_and_flat_softmax(dsb, cuda, dtype):
+    """Logits that span hundreds (one token takes all, and the running maximum
+    grows late), and logits that are all equal."""
+    c = _case(cuda, [(900, [910, 1000, 901], 1)], 32, 4, 16, dtype, 6, scale_q=1.0)
+    c["query"].mul_(16)
+    # keys grow along the sequence, so the maximum keeps moving
+    for r in range(3):
+        t = torch.arange(int(c["seq"][r]), device=cuda)
+        at = (c["table"][r, t // 16].long(), t % 16)
+        grown = c["key"][at].float() * (0.2 + 2.0 * t[:, None, None] / 1000)
+        c["key"][at] = grown.to(_T[dtype])
+    for s in range(1, 3):  # the copies of the started page stay copies
+        a, b = c["table"][0, 56].long(), c["table"][s, 56].long()
+        c["key"][b, :4] = c["key"][a, :4]
+    out, lse = _run(dsb, c)
+    _check(c, out, lse)
+    c["query"].zero_()
+    out, lse = _run(dsb, c)
+    _check(c, out, lse)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+def test_bad_indices_are_flagged(dsb, cuda):
+    P = dsb._lib
+    c = _case(cuda, [(200, [230, 260, 201], 1)], 8, 2, 16, "bf16", 8)
+    take = lambda: P.read_and_clear_error_flag(cuda)  # noqa: E731
+    # a row behind max_suffix_len is cut where the splits end, and flagged
+    out, lse = _run(dsb, c, max_suffix_len=10)
+    assert take() == P.DSB_FLAG_POSITION
+    # a table row outside the table: nothing for that row, the others right
+    c["trow"][1] = 9
+    out, lse = _run(dsb, c)
+    assert take() == P.DSB_FLAG_SLOT
+    c["trow"][1] = 1
+    seq = c["seq"].tolist()
+    for r in (0, 2):
+        one = {**c, "query": c["query"][r:r + 1], "trow": c["trow"][r:r + 1]}
+        _check(one, out[r:r + 1], lse[r:r + 1], seq=[seq[r]])
+    # pages outside the cache, in the prefix and behind it
+    for col in (3, 14):
+        bad = {**c, "table": c["table"].clone()}
+        bad["table"][0, col] = 10 ** 6 if col == 3 else -5
+        _run(dsb, bad)
+        assert take() == 4
+    # lengths that no table row holds (whose unused entries, -1, are no pages either)
+    long = {**c, "seq": c["seq"] + 10 ** 6}
+    _run(dsb, long)
+    assert take() in (P.DSB_FLAG_POSITION, P.DSB_FLAG_POSITION | 4)
+    # a prefix beyond the table is cut to it
+    cut = {**c, "prefix": c["prefix"] + 10 ** 6}
+    _run(dsb, cut)
+    assert take() in (0, P.DSB_FLAG_POSITION)
+    # groups that leave rows out: those rows have no shared prefix
+    part = {**c, "starts": torch.tensor([1, 3], dtype=torch.int32, device=cuda)}
+    out, lse = _run(dsb, part, max_suffix_len=260)
+    assert take() == 0
+    _check(c, out, lse)
+
+
+def test_two_streams_and_two_graphs(dsb, cuda):
+    c = _case(cuda, [(1000, [1001 + 13 * i for i in range(16)], 1)], 32, 4, 16, "bf16", 2)
+    ref, ref_lse = _run(dsb, c)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(_run(dsb, c))
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(_run(dsb, c))
+        graphs.append(g)
+    for s, g in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            g.replay()
+            g.replay()
+    torch.cuda.synchronize()
+    for out, lse in got:
+        assert torch.equal(out, ref) and torch.equal(lse, ref_lse)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+def test_a_cache_past_32_bits(dsb, cuda):
+    """Pages whose byte and element offsets pass 2^32 and 2^31."""
+    page, hk, hq = 16, 8, 64
+    pages = 2 ** 31 // (page * hk * _D) + 600
+    key, value = (torch.zeros((pages, page, hk, _D), dtype=torch.bfloat16, device=cuda)
+                  for _ in range(2))
+    c = _case(cuda, [(500, [530, 600], 1)], hq, hk, page, "bf16", 12)
+    n = c["key"].shape[0]
+    key[-n:], value[-n:] = c["key"], c["value"]
+    c["table"] = torch.where(c["table"] >= 0, c["table"] + (pages - n), c["table"])
+    c |= dict(key=key, value=value)
+    out, lse = _run(dsb, c)
+    torch.cuda.synchronize()
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+    _check(c, out, lse)

@@ -12,6 +12,7 @@ operator surface:
 * ``selection``   — ``select_context_chunks`` (+ batched/device plan helpers)
 * ``attention``   — ``draft_decode_attention``
 * ``runtime``     — ``DiffSpecDraftCache`` retrieval hook / rebuild / attention
+* ``pages``       — pages of the target's cache: resize, fork, compact, copy
 * ``parallel``    — head-sharded score exchange over NCCL
 * ``draft_layer`` — one Eagle3-style draft decoder layer built on the above
 * ``torch_ops``   — the same entry points as ``torch.ops.diffspec_b200.*`` custom
@@ -24,7 +25,7 @@ also registers it (and its submodules) as ``diffspec_b200``.
 
 import sys as _sys
 
-from . import _lib, attention, compact_kv, draft_layer, kernels, parallel, runtime, selection  # noqa: F401
+from . import _lib, attention, compact_kv, draft_layer, kernels, pages, parallel, runtime, selection  # noqa: F401
 from . import torch_ops  # noqa: F401  (registers torch.ops.diffspec_b200.*)
 from .attention import AttentionWorkspace, draft_decode_attention  # noqa: F401
 from .compact_kv import rebuild_compact_kv_from_plan  # noqa: F401
@@ -41,8 +42,8 @@ from .runtime import (  # noqa: F401
 from .selection import DiffSpecSelection, build_history_plan, select_context_chunks, select_rows  # noqa: F401
 
 _sys.modules.setdefault("diffspec_b200", _sys.modules[__name__])
-for _name in ("_lib", "attention", "compact_kv", "draft_layer", "kernels", "parallel", "runtime", "selection",
-              "torch_ops"):
+for _name in ("_lib", "attention", "compact_kv", "draft_layer", "kernels", "pages", "parallel", "runtime",
+              "selection", "torch_ops"):
     _sys.modules.setdefault(f"diffspec_b200.{_name}", _sys.modules[f"{__name__}.{_name}"])
 
 

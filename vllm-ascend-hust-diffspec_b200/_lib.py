@@ -165,6 +165,38 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int, [_P, _I32, _P, _I32, _P, _P, _P, _P, _P, _P],
     ),
     "dsb_rows_to_slots": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _P, _P]),
+    "dsb_qk_norm_rope": (
+        ctypes.c_int,
+        [_P, _I64, _P, _I64, _I32, _P, _I64, _P, _P, _I64, _P, _I32, _I32, _I32, _I32, _P, _P, _F32,
+         _P, _I32, _I32, _P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I32, _I64, _P, _P],
+    ),
+    "dsb_qk_norm_rope_paged": (
+        ctypes.c_int,
+        [_P, _I64, _P, _I64, _I32, _P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _F32, _P,
+         _I32, _P, _I64, _I32, _I32, _I32, _P, _P, _I64, _I32, _P, _I64, _I64, _I64, _P, _P, _P],
+    ),
+    "dsb_shared_prefix_scratch_floats": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "dsb_shared_prefix_attention_lse": (
+        ctypes.c_int,
+        [_P, _I32, _I32, _I32, _I32, _P, _P, _I64, _I32, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I32,
+         _I32, _I32, _F32, _I32, _P, _P, _P, _I64, _P, _P],
+    ),
+    "dsb_resize_requests": (
+        ctypes.c_int,
+        [_P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _I32, _I32, _P, _P, _P],
+    ),
+    "dsb_fork_scratch_ints": (_I64, [_I32]),
+    "dsb_fork_requests": (
+        ctypes.c_int,
+        [_P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I32, _I32, _P, _I32, _I64, _P, _P, _I64,
+         _P, _P],
+    ),
+    "dsb_compact_scratch_ints": (_I64, [_I64]),
+    "dsb_compact_pages": (
+        ctypes.c_int,
+        [_P, _I64, _P, _I64, _I64, _I64, _P, _I32, _P, _I32, _I64, _P, _P, _I64, _P, _P],
+    ),
+    "dsb_copy_pages": (ctypes.c_int, [_P, _I32, _I64, _I64, _P, _P, _I32, _P, _P]),
 }
 
 _lock = threading.Lock()
@@ -231,6 +263,16 @@ def check(status: int, what: str) -> None:
 
 def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """:func:`call` with ``device`` current (the kernels of tensors on another
+    device than the current one)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        check(getattr(load(), name)(*args), name)
+        return
+    with torch.cuda.device(device):
+        check(getattr(load(), name)(*args), name)
 
 
 _error_flags: dict[int, torch.Tensor] = {}

@@ -1,0 +1,270 @@
+// RMSNorm of every query and key head with the position rotation in the same
+// pass, and the step's K/V rows written where the next kernels read them.
+//
+// With x a head of the projection (fp32 math throughout):
+//   y   = x * rsqrt(mean(x^2) + eps) * w
+//   out = rotate(y, cos, sin of the token's position)
+// rounded once, when a value is stored.  The draft layer takes the rotated
+// keys and the values as contiguous rows for its attention, and the raw
+// cache the normed keys before the rotation (the working-cache rebuild
+// rotates them at their local positions); the target's step writes rotated
+// keys and values into its pages.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace dsb {
+namespace {
+
+enum { kDestNone = 0, kDestRaw = 1, kDestPaged = 2 };
+
+struct QkArgs {
+  const void *q, *k, *v;
+  void *q_out, *k_out, *v_out;  // k_out / v_out: contiguous rows, or null
+  int64_t q_stride, qo_stride, k_stride, v_stride;  // elements between tokens
+  const void *qw, *kw;
+  float eps;
+  const void *cos_sin;
+  int64_t cs_stride;
+  const int32_t *positions;
+  int pos_offset, rotary_rows;
+  int tokens, hq, hk, d, rot, neox;
+  // K/V destination: raw caches [dst_rows slots, max_len, hk, d] at
+  // [index[t], abs_pos[t]], or pages of table row index[t] (t when null)
+  int dest;
+  void *dst_k, *dst_v;
+  const int32_t *index;
+  const int64_t *abs_pos;
+  int64_t dst_rows, max_len;
+  const int32_t *bt;
+  int64_t bt_stride, bt_cols, nblocks;
+  int bs;
+  int32_t *err;
+};
+
+// Row (in units of hk * d elements) of the destination caches that token t's
+// K/V go to; -1: none (a padding token, or a bad index, which is flagged).
+__device__ __forceinline__ int64_t dest_row(const QkArgs &a, int t, int pos, bool report) {
+  if (a.dest == kDestRaw) {
+    const int slot = a.index[t];
+    if (slot < 0) return -1;
+    const int64_t p = a.abs_pos[t];
+    if (slot >= a.dst_rows || p < 0 || p >= a.max_len) {
+      if (report) flag_error(a.err, slot >= a.dst_rows ? DSB_FLAG_SLOT : DSB_FLAG_POSITION);
+      return -1;
+    }
+    return slot * a.max_len + p;
+  }
+  const int row = a.index != nullptr ? a.index[t] : t;
+  if (row < 0) return -1;
+  if (row >= a.dst_rows || pos < 0 || pos / a.bs >= a.bt_cols) {
+    if (report) flag_error(a.err, row >= a.dst_rows ? DSB_FLAG_SLOT : DSB_FLAG_POSITION);
+    return -1;
+  }
+  const int64_t page = a.bt[row * a.bt_stride + pos / a.bs];
+  if (page < 0 || page >= a.nblocks) {
+    if (report) flag_error(a.err, DSB_FLAG_BLOCK);
+    return -1;
+  }
+  return page * a.bs + pos % a.bs;
+}
+
+// One warp per (token, head), heads in the order q, k, v.  Element pairs that
+// rotate together are read and written by one lane, so q_out may be q.
+template <typename T, typename CS>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkArgs a) {
+  pdl_begin();
+  const int64_t warp = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  const int heads = a.hq + 2 * a.hk;
+  if (warp >= (int64_t)a.tokens * heads) return;
+  const int t = (int)(warp / heads), h = (int)(warp % heads);
+  const int d = a.d;
+  const int pos = a.positions[t] + a.pos_offset;
+  const bool is_q = h < a.hq;
+  const int kh = is_q ? 0 : (h - a.hq) % a.hk;
+  int64_t row = -1;
+  if (!is_q && a.dest != kDestNone)
+    row = dest_row(a, t, pos, lane == 0 && h == a.hq);
+  T *dst_v = nullptr, *dst_k = nullptr;
+  if (row >= 0) {
+    dst_k = static_cast<T *>(a.dst_k) + (row * a.hk + kh) * d;
+    dst_v = static_cast<T *>(a.dst_v) + (row * a.hk + kh) * d;
+  }
+  const int64_t out_row = ((int64_t)t * a.hk + kh) * d;
+  if (h >= a.hq + a.hk) {  // value head: copied
+    const T *src = static_cast<const T *>(a.v) + t * a.v_stride + (int64_t)kh * d;
+    T *out = a.v_out != nullptr ? static_cast<T *>(a.v_out) + out_row : nullptr;
+    for (int i = lane; i < d; i += 32) {
+      const T x = src[i];
+      if (out != nullptr) out[i] = x;
+      if (dst_v != nullptr) dst_v[i] = x;
+    }
+    return;
+  }
+  const T *src = is_q ? static_cast<const T *>(a.q) + t * a.q_stride + (int64_t)h * d
+                      : static_cast<const T *>(a.k) + t * a.k_stride + (int64_t)kh * d;
+  T *out = is_q ? static_cast<T *>(a.q_out) + t * a.qo_stride + (int64_t)h * d
+                : (a.k_out != nullptr ? static_cast<T *>(a.k_out) + out_row : nullptr);
+  const T *w = static_cast<const T *>(is_q ? a.qw : a.kw);
+  float ss = 0.f;
+  for (int i = lane; i < d; i += 32) {
+    const float x = Elem<T>::to_f(src[i]);
+    ss = fmaf(x, x, ss);
+  }
+  const float inv = rsqrtf(warp_sum(ss) / static_cast<float>(d) + a.eps);
+  bool turn = true;
+  if (pos < 0 || pos >= a.rotary_rows) {  // no such row of the table: normed only
+    if (lane == 0 && h == 0) flag_error(a.err, DSB_FLAG_POSITION);
+    turn = false;
+  }
+  const CS *cs = static_cast<const CS *>(a.cos_sin) + (turn ? pos : 0) * a.cs_stride;
+  const int half = a.rot / 2;
+  auto put = [&](int i, float y, float rotated) {
+    if (out != nullptr) out[i] = Elem<T>::from_f(rotated);
+    if (dst_k != nullptr) dst_k[i] = Elem<T>::from_f(a.dest == kDestRaw ? y : rotated);
+  };
+  for (int i = lane; i < half; i += 32) {
+    const int i1 = a.neox ? i : 2 * i, i2 = a.neox ? i + half : 2 * i + 1;
+    const float y1 = Elem<T>::to_f(src[i1]) * inv * Elem<T>::to_f(w[i1]);
+    const float y2 = Elem<T>::to_f(src[i2]) * inv * Elem<T>::to_f(w[i2]);
+    const float c = turn ? Elem<CS>::to_f(cs[i]) : 1.f;
+    const float s = turn ? Elem<CS>::to_f(cs[i + half]) : 0.f;
+    put(i1, y1, turn ? y1 * c - y2 * s : y1);
+    put(i2, y2, turn ? y2 * c + y1 * s : y2);
+  }
+  for (int i = a.rot + lane; i < d; i += 32) {
+    const float y = Elem<T>::to_f(src[i]) * inv * Elem<T>::to_f(w[i]);
+    put(i, y, y);
+  }
+}
+
+int launch(const QkArgs &a, int cos_sin_dtype, int dtype, cudaStream_t st) {
+  const int64_t warps = (int64_t)a.tokens * (a.hq + 2 * a.hk);
+  if ((warps + 7) / 8 > INT32_MAX) return fail(DSB_ERR_UNSUPPORTED, "grid too large");
+  const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
+  auto go = [&](auto tag) {
+    using T = decltype(tag);
+    if (cos_sin_dtype == DSB_F32)
+      launch_kernel(qk_norm_rope_kernel<T, float>, grid, block, 0, st, a);
+    else if (cos_sin_dtype == DSB_BF16)
+      launch_kernel(qk_norm_rope_kernel<T, __nv_bfloat16>, grid, block, 0, st, a);
+    else
+      launch_kernel(qk_norm_rope_kernel<T, __half>, grid, block, 0, st, a);
+  };
+  if (dtype == DSB_BF16)
+    go(__nv_bfloat16());
+  else
+    go(__half());
+  return check_launch("qk_norm_rope_kernel");
+}
+
+// What both entry points check; fills the common arguments.
+int prepare(QkArgs &a, const void *query, int64_t query_row_stride, void *query_out,
+            int64_t query_out_row_stride, int num_query_heads, const void *key,
+            int64_t key_row_stride, const void *value, int64_t value_row_stride, int num_kv_heads,
+            int head_dim, int rotary_dim, int is_neox, const void *q_weight, const void *k_weight,
+            float eps, const int32_t *positions, int position_offset, int tokens,
+            const void *cos_sin, int64_t cos_sin_row_stride, int rotary_rows, int cos_sin_dtype,
+            int dtype, int32_t *error_flag) {
+  if (dtype != DSB_BF16 && dtype != DSB_F16)
+    return fail(DSB_ERR_INVALID, "queries and keys must be BF16 or FP16");
+  if (cos_sin_dtype != DSB_BF16 && cos_sin_dtype != DSB_F16 && cos_sin_dtype != DSB_F32)
+    return fail(DSB_ERR_INVALID, "cos_sin must be BF16, FP16 or FP32");
+  if (num_query_heads <= 0 || num_kv_heads <= 0)
+    return fail(DSB_ERR_INVALID, "head counts must be positive");
+  if (head_dim <= 0 || rotary_dim < 0 || rotary_dim % 2 || rotary_dim > head_dim ||
+      rotary_rows <= 0 || cos_sin_row_stride < rotary_dim)
+    return fail(DSB_ERR_INVALID,
+                "rotary_dim must be even and at most head_dim; cos_sin rows hold [cos | sin] of it");
+  if (!(eps >= 0.f)) return fail(DSB_ERR_INVALID, "eps must be >= 0");
+  if (!query || !query_out || !key || !value || !q_weight || !k_weight || !positions || !cos_sin)
+    return fail(DSB_ERR_INVALID, "null pointer argument");
+  const int64_t q_row = (int64_t)num_query_heads * head_dim, kv_row = (int64_t)num_kv_heads * head_dim;
+  if (query_row_stride < q_row || query_out_row_stride < q_row || key_row_stride < kv_row ||
+      value_row_stride < kv_row)
+    return fail(DSB_ERR_INVALID, "row stride shorter than its heads");
+  if (query_out == query && query_out_row_stride != query_row_stride)
+    return fail(DSB_ERR_INVALID, "in-place queries need one row stride");
+  a.q = query, a.k = key, a.v = value;
+  a.q_out = query_out;
+  a.q_stride = query_row_stride, a.qo_stride = query_out_row_stride;
+  a.k_stride = key_row_stride, a.v_stride = value_row_stride;
+  a.qw = q_weight, a.kw = k_weight, a.eps = eps;
+  a.cos_sin = cos_sin, a.cs_stride = cos_sin_row_stride;
+  a.positions = positions, a.pos_offset = position_offset, a.rotary_rows = rotary_rows;
+  a.tokens = tokens, a.hq = num_query_heads, a.hk = num_kv_heads, a.d = head_dim;
+  a.rot = rotary_dim, a.neox = is_neox ? 1 : 0;
+  a.err = error_flag;
+  return DSB_OK;
+}
+
+}  // namespace
+}  // namespace dsb
+
+using namespace dsb;
+
+extern "C" int dsb_qk_norm_rope(
+    const void *query, int64_t query_row_stride, void *query_out, int64_t query_out_row_stride,
+    int32_t num_query_heads, const void *key, int64_t key_row_stride, void *key_out,
+    const void *value, int64_t value_row_stride, void *value_out, int32_t num_kv_heads,
+    int32_t head_dim, int32_t rotary_dim, int32_t is_neox, const void *q_weight,
+    const void *k_weight, float eps, const int32_t *positions, int32_t position_offset,
+    int32_t tokens, const void *cos_sin, int64_t cos_sin_row_stride, int32_t rotary_rows,
+    int32_t cos_sin_dtype, int32_t dtype, void *raw_key, void *raw_value, const int32_t *slots,
+    const int64_t *abs_positions, int32_t num_slots, int64_t max_model_len, int32_t *error_flag,
+    void *stream) {
+  if (tokens < 0) return fail(DSB_ERR_INVALID, "negative token count");
+  if (tokens == 0) return DSB_OK;
+  QkArgs a{};
+  if (int e = prepare(a, query, query_row_stride, query_out, query_out_row_stride, num_query_heads,
+                      key, key_row_stride, value, value_row_stride, num_kv_heads, head_dim,
+                      rotary_dim, is_neox, q_weight, k_weight, eps, positions, position_offset,
+                      tokens, cos_sin, cos_sin_row_stride, rotary_rows, cos_sin_dtype, dtype,
+                      error_flag))
+    return e;
+  if (!key_out || !value_out) return fail(DSB_ERR_INVALID, "null pointer argument");
+  a.k_out = key_out, a.v_out = value_out;
+  if (raw_key != nullptr || raw_value != nullptr) {
+    if (!raw_key || !raw_value || !slots || !abs_positions)
+      return fail(DSB_ERR_INVALID, "the raw caches come together, with slots and positions");
+    if (num_slots <= 0 || max_model_len <= 0)
+      return fail(DSB_ERR_INVALID, "raw cache geometry must be positive");
+    a.dest = kDestRaw;
+    a.dst_k = raw_key, a.dst_v = raw_value;
+    a.index = slots, a.abs_pos = abs_positions;
+    a.dst_rows = num_slots, a.max_len = max_model_len;
+  }
+  return launch(a, cos_sin_dtype, dtype, as_stream(stream));
+}
+
+extern "C" int dsb_qk_norm_rope_paged(
+    const void *query, int64_t query_row_stride, void *query_out, int64_t query_out_row_stride,
+    int32_t num_query_heads, const void *key, int64_t key_row_stride, const void *value,
+    int64_t value_row_stride, int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+    int32_t is_neox, const void *q_weight, const void *k_weight, float eps,
+    const int32_t *positions, int32_t tokens, const void *cos_sin, int64_t cos_sin_row_stride,
+    int32_t rotary_rows, int32_t cos_sin_dtype, int32_t dtype, void *key_cache, void *value_cache,
+    int64_t num_blocks, int32_t block_size, const int32_t *block_table, int64_t block_table_stride,
+    int64_t block_table_rows, int64_t block_table_cols, const int32_t *table_rows,
+    int32_t *error_flag, void *stream) {
+  if (tokens < 0) return fail(DSB_ERR_INVALID, "negative token count");
+  if (tokens == 0) return DSB_OK;
+  QkArgs a{};
+  if (int e = prepare(a, query, query_row_stride, query_out, query_out_row_stride, num_query_heads,
+                      key, key_row_stride, value, value_row_stride, num_kv_heads, head_dim,
+                      rotary_dim, is_neox, q_weight, k_weight, eps, positions, 0, tokens, cos_sin,
+                      cos_sin_row_stride, rotary_rows, cos_sin_dtype, dtype, error_flag))
+    return e;
+  if (!key_cache || !value_cache || !block_table)
+    return fail(DSB_ERR_INVALID, "null pointer argument");
+  if (num_blocks <= 0 || block_size <= 0 || block_table_rows <= 0 || block_table_cols <= 0 ||
+      block_table_stride < block_table_cols)
+    return fail(DSB_ERR_INVALID, "bad cache or block-table geometry");
+  a.dest = kDestPaged;
+  a.dst_k = key_cache, a.dst_v = value_cache;
+  a.index = table_rows, a.dst_rows = block_table_rows;
+  a.bt = block_table, a.bt_stride = block_table_stride, a.bt_cols = block_table_cols;
+  a.nblocks = num_blocks, a.bs = block_size;
+  return launch(a, cos_sin_dtype, dtype, as_stream(stream));
+}

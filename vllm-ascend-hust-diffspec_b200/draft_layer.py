@@ -24,11 +24,12 @@ import torch
 
 from . import _lib
 from .attention import AttentionWorkspace, draft_decode_attention
-from .kernels import qkv_projection_write_raw
+from .kernels import _qk_norm_inputs, qkv_projection_write_raw
 
 __all__ = ["Eagle3DraftLayer", "Eagle3DraftLayerTP", "add_rms_norm", "draft_linear",
            "draft_linear_peer", "peer_add_rms_norm",
-           "interleave_gate_up", "pack_linear_weight", "rms_norm", "rope_qk", "silu_mul"]
+           "interleave_gate_up", "pack_linear_weight", "qk_norm_rope", "rms_norm", "rope_qk",
+           "silu_mul"]
 
 
 def _rows(t: torch.Tensor, what: str) -> int:
@@ -240,6 +241,71 @@ def rope_qk(query: torch.Tensor, kv: torch.Tensor, positions: torch.Tensor,
               _lib.dtype_code(cos_sin.dtype), _lib.dtype_code(kv.dtype),
               _lib.ptr(_lib.error_flag(device)), _lib.stream_ptr(device))
     return key_out, value_out
+
+
+def qk_norm_rope(query: torch.Tensor, kv: torch.Tensor, positions: torch.Tensor,
+                 cos_sin: torch.Tensor, num_kv_heads: int, q_weight: torch.Tensor,
+                 k_weight: torch.Tensor, eps: float, *, query_out: torch.Tensor | None = None,
+                 key_out: torch.Tensor | None = None, value_out: torch.Tensor | None = None,
+                 position_offset: int = 0, rotary_dim: int | None = None,
+                 is_neox_style: bool = True, raw=None):
+    """:func:`rope_qk` with RMSNorm of every query and key head before the
+    rotation, one launch (``dsb_qk_norm_rope``).
+
+    ``y = x * rsqrt(mean(x^2) + eps) * weight`` over each head of ``query
+    [T, Hq * D]`` (``q_weight [D]``) and of the keys of ``kv [T, 2 * Hk * D]``
+    (``k_weight``), rotated at ``positions + position_offset`` of the
+    ``cos_sin`` table; ``query`` and ``kv`` may be column ranges of one
+    projection.  fp32 throughout, each value rounded once when stored.
+    Queries go to ``query_out`` (default: in place), keys and values to the
+    contiguous ``key_out`` / ``value_out [T, Hk, D]``.
+
+    ``raw = (raw_key, raw_value, slots, abs_positions)`` also writes the
+    normed keys before the rotation, and the values, to the raw caches
+    ``[S, max_model_len, Hk, D]`` at ``[slots[t], abs_positions[t]]`` (int32,
+    int64; a negative slot is padding), what
+    :func:`kernels.qkv_projection_write_raw` writes for keys without a norm.
+    A position outside the table is flagged and leaves the rows normed but
+    unrotated.  Returns ``(query_out, key_out, value_out)``."""
+    d, rot, query_out, q_weight, k_weight = _qk_norm_inputs(
+        query, kv, positions, cos_sin, num_kv_heads, q_weight, k_weight, rotary_dim, query_out)
+    tokens, hk = query.shape[0], num_kv_heads
+    raw_key, raw_value, slots, abs_positions = (None,) * 4 if raw is None else raw
+    num_slots = max_len = 0
+    if raw is not None:
+        if raw_key.ndim != 4 or raw_key.shape != raw_value.shape or raw_key.shape[2:] != (hk, d):
+            raise ValueError("raw key/value must have matching [S, max_model_len, Hk, D] shapes")
+        if not (raw_key.dtype == raw_value.dtype == kv.dtype):
+            raise ValueError("raw caches must have the keys' dtype")
+        if not (raw_key.is_contiguous() and raw_value.is_contiguous()):
+            raise ValueError("raw caches must be contiguous")
+        if slots.dtype != torch.int32 or abs_positions.dtype != torch.int64:
+            raise ValueError("slots must be int32 and positions int64")
+        if slots.numel() < tokens or abs_positions.numel() < tokens or not (
+                slots.is_contiguous() and abs_positions.is_contiguous()):
+            raise ValueError("slots/positions must cover every token, contiguously")
+        num_slots, max_len = raw_key.shape[:2]
+    device = _lib.require_cuda(query, kv, positions, cos_sin, q_weight, k_weight, query_out, key_out,
+                               value_out, raw_key, raw_value, slots, abs_positions)
+    shape = (tokens, hk, d)
+    for name, t in (("key_out", key_out), ("value_out", value_out)):
+        if t is not None and (t.shape != shape or t.dtype != kv.dtype or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous [T, Hk, D] in the kv dtype")
+    if key_out is None:
+        key_out = torch.empty(shape, dtype=kv.dtype, device=device)
+    if value_out is None:
+        value_out = torch.empty(shape, dtype=kv.dtype, device=device)
+    _lib.call_on(
+        device, "dsb_qk_norm_rope", _lib.ptr(query), query.stride(0), _lib.ptr(query_out),
+        query_out.stride(0), query.shape[1] // d, _lib.ptr(kv), kv.stride(0), _lib.ptr(key_out),
+        kv.data_ptr() + hk * d * kv.element_size(), kv.stride(0), _lib.ptr(value_out), hk, d, rot,
+        int(bool(is_neox_style)), _lib.ptr(q_weight), _lib.ptr(k_weight),
+        float(eps), _lib.ptr(positions), int(position_offset), tokens, _lib.ptr(cos_sin),
+        cos_sin.stride(0), cos_sin.shape[0], _lib.dtype_code(cos_sin.dtype),
+        _lib.dtype_code(kv.dtype), _lib.ptr(raw_key), _lib.ptr(raw_value), _lib.ptr(slots),
+        _lib.ptr(abs_positions), num_slots, max_len, _lib.ptr(_lib.error_flag(device)),
+        _lib.stream_ptr(device))
+    return query_out, key_out, value_out
 
 
 def silu_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -21,6 +21,8 @@ __all__ = [
     "kv_projection_write_raw",
     "qkv_projection_write_raw",
     "paged_decode_attention_lse",
+    "shared_prefix_attention_lse",
+    "qk_norm_rope_write_paged",
 ]
 
 
@@ -571,3 +573,194 @@ def paged_decode_attention_lse(
         _lib.stream_ptr(device),
     )
     return out, lse
+
+
+def shared_prefix_attention_lse(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    *,
+    scale: float,
+    max_prefix_len: int,
+    max_suffix_len: int,
+    group_starts: torch.Tensor | None = None,
+    table_rows: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`paged_decode_attention_lse` for rows that share a prefix, whose
+    keys and values are read once for all of them.
+
+    Rows ``[group_starts[i], group_starts[i + 1])`` (int32 ``[groups + 1]``,
+    ascending from 0 to the row count; one group of every row when omitted)
+    hold the same tokens at positions ``[0, prefix_lens[i])`` (int32
+    ``[groups]``; any length, whole pages or not): requests forked from one
+    prompt (:func:`pages.fork_requests`), or verify rows of theirs.  Row ``r``
+    sees the first ``seq_lens[r]`` tokens of block-table row ``table_rows[r]``
+    (default ``r``); the prefix is read through the group's first row.  A row
+    may see less than its prefix, or nothing (zeros, and an LSE of -inf); what
+    the prefix holds must be finite.
+
+    ``max_prefix_len`` sizes the split of the prefix (a longer one is still
+    read in whole); ``max_suffix_len`` is the most tokens that any row has
+    behind its prefix: a longer row is flagged and cut there, as by
+    ``max_seq_len`` of :func:`paged_decode_attention_lse`.  Up to 16 query
+    heads per kv head.  Returns ``(out [rows, Hq, 128], lse [rows, Hq]
+    fp32)``."""
+    if query.ndim != 3 or key_cache.ndim != 4 or key_cache.shape != value_cache.shape:
+        raise ValueError("query must be [rows, Hq, D] and the caches matching [blocks, bs, Hk, D]")
+    rows, hq, d = query.shape
+    num_blocks, block_size, hk, kd = key_cache.shape
+    if d != kd or hq % hk:
+        raise ValueError("head dims must match and Hq must be a multiple of Hk")
+    if not (query.dtype == key_cache.dtype == value_cache.dtype):
+        raise ValueError("query and caches must share a dtype")
+    if block_table.ndim != 2 or seq_lens.numel() < rows:
+        raise ValueError("block_table must be 2-D and seq_lens cover every row")
+    if table_rows is None and block_table.shape[0] < rows:
+        raise ValueError("block_table must have one row per query row without table_rows")
+    if table_rows is not None and table_rows.numel() < rows:
+        raise ValueError("table_rows must map every query row")
+    groups = prefix_lens.numel()
+    if group_starts is None and groups != 1:
+        raise ValueError("prefix_lens must have one entry without group_starts")
+    if group_starts is not None and group_starts.numel() != groups + 1:
+        raise ValueError("group_starts must have one entry more than prefix_lens")
+    if max_prefix_len < 0 or max_suffix_len < 0:
+        raise ValueError("max_prefix_len and max_suffix_len must be >= 0")
+    device = _lib.require_cuda(query, key_cache, value_cache, block_table, seq_lens, prefix_lens,
+                               group_starts, table_rows, out, lse)
+    if out is None:
+        out = torch.empty((rows, hq, d), dtype=query.dtype, device=device)
+    elif out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
+        raise ValueError("out must be contiguous and shaped like query")
+    if lse is None:
+        lse = torch.empty((rows, hq), dtype=torch.float32, device=device)
+    elif lse.shape != (rows, hq) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError("lse must be contiguous fp32 [rows, Hq]")
+    if rows == 0:
+        return out, lse
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    query = query.contiguous()
+    table = _prep_index(block_table)
+    if table.stride(1) != 1:
+        table = table.contiguous()
+    seq = _prep_index(seq_lens).contiguous()
+    prefix = _prep_index(prefix_lens).contiguous()
+    starts = None if group_starts is None else _prep_index(group_starts).contiguous()
+    trows = None if table_rows is None else _prep_index(table_rows).contiguous()
+    sizes = (int(max_prefix_len), int(max_suffix_len))
+    floats = _lib.load().dsb_shared_prefix_scratch_floats(rows, hq, hk, groups, block_size, *sizes)
+    scratch = torch.empty(max(floats, 1), dtype=torch.float32, device=device)
+    _lib.call_on(
+        device, "dsb_shared_prefix_attention_lse",
+        _lib.ptr(query), rows, hq, hk, d, _lib.ptr(key_cache), _lib.ptr(value_cache), num_blocks,
+        block_size, _lib.ptr(table), table.stride(0), table.shape[0], table.shape[1],
+        _lib.ptr(seq), _lib.ptr(trows), _lib.ptr(prefix), _lib.ptr(starts), groups, *sizes,
+        float(scale), _lib.dtype_code(query.dtype), _lib.ptr(out), _lib.ptr(lse),
+        _lib.ptr(scratch), scratch.numel(), _lib.ptr(_lib.error_flag(device)),
+        _lib.stream_ptr(device),
+    )
+    return out, lse
+
+
+def _qk_norm_inputs(query, kv, positions, cos_sin, num_kv_heads, q_weight, k_weight, rotary_dim,
+                    query_out):
+    """What the two query/key norm calls check alike; returns head_dim,
+    rotary_dim, query_out and the contiguous weights."""
+    tokens = query.shape[0]
+    if query.ndim != 2 or kv.ndim != 2 or kv.shape[0] != tokens:
+        raise ValueError("query must be [T, Hq * D] and kv [T, 2 * Hk * D]")
+    if num_kv_heads <= 0 or kv.shape[1] % (2 * num_kv_heads):
+        raise ValueError("kv must hold num_kv_heads keys, then as many values")
+    d = kv.shape[1] // (2 * num_kv_heads)
+    if d == 0 or query.shape[1] == 0 or query.shape[1] % d:
+        raise ValueError("query must be [T, Hq * D] and kv [T, 2 * Hk * D]")
+    if query.stride(1) != 1 or kv.stride(1) != 1:
+        raise ValueError("query and kv must have contiguous rows")
+    if q_weight.shape != (d,) or k_weight.shape != (d,):
+        raise ValueError("q_weight and k_weight must be [head_dim]")
+    if not (query.dtype == kv.dtype == q_weight.dtype == k_weight.dtype):
+        raise ValueError("query, kv and the weights must share a dtype")
+    rotary_dim = d if rotary_dim is None else int(rotary_dim)
+    if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > d:
+        raise ValueError("rotary_dim must be even and between zero and head_dim")
+    if cos_sin.ndim != 2 or cos_sin.shape[1] < rotary_dim or cos_sin.stride(1) != 1:
+        raise ValueError("cos_sin must be a [rows, cos | sin] table of rotary_dim columns")
+    if positions.dtype != torch.int32 or positions.numel() < tokens or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int32 with one entry per token")
+    if query_out is None:
+        query_out = query
+    elif (query_out.shape != query.shape or query_out.dtype != query.dtype
+          or query_out.stride(1) != 1):
+        raise ValueError("query_out must be shaped like query, in contiguous rows")
+    return d, rotary_dim, query_out, q_weight.contiguous(), k_weight.contiguous()
+
+
+def qk_norm_rope_write_paged(
+    query: torch.Tensor,
+    kv: torch.Tensor,
+    positions: torch.Tensor,
+    cos_sin: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    eps: float,
+    *,
+    table_rows: torch.Tensor | None = None,
+    query_out: torch.Tensor | None = None,
+    rotary_dim: int | None = None,
+    is_neox_style: bool = True,
+) -> torch.Tensor:
+    """Per-head RMSNorm of the target's queries and keys, RoPE at
+    ``positions`` and the K/V write into the paged cache, one launch.
+
+    ``query [T, Hq * D]`` and ``kv [T, 2 * Hk * D]`` (keys, then values; both
+    may be column ranges of one projection) give ``query_out`` (default: in
+    place) and, at the page that block-table row ``table_rows[t]`` (default
+    ``t``) has for ``positions[t]``, the rotated keys and the values.  Norm
+    and rotation are fp32 with one rounding at the store.  A token whose
+    table row is negative is padding: its queries are processed, nothing is
+    written.  Bad indices are flagged and their K/V skipped; a position
+    outside ``cos_sin`` is flagged and leaves the rows normed but unrotated.
+    Two tokens of a call must not share a place.  Returns ``query_out``.
+    """
+    if key_cache.ndim != 4 or key_cache.shape != value_cache.shape:
+        raise ValueError("the caches must be matching [blocks, bs, Hk, D]")
+    num_blocks, block_size, hk, kd = key_cache.shape
+    d, rot, query_out, q_weight, k_weight = _qk_norm_inputs(
+        query, kv, positions, cos_sin, hk, q_weight, k_weight, rotary_dim, query_out)
+    tokens = query.shape[0]
+    if kd != d or not (key_cache.dtype == value_cache.dtype == query.dtype):
+        raise ValueError("the caches must have the keys' head_dim and dtype")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    if block_table.ndim != 2 or (table_rows is None and block_table.shape[0] < tokens):
+        raise ValueError("block_table must be 2-D with a row for every token")
+    if table_rows is not None and table_rows.numel() < tokens:
+        raise ValueError("table_rows must map every token")
+    device = _lib.require_cuda(query, kv, positions, cos_sin, key_cache, value_cache, block_table,
+                               q_weight, k_weight, table_rows, query_out)
+    table = _prep_index(block_table)
+    if table.stride(1) != 1:
+        table = table.contiguous()
+    trows = None if table_rows is None else _prep_index(table_rows).contiguous()
+    item = kv.element_size()
+    _lib.call_on(
+        device, "dsb_qk_norm_rope_paged",
+        _lib.ptr(query), query.stride(0), _lib.ptr(query_out), query_out.stride(0),
+        query.shape[1] // d, _lib.ptr(kv), kv.stride(0), kv.data_ptr() + hk * d * item,
+        kv.stride(0), hk, d, rot, int(bool(is_neox_style)), _lib.ptr(q_weight),
+        _lib.ptr(k_weight), float(eps), _lib.ptr(positions), tokens,
+        _lib.ptr(cos_sin), cos_sin.stride(0), cos_sin.shape[0], _lib.dtype_code(cos_sin.dtype),
+        _lib.dtype_code(query.dtype), _lib.ptr(key_cache), _lib.ptr(value_cache), num_blocks,
+        block_size, _lib.ptr(table), table.stride(0), table.shape[0], table.shape[1],
+        _lib.ptr(trows), _lib.ptr(_lib.error_flag(device)), _lib.stream_ptr(device),
+    )
+    return query_out

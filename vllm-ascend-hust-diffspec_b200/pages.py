@@ -1,0 +1,180 @@
+"""Pages of the target's paged K/V cache, kept on the device.
+
+A pool of ``N`` pages serves requests that grow, shrink and leave, and
+requests forked from one another (parallel samples, agents on one prompt),
+which share the pages of the tokens they have in common:
+
+* ``ref_counts [N]``       — rows that hold each page; 0 is a free page
+* ``block_tables [R, C]``  — page of each row's ``block_size`` tokens, -1 none
+* ``held [R]``             — pages each row holds (its first entries)
+
+all int32 on the device and owned by the caller; a fresh pool is zeros, -1
+and zeros.  The calls are kernels on the current stream and read nothing
+back: a bad index is skipped and flagged in the error word, and ``status [2]``
+(int32) receives the rows that found no page and the free pages left.  Pages
+are handed out lowest id first, rows in call order.  The calls change the
+pool in place, so two of them on one pool belong on one stream.
+
+The tables are the ``block_table`` of the paged kernels
+(:func:`kernels.paged_decode_attention_lse`,
+:func:`kernels.shared_prefix_attention_lse`,
+:func:`kernels.paged_chunk_attention_scores`).
+"""
+
+from __future__ import annotations
+
+import ctypes
+from collections.abc import Sequence
+
+import torch
+
+from . import _lib
+from .kernels import _prep_index
+
+__all__ = ["resize_requests", "fork_requests", "compact_pages", "copy_pages"]
+
+
+def _pool(ref_counts, block_tables, held):
+    """The pool's arguments of every call."""
+    if ref_counts.ndim != 1 or block_tables.ndim != 2 or held.ndim != 1:
+        raise ValueError("ref_counts must be [pages], block_tables [rows, cols] and held [rows]")
+    if held.shape[0] != block_tables.shape[0]:
+        raise ValueError("held must have one entry per block-table row")
+    if not (ref_counts.dtype == block_tables.dtype == held.dtype == torch.int32):
+        raise ValueError("ref_counts, block_tables and held must be int32")
+    if not (ref_counts.is_contiguous() and held.is_contiguous()) or block_tables.stride(1) != 1:
+        raise ValueError("ref_counts and held must be contiguous, block_tables in contiguous rows")
+    return (_lib.ptr(ref_counts), ref_counts.shape[0], _lib.ptr(block_tables), block_tables.shape[0],
+            block_tables.stride(0), block_tables.shape[1], _lib.ptr(held))
+
+
+def _caches(caches: Sequence[torch.Tensor], pages: int):
+    """Pointers of the caches, their page size (tokens) and a token's bytes."""
+    caches = list(caches)
+    if not caches:
+        raise ValueError("caches must name at least one tensor")
+    first = caches[0]
+    if first.ndim < 3:
+        raise ValueError("caches must be [pages, block_size, ...]")
+    for t in caches:
+        if t.shape != first.shape or t.dtype != first.dtype or not t.is_contiguous():
+            raise ValueError("caches must be contiguous tensors of one shape and dtype")
+    if first.shape[0] != pages:
+        raise ValueError("caches must have one page per reference count")
+    token_bytes = first[0, 0].numel() * first.element_size()
+    array = (ctypes.c_void_p * len(caches))(*(t.data_ptr() for t in caches))
+    return caches, array, first.shape[1], token_bytes
+
+
+def _rows(n: int, **named):
+    out = []
+    for name, t in named.items():
+        if t.ndim != 1 or t.shape[0] != n:
+            raise ValueError(f"{name} must have one entry per request of the call")
+        if t.is_floating_point() or t.dtype == torch.bool:
+            raise ValueError(f"{name} must be whole numbers")
+        out.append(_prep_index(t).contiguous())
+    return out
+
+
+def _status(status, device):
+    if status is None:
+        return torch.empty(2, dtype=torch.int32, device=device)
+    if status.shape != (2,) or status.dtype != torch.int32 or not status.is_contiguous():
+        raise ValueError("status must be int32 [2]")
+    return status
+
+
+def resize_requests(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: torch.Tensor,
+                    rows: torch.Tensor, lens: torch.Tensor, *, block_size: int,
+                    status: torch.Tensor | None = None) -> torch.Tensor:
+    """Give table row ``rows[i]`` the pages of ``lens[i]`` tokens.
+
+    Surplus pages are let go first, those of every row of the call (length 0
+    frees a request; a page that another row holds stays), then the missing
+    ones are taken from the free pages, rows in call order: the first row
+    that does not fit, and every later one that needs pages, keeps what it
+    had and is counted in ``status[0]``.  A row outside the table or named
+    twice (the first counts), and a length that the table cannot hold, are
+    flagged and left alone.  Returns ``status``."""
+    if block_size <= 0:
+        raise ValueError("block_size must be positive")
+    pool = _pool(ref_counts, block_tables, held)
+    n = rows.shape[0] if rows.ndim == 1 else -1
+    rows, lens = _rows(n, rows=rows, lens=lens)
+    device = _lib.require_cuda(ref_counts, block_tables, held, rows, lens, status)
+    status = _status(status, device)
+    _lib.call_on(device, "dsb_resize_requests", *pool, _lib.ptr(rows), _lib.ptr(lens), n,
+                 int(block_size), _lib.ptr(status), _lib.ptr(_lib.error_flag(device)),
+                 _lib.stream_ptr(device))
+    return status
+
+
+def fork_requests(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: torch.Tensor,
+                  parents: torch.Tensor, children: torch.Tensor, lens: torch.Tensor,
+                  caches: Sequence[torch.Tensor], *,
+                  status: torch.Tensor | None = None) -> torch.Tensor:
+    """Start table row ``children[i]`` from the first ``lens[i]`` tokens of
+    row ``parents[i]``.
+
+    The parent's whole pages are shared (one reference more); the page that
+    ``lens[i]`` ends inside is the child's own, the lowest free one, with
+    those tokens copied in every cache of ``caches`` (each ``[N, block_size,
+    ...]``, all layers' keys and values).  A child must hold no page
+    (:func:`resize_requests` to length 0 frees one); one that holds some, is
+    named twice (the first counts) or lies outside the table, and a length
+    beyond the parent's pages, are flagged and not forked.  Children that
+    find no page for their started one are not forked and counted in
+    ``status[0]``.  Returns ``status``."""
+    pool = _pool(ref_counts, block_tables, held)
+    caches, array, block_size, token_bytes = _caches(caches, ref_counts.shape[0])
+    n = parents.shape[0] if parents.ndim == 1 else -1
+    parents, children, lens = _rows(n, parents=parents, children=children, lens=lens)
+    device = _lib.require_cuda(ref_counts, block_tables, held, parents, children, lens, status, *caches)
+    status = _status(status, device)
+    scratch = torch.empty(6 * n, dtype=torch.int32, device=device)
+    _lib.call_on(device, "dsb_fork_requests", *pool, _lib.ptr(parents), _lib.ptr(children),
+                 _lib.ptr(lens), n, block_size, array, len(caches), token_bytes, _lib.ptr(status),
+                 _lib.ptr(scratch), scratch.numel(), _lib.ptr(_lib.error_flag(device)),
+                 _lib.stream_ptr(device))
+    return status
+
+
+def compact_pages(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: torch.Tensor,
+                  caches: Sequence[torch.Tensor], *,
+                  status: torch.Tensor | None = None) -> torch.Tensor:
+    """Move the live pages to the front of the pool.
+
+    With ``n`` live pages, the k-th live page with an id of ``n`` or more
+    moves to the k-th free page below ``n``, in every cache; the reference
+    counts move along and every row's table names the new places.  Pages
+    below ``n`` stay where they are.  Returns ``status`` (``status[1]``: the
+    free pages, now the last ones)."""
+    pool = _pool(ref_counts, block_tables, held)
+    caches, array, block_size, token_bytes = _caches(caches, ref_counts.shape[0])
+    device = _lib.require_cuda(ref_counts, block_tables, held, status, *caches)
+    status = _status(status, device)
+    ints = _lib.load().dsb_compact_scratch_ints(ref_counts.shape[0])
+    scratch = torch.empty(ints, dtype=torch.int32, device=device)
+    _lib.call_on(device, "dsb_compact_pages", *pool, block_size, array, len(caches), token_bytes,
+                 _lib.ptr(status), _lib.ptr(scratch), scratch.numel(),
+                 _lib.ptr(_lib.error_flag(device)), _lib.stream_ptr(device))
+    return status
+
+
+def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
+    """``cache[dst[i]] = cache[src[i]]`` for every cache, one launch.
+
+    Pairs with a negative page are skipped, pages outside the caches flagged.
+    No page may be both a source and a target of one call, nor a target
+    twice: the copies run at the same time."""
+    first = caches[0] if len(caches) else None
+    if first is None or first.ndim < 3:
+        raise ValueError("caches must be [pages, block_size, ...] tensors")
+    caches, array, block_size, token_bytes = _caches(caches, first.shape[0])
+    n = src.shape[0] if src.ndim == 1 else -1
+    src, dst = _rows(n, src=src, dst=dst)
+    device = _lib.require_cuda(src, dst, *caches)
+    _lib.call_on(device, "dsb_copy_pages", array, len(caches), first.shape[0],
+                 block_size * token_bytes, _lib.ptr(src), _lib.ptr(dst), n,
+                 _lib.ptr(_lib.error_flag(device)), _lib.stream_ptr(device))
