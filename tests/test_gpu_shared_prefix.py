@@ -236,10 +236,11 @@ def test_bad_indices_are_flagged(dsb, cuda):
     long = {**c, "seq": c["seq"] + 10 ** 6}
     _run(dsb, long)
     assert take() in (P.DSB_FLAG_POSITION, P.DSB_FLAG_POSITION | 4)
-    # a prefix beyond the table is cut to it
+    # a prefix beyond the table is cut to it (the rows' own tokens are then read
+    # through the first row, which has no pages for the longest)
     cut = {**c, "prefix": c["prefix"] + 10 ** 6}
     _run(dsb, cut)
-    assert take() in (0, P.DSB_FLAG_POSITION)
+    assert take() in (0, 4)
     # groups that leave rows out: those rows have no shared prefix
     part = {**c, "starts": torch.tensor([1, 3], dtype=torch.int32, device=cuda)}
     out, lse = _run(dsb, part, max_suffix_len=260)
