@@ -126,6 +126,8 @@ CASES = {
     "pages of 24": ([(500, [510, 600, 501], 1)], 8, 2, 24, "f16"),
     "pages of 128": ([(1000, [1010, 1300], 1)], 8, 2, 128, "bf16"),
     "pages of 256": ([(700, [710, 1300], 1)], 8, 2, 256, "f16"),
+    "runs of one table row longer than a tile": ([(90, [400], 40), (0, [300], 33)], 32, 4, 16, "f16"),
+    "prefix off the boxes": ([(129, [140, 300], 2), (15, [20, 400], 1)], 8, 1, 128, "bf16"),
     "pages of 5": ([(203, [210, 280], 1)], 8, 1, 5, "bf16"),
     "pages of one": ([(97, [100, 98], 1)], 8, 2, 1, "f16"),
     "long": ([(20000, [20100, 22000, 20001], 1)], 32, 4, 16, "bf16"),
@@ -214,9 +216,10 @@ def test_bad_indices_are_flagged(dsb, cuda):
     P = dsb._lib
     c = _case(cuda, [(200, [230, 260, 201], 1)], 8, 2, 16, "bf16", 8)
     take = lambda: P.read_and_clear_error_flag(cuda)  # noqa: E731
-    # a row behind max_suffix_len is cut where the splits end, and flagged
-    out, lse = _run(dsb, c, max_suffix_len=10)
-    assert take() == P.DSB_FLAG_POSITION
+    # the two lengths of the call size its launches alone
+    out, lse = _run(dsb, c, max_prefix_len=3, max_suffix_len=10)
+    _check(c, out, lse)
+    assert take() == 0
     # a table row outside the table: nothing for that row, the others right
     c["trow"][1] = 9
     out, lse = _run(dsb, c)
@@ -243,9 +246,16 @@ def test_bad_indices_are_flagged(dsb, cuda):
     assert take() in (0, 4)
     # groups that leave rows out: those rows have no shared prefix
     part = {**c, "starts": torch.tensor([1, 3], dtype=torch.int32, device=cuda)}
-    out, lse = _run(dsb, part, max_suffix_len=260)
+    out, lse = _run(dsb, part)
     assert take() == 0
     _check(c, out, lse)
+    # groups that do not ascend within the rows: flagged, and nothing shared
+    for starts in ([0, 2, 1, 3], [0, 3, 3, 4], [-1, 3, 3, 3], [2, 0, 3, 3]):
+        part = {**c, "starts": torch.tensor(starts, dtype=torch.int32, device=cuda),
+                "prefix": c["prefix"].repeat(3)}
+        out, lse = _run(dsb, part)
+        assert take() == P.DSB_FLAG_SLOT
+        _check(c, out, lse)
 
 
 def test_two_streams_and_two_graphs(dsb, cuda):

@@ -1,7 +1,7 @@
-// Split-KV paged decode attention: the partial kernel shared by the target's
-// decode attention (one range per row, from its first token) and by the
-// shared-prefix attention (each row's own tokens behind the prefix).  In an
-// unnamed namespace, so each .cu file gets its own copy.
+// Split-KV paged decode attention: the kernels shared by the target's decode
+// attention and by the shared-prefix attention over pages that its tensor
+// tiles cannot take.  In an unnamed namespace, so each .cu file gets its own
+// copy.
 #pragma once
 
 #include <algorithm>
@@ -28,37 +28,7 @@ struct TaArgs {
   void *out;
   float *lse;
   int32_t *err;
-  // RANGE kernels only: rows [group_starts[i], group_starts[i + 1]) share the
-  // first prefix_lens[i] tokens, which another kernel has taken care of
-  const int32_t *prefix_lens, *group_starts;
-  int groups;
 };
-
-// The group of `row`: the last i < groups with group_starts[i] <= row, or -1
-// when the row lies outside all of them (starts ascending; null: one group of
-// every row).  Called by whole warps.
-__device__ __forceinline__ int ta_group_of(int row, const int32_t *starts, int groups) {
-  if (starts == nullptr) return 0;
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  bool inside = false;
-  for (int base = 0; base <= groups; base += 32) {
-    const int i = base + lane;
-    const bool le = i <= groups && starts[i] <= row;
-    before += __popc(__ballot_sync(0xffffffffu, le && i < groups));
-    inside |= __any_sync(0xffffffffu, i == groups && !le);
-  }
-  return inside ? before - 1 : -1;
-}
-
-// Tokens of `row`'s prefix: its group's length, at most what a table row holds.
-__device__ __forceinline__ int ta_prefix_of(int row, const TaArgs &a) {
-  if (a.prefix_lens == nullptr) return 0;
-  const int i = ta_group_of(row, a.group_starts, a.groups);
-  if (i < 0) return 0;
-  const int64_t cap = a.bt_cols * a.bs;
-  return (int)min((int64_t)max(a.prefix_lens[i], 0), cap);
-}
 
 constexpr int kTaTile = 16;                    // tokens per warp tile
 constexpr int kTaStages = 3;                   // tiles in a warp's ring (2 in flight while one computes)
@@ -108,13 +78,12 @@ __device__ __forceinline__ void ta_ldsm_x4_trans(uint32_t (&r)[4], uint32_t addr
 //                                         V rows by ldmatrix.trans).
 // Rows past the split (or past seq_lens) are zero-filled and masked; a page
 // entry outside the cache is flagged and its tokens read as zeros.
-// RANGE: the row's tokens from its group's prefix on (the range's first tile
-// starts on a multiple of 16 tokens, the prefix's tokens in it masked like
-// those past the end), for any group of up to G query heads.
-template <typename T, int GMAX, bool RANGE>
+// ANY: a group of any size up to GMAX query heads, and the row's tokens split
+// evenly over the launch's splits whatever its length.
+template <typename T, int GMAX, bool ANY>
 __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(const TaArgs a) {
   static_assert(GMAX <= 16, "at most 16 query heads per kv head");
-  const int G = RANGE ? a.hq / a.hk : GMAX;
+  const int G = ANY ? a.hq / a.hk : GMAX;
   extern __shared__ __align__(128) uint8_t s_raw[];  // rings, then the warps' states
   pdl_begin();
   // kv head fastest: the Hk CTAs of one (split, row) read the quarters of
@@ -125,7 +94,7 @@ __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(co
   int L = a.seq[r];
   const int trow = a.trows != nullptr ? a.trows[r] : r;
   if (trow < 0 || trow >= a.bt_rows) {
-    if (threadIdx.x == 0 && split == 0 && h == 0) flag_error(a.err, DSB_FLAG_SLOT);
+    if (threadIdx.x == 0 && split == 0 && h == 0 && (!ANY || L > 0)) flag_error(a.err, DSB_FLAG_SLOT);
     L = 0;
   }
   const int64_t cap = a.bt_cols * a.bs;  // tokens the table row can address
@@ -134,14 +103,15 @@ __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(co
     L = (int)cap;
   }
   if (L < 0) L = 0;
-  const int start = RANGE ? ta_prefix_of(r, a) : 0;  // the row's first token here
-  const int base = RANGE ? start / kTaTile * kTaTile : 0;
-  if (RANGE && L <= start) L = base;  // nothing behind the prefix
-  if ((int64_t)L > (int64_t)a.splits * a.tps + base) {  // seq_lens[r] above max_seq_len
+  int tps = a.tps;
+  if (ANY)
+    tps = (int)(((int64_t)L + a.splits - 1) / a.splits + kTaTile - 1) / kTaTile * kTaTile;
+  if (!ANY && (int64_t)L > (int64_t)a.splits * tps) {  // seq_lens[r] above max_seq_len
     if (threadIdx.x == 0 && split == 0 && h == 0) flag_error(a.err, DSB_FLAG_POSITION);
-    L = a.splits * a.tps + base;
+    L = a.splits * tps;
   }
-  const int s0 = base + split * a.tps, s1 = min(L, s0 + a.tps);
+  const int s0 = (int)min((int64_t)split * tps, (int64_t)L);
+  const int s1 = (int)min((int64_t)s0 + tps, (int64_t)L);
 
   // Q A-fragments of the 8 k-steps: rows g and g + 8 are query heads
   // h * G + g (+ 8) when < G; columns 16 s + 2 t (+ 8).
@@ -190,7 +160,7 @@ __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(co
     for (int i = 0; i < kTaTile / 2; ++i) {
       const int row = 2 * i + (lane >> 4), tok = T0 + row;
       int64_t off = -1;
-      if (tok < s1 && (!RANGE || tok >= start)) {
+      if (tok < s1) {
         if (a.page_tiles) {
           if (tile_base >= 0) off = tile_base + row * tok_stride;
         } else {
@@ -244,8 +214,7 @@ __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(co
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int tok = T0 + 8 * nt + 2 * t + (j & 1);
-        const bool seen = tok < s1 && (!RANGE || tok >= start);
-        sc[nt][j] = seen ? (ce[nt][j] + co[nt][j]) * a.scale_log2 : -INFINITY;
+        sc[nt][j] = tok < s1 ? (ce[nt][j] + co[nt][j]) * a.scale_log2 : -INFINITY;
       }
     // ---- online softmax (rows g: j = 0, 1; rows g + 8: j = 2, 3)
     float mx_lo = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
@@ -255,7 +224,7 @@ __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(co
       mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, off));
       mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, off));
     }
-    // finite: the last token of the tile's part of the range is visible to every row
+    // finite: token T0 is visible to every row of the tile
     const float mn_lo = fmaxf(m_lo, mx_lo), mn_hi = fmaxf(m_hi, mx_hi);
     const float c_lo = exp2f(m_lo - mn_lo), c_hi = exp2f(m_hi - mn_hi);
     m_lo = mn_lo;

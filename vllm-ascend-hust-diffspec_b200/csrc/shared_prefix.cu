@@ -5,65 +5,307 @@
 //   out[r, h] = sum_t softmax_t(scale * q[r, h] . k_t) v_t,  t < seq_lens[r]
 //   lse[r, h] = log sum_t exp(scale * q[r, h] . k_t)          (natural log)
 //
-// Two partial passes and a merge, all on the framework's split-KV pattern:
-//  * the prefix, once for the group: the queries of all its rows that read
-//    one kv head (rows x G of them) are the M = 128 rows of tensor-core
-//    tiles, so a K/V tile read from HBM serves all of them.  Bound by that
-//    stream up to ~200 query rows (K + V of 128 tokens are 64 KB, ~2800 SM
-//    clocks of the measured copy bandwidth, against ~1540 of products), by
-//    the products beyond;
-//  * each row's own tokens behind it: the split kernel of the plain decode
-//    attention (paged_split.cuh);
-//  * the merge of both, in a fixed order.
+// The work is cut into segments, a run of tokens that a set of query rows
+// reads through one table row:
+//   * the prefix of a group, with up to 256 of its query rows (rows x the G
+//     query heads of a kv head);
+//   * the tokens behind it of consecutive rows on one table row (the verify
+//     rows of a request), with up to 128 query rows.
+// A K/V tile read from HBM thus serves every query row that sees it.  Three
+// launches: a plan of the segments (one CTA), the partial sums (one
+// persistent CTA an SM, each with an equal share of all the 128-token tiles),
+// and the merge of the pieces in order.  Which CTA computes what depends on
+// the lengths alone, and the pieces are merged in token order: the same call
+// gives the same bits.
 #include "paged_split.cuh"
 #include "tma_umma.cuh"
 
 namespace dsb {
 namespace {
 
-// ------------------------------------------------------------ prefix pass
-// CTA (kv head, split, tile of query rows): warps 0-3 and 4-7 are two softmax
-// streams, warp 8 loads, warp 9 issues the products.  Per 128-token tile of
-// a stream:
-//   S[128 x 128] = Q . K^T                (tensor memory, fp32)
-//   P = exp2(scale S - m), m the row's running maximum; a thread has a row
-//   O[128 x 128] += P . V                 (A = P from tensor memory)
-// P overwrites S as two 16-bit terms, hi + lo (the weights keep ~16 bits; one
-// term alone costs half an output step more), so P . V is two products.  O
-// is rescaled only when a row's maximum has grown by more than 2^8 since the
-// last time: until then P stays below 2^8 and sums in fp32 as well.
-//   one query tile a CTA (up to 128 query rows in a group): the streams take
-//   the split's even and odd token tiles and are merged at its end;
-//   two (more rows): each stream has 128 query rows of its own, and a K/V
-//   tile serves 256.
-// K and V tiles pass through one ring of 32 KB slots in the order of use.
 constexpr int kSpTile = 32768;      // 128 tokens x 128 dims, 16-bit: two 64-dim halves
 constexpr int kSpHalf = 16384;
 constexpr int kSpTok = 128;
+constexpr int kSpSlots = 5;         // K / V tiles in flight
 constexpr int kSpThreads = 320;
-constexpr int kSpSmem = 1024 + 7 * kSpTile + 256;  // query tiles + ring, barriers
+constexpr int kSpSmem = 1024 + (2 + kSpSlots) * kSpTile + 256;  // queries, ring, barriers
 constexpr float kSpGrow = 8.f;      // log2 of the growth that rescales O
+// A piece costs about two tiles beside its tiles (its queries, first loads
+// and sums), so each segment counts two units more than its tiles.
+constexpr int kSpStart = 2;
+
+// Tokens [tok0, tok1) for query rows m < nq: (row0 + (q0 + m) / G, head
+// (q0 + m) % G).  Tiles start at `base`, tok0 rounded down to a TMA box.
+struct alignas(16) SpSeg {
+  int32_t row0, q0, nq, trow, tok0, tok1, base;
+  int32_t len;     // units of one kv head: tiles + kSpStart, 0: nothing to do
+  int64_t unit0;   // units before this segment
+  int64_t acc;     // first row of its partial sums
+  int32_t maxp;    // pieces that one kv head may be cut into
+  int32_t pad[3];
+};
+static_assert(sizeof(SpSeg) == 64, "one segment per 64 bytes");
+
+struct SpPlanHead {
+  int64_t units;
+  int32_t segs, pad;
+};
+
+// Where a row's partial sums are: its group's first prefix segment and row,
+// its own segment and its place in it (-1: none).
+struct alignas(16) SpRow {
+  int32_t row0, pseg, sseg, srow;
+};
 
 struct SpArgs {
   TaArgs a;
-  int psplits;
-  float *acc;    // [rows * hq, psplits, D]: sums of the prefix's splits
-  float2 *ml;    // [rows * hq, psplits]: (maximum, sum)
+  const int32_t *prefix_lens, *group_starts;  // (group_starts null: one group)
+  int groups, ctas;
+  int box;             // tokens of a TMA box: 8 .. 128, dividing the page
   int64_t token_rows;  // num_blocks * block_size
-  int box;       // tokens of a TMA box: 8 .. 128, dividing the page
+  SpPlanHead *head;
+  SpSeg *segs;
+  SpRow *rows;
+  int32_t *gseg;       // [groups] first prefix segment of each
+  float *acc;          // [rows of partial sums, D]
+  float2 *ml;          // [rows of partial sums]: maximum (log2), sum
 };
 
-// One try first: most waits are over when they begin, and the bounded wait
-// reads the timer.
+// The CTA that owns unit u of `units`, and a CTA's first unit.
+__device__ __forceinline__ int sp_owner(int64_t u, int64_t units, int ctas) {
+  return (int)(((u + 1) * ctas - 1) / units);
+}
+__device__ __forceinline__ int64_t sp_first(int64_t cta, int64_t units, int ctas) {
+  return cta * units / ctas;
+}
+
+// Tokens that row r may see, 0 for a row without a valid table row.
+__device__ __forceinline__ int sp_visible(const TaArgs &a, int r, int64_t &trow, bool report) {
+  const int L = a.seq[r];
+  trow = a.trows != nullptr ? a.trows[r] : r;
+  if (L <= 0) return 0;
+  if (trow < 0 || trow >= a.bt_rows) {
+    if (report) flag_error(a.err, DSB_FLAG_SLOT);
+    return 0;
+  }
+  const int64_t cap = a.bt_cols * a.bs;
+  if (L > cap) {
+    if (report) flag_error(a.err, DSB_FLAG_POSITION);
+    return (int)cap;
+  }
+  return L;
+}
+
+// ------------------------------------------------------------------- plan
+constexpr int kPlanThreads = 1024;
+
+// Inclusive scan over the block (sum, or maximum); the last value in `total`.
+template <typename V, bool MAX> __device__ V plan_scan(V v, V *warp_v, V &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto join = [](V x, V y) { return MAX ? (x > y ? x : y) : x + y; };
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v = join(x, v);
+  }
+  __syncthreads();
+  if (lane == 31) warp_v[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    V w = warp_v[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const V x = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w = join(x, w);
+    }
+    warp_v[lane] = w;
+  }
+  __syncthreads();
+  total = warp_v[31];
+  return warp > 0 ? join(warp_v[warp - 1], v) : v;
+}
+
+__device__ __forceinline__ void sp_group(const SpArgs &s, int i, int &lo, int &hi) {
+  lo = s.group_starts != nullptr ? s.group_starts[i] : 0;
+  hi = s.group_starts != nullptr ? s.group_starts[i + 1] : s.a.rows;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const SpArgs s) {
+  __shared__ int32_t warp_i[32];
+  __shared__ int64_t warp_l[32];
+  const TaArgs &a = s.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = a.hq / a.hk, run_rows = 128 / G;
+  pdl_begin();
+
+  // prefix segments: each group's query rows, 256 at a time
+  int nprefix = 0;
+  bool bad = false;  // groups that do not ascend within the rows: nothing is shared
+  if (s.group_starts != nullptr)
+    for (int i = tid; i < s.groups; i += kPlanThreads)
+      bad |= s.group_starts[i] < 0 || s.group_starts[i + 1] < s.group_starts[i] ||
+             s.group_starts[i + 1] > a.rows;
+  bad = __syncthreads_or(bad);
+  if (bad && tid == 0) flag_error(a.err, DSB_FLAG_SLOT);
+  const int groups = bad ? 0 : s.groups;
+  for (int base = 0; base < groups; base += kPlanThreads) {
+    const int i = base + tid;
+    int tiles = 0, total;
+    if (i < groups) {
+      int lo, hi;
+      sp_group(s, i, lo, hi);
+      tiles = (int)(((int64_t)(hi - lo) * G + 255) / 256);
+    }
+    const int cum = plan_scan<int32_t, false>(tiles, warp_i, total);
+    if (i < groups) s.gseg[i] = nprefix + cum - tiles;
+    nprefix += total;
+  }
+  // every row's group
+  for (int r = tid; r < a.rows; r += kPlanThreads) s.rows[r] = SpRow{0, -1, -1, 0};
+  __syncthreads();
+
+  // segments of the rows' own tokens: rows of a group on one table row
+  int nown = 0, carry = -1;
+  for (int base = 0; base < a.rows; base += kPlanThreads) {
+    const int r = base + tid;
+    int gi = -1, lo = 0, hi = a.rows, prefix = 0;
+    int64_t trow = -1;
+    bool starts = false;
+    if (r < a.rows) {
+      if (s.group_starts == nullptr) {
+        gi = 0;
+      } else if (groups > 0) {  // the last group that begins at or before the row
+        int x = 0, y = groups;
+        while (x < y) {
+          const int mid = (x + y) / 2;
+          if (s.group_starts[mid] <= r) x = mid + 1;
+          else y = mid;
+        }
+        gi = x - 1;
+        if (gi >= 0) sp_group(s, gi, lo, hi);
+        if (gi < 0 || r >= hi) {  // outside every group: no shared prefix
+          lo = gi < 0 ? 0 : hi;
+          hi = gi < 0 ? s.group_starts[0] : a.rows;
+          gi = -1;
+        }
+      }
+      if (gi >= 0) {
+        prefix = (int)min((int64_t)max(s.prefix_lens[gi], 0), a.bt_cols * a.bs);
+        s.rows[r].row0 = lo;
+        s.rows[r].pseg = s.gseg[gi];
+      }
+      sp_visible(a, r, trow, true);
+      const int64_t before = r > lo ? (a.trows != nullptr ? a.trows[r - 1] : r - 1) : -1;
+      starts = r == lo || before != trow;
+    }
+    int total;
+    const int first = max(carry, plan_scan<int32_t, true>(starts ? r : -1, warp_i, total));
+    carry = max(carry, total);
+    // a run is taken run_rows rows at a time, by the first of them
+    const bool leads = r < a.rows && trow >= 0 && trow < a.bt_rows && (r - first) % run_rows == 0;
+    int nrows = 0, most = 0;
+    if (leads)
+      for (; nrows < run_rows && r + nrows < hi; ++nrows) {
+        const int64_t t = a.trows != nullptr ? a.trows[r + nrows] : r + nrows;
+        if (t != trow) break;
+        most = max(most, (int)min((int64_t)a.seq[r + nrows], a.bt_cols * a.bs));
+      }
+    const bool has = leads && most > prefix;
+    const int at = nprefix + nown + plan_scan<int32_t, false>(has ? 1 : 0, warp_i, total) - 1;
+    nown += total;
+    if (has) {
+      SpSeg g{};
+      g.row0 = r, g.q0 = 0, g.nq = nrows * G, g.trow = (int)trow;
+      g.tok0 = prefix, g.tok1 = most;
+      g.base = prefix / s.box * s.box;
+      g.len = (most - g.base + kSpTok - 1) / kSpTok + kSpStart;
+      s.segs[at] = g;
+      for (int j = 0; j < nrows; ++j) {
+        s.rows[r + j].sseg = at;
+        s.rows[r + j].srow = j;
+      }
+    }
+  }
+
+  // the prefix segments, a warp each: as far as any of their rows sees
+  for (int p = warp; p < nprefix; p += kPlanThreads / 32) {
+    int x = 0, y = groups;
+    while (x < y) {
+      const int mid = (x + y) / 2;
+      if (s.gseg[mid] <= p) x = mid + 1;
+      else y = mid;
+    }
+    // (groups without rows share their segment's number with the next one)
+    const int gi = x - 1;
+    int lo, hi;
+    sp_group(s, gi, lo, hi);
+    const int prefix = (int)min((int64_t)max(s.prefix_lens[gi], 0), a.bt_cols * a.bs);
+    SpSeg g{};
+    g.row0 = lo, g.q0 = (p - s.gseg[gi]) * 256;
+    g.nq = (int)min((int64_t)256, (int64_t)(hi - lo) * G - g.q0);
+    const int r0 = lo + g.q0 / G, r1 = lo + (g.q0 + g.nq - 1) / G;
+    int most = 0, trow = -1;
+    for (int r = r0 + lane; r - lane <= r1; r += 32) {
+      int64_t t = -1;
+      int L = 0;
+      if (r <= r1) L = min(sp_visible(a, r, t, false), prefix);
+      most = max(most, L);
+      const unsigned sees = __ballot_sync(0xffffffffu, L > 0);
+      const int tr = __shfl_sync(0xffffffffu, (int)t, sees ? __ffs(sees) - 1 : 0);
+      if (trow < 0 && sees) trow = tr;
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    g.trow = max(trow, 0);
+    g.tok1 = most;
+    g.len = most > 0 ? (most + kSpTok - 1) / kSpTok + kSpStart : 0;
+    if (lane == 0) s.segs[p] = g;
+  }
+  __syncthreads();
+
+  // units before each segment, then the places of their partial sums
+  const int nseg = nprefix + nown;
+  int64_t units = 0, total;
+  for (int base = 0; base < nseg; base += kPlanThreads) {
+    const int i = base + tid;
+    const int64_t mine = i < nseg ? (int64_t)s.segs[i].len * a.hk : 0;
+    const int64_t cum = plan_scan<int64_t, false>(mine, warp_l, total);
+    if (i < nseg) s.segs[i].unit0 = units + cum - mine;
+    units += total;
+  }
+  int64_t sums = 0;
+  for (int base = 0; base < nseg; base += kPlanThreads) {
+    const int i = base + tid;
+    int64_t mine = 0;
+    int maxp = 0;
+    if (i < nseg && s.segs[i].len > 0) {
+      maxp = (int)((int64_t)s.segs[i].len * s.ctas / units) + 2;
+      mine = (int64_t)a.hk * maxp * s.segs[i].nq;
+    }
+    const int64_t cum = plan_scan<int64_t, false>(mine, warp_l, total);
+    if (i < nseg) {
+      s.segs[i].maxp = maxp;
+      s.segs[i].acc = sums + cum - mine;
+    }
+    sums += total;
+  }
+  if (tid == 0) *s.head = SpPlanHead{units, nseg, 0};
+}
+
+// ---------------------------------------------------------- partial sums
+// A few tries before the bounded wait, whose timer reads cost more than a try.
 __device__ __forceinline__ bool sp_wait(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done || mbar_wait(bar, parity);
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return mbar_wait(bar, parity);
 }
 
 __device__ __forceinline__ float sp_exp2(float x) {
@@ -84,13 +326,6 @@ __device__ __forceinline__ void sp_ld32(uint32_t addr, uint32_t *r) {
       : SP_R8(r, 0), SP_R8(r, 8), SP_R8(r, 16), SP_R8(r, 24)
       : "r"(addr));
 }
-__device__ __forceinline__ void sp_st16(uint32_t addr, const uint32_t *r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15};" ::SP_U8(r, 0),
-      SP_U8(r, 8), "r"(addr)
-      : "memory");
-}
 __device__ __forceinline__ void sp_st32(uint32_t addr, const uint32_t *r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
@@ -98,8 +333,13 @@ __device__ __forceinline__ void sp_st32(uint32_t addr, const uint32_t *r) {
       SP_U8(r, 8), SP_U8(r, 16), SP_U8(r, 24), "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void sp_wait_ld() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#define SP_M8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), \
+                    "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
+// The loads are done: `r` holds its columns (named as an operand, so that
+// nothing that reads it moves before the wait).
+__device__ __forceinline__ void sp_wait_ld(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : SP_M8(r, 0), SP_M8(r, 8), SP_M8(r, 16), SP_M8(r, 24)::"memory");
 }
 __device__ __forceinline__ void sp_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -114,99 +354,121 @@ __device__ __forceinline__ void sp_umma_ts(uint32_t d, uint32_t a, uint64_t b, u
       : "memory");
 }
 
-// What a CTA works on.
-struct SpTask {
-  int row0, nrows;   // the group's rows
-  int tile;          // query tile of the group
-  int prefix;        // its tokens
-  int64_t trow;      // the table row that they are read through
-};
 
-// The CTA's (group, query tile) from blockIdx.z, by one warp; false: none.
-__device__ bool sp_find(const SpArgs &s, int per_tile, int heads, SpTask &task) {
-  const TaArgs &a = s.a;
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int base = 0; base < a.groups; base += 32) {
-    const int i = base + lane;
-    int lo = 0, hi = 0;
-    if (i < a.groups) {
-      lo = a.group_starts != nullptr ? a.group_starts[i] : 0;
-      hi = a.group_starts != nullptr ? a.group_starts[i + 1] : a.rows;
-      if ((hi < lo || lo < 0 || hi > a.rows) && blockIdx.x + blockIdx.y + blockIdx.z == 0)
-        flag_error(a.err, DSB_FLAG_SLOT);
-      lo = min(max(lo, 0), a.rows);
-      hi = min(max(hi, lo), a.rows);
-    }
-    const int tiles = (int)(((int64_t)(hi - lo) * heads + per_tile - 1) / per_tile);
-    int cum = tiles;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, cum, o);
-      if (lane >= o) cum += x;
-    }
-    const int z = (int)blockIdx.z - before;
-    const unsigned hit = __ballot_sync(0xffffffffu, cum > z);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      task.row0 = __shfl_sync(0xffffffffu, lo, src);
-      task.nrows = __shfl_sync(0xffffffffu, hi - lo, src);
-      task.tile = z - __shfl_sync(0xffffffffu, cum - tiles, src);
-      task.prefix = 0;
-      task.trow = 0;
-      // the first row of the group that sees anything
-      for (int r0 = 0; r0 < task.nrows; r0 += 32) {
-        const int r = task.row0 + r0 + lane;
-        int64_t trow = -1;
-        if (r0 + lane < task.nrows && a.seq[r] > 0) trow = a.trows != nullptr ? a.trows[r] : r;
-        const unsigned ok = __ballot_sync(0xffffffffu, trow >= 0 && trow < a.bt_rows);
-        if (ok) {
-          task.trow = __shfl_sync(0xffffffffu, trow, __ffs(ok) - 1);
-          const int p = a.prefix_lens[base + src];
-          task.prefix = (int)min((int64_t)max(p, 0), a.bt_cols * a.bs);
-          break;
-        }
-      }
-      return true;
-    }
-    before += __shfl_sync(0xffffffffu, cum, 31);
-  }
-  return false;
+// d = max(a, b, c)
+__device__ __forceinline__ float sp_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// pairs of fp32 in one 64-bit register
+__device__ __forceinline__ uint64_t sp_pair(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ float2 sp_unpair(uint64_t d) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(d));
+  return v;
+}
+__device__ __forceinline__ uint64_t sp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t sp_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 32 bytes of a row (32-byte aligned)
+__device__ __forceinline__ void sp_st_global8(float *p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]),
+               "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
 }
 
-template <typename T, int MT>  // MT query tiles a CTA
+// A CTA's share of a segment's kv head: tiles [t0, t0 + n) from `base`.
+struct SpPiece {
+  SpSeg g;
+  int h, t0, n, index;
+};
+
+// The pieces of this CTA, in order; every role walks them for itself.
+struct SpWalk {
+  int64_t u, end, units;
+  int seg;
+  __device__ bool next(const SpArgs &s, SpPiece &p) {
+    while (u < end) {
+      p.g = s.segs[seg];
+      if (u >= p.g.unit0 + (int64_t)p.g.len * s.a.hk) {
+        ++seg;
+        continue;
+      }
+      const int64_t off = u - p.g.unit0;
+      p.h = (int)(off / p.g.len);
+      const int a = (int)(off % p.g.len);
+      const int b = (int)min((int64_t)p.g.len, a + (end - u));
+      u += b - a;
+      p.t0 = max(a - kSpStart, 0);
+      p.n = max(b - kSpStart, 0) - p.t0;
+      if (p.n <= 0) continue;
+      p.index = (int)blockIdx.x -
+                sp_owner(p.g.unit0 + (int64_t)p.h * p.g.len, units, s.ctas);
+      return true;
+    }
+    return false;
+  }
+};
+
+// Warps 0-3 and 4-7 are two softmax streams, warp 8 loads, warp 9 issues the
+// products.  Per 128-token tile of a stream:
+//   S[128 x 128] = Q . K^T                (tensor memory, fp32)
+//   P = exp2(scale S - m), m the row's running maximum; a thread has a row
+//   O[128 x 128] += P . V                 (A = P from tensor memory)
+// P takes S's place as two 16-bit terms, hi + lo (the weights keep ~16 bits;
+// one term alone costs the output half a step more), so P . V is two
+// products.  O is rescaled only when a row's maximum has grown by more than
+// 2^8 since the last time: until then P stays below 2^8, in fp32 sums.
+//   up to 128 query rows in the segment: the streams take its even and odd
+//   tiles, and their sums are joined at the piece's end;
+//   more: each stream has 128 of the query rows, and takes every tile.
+// K and V tiles pass through one ring of 32 KB slots in the order of use; the
+// loads of a piece begin while the one before it is still being computed.
+template <typename T>
 __global__ void __launch_bounds__(kSpThreads, 1)
     shared_prefix_kernel(const __grid_constant__ CUtensorMap tk,
                          const __grid_constant__ CUtensorMap tv, const SpArgs s) {
-  constexpr int kSlots = MT == 1 ? 6 : 5;
   const TaArgs &a = s.a;
   extern __shared__ uint8_t sp_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(sp_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const uint32_t s_q = smem_u32(smem), s_kv = s_q + MT * kSpTile;
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + 7 * kSpTile);
-  const uint32_t full = smem_u32(bars), empty = full + 8 * kSlots, s_full = empty + 8 * kSlots,
-                 p_ready = s_full + 16, done = p_ready + 16, tail = done + 8;
+  const uint32_t s_q = smem_u32(smem), s_kv = s_q + 2 * kSpTile;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + kSpSlots) * kSpTile);
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kSpSlots, s_full = empty + 8 * kSpSlots,
+                 p_ready = s_full + 16, o_done = p_ready + 16, q_ready = o_done + 8,
+                 joint = q_ready + 8, drain = joint + 8;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_found, s_issued, s_seen;
-  __shared__ SpTask s_task;
+  __shared__ int s_abort, s_issued, s_seg;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int G = a.hq / a.hk, h = blockIdx.x, split = blockIdx.y;
+  const int G = a.hq / a.hk;
 
   if (tid == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tk)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tv)) : "memory");
-    for (int i = 0; i < 2 * kSlots; ++i) mbar_init(full + 8 * i);
+    for (int i = 0; i < 2 * kSpSlots; ++i) mbar_init(full + 8 * i);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + 8 * i);
       mbar_init_count(p_ready + 8 * i, 128);
     }
-    mbar_init(done);
-    mbar_init(tail);
+    mbar_init(o_done);
+    mbar_init_count(q_ready, 256);
+    mbar_init_count(joint, 256);
+    mbar_init(drain);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_abort = 0;
     s_issued = 0;
-    s_seen = 0;
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
@@ -215,467 +477,563 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_begin();
-  if (warp == 8) {
-    SpTask t{0, 0, 0, 0, 0};  // (no task: no rows)
-    const bool found = sp_find(s, 128 * MT, G, t);
-    if (lane == 0) {
-      s_task = t;
-      s_found = found;
+  SpWalk walk;
+  walk.units = s.head->units;
+  walk.u = sp_first(blockIdx.x, walk.units, s.ctas);
+  walk.end = sp_first(blockIdx.x + 1, walk.units, s.ctas);
+  if (warp == 8) {  // the segment that the first unit is in
+    const int nseg = s.head->segs;
+    int before = 0;  // segments that begin at or before it
+    for (int base = 0; base < nseg; base += 32) {
+      const int i = base + lane;
+      const unsigned le = __ballot_sync(0xffffffffu, i < nseg && s.segs[i].unit0 <= walk.u);
+      before += __popc(le);
+      if (le != 0xffffffffu) break;
     }
+    if (lane == 0) s_seg = max(before - 1, 0);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const SpTask task = s_task;
-  const int heads = s_found ? task.nrows * G : 0;  // query rows of the group for this kv head
+  // (empty segments begin where the next one does: none is skipped)
+  walk.seg = s_seg;
+  auto stop = [&]() {
+    atomicExch(&s_abort, 1);
+    flag_error(a.err, DSB_FLAG_TIMEOUT);
+  };
+  int pieces = 0;
+  SpPiece p;
 
-  // this thread's query row: (row, query head), or none
-  const int stream = warp >> 2;
-  const int m = task.tile * 128 * MT + (MT == 2 ? stream * 128 : 0) + (tid & 127);
-  const bool mine = warp < 8 && m < heads;
-  const int row = mine ? task.row0 + m / G : 0;
-  const int64_t rh = (int64_t)row * a.hq + h * G + (mine ? m % G : 0);
-  int lim = 0;  // the prefix tokens that it sees
-  if (mine) {
-    const int64_t trow = a.trows != nullptr ? a.trows[row] : row;
-    lim = trow >= 0 && trow < a.bt_rows ? min(max(a.seq[row], 0), task.prefix) : 0;
-  }
-  if (warp < 8) {
-    const int most = __reduce_max_sync(0xffffffffu, lim);
-    if (lane == 0) atomicMax(&s_seen, most);
-    // query tiles, swizzled as the operand wants them; rows past the group are zero
-    for (int i = tid; i < MT * 128 * 16; i += 256) {
-      const int q = i >> 4, c = i & 15;  // query row of the CTA, 16-byte piece of its 256 bytes
-      const int mm = task.tile * 128 * MT + q;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (mm < heads)
-        v = *reinterpret_cast<const uint4 *>(
-            static_cast<const T *>(a.q) +
-            ((int64_t)(task.row0 + mm / G) * a.hq + h * G + mm % G) * kTaD + c * 8);
-      const int r = q & 127;
-      *reinterpret_cast<uint4 *>(smem + (q >> 7) * kSpTile + (c >> 3) * kSpHalf + r * 128 +
-                                 (((c & 7) ^ (r & 7)) * 16)) = v;
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
-  __syncthreads();
-  const int seen = s_seen;  // prefix tokens that any of these query rows sees
-  const int ntok = (seen + kSpTok - 1) / kSpTok;
-  const int t0 = (int)((int64_t)split * ntok / s.psplits);
-  const int n = (int)((int64_t)(split + 1) * ntok / s.psplits) - t0;  // token tiles of this CTA
-
-  if (n > 0) {
-    // index of a tile's load in the order of use
-    auto k_index = [&](int j) { return MT == 2 ? 2 * j : (j < 2 ? j : 2 * j - 1); };
-    auto v_index = [&](int j) { return MT == 2 ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1); };
-
-    if (warp == 8) {
-      const int32_t *bt = a.bt + task.trow * a.bt_stride;
-      int i = 0;
-      bool bad = false, ok = true;
+  if (warp == 8) {
+    int i = 0;  // loads so far
+    bool bad = false, ok = true;
+    while (ok && walk.next(s, p)) {
+      const int32_t *bt = a.bt + (int64_t)p.g.trow * a.bt_stride;
+      const bool two = p.g.nq > 128;
       auto load = [&](int j, bool is_v) {
         if (!ok) return;
-        const int slot = i % kSlots;
-        if (i >= kSlots) ok = sp_wait(empty + 8 * slot, (uint32_t)(i / kSlots - 1) & 1u);
+        const int slot = i % kSpSlots;
+        if (i >= kSpSlots) ok = sp_wait(empty + 8 * slot, (uint32_t)(i / kSpSlots - 1) & 1u);
         ok = __all_sync(0xffffffffu, ok && !*reinterpret_cast<volatile int *>(&s_abort));
         if (!ok) return;
-        const int T0 = (t0 + j) * kSpTok;
-        const uint32_t dst = s_kv + slot * kSpTile;
-        // the values behind the last token seen are zeroed once they are here
-        // (their weights are zero, but zero times what lies there may not be)
-        const bool cut = is_v && T0 + kSpTok > seen;
-        const uint32_t bar = cut ? tail : full + 8 * slot;
+        const int T0 = p.g.base + (p.t0 + j) * kSpTok;
+        const uint32_t dst = s_kv + slot * kSpTile, bar = full + 8 * slot;
         if (lane == 0) mbar_expect_tx(bar, kSpTile);
         __syncwarp();
         const int boxes = kSpTok / s.box;
         for (int b = lane; b < 2 * boxes; b += 32) {
           const int half = b / boxes, first = (b % boxes) * s.box, tok = T0 + first;
           int y = (int)s.token_rows;  // out of range: zeros
-          if (tok < seen) {
+          if (tok < p.g.tok1) {
             const int64_t page = bt[tok / a.bs];
             if (page >= 0 && page < a.nblocks)
               y = (int)(page * a.bs + tok % a.bs);
             else
               bad = true;
           }
-          tma_load_3d(dst + half * kSpHalf + first * 128, is_v ? &tv : &tk, half * 64, h, y, bar);
+          tma_load_3d(dst + half * kSpHalf + first * 128, is_v ? &tv : &tk, half * 64, p.h, y, bar);
         }
         __syncwarp();
-        if (lane == 0) s_issued = i + 1;
-        if (cut) {
-          ok = __all_sync(0xffffffffu, sp_wait(tail, 0));
-          if (ok) {
-            const int keep = seen - T0;
-            for (int z = keep * 8 + lane; z < kSpTok * 8; z += 32) {
-              const uint32_t p = dst + (z >> 3) * 128 + (z & 7) * 16;
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(p), "r"(0u) : "memory");
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(p + kSpHalf), "r"(0u)
-                           : "memory");
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * slot);
-          }
-        }
         ++i;
       };
       load(0, false);
-      if (MT == 1 && n > 1) load(1, false);
-      for (int j = 0; j < n; ++j) {
+      if (!two && p.n > 1) load(1, false);
+      for (int j = 0; j < p.n; ++j) {
         load(j, true);
-        if (j + MT % 2 + 1 < n) load(j + MT % 2 + 1, false);
+        if (j + (two ? 1 : 2) < p.n) load(j + (two ? 1 : 2), false);
       }
-      if (bad) flag_error(a.err, DSB_FLAG_BLOCK);
-      if (!ok && lane == 0) {
-        atomicExch(&s_abort, 1);
-        flag_error(a.err, DSB_FLAG_TIMEOUT);
-      }
-    } else if (tid == 9 * 32) {
-      const uint32_t qk = umma_idesc<T, 128>(false), pv = qk | (1u << 16);  // V is dim-contiguous
-      auto slot_of = [&](int i) { return s_kv + (i % kSlots) * kSpTile; };
-      auto filled = [&](int i) {
-        const bool got = sp_wait(full + 8 * (i % kSlots), (uint32_t)(i / kSlots) & 1u);
-        tc_fence_after();
-        return got;
-      };
-      auto product_s = [&](int st, int j) {  // S of stream st
-        const uint32_t q = s_q + (MT == 2 ? st * kSpTile : 0), k = slot_of(k_index(j));
+    }
+    if (bad) flag_error(a.err, DSB_FLAG_BLOCK);
+    if (!ok && lane == 0) stop();
+    if (lane == 0) s_issued = i;
+  } else if (tid == 9 * 32) {
+    const uint32_t qk = umma_idesc<T, 128>(false), pv = qk | (1u << 16);  // V is dim-contiguous
+    int i0 = 0, kt[2] = {0, 0};  // loads and tiles of the pieces before
+    auto slot_of = [&](int i) { return s_kv + (i % kSpSlots) * kSpTile; };
+    auto filled = [&](int i) {
+      const bool got = sp_wait(full + 8 * (i % kSpSlots), (uint32_t)(i / kSpSlots) & 1u);
+      tc_fence_after();
+      return got;
+    };
+    auto freed = [&](int i) { umma_commit(empty + 8 * (i % kSpSlots)); };
+    auto product_s = [&](int st, uint32_t q, int i) {  // S of stream st, from K in load i
+      const uint32_t k = slot_of(i);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const uint32_t off = (x >> 2) * kSpHalf + (x & 3) * 32;
-          umma(tmem + st * 128, umma_desc(q + off, 16, 1024), umma_desc(k + off, 16, 1024), qk, x > 0);
-        }
-        umma_commit(s_full + 8 * st);
-      };
-      auto product_o = [&](int st, int j, bool first) {  // O of stream st
-        const uint32_t v = slot_of(v_index(j)), p = tmem + st * 128, o = tmem + 256 + st * 128;
+      for (int x = 0; x < 8; ++x) {
+        const uint32_t off = (x >> 2) * kSpHalf + (x & 3) * 32;
+        umma(tmem + st * 128, umma_desc(q + off, 16, 1024), umma_desc(k + off, 16, 1024), qk, x > 0);
+      }
+      umma_commit(s_full + 8 * st);
+    };
+    auto product_o = [&](int st, int i, bool first) {  // O of stream st, from V in load i
+      const uint32_t v = slot_of(i), o = tmem + 256 + st * 128;
 #pragma unroll
-        for (int x = 0; x < 16; ++x)  // the hi terms, then the lo ones
-          sp_umma_ts(o, p + x * 8, umma_desc(v + (x & 7) * 2048, kSpHalf, 1024), pv, !(first && x == 0));
-      };
-      auto freed = [&](int i) { umma_commit(empty + 8 * (i % kSlots)); };
-      bool ok = filled(k_index(0));
-      if (ok) {
-        product_s(0, 0);
-        if (MT == 2) product_s(1, 0);
-        freed(k_index(0));
+      for (int x = 0; x < 16; ++x) {  // 16 tokens: the hi terms, then the lo ones
+        const int c = x >> 1;
+        const uint32_t pt = tmem + st * 128 + (c >> 1) * 32 + (c & 1) * 8 + (x & 1) * 16;
+        sp_umma_ts(o, pt, umma_desc(v + c * 2048, kSpHalf, 1024), pv, !(first && x == 0));
       }
-      if (MT == 1 && n > 1 && ok) {
-        ok = filled(k_index(1));
-        if (ok) {
-          product_s(1, 1);
-          freed(k_index(1));
-        }
-      }
-      for (int j = 0; j < n && ok; ++j) {
-        ok = filled(v_index(j));
-        if (MT == 2) {
+    };
+    auto weighted = [&](int st) {  // P of stream st's next tile is in place
+      const bool got = sp_wait(p_ready + 8 * st, (uint32_t)kt[st]++ & 1u);
+      tc_fence_after();
+      return got;
+    };
+    bool ok = true;
+    while (ok && walk.next(s, p)) {
+      const int n = p.n;
+      const bool two = p.g.nq > 128;
+      // one query tile alternates between the two places
+      const uint32_t q0 = s_q + (two ? 0 : (pieces & 1) * kSpTile);
+      ok = sp_wait(q_ready, (uint32_t)pieces & 1u);
+      tc_fence_after();
+      if (two) {  // loads: K0 V0 K1 V1 ...
+        ok = ok && filled(i0);
+        if (!ok) break;
+        product_s(0, q0, i0);
+        product_s(1, q0 + kSpTile, i0);
+        freed(i0);
+        for (int j = 0; j < n && ok; ++j) {
+          const int v = i0 + 2 * j + 1, k = v + 1;
+          ok = filled(v);
           for (int st = 0; st < 2 && ok; ++st) {
-            ok = sp_wait(p_ready + 8 * st, (uint32_t)j & 1u);
+            ok = weighted(st);
             if (!ok) break;
-            tc_fence_after();
-            product_o(st, j, j == 0);
-            if (st == 1) freed(v_index(j));
+            product_o(st, v, j == 0);
+            if (st == 1) freed(v);
             if (j + 1 < n) {
-              if (st == 0) ok = filled(k_index(j + 1));
+              if (st == 0) ok = filled(k);
               if (!ok) break;
-              product_s(st, j + 1);
-              if (st == 1) freed(k_index(j + 1));
+              product_s(st, q0 + st * kSpTile, k);
+              if (st == 1) freed(k);
             }
           }
-        } else if (ok) {
-          const int st = j & 1;
-          ok = sp_wait(p_ready + 8 * st, (uint32_t)(j >> 1) & 1u);
+        }
+      } else {  // loads: K0 K1 V0 K2 V1 ... (without the K's past the last)
+        for (int st = 0; st < min(n, 2) && ok; ++st) {
+          ok = filled(i0 + st);
           if (!ok) break;
-          tc_fence_after();
-          product_o(st, j, j < 2);
-          freed(v_index(j));
+          product_s(st, q0, i0 + st);
+          freed(i0 + st);
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          const int v = i0 + min(2 * j + 2, 2 * n - 1);
+          ok = filled(v) && weighted(j & 1);
+          if (!ok) break;
+          product_o(j & 1, v, j < 2);
+          freed(v);
           if (j + 2 < n) {
-            ok = filled(k_index(j + 2));
+            const int k = i0 + 2 * j + 3;
+            ok = filled(k);
             if (!ok) break;
-            product_s(st, j + 2);
-            freed(k_index(j + 2));
+            product_s(j & 1, q0, k);
+            freed(k);
           }
         }
       }
-      if (!ok) {
-        atomicExch(&s_abort, 1);
-        flag_error(a.err, DSB_FLAG_TIMEOUT);
-      }
-      umma_commit(done);  // arrives once every issued product is done
+      if (!ok) break;
+      i0 += 2 * n;
+      umma_commit(o_done);
+      ++pieces;
     }
-
-    float m_ref = -INFINITY, l = 0.f;
+    if (!ok) stop();
+  } else if (warp < 8) {
+    const int stream = warp >> 2, m128 = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + lanes + stream * 128, to = ts + 256;
-    const int count = warp >= 8 ? 0 : (MT == 2 ? n : (n - stream + 1) / 2);
-    for (int k = 0; k < count; ++k) {
-      const int T0 = (t0 + (MT == 2 ? k : 2 * k + stream)) * kSpTok;
-      if (!__all_sync(0xffffffffu, sp_wait(s_full + 8 * stream, (uint32_t)k & 1u))) {
-        if (lane == 0) {
-          atomicExch(&s_abort, 1);
-          flag_error(a.err, DSB_FLAG_TIMEOUT);
+    const uint64_t scale2 = sp_pair(a.scale_log2, a.scale_log2);
+    const uint64_t neg1 = sp_pair(-1.f, -1.f);
+    int i0 = 0, kt = 0;  // loads and this stream's tiles of the pieces before
+    int joints = 0;
+    bool ok = true;
+    auto both = [&]() {  // all 256 threads are here (a bounded wait, unlike bar.sync)
+      mbar_arrive(joint);
+      ok = __all_sync(0xffffffffu, sp_wait(joint, (uint32_t)joints++ & 1u));
+    };
+    while (ok && walk.next(s, p)) {
+      const int n = p.n, nq = p.g.nq;
+      const bool two = nq > 128;
+      // the queries, swizzled as the operand wants them (places behind nq hold
+      // anything: a query row meets only its own sums)
+      uint8_t *qdst = smem + (two ? 0 : (pieces & 1) * kSpTile);
+      for (int b = 0; b < (two ? 2 : 1); ++b) {
+        uint4 v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int q = b * 128 + x * 16 + (tid >> 4);
+          const int mm = p.g.q0 + min(q, nq - 1);
+          v[x] = *reinterpret_cast<const uint4 *>(
+              static_cast<const T *>(a.q) +
+              ((int64_t)(p.g.row0 + mm / G) * a.hq + p.h * G + mm % G) * kTaD + (tid & 15) * 8);
         }
-        break;
-      }
-      tc_fence_after();
-      uint32_t x[128];
-      sp_ld32(ts, x);
-      sp_ld32(ts + 32, x + 32);
-      sp_ld32(ts + 64, x + 64);
-      sp_ld32(ts + 96, x + 96);
-      sp_wait_ld();
-      const int vis = lim - T0;
-      if (vis < kSpTok) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i >= vis) x[i] = __float_as_uint(-INFINITY);
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[i]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
-      if (__any_sync(0xffffffffu, top > m_ref + kSpGrow)) {
-        const float now = fmaxf(m_ref, top);
-        const float f = now == -INFINITY ? 1.f : sp_exp2(m_ref - now);
-        m_ref = now;
-        l *= f;
-        if (k > 0) {
-#pragma unroll
-          for (int c = 0; c < 128; c += 32) {
-            uint32_t o[32];
-            sp_ld32(to + c, o);
-            sp_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            sp_st32(to + c, o);
-          }
+        for (int x = 0; x < 8; ++x) {
+          const int r = x * 16 + (tid >> 4), c = tid & 15;
+          *reinterpret_cast<uint4 *>(qdst + b * kSpTile + (c >> 3) * kSpHalf + r * 128 +
+                                     (((c & 7) ^ (r & 7)) * 16)) = v[x];
         }
       }
-      const float base = m_ref == -INFINITY ? 0.f : m_ref;
-      float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 128; c += 32) {
-        uint32_t hi[16], lo[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p0 = sp_exp2(fmaf(__uint_as_float(x[c + 2 * i]), a.scale_log2, -base));
-          const float p1 = sp_exp2(fmaf(__uint_as_float(x[c + 2 * i + 1]), a.scale_log2, -base));
-          ls[(2 * i) & 3] += p0;
-          ls[(2 * i + 1) & 3] += p1;
-          pack2_split<T>(p0, p1, hi[i], lo[i]);
-        }
-        sp_st16(ts + c / 2, hi);
-        sp_st16(ts + 64 + c / 2, lo);
-      }
-      l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-      sp_wait_st();
-      tc_fence_before();
-      mbar_arrive(p_ready + 8 * stream);
-    }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(q_ready);
 
-    // every product done, every load landed: the partial sums
-    bool good = true;
-    if (warp < 8 || tid == 9 * 32) good = sp_wait(done, 0);
-    good = __syncthreads_and(good) && !s_abort;
-    if (!good) {
-      if (tid == 0) flag_error(a.err, DSB_FLAG_TIMEOUT);
-      if (tid == 8 * 32)  // (the copies in flight land, or their waits run out)
-        for (int i = max(0, s_issued - kSlots); i < s_issued; ++i)
-          mbar_wait(full + 8 * (i % kSlots), (uint32_t)(i / kSlots) & 1u);
-      if (tid == 0) mbar_wait(done, 0);
-      __syncthreads();
-      m_ref = -INFINITY;
-      l = 0.f;
-    }
-    tc_fence_after();
-    float *stage = reinterpret_cast<float *>(smem + MT * kSpTile);  // [128][132], the ring's place
-    float *part = s.acc + (rh * s.psplits + split) * kTaD;
-    if (MT == 2) {
-      if (warp < 8) {
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t o[32];
-          sp_ld32(to + c, o);
-          sp_wait_ld();
-          if (mine)
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<uint4 *>(part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        }
-        if (mine) s.ml[rh * s.psplits + split] = make_float2(m_ref, l);
+      // this thread's query row, and the tokens [tok0, lim) that it sees
+      const int m = (two ? stream * 128 : 0) + m128;
+      const bool mine = m < nq;
+      int lim = 0;
+      if (mine) {
+        int64_t t;
+        lim = min(sp_visible(a, p.g.row0 + (p.g.q0 + m) / G, t, false), p.g.tok1);
       }
-    } else {
-      __shared__ float2 s_ml[128];
-      if (stream == 1 && warp < 8) {
-        s_ml[tid & 127] = make_float2(m_ref, l);
-        if (n > 1) {
-#pragma unroll 1
-          for (int c = 0; c < 128; c += 32) {
-            uint32_t o[32];
-            sp_ld32(to + c, o);
-            sp_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<uint4 *>(stage + (tid & 127) * 132 + c + i) =
-                  make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+      const bool works = __any_sync(0xffffffffu, mine);
+      const int count = two ? n : (n - stream + 1) / 2;
+      float m_ref = -INFINITY, l = 0.f;
+      for (int k = 0; k < count; ++k) {
+        const int j = two ? k : 2 * k + stream;
+        const int T0 = p.g.base + (p.t0 + j) * kSpTok;
+        ok = __all_sync(0xffffffffu, sp_wait(s_full + 8 * stream, (uint32_t)(kt + k) & 1u));
+        if (!ok) break;
+        tc_fence_after();
+        // What a page holds behind the segment's end has weights of zero, but
+        // zero times what lies there may not be: those values become zeros.
+        if (T0 + kSpTok > p.g.tok1 && (!two || stream == 0)) {
+          const int i = i0 + (two ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1));
+          ok = __all_sync(0xffffffffu, sp_wait(full + 8 * (i % kSpSlots),
+                                               (uint32_t)(i / kSpSlots) & 1u));
+          if (!ok) break;
+          const uint32_t v = s_kv + (i % kSpSlots) * kSpTile;
+          for (int z = (p.g.tok1 - T0) * 8 + m128; z < kSpTok * 8; z += 128) {
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + z * 16), "r"(0u)
+                         : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + kSpHalf + z * 16),
+                         "r"(0u)
+                         : "memory");
           }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-      }
-      __syncthreads();
-      if (stream == 0) {
-        const float2 other = s_ml[tid];
-        const float M = fmaxf(m_ref, other.x);
-        const float f0 = M == -INFINITY ? 0.f : sp_exp2(m_ref - M);
-        const float f1 = M == -INFINITY ? 0.f : sp_exp2(other.x - M);
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t o[32];
-          sp_ld32(to + c, o);
-          sp_wait_ld();
-          if (mine)
+        if (works) {
+          const int from = p.g.tok0 - T0, till = lim - T0;  // columns seen
+          const bool whole = __all_sync(0xffffffffu, from <= 0 && till >= kSpTok);
+          auto hide = [&](uint32_t(&x)[32], int c) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c + i < from || c + i >= till) x[i] = __float_as_uint(-INFINITY);
+          };
+          // the tile's maximum, 32 columns at a time, the next ones on their way
+          float top = -INFINITY;
+          uint32_t x0[32], x1[32];
+          auto maximum = [&](uint32_t(&x)[32], int c) {
+            if (!whole) hide(x, c);
+            float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (n > 1) w = *reinterpret_cast<const float4 *>(stage + tid * 132 + c + i);
-              float4 y;
-              y.x = __uint_as_float(o[i]) * f0 + w.x * f1;
-              y.y = __uint_as_float(o[i + 1]) * f0 + w.y * f1;
-              y.z = __uint_as_float(o[i + 2]) * f0 + w.z * f1;
-              y.w = __uint_as_float(o[i + 3]) * f0 + w.w * f1;
-              *reinterpret_cast<float4 *>(part + c + i) = y;
+              t0 = sp_max3(t0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+              t1 = sp_max3(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+            }
+            top = sp_max3(top, t0, t1);
+          };
+          sp_ld32(ts, x0);
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 64) {
+            sp_wait_ld(x0);
+            sp_ld32(ts + c + 32, x1);
+            maximum(x0, c);
+            sp_wait_ld(x1);
+            sp_ld32(ts + ((c + 64) & 127), x0);  // (at the end the first again, for the weights)
+            maximum(x1, c + 32);
+          }
+          top *= a.scale_log2;
+          if (__any_sync(0xffffffffu, top > m_ref + kSpGrow)) {
+            const float now = fmaxf(m_ref, top);
+            const float f = now == -INFINITY ? 1.f : sp_exp2(m_ref - now);
+            m_ref = now;
+            l *= f;
+            if (k > 0) {
+#pragma unroll 1
+              for (int c = 0; c < 128; c += 32) {
+                uint32_t o[32];
+                sp_ld32(to + c, o);
+                sp_wait_ld(o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                sp_st32(to + c, o);
+              }
+            }
+          }
+          const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+          const uint64_t neg2 = sp_pair(neg, neg);
+          uint64_t sum0 = 0, sum1 = 0;
+          auto weights = [&](uint32_t(&x)[32], int c) {
+            if (!whole) hide(x, c);
+            uint32_t w[32];  // 16 pairs of hi terms, 16 of lo terms
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 e = sp_unpair(
+                  sp_fma2(sp_pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, neg2));
+              const float p0 = sp_exp2(e.x), p1 = sp_exp2(e.y);
+              const uint64_t pp = sp_pair(p0, p1);
+              if (i & 1) sum1 = sp_add2(sum1, pp);
+              else sum0 = sp_add2(sum0, pp);
+              w[i] = pack2<T>(p0, p1);
+              const float2 h = unpack2<T>(w[i]);
+              const float2 r = sp_unpair(sp_fma2(sp_pair(h.x, h.y), neg1, pp));
+              w[16 + i] = pack2<T>(r.x, r.y);
+            }
+            sp_st32(ts + c, w);
+          };
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 64) {
+            sp_wait_ld(x0);
+            sp_ld32(ts + c + 32, x1);
+            weights(x0, c);
+            sp_wait_ld(x1);
+            if (c == 0) sp_ld32(ts + 64, x0);
+            weights(x1, c + 32);
+          }
+          const float2 t = sp_unpair(sp_add2(sum0, sum1));
+          l += t.x + t.y;
+          sp_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(p_ready + 8 * stream);
+      }
+      if (!ok) break;
+      kt += count;
+      i0 += 2 * n;
+
+      // the piece's sums (its products are done): [nq][D], and (maximum, sum)
+      ok = __all_sync(0xffffffffu, sp_wait(o_done, (uint32_t)pieces & 1u));
+      if (!ok) break;
+      tc_fence_after();
+      const int64_t at = p.g.acc + ((int64_t)p.h * p.g.maxp + p.index) * nq + m;
+      float *part = s.acc + at * kTaD;
+      if (two) {
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t o[32];
+          sp_ld32(to + c, o);
+          sp_wait_ld(o);
+          if (mine)
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              float y[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[i + e]);
+              sp_st_global8(part + c + i, y);
             }
         }
-        if (mine) s.ml[rh * s.psplits + split] = make_float2(M, l * f0 + other.y * f1);
+        if (mine) s.ml[at] = make_float2(l != l ? 0.f : m_ref, l);  // (NaN is no empty sum)
+      } else {
+        // both streams' sums of a row lie in the same lane: each stream joins
+        // half of the columns (maxima and sums pass where the queries were)
+        float2 *ml = reinterpret_cast<float2 *>(qdst);
+        ml[stream * 128 + m128] = make_float2(m_ref, l);
+        both();
+        if (!ok) break;
+        const float2 x0 = ml[m128], x1 = ml[128 + m128];
+        const float M = fmaxf(x0.x, x1.x);
+        const float f0 = M == -INFINITY ? 0.f : sp_exp2(x0.x - M);
+        const float f1 = M == -INFINITY ? 0.f : sp_exp2(x1.x - M);
+        const uint32_t t0 = tmem + lanes + 256 + stream * 64;
+        if (works)
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t o0[32], o1[32];
+            sp_ld32(t0 + c, o0);
+            sp_ld32(t0 + 128 + c, o1);
+            sp_wait_ld(o0);
+            sp_wait_ld(o1);
+            if (mine)
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  y[e] = __uint_as_float(o0[i + e]) * f0;
+                  if (n > 1) y[e] = fmaf(__uint_as_float(o1[i + e]), f1, y[e]);
+                }
+                sp_st_global8(part + stream * 64 + c + i, y);
+              }
+          }
+        const float sum = x0.y * f0 + x1.y * f1;
+        if (mine && stream == 0) s.ml[at] = make_float2(sum != sum ? 0.f : M, sum);
+        // all of it is read before the next piece's queries and products
+        tc_fence_before();
+        both();
       }
+      ++pieces;
     }
-  } else if (mine && (MT == 2 || stream == 0)) {
-    s.ml[rh * s.psplits + split] = make_float2(-INFINITY, 0.f);  // no tokens for this split
+    if (!ok && lane == 0) stop();
   }
   tc_fence_before();
   __syncthreads();
+  if (s_abort) {
+    // A wait ran out: let the copies land and the products end before the
+    // shared and tensor memory go.
+    if (tid == 0) {
+      for (int i = max(0, s_issued - kSpSlots); i < s_issued; ++i)
+        mbar_wait(full + 8 * (i % kSpSlots), (uint32_t)(i / kSpSlots) & 1u);
+    }
+    if (tid == 9 * 32) {
+      umma_commit(drain);
+      mbar_wait(drain, 0);
+    }
+    __syncthreads();
+  }
   if (warp == 9)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// One CTA per (row, query head), thread = output element: the prefix's
-// splits, then the row's own, in order.
+// ------------------------------------------------------------------ merge
+constexpr int kMergeWarps = 4;
+
+// A warp a (row, query head), a lane four of its dims: the pieces of the
+// prefix, then of the row's own tokens, in order.
 template <typename T>
-__global__ void __launch_bounds__(kTaD) shared_prefix_merge_kernel(const SpArgs s) {
+__global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(const SpArgs s) {
   pdl_begin();
   const TaArgs &a = s.a;
-  const int64_t rh = blockIdx.x;
-  const int row = (int)(rh / a.hq), d = threadIdx.x;
-  const int np = ta_group_of(row, a.group_starts, a.groups) >= 0 ? s.psplits : 0;
-  const float2 *ml = s.ml + rh * s.psplits;
-  const float *own = a.part + rh * a.splits * (kTaD + 2);
-  float M = -INFINITY;
-  for (int i = 0; i < np; ++i) M = fmaxf(M, ml[i].x);
-  for (int i = 0; i < a.splits; ++i) M = fmaxf(M, own[i * (kTaD + 2) + kTaD]);
-  float sum = 0.f, ac = 0.f;
-  if (M != -INFINITY) {
-    for (int i = 0; i < np; ++i) {
-      const float2 x = ml[i];
-      if (x.x == -INFINITY) continue;  // (its sums were not written)
-      const float f = exp2f(x.x - M);
-      sum = fmaf(x.y, f, sum);
-      ac = fmaf(s.acc[(rh * s.psplits + i) * kTaD + d], f, ac);
-    }
-    for (int i = 0; i < a.splits; ++i) {
-      const float *q = own + i * (kTaD + 2);
-      const float f = exp2f(q[kTaD] - M);
-      sum = fmaf(q[kTaD + 1], f, sum);
-      ac = fmaf(q[d], f, ac);
+  const int64_t rh = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+  if (rh >= (int64_t)a.rows * a.hq) return;
+  const int lane = threadIdx.x & 31, G = a.hq / a.hk;
+  const int row = (int)(rh / a.hq), head = (int)(rh % a.hq), h = head / G;
+  const int64_t units = s.head->units;
+  const SpRow at = s.rows[row];
+  float M = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int m = (row - at.row0) * G + head % G;  // query row in the group
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {
+    const int seg = part == 0 ? (at.pseg < 0 ? -1 : at.pseg + m / 256) : at.sseg;
+    if (seg < 0) continue;
+    const SpSeg g = s.segs[seg];
+    if (g.len == 0) continue;
+    const int q = part == 0 ? m % 256 : at.srow * G + head % G;
+    const int64_t A = g.unit0 + (int64_t)h * g.len;
+    const int b0 = sp_owner(A, units, s.ctas), b1 = sp_owner(A + g.len - 1, units, s.ctas);
+    const int64_t first = g.acc + (int64_t)h * g.maxp * g.nq + q;
+    for (int base = b0; base <= b1; base += 32) {
+      const int b = base + lane;
+      float2 x = make_float2(-INFINITY, 0.f);
+      if (b <= b1) {  // (a piece without tiles wrote nothing)
+        const int from = (int)max(sp_first(b, units, s.ctas) - A, (int64_t)0);
+        const int till = (int)min(sp_first(b + 1, units, s.ctas) - A, (int64_t)g.len);
+        if (max(till - kSpStart, 0) > max(from - kSpStart, 0))
+          x = s.ml[first + (int64_t)(b - b0) * g.nq];
+      }
+      float top = x.x;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float now = fmaxf(M, top);
+      if (now == -INFINITY) continue;
+      const float f = exp2f(M - now);
+      M = now;
+      acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+      const float w = x.x == -INFINITY ? 0.f : exp2f(x.x - now);
+      sum = fmaf(sum, f, warp_sum(w * x.y));
+      const int n = min(32, b1 - base + 1);
+      const unsigned live = __ballot_sync(0xffffffffu, x.x != -INFINITY);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);
+        if (!(live >> i & 1)) continue;
+        const float4 v = *reinterpret_cast<const float4 *>(
+            s.acc + (first + (int64_t)(base + i - b0) * g.nq) * kTaD + 4 * lane);
+        acc.x = fmaf(v.x, wi, acc.x);
+        acc.y = fmaf(v.y, wi, acc.y);
+        acc.z = fmaf(v.z, wi, acc.z);
+        acc.w = fmaf(v.w, wi, acc.w);
+      }
     }
   }
-  const float y = sum > 0.f ? ac / sum : 0.f;
-  static_cast<T *>(a.out)[rh * kTaD + d] = Elem<T>::from_f(y);
-  if (d == 0) a.lse[rh] = sum > 0.f ? (M + log2f(sum)) * kTaLn2 : -INFINITY;
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  uint2 out;
+  out.x = pack2<T>(acc.x * inv, acc.y * inv);
+  out.y = pack2<T>(acc.z * inv, acc.w * inv);
+  if (!(sum > 0.f) && !(sum != sum)) out = make_uint2(0, 0);
+  if (sum != sum) out.x = out.y = pack2<T>(sum, sum);
+  *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + rh * kTaD + 4 * lane) = out;
+  if (lane == 0)
+    a.lse[rh] = sum != sum ? sum : (sum > 0.f ? (M + log2f(sum)) * kTaLn2 : -INFINITY);
 }
 
 // ------------------------------------------------------------------- host
-// Tokens of a split of the rows' own range: long ones when the rows alone
-// fill the GPU, else shorter ones for more CTAs (a multiple of the tile).
-int own_tokens_per_split(int64_t own, int rows, int hk) {
-  const int64_t ctas = 4LL * 148 / std::max<int64_t>(1, (int64_t)rows * hk);  // splits wanted
-  const int64_t tps = (own + std::max<int64_t>(ctas, 1) - 1) / std::max<int64_t>(ctas, 1);
-  return (int)std::min<int64_t>(1024, std::max<int64_t>(64, (tps + 15) / 16 * 16));
-}
-
 struct SpPlan {
-  bool shared;         // the prefix pass runs (else every row reads its whole sequence)
-  int box, query_tiles, psplits, ztiles;
-  int64_t own, splits; // tokens and splits of the rows' own range
-  int tps;
-  int64_t acc_floats, ml_floats, own_floats;
+  int box;             // 0: pages that no TMA box fits (every row for itself)
+  int64_t splits;      // of a row, without boxes
+  // scratch, in floats (every part a multiple of 16 bytes)
+  int64_t head, segs, rows, gseg, acc, ml, total;
 };
 
 SpPlan plan_for(int rows, int hq, int hk, int groups, int bs, int max_prefix, int max_suffix) {
   SpPlan p{};
-  // The prefix is copied in boxes of whole 8-row swizzle atoms inside a page;
-  // pages that are no multiple of 8 tokens take the rows' own pass alone.
+  // The tiles are copied in boxes of whole 8-row swizzle atoms inside a page;
+  // pages that are no multiple of 8 tokens take a pass of every row by
+  // itself (one row of 40960 tokens by itself costs what all rows do here).
   p.box = kSpTok;
   while (p.box >= 8 && bs % p.box) p.box /= 2;
-  p.shared = p.box >= 8 && max_prefix > 0;
-  if (p.shared) {
-    const int g = hq / hk;
-    const int64_t each = ((int64_t)rows + groups - 1) / groups * g;  // query rows of a group
-    p.query_tiles = each > 128 ? 2 : 1;
-    const int per = 128 * p.query_tiles;
-    p.ztiles = (int)((int64_t)rows * g / per) + groups;
-    // splits of the prefix: the fewest rounds of 148 CTAs, each with ~3 tiles'
-    // worth of start and end
-    const int64_t columns = hk * groups * ((each + per - 1) / per);
-    const int64_t tiles = ((int64_t)max_prefix + kSpTok - 1) / kSpTok;
-    int64_t best = -1;
-    for (int64_t k = 1; k <= std::min<int64_t>(tiles, 148); ++k) {
-      const int64_t rounds = (columns * k + 147) / 148, cost = rounds * ((tiles + k - 1) / k + 3);
-      if (best < 0 || cost < best) {
-        best = cost;
-        p.psplits = (int)k;
-      }
-    }
-    p.acc_floats = (int64_t)rows * hq * p.psplits * kTaD;
-    p.ml_floats = (int64_t)rows * hq * p.psplits * 2;
+  if (p.box < 8) {
+    p.box = 0;
+    // splits that give the GPU four CTAs an SM, of 64 to 1024 tokens
+    const int64_t most = (int64_t)max_prefix + max_suffix;
+    const int64_t ctas = std::max<int64_t>(1, 4LL * sm_count() / ((int64_t)rows * hk));
+    p.splits = std::max<int64_t>(std::min<int64_t>(ctas, (most + 63) / 64), (most + 1023) / 1024);
+    p.splits = std::max<int64_t>(p.splits, 1);
+    p.total = (int64_t)rows * hq * p.splits * (kTaD + 2);
+    return p;
   }
-  // the rows' own range starts on a tile of 16 tokens at or before its first
-  p.own = p.shared ? (int64_t)max_suffix + kTaTile - 1 : (int64_t)max_prefix + max_suffix;
-  p.tps = own_tokens_per_split(p.own, rows, hk);
-  p.splits = std::max<int64_t>(1, (p.own + p.tps - 1) / p.tps);
-  p.own_floats = (int64_t)rows * hq * p.splits * (kTaD + 2);
+  const int64_t g = hq / hk, ctas = sm_count();
+  const int64_t segs = ((int64_t)rows * g + 255) / 256 + groups + rows;
+  // pieces x query rows: each (row, head) is in two segments, each of which
+  // is in two pieces more than its share of the CTAs
+  const int64_t sums = 4 * (int64_t)rows * hq + 256 * ctas;
+  auto round = [](int64_t n) { return (n + 7) / 8 * 8; };
+  p.head = 0;
+  p.segs = 8;
+  p.rows = p.segs + segs * 16;
+  p.gseg = p.rows + (int64_t)rows * 4;
+  p.ml = round(p.gseg + groups);
+  p.acc = round(p.ml + 2 * sums);
+  p.total = p.acc + sums * kTaD;
   return p;
 }
 
-template <typename T, int MT> int run_prefix(const SpArgs &s, const SpPlan &p, int dtype, cudaStream_t st) {
-  auto kern = shared_prefix_kernel<T, MT>;
+template <typename T> int run_typed(SpArgs &s, const SpPlan &p, float *scratch, int dtype, cudaStream_t st) {
+  TaArgs &a = s.a;
+  const int64_t rh = (int64_t)a.rows * a.hq;
+  if (p.box == 0) {
+    a.splits = (int)p.splits;
+    a.part = scratch;
+    a.page_tiles = 0;
+    auto kern = paged_decode_split_kernel<T, 16, true>;
+    constexpr size_t smem = TaSmem<16>::kBytes;
+    if (int e = ensure_smem((const void *)kern, smem); e != DSB_OK) return e;
+    launch_kernel(kern, dim3(a.hk, a.splits, a.rows), dim3(kTaWarps * 32), smem, st, a);
+    if (int e = check_launch("paged_decode_split_kernel")) return e;
+    launch_kernel(paged_decode_merge_kernel<T>, dim3((unsigned)rh), dim3(kTaD), 0, st, a);
+    return check_launch("paged_decode_merge_kernel");
+  }
+  s.box = p.box;
+  s.ctas = sm_count();
+  s.head = reinterpret_cast<SpPlanHead *>(scratch);
+  s.segs = reinterpret_cast<SpSeg *>(scratch + p.segs);
+  s.rows = reinterpret_cast<SpRow *>(scratch + p.rows);
+  s.gseg = reinterpret_cast<int32_t *>(scratch + p.gseg);
+  s.ml = reinterpret_cast<float2 *>(scratch + p.ml);
+  s.acc = scratch + p.acc;
+  auto kern = shared_prefix_kernel<T>;
   if (int e = ensure_smem((const void *)kern, kSpSmem); e != DSB_OK) return e;
   CUtensorMap tk, tv;
-  if (!encode_paged_map(&tk, s.a.k, s.token_rows, s.a.hk, kTaD, dtype, p.box) ||
-      !encode_paged_map(&tv, s.a.v, s.token_rows, s.a.hk, kTaD, dtype, p.box))
+  if (!encode_paged_map(&tk, a.k, s.token_rows, a.hk, kTaD, dtype, p.box) ||
+      !encode_paged_map(&tv, a.v, s.token_rows, a.hk, kTaD, dtype, p.box))
     return fail(DSB_ERR_CUDA, "tensor map of the paged cache");
-  launch_kernel(kern, dim3(s.a.hk, p.psplits, p.ztiles), dim3(kSpThreads), kSpSmem, st, tk, tv, s);
-  return check_launch("shared_prefix_kernel");
-}
-
-template <typename T> int run_typed(const SpArgs &s, const SpPlan &p, int dtype, cudaStream_t st) {
-  if (p.shared) {
-    const int e = p.query_tiles == 1 ? run_prefix<T, 1>(s, p, dtype, st)
-                                     : run_prefix<T, 2>(s, p, dtype, st);
-    if (e != DSB_OK) return e;
-  }
-  const TaArgs &a = s.a;
-  auto kern = paged_decode_split_kernel<T, 16, true>;
-  constexpr size_t smem = TaSmem<16>::kBytes;
-  if (int e = ensure_smem((const void *)kern, smem); e != DSB_OK) return e;
-  launch_kernel(kern, dim3(a.hk, a.splits, a.rows), dim3(kTaWarps * 32), smem, st, a);
-  if (int e = check_launch("paged_decode_split_kernel (own range)")) return e;
-  const dim3 grid((unsigned)((int64_t)a.rows * a.hq));
-  if (p.shared)
-    launch_kernel(shared_prefix_merge_kernel<T>, grid, dim3(kTaD), 0, st, s);
-  else
-    launch_kernel(paged_decode_merge_kernel<T>, grid, dim3(kTaD), 0, st, a);
-  return check_launch("merge kernel");
+  launch_kernel(shared_prefix_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, s);
+  if (int e = check_launch("shared_prefix_plan_kernel")) return e;
+  launch_kernel(kern, dim3(s.ctas), dim3(kSpThreads), kSpSmem, st, tk, tv, s);
+  if (int e = check_launch("shared_prefix_kernel")) return e;
+  launch_kernel(shared_prefix_merge_kernel<T>, dim3((unsigned)((rh + kMergeWarps - 1) / kMergeWarps)),
+                dim3(kMergeWarps * 32), 0, st, s);
+  return check_launch("shared_prefix_merge_kernel");
 }
 
 }  // namespace
@@ -692,7 +1050,7 @@ extern "C" int64_t dsb_shared_prefix_scratch_floats(int32_t query_rows, int32_t 
     return 0;
   const SpPlan p = plan_for(query_rows, num_query_heads, num_kv_heads, num_groups, block_size,
                             max_prefix_len, max_suffix_len);
-  return p.acc_floats + p.ml_floats + p.own_floats;
+  return p.total;
 }
 
 extern "C" int dsb_shared_prefix_attention_lse(
@@ -725,16 +1083,17 @@ extern "C" int dsb_shared_prefix_attention_lse(
     return fail(DSB_ERR_INVALID, "null pointer argument");
   const SpPlan p = plan_for(query_rows, num_query_heads, num_kv_heads, num_groups, block_size,
                             max_prefix_len, max_suffix_len);
-  if (p.splits > 65535 || num_kv_heads > 65535 || query_rows > 65535 || p.ztiles > 65535 ||
+  if (p.splits > 65535 || num_kv_heads > 65535 || query_rows > 65535 ||
       (int64_t)query_rows * num_query_heads > INT32_MAX)
     return fail(DSB_ERR_UNSUPPORTED, "grid too large");
   if (num_blocks * block_size >= INT32_MAX)
     return fail(DSB_ERR_UNSUPPORTED, "the cache must hold fewer than 2^31 - 1 tokens");
-  if (scratch_floats < p.acc_floats + p.ml_floats + p.own_floats)
+  if (scratch_floats < p.total)
     return fail(DSB_ERR_INVALID, "scratch smaller than dsb_shared_prefix_scratch_floats");
   if (reinterpret_cast<uintptr_t>(query) % 16 || reinterpret_cast<uintptr_t>(key_cache) % 16 ||
-      reinterpret_cast<uintptr_t>(value_cache) % 16 || reinterpret_cast<uintptr_t>(scratch) % 16)
-    return fail(DSB_ERR_UNSUPPORTED, "query, caches and scratch must be 16-byte aligned");
+      reinterpret_cast<uintptr_t>(value_cache) % 16 || reinterpret_cast<uintptr_t>(scratch) % 32)
+    return fail(DSB_ERR_UNSUPPORTED,
+                "query and caches must be 16-byte aligned, scratch 32-byte");
   SpArgs s{};
   TaArgs &a = s.a;
   a.q = query;
@@ -751,25 +1110,15 @@ extern "C" int dsb_shared_prefix_attention_lse(
   a.hq = num_query_heads;
   a.hk = num_kv_heads;
   a.rows = query_rows;
-  a.splits = (int)p.splits;
-  a.tps = p.tps;
-  a.page_tiles = block_size % kTaTile == 0 ? 1 : 0;
   a.scale_log2 = scale * kTaLog2e;
   a.out = out;
   a.lse = lse;
   a.err = error_flag;
-  if (p.shared) {
-    a.prefix_lens = prefix_lens;
-    a.group_starts = group_starts;
-    a.groups = num_groups;
-  }
-  s.acc = scratch;
-  s.ml = reinterpret_cast<float2 *>(scratch + p.acc_floats);
-  a.part = scratch + p.acc_floats + p.ml_floats;
-  s.psplits = p.psplits;
+  s.prefix_lens = prefix_lens;
+  s.group_starts = group_starts;
+  s.groups = num_groups;
   s.token_rows = num_blocks * block_size;
-  s.box = p.box;
   cudaStream_t st = as_stream(stream);
-  return dtype == DSB_BF16 ? run_typed<__nv_bfloat16>(s, p, dtype, st)
-                           : run_typed<__half>(s, p, dtype, st);
+  return dtype == DSB_BF16 ? run_typed<__nv_bfloat16>(s, p, scratch, dtype, st)
+                           : run_typed<__half>(s, p, scratch, dtype, st);
 }

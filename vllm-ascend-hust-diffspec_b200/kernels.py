@@ -597,19 +597,20 @@ def shared_prefix_attention_lse(
     Rows ``[group_starts[i], group_starts[i + 1])`` (int32 ``[groups + 1]``,
     ascending from 0 to the row count; one group of every row when omitted)
     hold the same tokens at positions ``[0, prefix_lens[i])`` (int32
-    ``[groups]``; any length, whole pages or not): requests forked from one
+    ``[groups]``; any length, whole pages or not; groups that do not ascend
+    are flagged and share nothing): requests forked from one
     prompt (:func:`pages.fork_requests`), or verify rows of theirs.  Row ``r``
     sees the first ``seq_lens[r]`` tokens of block-table row ``table_rows[r]``
-    (default ``r``); the prefix is read through the group's first row.  A row
-    may see less than its prefix, or nothing (zeros, and an LSE of -inf); what
-    the prefix holds must be finite.
+    (default ``r``); the prefix is read through the table row of the first row
+    that sees any of it.  A row may see less than its prefix, or nothing
+    (zeros, and an LSE of -inf); what the rows of a group see must be finite.
 
-    ``max_prefix_len`` sizes the split of the prefix (a longer one is still
-    read in whole); ``max_suffix_len`` is the most tokens that any row has
-    behind its prefix: a longer row is flagged and cut there, as by
-    ``max_seq_len`` of :func:`paged_decode_attention_lse`.  Up to 16 query
-    heads per kv head.  Returns ``(out [rows, Hq, 128], lse [rows, Hq]
-    fp32)``."""
+    ``max_prefix_len`` and ``max_suffix_len`` (the most tokens that a row has
+    behind its prefix) size the launches; longer ones are read all the same.
+    Consecutive rows on one table row read their own tokens once for all of
+    them.  Pages of a multiple of 8 tokens share; with other page sizes every
+    row reads its whole sequence.  Up to 16 query heads per kv head.  Returns
+    ``(out [rows, Hq, 128], lse [rows, Hq] fp32)``."""
     if query.ndim != 3 or key_cache.ndim != 4 or key_cache.shape != value_cache.shape:
         raise ValueError("query must be [rows, Hq, D] and the caches matching [blocks, bs, Hk, D]")
     rows, hq, d = query.shape
