@@ -23,11 +23,11 @@
 namespace dsb {
 namespace {
 
-constexpr int kSpTile = 32768;      // 128 tokens x 128 dims, 16-bit: two 64-dim halves
-constexpr int kSpHalf = 16384;
+constexpr int kSpTile = 32768;      // 128 rows x 128 dims, 16-bit
+constexpr int kSpHalf = 16384;      // (queries: 64 dims of all rows, then the other 64)
 constexpr int kSpTok = 128;
 constexpr int kSpSlots = 5;         // K / V tiles in flight
-constexpr int kSpThreads = 320;
+constexpr int kSpThreads = 352;
 constexpr int kSpSmem = 1024 + (2 + kSpSlots) * kSpTile + 256;  // queries, ring, barriers
 constexpr float kSpGrow = 8.f;      // log2 of the growth that rescales O
 // A piece costs about two tiles beside its tiles (its queries, first loads
@@ -344,6 +344,17 @@ __device__ __forceinline__ void sp_wait_ld(uint32_t *r) {
 __device__ __forceinline__ void sp_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
+// A box of a head's tokens: x (64 dims, two halves), 8-token rows from `row8`.
+// It lands as [8 tokens][half][8 rows of 128 bytes] (swizzled atoms of 1 KB):
+// one box a page, with both halves of the head's 256 bytes.
+__device__ __forceinline__ void sp_load(uint32_t dst, const CUtensorMap *map, int row8, int head,
+                                        uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %2, %2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row8), "r"(head), "r"(bar)
+      : "memory");
+}
 // D[tmem] (+)= A[tmem] . B[smem]
 __device__ __forceinline__ void sp_umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
                                            bool accumulate) {
@@ -399,6 +410,23 @@ struct SpPiece {
 struct SpWalk {
   int64_t u, end, units;
   int seg;
+  // By whole warps: the segment that the first unit is in is the last one
+  // that begins at or before it (empty ones begin where the next does).
+  __device__ void begin(const SpArgs &s) {
+    const int lane = threadIdx.x & 31;
+    units = s.head->units;
+    u = sp_first(blockIdx.x, units, s.ctas);
+    end = sp_first(blockIdx.x + 1, units, s.ctas);
+    seg = 0;
+    for (int span = u < end ? s.head->segs : 0; span > 1;) {
+      const int step = (span + 31) / 32, i = seg + lane * step;
+      const bool le = lane * step < span && s.segs[i].unit0 <= u;
+      const int n = __popc(__ballot_sync(0xffffffffu, le));
+      const int skip = max(n - 1, 0) * step;
+      seg += skip;
+      span = min(step, span - skip);
+    }
+  }
   __device__ bool next(const SpArgs &s, SpPiece &p) {
     while (u < end) {
       p.g = s.segs[seg];
@@ -447,10 +475,10 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   const uint32_t s_q = smem_u32(smem), s_kv = s_q + 2 * kSpTile;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + kSpSlots) * kSpTile);
   const uint32_t full = smem_u32(bars), empty = full + 8 * kSpSlots, s_full = empty + 8 * kSpSlots,
-                 p_ready = s_full + 16, o_done = p_ready + 16, q_ready = o_done + 8,
+                 p_ready = s_full + 16, o_done = p_ready + 32, q_ready = o_done + 8,
                  joint = q_ready + 8, drain = joint + 8;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_issued, s_seg;
+  __shared__ int s_abort, s_issued[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.hq / a.hk;
 
@@ -458,17 +486,14 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tk)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tv)) : "memory");
     for (int i = 0; i < 2 * kSpSlots; ++i) mbar_init(full + 8 * i);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + 8 * i);
-      mbar_init_count(p_ready + 8 * i, 128);
-    }
+    for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i);
+    for (int i = 0; i < 4; ++i) mbar_init_count(p_ready + 8 * i, 128);
     mbar_init(o_done);
     mbar_init_count(q_ready, 256);
     mbar_init_count(joint, 256);
     mbar_init(drain);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    s_abort = 0;
-    s_issued = 0;
+    s_abort = s_issued[0] = s_issued[1] = 0;
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
@@ -476,28 +501,11 @@ __global__ void __launch_bounds__(kSpThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_begin();
-  SpWalk walk;
-  walk.units = s.head->units;
-  walk.u = sp_first(blockIdx.x, walk.units, s.ctas);
-  walk.end = sp_first(blockIdx.x + 1, walk.units, s.ctas);
-  if (warp == 8) {  // the segment that the first unit is in
-    const int nseg = s.head->segs;
-    int before = 0;  // segments that begin at or before it
-    for (int base = 0; base < nseg; base += 32) {
-      const int i = base + lane;
-      const unsigned le = __ballot_sync(0xffffffffu, i < nseg && s.segs[i].unit0 <= walk.u);
-      before += __popc(le);
-      if (le != 0xffffffffu) break;
-    }
-    if (lane == 0) s_seg = max(before - 1, 0);
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  // (empty segments begin where the next one does: none is skipped)
-  walk.seg = s_seg;
+  SpWalk walk;
   auto stop = [&]() {
     atomicExch(&s_abort, 1);
     flag_error(a.err, DSB_FLAG_TIMEOUT);
@@ -505,49 +513,52 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   int pieces = 0;
   SpPiece p;
 
-  if (warp == 8) {
-    int i = 0;  // loads so far
+  if (warp == 8 || warp == 10) {  // the keys, and the values
+    pdl_begin();
+    walk.begin(s);
+    const bool is_v = warp == 10;
+    const CUtensorMap *map = is_v ? &tv : &tk;
+    const int boxes = kSpTok / s.box;  // of a tile, at most 16: a lane each
+    int i0 = 0, last = 0;  // loads of the pieces before; this warp's last load + 1
     bool bad = false, ok = true;
     while (ok && walk.next(s, p)) {
       const int32_t *bt = a.bt + (int64_t)p.g.trow * a.bt_stride;
       const bool two = p.g.nq > 128;
-      auto load = [&](int j, bool is_v) {
-        if (!ok) return;
+      // where lane's box of tile j begins, in 8-token rows of the cache
+      auto place = [&](int j) {
+        const int tok = p.g.base + (p.t0 + j) * kSpTok + lane * s.box;
+        if (lane >= boxes || tok >= p.g.tok1) return (int)(s.token_rows / 8);  // out of range: zeros
+        const int64_t page = bt[tok / a.bs];
+        if (page < 0 || page >= a.nblocks) {
+          bad = true;
+          return (int)(s.token_rows / 8);
+        }
+        return (int)((page * a.bs + tok % a.bs) / 8);
+      };
+      int at = place(0);
+      for (int j = 0; j < p.n; ++j) {
+        // loads in the order of use: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 ...
+        const int i = i0 + (is_v ? (two ? 2 * j + 1 : min(2 * j + 2, 2 * p.n - 1))
+                                 : (two ? 2 * j : (j < 2 ? j : 2 * j - 1)));
         const int slot = i % kSpSlots;
         if (i >= kSpSlots) ok = sp_wait(empty + 8 * slot, (uint32_t)(i / kSpSlots - 1) & 1u);
         ok = __all_sync(0xffffffffu, ok && !*reinterpret_cast<volatile int *>(&s_abort));
-        if (!ok) return;
-        const int T0 = p.g.base + (p.t0 + j) * kSpTok;
-        const uint32_t dst = s_kv + slot * kSpTile, bar = full + 8 * slot;
+        if (!ok) break;
+        const uint32_t bar = full + 8 * slot;
         if (lane == 0) mbar_expect_tx(bar, kSpTile);
         __syncwarp();
-        const int boxes = kSpTok / s.box;
-        for (int b = lane; b < 2 * boxes; b += 32) {
-          const int half = b / boxes, first = (b % boxes) * s.box, tok = T0 + first;
-          int y = (int)s.token_rows;  // out of range: zeros
-          if (tok < p.g.tok1) {
-            const int64_t page = bt[tok / a.bs];
-            if (page >= 0 && page < a.nblocks)
-              y = (int)(page * a.bs + tok % a.bs);
-            else
-              bad = true;
-          }
-          tma_load_3d(dst + half * kSpHalf + first * 128, is_v ? &tv : &tk, half * 64, p.h, y, bar);
-        }
-        __syncwarp();
-        ++i;
-      };
-      load(0, false);
-      if (!two && p.n > 1) load(1, false);
-      for (int j = 0; j < p.n; ++j) {
-        load(j, true);
-        if (j + (two ? 1 : 2) < p.n) load(j + (two ? 1 : 2), false);
+        if (lane < boxes) sp_load(s_kv + slot * kSpTile + lane * s.box * 256, map, at, p.h, bar);
+        last = i + 1;
+        if (j + 1 < p.n) at = place(j + 1);
       }
+      i0 += 2 * p.n;
     }
     if (bad) flag_error(a.err, DSB_FLAG_BLOCK);
-    if (!ok && lane == 0) stop();
-    if (lane == 0) s_issued = i;
-  } else if (tid == 9 * 32) {
+    if (lane == 0) {
+      if (!ok) stop();
+      s_issued[is_v] = last;
+    }
+  } else if (warp == 9) {
     const uint32_t qk = umma_idesc<T, 128>(false), pv = qk | (1u << 16);  // V is dim-contiguous
     int i0 = 0, kt[2] = {0, 0};  // loads and tiles of the pieces before
     auto slot_of = [&](int i) { return s_kv + (i % kSpSlots) * kSpTile; };
@@ -561,27 +572,34 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       const uint32_t k = slot_of(i);
 #pragma unroll
       for (int x = 0; x < 8; ++x) {
-        const uint32_t off = (x >> 2) * kSpHalf + (x & 3) * 32;
-        umma(tmem + st * 128, umma_desc(q + off, 16, 1024), umma_desc(k + off, 16, 1024), qk, x > 0);
+        const uint32_t d = (x & 3) * 32;
+        umma(tmem + st * 128, umma_desc(q + (x >> 2) * kSpHalf + d, 16, 1024),
+             umma_desc(k + (x >> 2) * 1024 + d, 16, 2048), qk, x > 0);
       }
       umma_commit(s_full + 8 * st);
     };
-    auto product_o = [&](int st, int i, bool first) {  // O of stream st, from V in load i
+    // O of stream st, from V in load i: the two halves of the tile's tokens as
+    // their weights come
+    auto product_o = [&](int st, int i, bool first) {
       const uint32_t v = slot_of(i), o = tmem + 256 + st * 128;
+      const uint32_t phase = (uint32_t)kt[st]++ & 1u;
 #pragma unroll
-      for (int x = 0; x < 16; ++x) {  // 16 tokens: the hi terms, then the lo ones
-        const int c = x >> 1;
-        const uint32_t pt = tmem + st * 128 + (c >> 1) * 32 + (c & 1) * 8 + (x & 1) * 16;
-        sp_umma_ts(o, pt, umma_desc(v + c * 2048, kSpHalf, 1024), pv, !(first && x == 0));
+      for (int part = 0; part < 2; ++part) {
+        if (!sp_wait(p_ready + 16 * st + 8 * part, phase)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {  // 16 tokens, the hi terms, then the lo ones
+          const int c = part * 4 + (x >> 1);
+          const uint32_t pt = tmem + st * 128 + (c >> 1) * 32 + (c & 1) * 8 + (x & 1) * 16;
+          sp_umma_ts(o, pt, umma_desc(v + c * 4096, 1024, 2048), pv, !(first && part + x == 0));
+        }
       }
+      return true;
     };
-    auto weighted = [&](int st) {  // P of stream st's next tile is in place
-      const bool got = sp_wait(p_ready + 8 * st, (uint32_t)kt[st]++ & 1u);
-      tc_fence_after();
-      return got;
-    };
+    pdl_begin();
+    walk.begin(s);
     bool ok = true;
-    while (ok && walk.next(s, p)) {
+    while (lane == 0 && ok && walk.next(s, p)) {  // one thread issues them
       const int n = p.n;
       const bool two = p.g.nq > 128;
       // one query tile alternates between the two places
@@ -598,9 +616,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           const int v = i0 + 2 * j + 1, k = v + 1;
           ok = filled(v);
           for (int st = 0; st < 2 && ok; ++st) {
-            ok = weighted(st);
+            ok = product_o(st, v, j == 0);
             if (!ok) break;
-            product_o(st, v, j == 0);
             if (st == 1) freed(v);
             if (j + 1 < n) {
               if (st == 0) ok = filled(k);
@@ -619,9 +636,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         }
         for (int j = 0; j < n && ok; ++j) {
           const int v = i0 + min(2 * j + 2, 2 * n - 1);
-          ok = filled(v) && weighted(j & 1);
+          ok = filled(v) && product_o(j & 1, v, j < 2);
           if (!ok) break;
-          product_o(j & 1, v, j < 2);
           freed(v);
           if (j + 2 < n) {
             const int k = i0 + 2 * j + 3;
@@ -651,68 +667,90 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       mbar_arrive(joint);
       ok = __all_sync(0xffffffffu, sp_wait(joint, (uint32_t)joints++ & 1u));
     };
-    while (ok && walk.next(s, p)) {
-      const int n = p.n, nq = p.g.nq;
-      const bool two = nq > 128;
-      // the queries, swizzled as the operand wants them (places behind nq hold
-      // anything: a query row meets only its own sums)
-      uint8_t *qdst = smem + (two ? 0 : (pieces & 1) * kSpTile);
-      for (int b = 0; b < (two ? 2 : 1); ++b) {
-        uint4 v[8];
+    // A piece's queries, swizzled as the operand wants them (places behind nq
+    // hold anything: a query row meets only its own sums).  One query tile
+    // alternates between the two places.
+    auto fetch = [&](const SpPiece &x, int place) {
+      for (int b = 0; b < (x.g.nq > 128 ? 2 : 1); ++b) {
+        const uint32_t dst = s_q + (x.g.nq > 128 ? b : place & 1) * kSpTile;
+        const int c = tid & 15;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int q = b * 128 + x * 16 + (tid >> 4);
-          const int mm = p.g.q0 + min(q, nq - 1);
-          v[x] = *reinterpret_cast<const uint4 *>(
-              static_cast<const T *>(a.q) +
-              ((int64_t)(p.g.row0 + mm / G) * a.hq + p.h * G + mm % G) * kTaD + (tid & 15) * 8);
-        }
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int r = x * 16 + (tid >> 4), c = tid & 15;
-          *reinterpret_cast<uint4 *>(qdst + b * kSpTile + (c >> 3) * kSpHalf + r * 128 +
-                                     (((c & 7) ^ (r & 7)) * 16)) = v[x];
+        for (int y = 0; y < 8; ++y) {
+          const int r = y * 16 + (tid >> 4);
+          const int mm = x.g.q0 + min(b * 128 + r, x.g.nq - 1);
+          const T *src = static_cast<const T *>(a.q) +
+                         ((int64_t)(x.g.row0 + mm / G) * a.hq + x.h * G + mm % G) * kTaD + c * 8;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                           dst + (c >> 3) * kSpHalf + r * 128 + (((c & 7) ^ (r & 7)) * 16)),
+                       "l"(src)
+                       : "memory");
         }
       }
+      cp_async_commit();
+    };
+    auto fetched = [&]() {
+      cp_async_wait<0>();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(q_ready);
-
-      // this thread's query row, and the tokens [tok0, lim) that it sees
-      const int m = (two ? stream * 128 : 0) + m128;
+    };
+    // The first turn of the loop is a rehearsal on whatever the tensor memory
+    // holds: it brings the instructions in (~7000 clocks of misses) while the
+    // plan is still being made.
+    bool rehearsal = true, has_next = false, early = false;
+    SpPiece after;
+    p.n = 1;
+    p.g.tok0 = p.g.base = p.t0 = 0;
+    p.g.nq = 128;
+    p.g.tok1 = kSpTok;
+    while (ok) {
+      const int n = p.n, nq = p.g.nq;
+      const bool two = nq > 128;
+      const int m = (two ? stream * 128 : 0) + m128;  // this thread's query row
       const bool mine = m < nq;
-      int lim = 0;
-      if (mine) {
-        int64_t t;
-        lim = min(sp_visible(a, p.g.row0 + (p.g.q0 + m) / G, t, false), p.g.tok1);
+      int lim = kSpTok;  // the tokens [tok0, lim) are what it sees
+      if (!rehearsal) {
+        if (!early) {
+          fetch(p, pieces);
+          fetched();
+        }
+        has_next = walk.next(s, after);
+        early = has_next && !two && after.g.nq <= 128;
+        if (early) fetch(after, pieces + 1);
+        lim = 0;
+        if (mine) {
+          int64_t t;
+          lim = min(sp_visible(a, p.g.row0 + (p.g.q0 + m) / G, t, false), p.g.tok1);
+        }
       }
       const bool works = __any_sync(0xffffffffu, mine);
-      const int count = two ? n : (n - stream + 1) / 2;
+      const int count = rehearsal ? 1 : two ? n : (n - stream + 1) / 2;
       float m_ref = -INFINITY, l = 0.f;
       for (int k = 0; k < count; ++k) {
         const int j = two ? k : 2 * k + stream;
         const int T0 = p.g.base + (p.t0 + j) * kSpTok;
-        ok = __all_sync(0xffffffffu, sp_wait(s_full + 8 * stream, (uint32_t)(kt + k) & 1u));
-        if (!ok) break;
-        tc_fence_after();
-        // What a page holds behind the segment's end has weights of zero, but
-        // zero times what lies there may not be: those values become zeros.
-        if (T0 + kSpTok > p.g.tok1 && (!two || stream == 0)) {
-          const int i = i0 + (two ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1));
-          ok = __all_sync(0xffffffffu, sp_wait(full + 8 * (i % kSpSlots),
-                                               (uint32_t)(i / kSpSlots) & 1u));
+        if (!rehearsal) {
+          ok = __all_sync(0xffffffffu, sp_wait(s_full + 8 * stream, (uint32_t)(kt + k) & 1u));
           if (!ok) break;
-          const uint32_t v = s_kv + (i % kSpSlots) * kSpTile;
-          for (int z = (p.g.tok1 - T0) * 8 + m128; z < kSpTok * 8; z += 128) {
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + z * 16), "r"(0u)
-                         : "memory");
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + kSpHalf + z * 16),
-                         "r"(0u)
-                         : "memory");
+          tc_fence_after();
+          // What a page holds behind the segment's end has weights of zero, but
+          // zero times what lies there may not be: those values become zeros.
+          if (T0 + kSpTok > p.g.tok1 && (!two || stream == 0)) {
+            const int i = i0 + (two ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1));
+            ok = __all_sync(0xffffffffu, sp_wait(full + 8 * (i % kSpSlots),
+                                                 (uint32_t)(i / kSpSlots) & 1u));
+            if (!ok) break;
+            const uint32_t v = s_kv + (i % kSpSlots) * kSpTile;
+            for (int z = (p.g.tok1 - T0) * 8 + m128; z < kSpTok * 8; z += 128) {
+              const uint32_t at = v + (z >> 6) * 2048 + (z & 63) * 16;
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at + 1024), "r"(0u)
+                           : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         if (works) {
-          const int from = p.g.tok0 - T0, till = lim - T0;  // columns seen
+          const int from = p.g.tok0 - T0, till = (rehearsal ? kSpTok : lim - T0);  // columns seen
           const bool whole = __all_sync(0xffffffffu, from <= 0 && till >= kSpTok);
           auto hide = [&](uint32_t(&x)[32], int c) {
 #pragma unroll
@@ -789,17 +827,32 @@ __global__ void __launch_bounds__(kSpThreads, 1)
             sp_wait_ld(x1);
             if (c == 0) sp_ld32(ts + 64, x0);
             weights(x1, c + 32);
+            if (c == 0 && !rehearsal) {  // half of the tile's weights are there
+              sp_wait_st();
+              tc_fence_before();
+              mbar_arrive(p_ready + 16 * stream);
+            }
           }
           const float2 t = sp_unpair(sp_add2(sum0, sum1));
           l += t.x + t.y;
           sp_wait_st();
+        } else if (!rehearsal) {
+          mbar_arrive(p_ready + 16 * stream);
         }
         tc_fence_before();
-        mbar_arrive(p_ready + 8 * stream);
+        if (!rehearsal) mbar_arrive(p_ready + 16 * stream + 8);
       }
       if (!ok) break;
+      if (rehearsal) {
+        rehearsal = false;
+        pdl_begin();
+        walk.begin(s);
+        if (!walk.next(s, p)) break;
+        continue;
+      }
       kt += count;
       i0 += 2 * n;
+      if (early) fetched();  // the next piece's first products run beside the sums
 
       // the piece's sums (its products are done): [nq][D], and (maximum, sum)
       ok = __all_sync(0xffffffffu, sp_wait(o_done, (uint32_t)pieces & 1u));
@@ -826,7 +879,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       } else {
         // both streams' sums of a row lie in the same lane: each stream joins
         // half of the columns (maxima and sums pass where the queries were)
-        float2 *ml = reinterpret_cast<float2 *>(qdst);
+        float2 *ml = reinterpret_cast<float2 *>(smem + (pieces & 1) * kSpTile);
         ml[stream * 128 + m128] = make_float2(m_ref, l);
         both();
         if (!ok) break;
@@ -862,7 +915,10 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         both();
       }
       ++pieces;
+      if (!has_next) break;
+      p = after;
     }
+    cp_async_wait<0>();
     if (!ok && lane == 0) stop();
   }
   tc_fence_before();
@@ -870,10 +926,9 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   if (s_abort) {
     // A wait ran out: let the copies land and the products end before the
     // shared and tensor memory go.
-    if (tid == 0) {
-      for (int i = max(0, s_issued - kSpSlots); i < s_issued; ++i)
+    if (tid < 2)  // (of the keys, and of the values: no more than the ring holds)
+      for (int i = max(0, s_issued[tid] - kSpSlots); i < s_issued[tid]; ++i)
         mbar_wait(full + 8 * (i % kSpSlots), (uint32_t)(i / kSpSlots) & 1u);
-    }
     if (tid == 9 * 32) {
       umma_commit(drain);
       mbar_wait(drain, 0);
@@ -887,15 +942,17 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 // ------------------------------------------------------------------ merge
 constexpr int kMergeWarps = 4;
 
-// A warp a (row, query head), a lane four of its dims: the pieces of the
-// prefix, then of the row's own tokens, in order.
+// A CTA a (row, query head), a lane four of its dims: warp w takes pieces w,
+// w + 4, ... of the prefix, then of the row's own tokens, and the warps' sums
+// are joined in order.
 template <typename T>
 __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(const SpArgs s) {
+  __shared__ float4 s_acc[kMergeWarps][32];
+  __shared__ float2 s_ml[kMergeWarps];
   pdl_begin();
   const TaArgs &a = s.a;
-  const int64_t rh = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
-  if (rh >= (int64_t)a.rows * a.hq) return;
-  const int lane = threadIdx.x & 31, G = a.hq / a.hk;
+  const int64_t rh = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.hq / a.hk;
   const int row = (int)(rh / a.hq), head = (int)(rh % a.hq), h = head / G;
   const int64_t units = s.head->units;
   const SpRow at = s.rows[row];
@@ -912,8 +969,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(c
     const int64_t A = g.unit0 + (int64_t)h * g.len;
     const int b0 = sp_owner(A, units, s.ctas), b1 = sp_owner(A + g.len - 1, units, s.ctas);
     const int64_t first = g.acc + (int64_t)h * g.maxp * g.nq + q;
-    for (int base = b0; base <= b1; base += 32) {
-      const int b = base + lane;
+    for (int base = b0 + warp; base <= b1; base += 32 * kMergeWarps) {
+      const int b = base + lane * kMergeWarps;
       float2 x = make_float2(-INFINITY, 0.f);
       if (b <= b1) {  // (a piece without tiles wrote nothing)
         const int from = (int)max(sp_first(b, units, s.ctas) - A, (int64_t)0);
@@ -931,14 +988,15 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(c
       acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
       const float w = x.x == -INFINITY ? 0.f : exp2f(x.x - now);
       sum = fmaf(sum, f, warp_sum(w * x.y));
-      const int n = min(32, b1 - base + 1);
+      const int n = min(32, (b1 - base) / kMergeWarps + 1);
       const unsigned live = __ballot_sync(0xffffffffu, x.x != -INFINITY);
-#pragma unroll 4
+      const float *src = s.acc + (first + (int64_t)(base - b0) * g.nq) * kTaD + 4 * lane;
+#pragma unroll 8
       for (int i = 0; i < n; ++i) {
         const float wi = __shfl_sync(0xffffffffu, w, i);
-        if (!(live >> i & 1)) continue;
-        const float4 v = *reinterpret_cast<const float4 *>(
-            s.acc + (first + (int64_t)(base + i - b0) * g.nq) * kTaD + 4 * lane);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (live >> i & 1)
+          v = *reinterpret_cast<const float4 *>(src + (int64_t)i * kMergeWarps * g.nq * kTaD);
         acc.x = fmaf(v.x, wi, acc.x);
         acc.y = fmaf(v.y, wi, acc.y);
         acc.z = fmaf(v.z, wi, acc.z);
@@ -946,18 +1004,54 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(c
       }
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  s_acc[warp][lane] = acc;
+  if (lane == 0) s_ml[warp] = make_float2(M, sum);
+  __syncthreads();
+  if (warp != 0) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, s_ml[w].x);
+  sum = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) {
+    if (s_ml[w].x == -INFINITY) continue;
+    const float f = exp2f(s_ml[w].x - top);
+    const float4 v = s_acc[w][lane];
+    sum = fmaf(s_ml[w].y, f, sum);
+    acc.x = fmaf(v.x, f, acc.x);
+    acc.y = fmaf(v.y, f, acc.y);
+    acc.z = fmaf(v.z, f, acc.z);
+    acc.w = fmaf(v.w, f, acc.w);
+  }
+  // nothing seen: zeros and -inf (a sum that is NaN says so)
+  const bool none = top == -INFINITY;
+  const float inv = none ? 0.f : 1.f / sum;
   uint2 out;
   out.x = pack2<T>(acc.x * inv, acc.y * inv);
   out.y = pack2<T>(acc.z * inv, acc.w * inv);
-  if (!(sum > 0.f) && !(sum != sum)) out = make_uint2(0, 0);
-  if (sum != sum) out.x = out.y = pack2<T>(sum, sum);
   *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + rh * kTaD + 4 * lane) = out;
-  if (lane == 0)
-    a.lse[rh] = sum != sum ? sum : (sum > 0.f ? (M + log2f(sum)) * kTaLn2 : -INFINITY);
+  if (lane == 0) a.lse[rh] = none ? -INFINITY : (top + log2f(sum)) * kTaLn2;
 }
 
 // ------------------------------------------------------------------- host
+// The paged cache as (64 dims, 8 tokens, 2 halves, rows of 8 tokens, heads);
+// a box holds `box` tokens of one head.
+bool sp_encode_map(CUtensorMap *map, const void *base, int64_t token_rows, int heads, int dtype,
+                   int box) {
+  auto fn = tensor_map_encoder();
+  if (fn == nullptr) return false;
+  const cuuint64_t token = (cuuint64_t)heads * kTaD * 2;
+  cuuint64_t dims[5] = {64, 8, 2, (cuuint64_t)token_rows / 8, (cuuint64_t)heads};
+  cuuint64_t strides[4] = {token, 128, 8 * token, kTaD * 2};
+  cuuint32_t boxes[5] = {64, 8, 2, (cuuint32_t)box / 8, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn(map, dtype == DSB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+            5, const_cast<void *>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct SpPlan {
   int box;             // 0: pages that no TMA box fits (every row for itself)
   int64_t splits;      // of a row, without boxes
@@ -1024,15 +1118,14 @@ template <typename T> int run_typed(SpArgs &s, const SpPlan &p, float *scratch, 
   auto kern = shared_prefix_kernel<T>;
   if (int e = ensure_smem((const void *)kern, kSpSmem); e != DSB_OK) return e;
   CUtensorMap tk, tv;
-  if (!encode_paged_map(&tk, a.k, s.token_rows, a.hk, kTaD, dtype, p.box) ||
-      !encode_paged_map(&tv, a.v, s.token_rows, a.hk, kTaD, dtype, p.box))
+  if (!sp_encode_map(&tk, a.k, s.token_rows, a.hk, dtype, p.box) ||
+      !sp_encode_map(&tv, a.v, s.token_rows, a.hk, dtype, p.box))
     return fail(DSB_ERR_CUDA, "tensor map of the paged cache");
   launch_kernel(shared_prefix_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, s);
   if (int e = check_launch("shared_prefix_plan_kernel")) return e;
   launch_kernel(kern, dim3(s.ctas), dim3(kSpThreads), kSpSmem, st, tk, tv, s);
   if (int e = check_launch("shared_prefix_kernel")) return e;
-  launch_kernel(shared_prefix_merge_kernel<T>, dim3((unsigned)((rh + kMergeWarps - 1) / kMergeWarps)),
-                dim3(kMergeWarps * 32), 0, st, s);
+  launch_kernel(shared_prefix_merge_kernel<T>, dim3((unsigned)rh), dim3(kMergeWarps * 32), 0, st, s);
   return check_launch("shared_prefix_merge_kernel");
 }
 
