@@ -27,7 +27,7 @@ constexpr int kSpTile = 32768;      // 128 rows x 128 dims, 16-bit
 constexpr int kSpHalf = 16384;      // (queries: 64 dims of all rows, then the other 64)
 constexpr int kSpTok = 128;
 constexpr int kSpSlots = 5;         // K / V tiles in flight
-constexpr int kSpThreads = 352;
+constexpr int kSpThreads = 384;
 constexpr int kSpSmem = 1024 + (2 + kSpSlots) * kSpTile + 256;  // queries, ring, barriers
 constexpr float kSpGrow = 8.f;      // log2 of the growth that rescales O
 // A piece costs about two tiles beside its tiles (its queries, first loads
@@ -46,9 +46,10 @@ struct alignas(16) SpSeg {
 };
 static_assert(sizeof(SpSeg) == 64, "one segment per 64 bytes");
 
-struct SpPlanHead {
+// Where a CTA begins: all the units, and the segment its first one is in.
+struct alignas(16) SpBegin {
   int64_t units;
-  int32_t segs, pad;
+  int32_t seg, pad;
 };
 
 // Where a row's partial sums are: its group's first prefix segment and row,
@@ -63,7 +64,7 @@ struct SpArgs {
   int groups, ctas;
   int box;             // tokens of a TMA box: 8 .. 128, dividing the page
   int64_t token_rows;  // num_blocks * block_size
-  SpPlanHead *head;
+  SpBegin *begin;      // [ctas]
   SpSeg *segs;
   SpRow *rows;
   int32_t *gseg;       // [groups] first prefix segment of each
@@ -71,12 +72,20 @@ struct SpArgs {
   float2 *ml;          // [rows of partial sums]: maximum (log2), sum
 };
 
+// floor(x / y) of whole numbers below 2^52 without a 64-bit division: the
+// rounded quotient, put right by at most one.
+__device__ __forceinline__ int64_t sp_div(int64_t x, int64_t y) {
+  int64_t q = (int64_t)((double)x / (double)y);
+  if (q * y > x) --q;
+  if ((q + 1) * y <= x) ++q;
+  return q;
+}
 // The CTA that owns unit u of `units`, and a CTA's first unit.
 __device__ __forceinline__ int sp_owner(int64_t u, int64_t units, int ctas) {
-  return (int)(((u + 1) * ctas - 1) / units);
+  return (int)sp_div((u + 1) * ctas - 1, units);
 }
 __device__ __forceinline__ int64_t sp_first(int64_t cta, int64_t units, int ctas) {
-  return cta * units / ctas;
+  return sp_div(cta * units, ctas);
 }
 
 // Tokens that row r may see, 0 for a row without a valid table row.
@@ -97,10 +106,15 @@ __device__ __forceinline__ int sp_visible(const TaArgs &a, int r, int64_t &trow,
 }
 
 // ------------------------------------------------------------------- plan
-constexpr int kPlanThreads = 1024;
+// One CTA of 256 threads: the plan's time is the latency of its dependent
+// reads and of its barriers (1024 threads: 1200 clocks a scan; 9 us in all
+// for 16 rows).  What it reads again is kept in shared memory: the first
+// kPlanKeep groups and segments, and the rows of a turn of the loop.
+constexpr int kPlanThreads = 256, kPlanKeep = 1024;
 
 // Inclusive scan over the block (sum, or maximum); the last value in `total`.
 template <typename V, bool MAX> __device__ V plan_scan(V v, V *warp_v, V &total) {
+  constexpr int kWarps = kPlanThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto join = [](V x, V y) { return MAX ? (x > y ? x : y) : x + y; };
 #pragma unroll
@@ -108,147 +122,113 @@ template <typename V, bool MAX> __device__ V plan_scan(V v, V *warp_v, V &total)
     const V x = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v = join(x, v);
   }
-  __syncthreads();
   if (lane == 31) warp_v[warp] = v;
   __syncthreads();
-  if (warp == 0) {
-    V w = warp_v[lane];
+  V before = v;
+  total = warp_v[0];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const V x = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w = join(x, w);
-    }
-    warp_v[lane] = w;
+  for (int w = 1; w < kWarps; ++w) {
+    if (w == warp) before = join(total, v);
+    total = join(total, warp_v[w]);
   }
-  __syncthreads();
-  total = warp_v[31];
-  return warp > 0 ? join(warp_v[warp - 1], v) : v;
-}
-
-__device__ __forceinline__ void sp_group(const SpArgs &s, int i, int &lo, int &hi) {
-  lo = s.group_starts != nullptr ? s.group_starts[i] : 0;
-  hi = s.group_starts != nullptr ? s.group_starts[i + 1] : s.a.rows;
+  __syncthreads();  // (warp_v is written again by the next scan)
+  return warp > 0 ? before : v;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const SpArgs s) {
-  __shared__ int32_t warp_i[32];
-  __shared__ int64_t warp_l[32];
+  __shared__ int32_t warp_i[kPlanThreads / 32];
+  __shared__ int64_t warp_l[kPlanThreads / 32];
+  __shared__ int32_t s_start[kPlanKeep + 1], s_prefix[kPlanKeep], s_gseg[kPlanKeep];
+  __shared__ int32_t s_trow[kPlanThreads + 128], s_seen[kPlanThreads + 128];
+  __shared__ int32_t s_len[kPlanKeep], s_nq[kPlanKeep];
+  __shared__ int64_t s_unit0[kPlanKeep];
   const TaArgs &a = s.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = a.hq / a.hk, run_rows = 128 / G;
+  const int64_t cap = a.bt_cols * a.bs;  // tokens a table row can address
   pdl_begin();
 
-  // prefix segments: each group's query rows, 256 at a time
-  int nprefix = 0;
-  bool bad = false;  // groups that do not ascend within the rows: nothing is shared
-  if (s.group_starts != nullptr)
-    for (int i = tid; i < s.groups; i += kPlanThreads)
-      bad |= s.group_starts[i] < 0 || s.group_starts[i + 1] < s.group_starts[i] ||
-             s.group_starts[i + 1] > a.rows;
+  // The rows of a turn: what each sees, and its table row (-1: none).  A run
+  // may reach into the rows of the next turn.
+  auto read_rows = [&](int base) {
+    for (int i = tid; i < kPlanThreads + run_rows && base + i < a.rows; i += kPlanThreads) {
+      int64_t t;
+      s_seen[i] = sp_visible(a, base + i, t, i < kPlanThreads);
+      t = a.trows != nullptr ? a.trows[base + i] : base + i;
+      s_trow[i] = t >= 0 && t < a.bt_rows ? (int)t : -1;
+    }
+  };
+  read_rows(0);
+  // the groups; if they do not ascend within the rows, nothing is shared
+  bool bad = false;
+  for (int i = tid; i <= s.groups; i += kPlanThreads) {
+    const int at = s.group_starts != nullptr ? s.group_starts[i] : (i == 0 ? 0 : a.rows);
+    if (i <= kPlanKeep) s_start[i] = at;
+    if (i < s.groups && i < kPlanKeep) s_prefix[i] = s.prefix_lens[i];
+    bad |= at < 0 || at > a.rows ||
+           (i > 0 && s.group_starts != nullptr && s.group_starts[i - 1] > at);
+  }
+  for (int r = tid; r < a.rows; r += kPlanThreads) s.rows[r] = SpRow{0, -1, -1, 0};
   bad = __syncthreads_or(bad);
   if (bad && tid == 0) flag_error(a.err, DSB_FLAG_SLOT);
   const int groups = bad ? 0 : s.groups;
+  auto start_of = [&](int i) { return i <= kPlanKeep ? s_start[i] : s.group_starts[i]; };
+  auto prefix_of = [&](int i) {
+    const int p = i < kPlanKeep ? s_prefix[i] : s.prefix_lens[i];
+    return (int)min((int64_t)max(p, 0), cap);
+  };
+  auto gseg_of = [&](int i) { return i < kPlanKeep ? s_gseg[i] : s.gseg[i]; };
+  auto keep = [&](int i, const SpSeg &g) {
+    s.segs[i] = g;
+    if (i < kPlanKeep) s_len[i] = g.len, s_nq[i] = g.nq;
+  };
+
+  // prefix segments: each group's query rows, 256 at a time
+  int nprefix = 0;
   for (int base = 0; base < groups; base += kPlanThreads) {
     const int i = base + tid;
-    int tiles = 0, total;
-    if (i < groups) {
-      int lo, hi;
-      sp_group(s, i, lo, hi);
-      tiles = (int)(((int64_t)(hi - lo) * G + 255) / 256);
+    int tiles = 0, total, cum;
+    if (i < groups) tiles = (int)(((int64_t)(start_of(i + 1) - start_of(i)) * G + 255) / 256);
+    if (groups == 1) {
+      cum = tiles;
+      total = (int)(((int64_t)(start_of(1) - start_of(0)) * G + 255) / 256);
+    } else {
+      cum = plan_scan<int32_t, false>(tiles, warp_i, total);
     }
-    const int cum = plan_scan<int32_t, false>(tiles, warp_i, total);
-    if (i < groups) s.gseg[i] = nprefix + cum - tiles;
+    if (i < groups) {
+      s.gseg[i] = nprefix + cum - tiles;
+      if (i < kPlanKeep) s_gseg[i] = nprefix + cum - tiles;
+    }
     nprefix += total;
   }
-  // every row's group
-  for (int r = tid; r < a.rows; r += kPlanThreads) s.rows[r] = SpRow{0, -1, -1, 0};
   __syncthreads();
-
-  // segments of the rows' own tokens: rows of a group on one table row
-  int nown = 0, carry = -1;
-  for (int base = 0; base < a.rows; base += kPlanThreads) {
-    const int r = base + tid;
-    int gi = -1, lo = 0, hi = a.rows, prefix = 0;
-    int64_t trow = -1;
-    bool starts = false;
-    if (r < a.rows) {
-      if (s.group_starts == nullptr) {
-        gi = 0;
-      } else if (groups > 0) {  // the last group that begins at or before the row
-        int x = 0, y = groups;
-        while (x < y) {
-          const int mid = (x + y) / 2;
-          if (s.group_starts[mid] <= r) x = mid + 1;
-          else y = mid;
-        }
-        gi = x - 1;
-        if (gi >= 0) sp_group(s, gi, lo, hi);
-        if (gi < 0 || r >= hi) {  // outside every group: no shared prefix
-          lo = gi < 0 ? 0 : hi;
-          hi = gi < 0 ? s.group_starts[0] : a.rows;
-          gi = -1;
-        }
-      }
-      if (gi >= 0) {
-        prefix = (int)min((int64_t)max(s.prefix_lens[gi], 0), a.bt_cols * a.bs);
-        s.rows[r].row0 = lo;
-        s.rows[r].pseg = s.gseg[gi];
-      }
-      sp_visible(a, r, trow, true);
-      const int64_t before = r > lo ? (a.trows != nullptr ? a.trows[r - 1] : r - 1) : -1;
-      starts = r == lo || before != trow;
-    }
-    int total;
-    const int first = max(carry, plan_scan<int32_t, true>(starts ? r : -1, warp_i, total));
-    carry = max(carry, total);
-    // a run is taken run_rows rows at a time, by the first of them
-    const bool leads = r < a.rows && trow >= 0 && trow < a.bt_rows && (r - first) % run_rows == 0;
-    int nrows = 0, most = 0;
-    if (leads)
-      for (; nrows < run_rows && r + nrows < hi; ++nrows) {
-        const int64_t t = a.trows != nullptr ? a.trows[r + nrows] : r + nrows;
-        if (t != trow) break;
-        most = max(most, (int)min((int64_t)a.seq[r + nrows], a.bt_cols * a.bs));
-      }
-    const bool has = leads && most > prefix;
-    const int at = nprefix + nown + plan_scan<int32_t, false>(has ? 1 : 0, warp_i, total) - 1;
-    nown += total;
-    if (has) {
-      SpSeg g{};
-      g.row0 = r, g.q0 = 0, g.nq = nrows * G, g.trow = (int)trow;
-      g.tok0 = prefix, g.tok1 = most;
-      g.base = prefix / s.box * s.box;
-      g.len = (most - g.base + kSpTok - 1) / kSpTok + kSpStart;
-      s.segs[at] = g;
-      for (int j = 0; j < nrows; ++j) {
-        s.rows[r + j].sseg = at;
-        s.rows[r + j].srow = j;
-      }
-    }
-  }
 
   // the prefix segments, a warp each: as far as any of their rows sees
   for (int p = warp; p < nprefix; p += kPlanThreads / 32) {
     int x = 0, y = groups;
     while (x < y) {
       const int mid = (x + y) / 2;
-      if (s.gseg[mid] <= p) x = mid + 1;
+      if (gseg_of(mid) <= p) x = mid + 1;
       else y = mid;
     }
     // (groups without rows share their segment's number with the next one)
-    const int gi = x - 1;
-    int lo, hi;
-    sp_group(s, gi, lo, hi);
-    const int prefix = (int)min((int64_t)max(s.prefix_lens[gi], 0), a.bt_cols * a.bs);
+    const int gi = x - 1, lo = start_of(gi), prefix = prefix_of(gi);
     SpSeg g{};
-    g.row0 = lo, g.q0 = (p - s.gseg[gi]) * 256;
-    g.nq = (int)min((int64_t)256, (int64_t)(hi - lo) * G - g.q0);
+    g.row0 = lo, g.q0 = (p - gseg_of(gi)) * 256;
+    g.nq = (int)min((int64_t)256, (int64_t)(start_of(gi + 1) - lo) * G - g.q0);
     const int r0 = lo + g.q0 / G, r1 = lo + (g.q0 + g.nq - 1) / G;
     int most = 0, trow = -1;
     for (int r = r0 + lane; r - lane <= r1; r += 32) {
       int64_t t = -1;
       int L = 0;
-      if (r <= r1) L = min(sp_visible(a, r, t, false), prefix);
+      if (r <= r1) {
+        if (r < kPlanThreads) {
+          L = s_seen[r], t = s_trow[r];
+        } else {
+          L = sp_visible(a, r, t, false);
+        }
+        L = min(L, prefix);
+      }
       most = max(most, L);
       const unsigned sees = __ballot_sync(0xffffffffu, L > 0);
       const int tr = __shfl_sync(0xffffffffu, (int)t, sees ? __ffs(sees) - 1 : 0);
@@ -258,37 +238,123 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
     g.trow = max(trow, 0);
     g.tok1 = most;
     g.len = most > 0 ? (most + kSpTok - 1) / kSpTok + kSpStart : 0;
-    if (lane == 0) s.segs[p] = g;
+    if (lane == 0) keep(p, g);
+  }
+
+  // segments of the rows' own tokens: rows of a group on one table row
+  int nown = 0, carry = -1;
+  for (int base = 0; base < a.rows; base += kPlanThreads) {
+    if (base > 0) {
+      __syncthreads();
+      read_rows(base);
+      __syncthreads();
+    }
+    const int r = base + tid;
+    int gi = -1, lo = 0, hi = a.rows, prefix = 0, trow = -1;
+    bool starts = false;
+    if (r < a.rows) {
+      if (groups > 0) {  // the last group that begins at or before the row
+        int x = 0, y = groups;
+        while (x < y) {
+          const int mid = (x + y) / 2;
+          if (start_of(mid) <= r) x = mid + 1;
+          else y = mid;
+        }
+        gi = x - 1;
+        if (gi >= 0) lo = start_of(gi), hi = start_of(gi + 1);
+        if (gi < 0 || r >= hi) {  // outside every group: no shared prefix
+          lo = gi < 0 ? 0 : hi;
+          hi = gi < 0 ? start_of(0) : a.rows;
+          gi = -1;
+        }
+      }
+      if (gi >= 0) {
+        prefix = prefix_of(gi);
+        s.rows[r].row0 = lo;
+        s.rows[r].pseg = gseg_of(gi);
+      }
+      trow = s_trow[tid];
+      int before = -1;
+      if (r > lo) {
+        if (tid > 0) {
+          before = s_trow[tid - 1];
+        } else {
+          const int64_t t = a.trows != nullptr ? a.trows[r - 1] : r - 1;
+          before = t >= 0 && t < a.bt_rows ? (int)t : -1;
+        }
+      }
+      starts = r == lo || before != trow;
+    }
+    int total;
+    const int first = max(carry, plan_scan<int32_t, true>(starts ? r : -1, warp_i, total));
+    carry = max(carry, total);
+    // a run is taken run_rows rows at a time, by the first of them
+    const bool leads = trow >= 0 && (r - first) % run_rows == 0;
+    int nrows = 0, most = 0;
+    if (leads)
+      for (; nrows < run_rows && r + nrows < hi && s_trow[tid + nrows] == trow; ++nrows)
+        most = max(most, s_seen[tid + nrows]);
+    const bool has = leads && most > prefix;
+    const int at = nprefix + nown + plan_scan<int32_t, false>(has ? 1 : 0, warp_i, total) - 1;
+    nown += total;
+    if (has) {
+      SpSeg g{};
+      g.row0 = r, g.q0 = 0, g.nq = nrows * G, g.trow = trow;
+      g.tok0 = prefix, g.tok1 = most;
+      g.base = prefix / s.box * s.box;
+      g.len = (most - g.base + kSpTok - 1) / kSpTok + kSpStart;
+      keep(at, g);
+      for (int j = 0; j < nrows; ++j) {
+        s.rows[r + j].sseg = at;
+        s.rows[r + j].srow = j;
+      }
+    }
   }
   __syncthreads();
 
   // units before each segment, then the places of their partial sums
   const int nseg = nprefix + nown;
-  int64_t units = 0, total;
+  auto len_of = [&](int i) { return i < kPlanKeep ? s_len[i] : s.segs[i].len; };
+  auto nq_of = [&](int i) { return i < kPlanKeep ? s_nq[i] : s.segs[i].nq; };
+  int64_t units = 0, total = 0;
   for (int base = 0; base < nseg; base += kPlanThreads) {
     const int i = base + tid;
-    const int64_t mine = i < nseg ? (int64_t)s.segs[i].len * a.hk : 0;
-    const int64_t cum = plan_scan<int64_t, false>(mine, warp_l, total);
-    if (i < nseg) s.segs[i].unit0 = units + cum - mine;
+    const int64_t mine = i < nseg ? (int64_t)len_of(i) * a.hk : 0;
+    const int64_t u0 = units + plan_scan<int64_t, false>(mine, warp_l, total) - mine;
     units += total;
+    if (i < nseg) {
+      s.segs[i].unit0 = u0;
+      if (i < kPlanKeep) s_unit0[i] = u0;
+    }
   }
+  const float share = units > 0 ? (float)s.ctas / (float)units : 0.f;
   int64_t sums = 0;
   for (int base = 0; base < nseg; base += kPlanThreads) {
     const int i = base + tid;
-    int64_t mine = 0;
-    int maxp = 0;
-    if (i < nseg && s.segs[i].len > 0) {
-      maxp = (int)((int64_t)s.segs[i].len * s.ctas / units) + 2;
-      mine = (int64_t)a.hk * maxp * s.segs[i].nq;
-    }
-    const int64_t cum = plan_scan<int64_t, false>(mine, warp_l, total);
-    if (i < nseg) {
-      s.segs[i].maxp = maxp;
-      s.segs[i].acc = sums + cum - mine;
-    }
+    const int len = i < nseg ? len_of(i) : 0;
+    // pieces that a kv head's `len` units can fall into: two more than its
+    // share of the CTAs (one more again for the rounding of the share)
+    const int maxp = len > 0 ? (int)((float)len * share) + 3 : 0;
+    const int64_t rows = len > 0 ? (int64_t)a.hk * maxp * nq_of(i) : 0;
+    const int64_t acc = sums + plan_scan<int64_t, false>(rows, warp_l, total) - rows;
     sums += total;
+    if (i < nseg) {
+      s.segs[i].acc = acc;
+      s.segs[i].maxp = maxp;
+    }
   }
-  if (tid == 0) *s.head = SpPlanHead{units, nseg, 0};
+  // where each CTA begins: the last segment that starts at or before its first
+  // unit (an empty one starts where the next does)
+  for (int b = tid; b < s.ctas; b += kPlanThreads) {
+    const int64_t u = sp_first(b, units, s.ctas);
+    int x = 0, y = nseg;
+    while (x < y) {
+      const int mid = (x + y) / 2;
+      if ((mid < kPlanKeep ? s_unit0[mid] : s.segs[mid].unit0) <= u) x = mid + 1;
+      else y = mid;
+    }
+    s.begin[b] = SpBegin{units, max(x - 1, 0), 0};
+  }
 }
 
 // ---------------------------------------------------------- partial sums
@@ -355,16 +421,25 @@ __device__ __forceinline__ void sp_load(uint32_t dst, const CUtensorMap *map, in
       "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row8), "r"(head), "r"(bar)
       : "memory");
 }
-// D[tmem] (+)= A[tmem] . B[smem]
-__device__ __forceinline__ void sp_umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                           bool accumulate) {
+// D[tmem] (+)= A[smem] . B[smem], and A[tmem] . B[smem]; descriptors as words
+__device__ __forceinline__ void sp_umma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                           uint32_t b_hi, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %6, 0;\n"
+      " mov.b64 a, {%1, %2};\n mov.b64 b, {%3, %4};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate ? 1u : 0u)
       : "memory");
 }
-
+__device__ __forceinline__ void sp_umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
+                                           uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n"
+      " mov.b64 b, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
 
 // d = max(a, b, c)
 __device__ __forceinline__ float sp_max3(float a, float b, float c) {
@@ -410,22 +485,12 @@ struct SpPiece {
 struct SpWalk {
   int64_t u, end, units;
   int seg;
-  // By whole warps: the segment that the first unit is in is the last one
-  // that begins at or before it (empty ones begin where the next does).
   __device__ void begin(const SpArgs &s) {
-    const int lane = threadIdx.x & 31;
-    units = s.head->units;
+    const SpBegin x = s.begin[blockIdx.x];
+    units = x.units;
+    seg = x.seg;
     u = sp_first(blockIdx.x, units, s.ctas);
     end = sp_first(blockIdx.x + 1, units, s.ctas);
-    seg = 0;
-    for (int span = u < end ? s.head->segs : 0; span > 1;) {
-      const int step = (span + 31) / 32, i = seg + lane * step;
-      const bool le = lane * step < span && s.segs[i].unit0 <= u;
-      const int n = __popc(__ballot_sync(0xffffffffu, le));
-      const int skip = max(n - 1, 0) * step;
-      seg += skip;
-      span = min(step, span - skip);
-    }
   }
   __device__ bool next(const SpArgs &s, SpPiece &p) {
     while (u < end) {
@@ -435,8 +500,8 @@ struct SpWalk {
         continue;
       }
       const int64_t off = u - p.g.unit0;
-      p.h = (int)(off / p.g.len);
-      const int a = (int)(off % p.g.len);
+      p.h = (int)sp_div(off, p.g.len);
+      const int a = (int)(off - (int64_t)p.h * p.g.len);
       const int b = (int)min((int64_t)p.g.len, a + (end - u));
       u += b - a;
       p.t0 = max(a - kSpStart, 0);
@@ -450,8 +515,9 @@ struct SpWalk {
   }
 };
 
-// Warps 0-3 and 4-7 are two softmax streams, warp 8 loads, warp 9 issues the
-// products.  Per 128-token tile of a stream:
+// Warps 0-3 and 4-7 are two softmax streams; warps 8 and 10 load keys and
+// values, warps 9 and 11 issue the products of a stream each (the waits of one
+// pass beside the products of the other).  Per 128-token tile of a stream:
 //   S[128 x 128] = Q . K^T                (tensor memory, fp32)
 //   P = exp2(scale S - m), m the row's running maximum; a thread has a row
 //   O[128 x 128] += P . V                 (A = P from tensor memory)
@@ -476,7 +542,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + kSpSlots) * kSpTile);
   const uint32_t full = smem_u32(bars), empty = full + 8 * kSpSlots, s_full = empty + 8 * kSpSlots,
                  p_ready = s_full + 16, o_done = p_ready + 32, q_ready = o_done + 8,
-                 joint = q_ready + 8, drain = joint + 8;
+                 joint = q_ready + 8, drain = joint + 8,
+                 turn_of = drain + 8;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_issued[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -485,13 +552,17 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   if (tid == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tk)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tv)) : "memory");
-    for (int i = 0; i < 2 * kSpSlots; ++i) mbar_init(full + 8 * i);
+    for (int i = 0; i < kSpSlots; ++i) {
+      mbar_init(full + 8 * i);
+      mbar_init_count(empty + 8 * i, 2);  // both streams, or one of them twice
+    }
     for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i);
     for (int i = 0; i < 4; ++i) mbar_init_count(p_ready + 8 * i, 128);
-    mbar_init(o_done);
+    mbar_init_count(o_done, 2);
     mbar_init_count(q_ready, 256);
     mbar_init_count(joint, 256);
-    mbar_init(drain);
+    mbar_init_count(drain, 2);
+    for (int i = 0; i < 2; ++i) mbar_init(turn_of + 8 * i);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_abort = s_issued[0] = s_issued[1] = 0;
   }
@@ -558,97 +629,100 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       if (!ok) stop();
       s_issued[is_v] = last;
     }
-  } else if (warp == 9) {
+  } else if (warp == 9 || warp == 11) {
     const uint32_t qk = umma_idesc<T, 128>(false), pv = qk | (1u << 16);  // V is dim-contiguous
-    int i0 = 0, kt[2] = {0, 0};  // loads and tiles of the pieces before
-    auto slot_of = [&](int i) { return s_kv + (i % kSpSlots) * kSpTile; };
-    auto filled = [&](int i) {
-      const bool got = sp_wait(full + 8 * (i % kSpSlots), (uint32_t)(i / kSpSlots) & 1u);
-      tc_fence_after();
-      return got;
-    };
-    auto freed = [&](int i) { umma_commit(empty + 8 * (i % kSpSlots)); };
-    auto product_s = [&](int st, uint32_t q, int i) {  // S of stream st, from K in load i
-      const uint32_t k = slot_of(i);
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const uint32_t d = (x & 3) * 32;
-        umma(tmem + st * 128, umma_desc(q + (x >> 2) * kSpHalf + d, 16, 1024),
-             umma_desc(k + (x >> 2) * 1024 + d, 16, 2048), qk, x > 0);
-      }
-      umma_commit(s_full + 8 * st);
-    };
-    // O of stream st, from V in load i: the two halves of the tile's tokens as
-    // their weights come
-    auto product_o = [&](int st, int i, bool first) {
-      const uint32_t v = slot_of(i), o = tmem + 256 + st * 128;
-      const uint32_t phase = (uint32_t)kt[st]++ & 1u;
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        if (!sp_wait(p_ready + 16 * st + 8 * part, phase)) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {  // 16 tokens, the hi terms, then the lo ones
-          const int c = part * 4 + (x >> 1);
-          const uint32_t pt = tmem + st * 128 + (c >> 1) * 32 + (c & 1) * 8 + (x & 1) * 16;
-          sp_umma_ts(o, pt, umma_desc(v + c * 4096, 1024, 2048), pv, !(first && part + x == 0));
-        }
-      }
-      return true;
-    };
-    pdl_begin();
-    walk.begin(s);
-    bool ok = true;
-    while (lane == 0 && ok && walk.next(s, p)) {  // one thread issues them
-      const int n = p.n;
-      const bool two = p.g.nq > 128;
-      // one query tile alternates between the two places
-      const uint32_t q0 = s_q + (two ? 0 : (pieces & 1) * kSpTile);
-      ok = sp_wait(q_ready, (uint32_t)pieces & 1u);
-      tc_fence_after();
-      if (two) {  // loads: K0 V0 K1 V1 ...
-        ok = ok && filled(i0);
+    // Operand descriptors as two words; only the address (16-byte units, in
+    // the low word) changes, so a product costs two additions to issue.
+    constexpr uint32_t kHi = (1u << 14) | (2u << 29);  // version, 128-byte swizzle
+    constexpr uint32_t kHiQ = kHi | 1024 / 16, kHiKv = kHi | 2048 / 16;
+    const int st = warp == 11;
+    const uint32_t ts = tmem + st * 128;
+    int i0 = 0, tiles = 0;  // loads, and this stream's tiles, of the pieces before
+    int turns = 0;
+    bool ok = true, rehearsal = true;
+    // S of the stream's first tile, then O and the next S in turn.  `e` counts
+    // the tiles of both streams, this one's are those of its parity.  The
+    // second half of O with the next S is issued in the order of `e`: the
+    // streams then work half a period apart, one's products beside the other's
+    // exponentials (left alone they fall into step and wait for each other).
+    while (lane == 0 && ok) {  // one thread issues them
+      bool two = false;
+      int n = 2;
+      if (!rehearsal) {
+        if (!walk.next(s, p)) break;
+        n = p.n;
+        two = p.g.nq > 128;
+        ok = sp_wait(q_ready, (uint32_t)pieces & 1u);
         if (!ok) break;
-        product_s(0, q0, i0);
-        product_s(1, q0 + kSpTile, i0);
-        freed(i0);
-        for (int j = 0; j < n && ok; ++j) {
-          const int v = i0 + 2 * j + 1, k = v + 1;
-          ok = filled(v);
-          for (int st = 0; st < 2 && ok; ++st) {
-            ok = product_o(st, v, j == 0);
+      }
+      // one query tile alternates between the two places
+      const uint32_t q0 = s_q + (two ? st : pieces & 1) * kSpTile;
+      const uint32_t a0 = (q0 >> 4) | 1u << 16;
+      const int all = two ? 2 * n : n;
+      for (int e = st - 2; e < all; e += 2) {
+        if (e >= 0) {
+          const int v = i0 + (two ? e | 1 : min(2 * e + 2, 2 * n - 1));  // the load of its V
+          const uint32_t slot = (uint32_t)v % kSpSlots, turn = (uint32_t)v / kSpSlots;
+          const uint32_t b0 = ((s_kv + slot * kSpTile) >> 4) | (1024 / 16) << 16;
+          if (!rehearsal) {
+            ok = sp_wait(full + 8 * slot, turn & 1u);
             if (!ok) break;
-            if (st == 1) freed(v);
-            if (j + 1 < n) {
-              if (st == 0) ok = filled(k);
+          }
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {  // 64 tokens, as their weights come
+            if (!rehearsal) {
+              ok = sp_wait(p_ready + 16 * st + 8 * part, (uint32_t)tiles & 1u) &&
+                   (part == 0 || e == 0 || sp_wait(turn_of + 8 * st, (uint32_t)turns++ & 1u));
               if (!ok) break;
-              product_s(st, q0 + st * kSpTile, k);
-              if (st == 1) freed(k);
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {  // 16 tokens, the hi terms, then the lo ones
+              const int c = part * 4 + (x >> 1);
+              sp_umma_ts(ts + 256, ts + (c >> 1) * 32 + (c & 1) * 8 + (x & 1) * 16,
+                         b0 + c * (4096 / 16), kHiKv, pv, part + x > 0 || e >= 2);
             }
           }
-        }
-      } else {  // loads: K0 K1 V0 K2 V1 ... (without the K's past the last)
-        for (int st = 0; st < min(n, 2) && ok; ++st) {
-          ok = filled(i0 + st);
           if (!ok) break;
-          product_s(st, q0, i0 + st);
-          freed(i0 + st);
-        }
-        for (int j = 0; j < n && ok; ++j) {
-          const int v = i0 + min(2 * j + 2, 2 * n - 1);
-          ok = filled(v) && product_o(j & 1, v, j < 2);
-          if (!ok) break;
-          freed(v);
-          if (j + 2 < n) {
-            const int k = i0 + 2 * j + 3;
-            ok = filled(k);
-            if (!ok) break;
-            product_s(j & 1, q0, k);
-            freed(k);
+          ++tiles;
+          if (!rehearsal) {
+            umma_commit(empty + 8 * slot);
+            if (!two) mbar_arrive(empty + 8 * slot);
           }
         }
+        if (e + 2 < all) {
+          const int k = i0 + (two ? (e + 2) & ~1 : (e < 0 ? e + 2 : 2 * e + 3));  // of its K
+          const uint32_t slot = (uint32_t)k % kSpSlots, turn = (uint32_t)k / kSpSlots;
+          const uint32_t b0 = ((s_kv + slot * kSpTile) >> 4) | 1u << 16;
+          if (!rehearsal) {
+            ok = sp_wait(full + 8 * slot, turn & 1u);
+            if (!ok) break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const uint32_t d = (x & 3) * (32 / 16);
+            sp_umma_ss(ts, a0 + (x >> 2) * (kSpHalf / 16) + d, kHiQ,
+                       b0 + (x >> 2) * (1024 / 16) + d, kHiKv, qk, x > 0);
+          }
+          if (!rehearsal) {
+            umma_commit(s_full + 8 * st);
+            umma_commit(empty + 8 * slot);
+            if (!two) mbar_arrive(empty + 8 * slot);
+          }
+        }
+        if (!rehearsal && e >= 0 && e + 1 < all) mbar_arrive(turn_of + 8 * (st ^ 1));
       }
       if (!ok) break;
+      if (rehearsal) {  // (on whatever shared memory holds; the sums are not used)
+        rehearsal = false;
+        tiles = 0;
+        umma_commit(drain);
+        ok = sp_wait(drain, 0);
+        pdl_begin();
+        walk.begin(s);
+        continue;
+      }
       i0 += 2 * n;
       umma_commit(o_done);
       ++pieces;
@@ -929,9 +1003,9 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     if (tid < 2)  // (of the keys, and of the values: no more than the ring holds)
       for (int i = max(0, s_issued[tid] - kSpSlots); i < s_issued[tid]; ++i)
         mbar_wait(full + 8 * (i % kSpSlots), (uint32_t)(i / kSpSlots) & 1u);
-    if (tid == 9 * 32) {
+    if (tid == 9 * 32 || tid == 11 * 32) {
       umma_commit(drain);
-      mbar_wait(drain, 0);
+      mbar_wait(drain, 1);
     }
     __syncthreads();
   }
@@ -943,86 +1017,104 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 constexpr int kMergeWarps = 4;
 
 // A CTA a (row, query head), a lane four of its dims: warp w takes pieces w,
-// w + 4, ... of the prefix, then of the row's own tokens, and the warps' sums
-// are joined in order.
-template <typename T>
+// w + 4, ... of the prefix and, behind them, of the row's own tokens, and the
+// warps' sums are joined in order.  One warp a (row, head) instead (SPREAD
+// false) when they alone fill the GPU: 2560 of a few pieces each, 11.8 us
+// against 19.8.
+template <typename T, bool SPREAD>
 __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(const SpArgs s) {
   __shared__ float4 s_acc[kMergeWarps][32];
   __shared__ float2 s_ml[kMergeWarps];
   pdl_begin();
   const TaArgs &a = s.a;
-  const int64_t rh = blockIdx.x;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.hq / a.hk;
+  constexpr int kStep = SPREAD ? kMergeWarps : 1;
+  const int lane = threadIdx.x & 31, G = a.hq / a.hk;
+  const int warp = SPREAD ? threadIdx.x >> 5 : 0;
+  const int64_t rh = SPREAD ? blockIdx.x : (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+  if (rh >= (int64_t)a.rows * a.hq) return;  // (whole warps, none of SPREAD's)
   const int row = (int)(rh / a.hq), head = (int)(rh % a.hq), h = head / G;
-  const int64_t units = s.head->units;
+  const int64_t units = s.begin[0].units;
   const SpRow at = s.rows[row];
-  float M = -INFINITY, sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const int m = (row - at.row0) * G + head % G;  // query row in the group
-#pragma unroll 1
+  // the two segments: pieces, first owner, first place, places between pieces
+  int count[2] = {0, 0}, b0[2] = {0, 0}, len[2] = {0, 0}, stride[2] = {0, 0};
+  int64_t A[2] = {0, 0}, place[2] = {0, 0};
+#pragma unroll
   for (int part = 0; part < 2; ++part) {
     const int seg = part == 0 ? (at.pseg < 0 ? -1 : at.pseg + m / 256) : at.sseg;
     if (seg < 0) continue;
-    const SpSeg g = s.segs[seg];
+    const SpSeg &g = s.segs[seg];
+    len[part] = g.len;
     if (g.len == 0) continue;
-    const int q = part == 0 ? m % 256 : at.srow * G + head % G;
-    const int64_t A = g.unit0 + (int64_t)h * g.len;
-    const int b0 = sp_owner(A, units, s.ctas), b1 = sp_owner(A + g.len - 1, units, s.ctas);
-    const int64_t first = g.acc + (int64_t)h * g.maxp * g.nq + q;
-    for (int base = b0 + warp; base <= b1; base += 32 * kMergeWarps) {
-      const int b = base + lane * kMergeWarps;
-      float2 x = make_float2(-INFINITY, 0.f);
-      if (b <= b1) {  // (a piece without tiles wrote nothing)
-        const int from = (int)max(sp_first(b, units, s.ctas) - A, (int64_t)0);
-        const int till = (int)min(sp_first(b + 1, units, s.ctas) - A, (int64_t)g.len);
-        if (max(till - kSpStart, 0) > max(from - kSpStart, 0))
-          x = s.ml[first + (int64_t)(b - b0) * g.nq];
-      }
-      float top = x.x;
+    A[part] = g.unit0 + (int64_t)h * g.len;
+    b0[part] = sp_owner(A[part], units, s.ctas);
+    count[part] = sp_owner(A[part] + g.len - 1, units, s.ctas) - b0[part] + 1;
+    stride[part] = g.nq;
+    place[part] = g.acc + (int64_t)h * g.maxp * g.nq + (part == 0 ? m % 256 : at.srow * G + head % G);
+  }
+  const int all = count[0] + count[1];
+  float M = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = warp; base < all; base += 32 * kStep) {
+    const int i = base + lane * kStep;
+    float2 x = make_float2(-INFINITY, 0.f);
+    int64_t src = 0;
+    if (i < all) {
+      const bool own = i >= count[0];
+      const int k = own ? i - count[0] : i;
+      const int64_t u0 = own ? A[1] : A[0];
+      const int b = (own ? b0[1] : b0[0]) + k;
+      const int from = (int)max(sp_first(b, units, s.ctas) - u0, (int64_t)0);
+      const int till = (int)min(sp_first(b + 1, units, s.ctas) - u0, (int64_t)(own ? len[1] : len[0]));
+      src = (own ? place[1] : place[0]) + (int64_t)k * (own ? stride[1] : stride[0]);
+      if (max(till - kSpStart, 0) > max(from - kSpStart, 0)) x = s.ml[src];  // (else nothing was written)
+    }
+    float top = x.x;
 #pragma unroll
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float now = fmaxf(M, top);
-      if (now == -INFINITY) continue;
-      const float f = exp2f(M - now);
-      M = now;
-      acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-      const float w = x.x == -INFINITY ? 0.f : exp2f(x.x - now);
-      sum = fmaf(sum, f, warp_sum(w * x.y));
-      const int n = min(32, (b1 - base) / kMergeWarps + 1);
-      const unsigned live = __ballot_sync(0xffffffffu, x.x != -INFINITY);
-      const float *src = s.acc + (first + (int64_t)(base - b0) * g.nq) * kTaD + 4 * lane;
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float now = fmaxf(M, top);
+    if (now == -INFINITY) continue;
+    const float f = exp2f(M - now);
+    M = now;
+    acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+    const float w = x.x == -INFINITY ? 0.f : exp2f(x.x - now);
+    sum = fmaf(sum, f, warp_sum(w * x.y));
+    const int n = min(32, (all - 1 - base) / kStep + 1);
+    const unsigned live = __ballot_sync(0xffffffffu, x.x != -INFINITY);
 #pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float wi = __shfl_sync(0xffffffffu, w, i);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (live >> i & 1)
-          v = *reinterpret_cast<const float4 *>(src + (int64_t)i * kMergeWarps * g.nq * kTaD);
-        acc.x = fmaf(v.x, wi, acc.x);
-        acc.y = fmaf(v.y, wi, acc.y);
-        acc.z = fmaf(v.z, wi, acc.z);
-        acc.w = fmaf(v.w, wi, acc.w);
-      }
+    for (int j = 0; j < n; ++j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      const int64_t sj = __shfl_sync(0xffffffffu, src, j);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (live >> j & 1) v = *reinterpret_cast<const float4 *>(s.acc + sj * kTaD + 4 * lane);
+      acc.x = fmaf(v.x, wj, acc.x);
+      acc.y = fmaf(v.y, wj, acc.y);
+      acc.z = fmaf(v.z, wj, acc.z);
+      acc.w = fmaf(v.w, wj, acc.w);
     }
   }
-  s_acc[warp][lane] = acc;
-  if (lane == 0) s_ml[warp] = make_float2(M, sum);
-  __syncthreads();
-  if (warp != 0) return;
-  float top = -INFINITY;
+  float top = M;
+  if (SPREAD) {
+    s_acc[warp][lane] = acc;
+    if (lane == 0) s_ml[warp] = make_float2(M, sum);
+    __syncthreads();
+    if (warp != 0) return;
+    top = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, s_ml[w].x);
-  sum = 0.f;
-  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, s_ml[w].x);
+    sum = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) {
-    if (s_ml[w].x == -INFINITY) continue;
-    const float f = exp2f(s_ml[w].x - top);
-    const float4 v = s_acc[w][lane];
-    sum = fmaf(s_ml[w].y, f, sum);
-    acc.x = fmaf(v.x, f, acc.x);
-    acc.y = fmaf(v.y, f, acc.y);
-    acc.z = fmaf(v.z, f, acc.z);
-    acc.w = fmaf(v.w, f, acc.w);
+    for (int w = 0; w < kMergeWarps; ++w) {
+      if (s_ml[w].x == -INFINITY) continue;
+      const float f = exp2f(s_ml[w].x - top);
+      const float4 v = s_acc[w][lane];
+      sum = fmaf(s_ml[w].y, f, sum);
+      acc.x = fmaf(v.x, f, acc.x);
+      acc.y = fmaf(v.y, f, acc.y);
+      acc.z = fmaf(v.z, f, acc.z);
+      acc.w = fmaf(v.w, f, acc.w);
+    }
   }
   // nothing seen: zeros and -inf (a sum that is NaN says so)
   const bool none = top == -INFINITY;
@@ -1056,7 +1148,7 @@ struct SpPlan {
   int box;             // 0: pages that no TMA box fits (every row for itself)
   int64_t splits;      // of a row, without boxes
   // scratch, in floats (every part a multiple of 16 bytes)
-  int64_t head, segs, rows, gseg, acc, ml, total;
+  int64_t begin, segs, rows, gseg, acc, ml, total;
 };
 
 SpPlan plan_for(int rows, int hq, int hk, int groups, int bs, int max_prefix, int max_suffix) {
@@ -1079,11 +1171,11 @@ SpPlan plan_for(int rows, int hq, int hk, int groups, int bs, int max_prefix, in
   const int64_t g = hq / hk, ctas = sm_count();
   const int64_t segs = ((int64_t)rows * g + 255) / 256 + groups + rows;
   // pieces x query rows: each (row, head) is in two segments, each of which
-  // is in two pieces more than its share of the CTAs
-  const int64_t sums = 4 * (int64_t)rows * hq + 256 * ctas;
+  // has places for three pieces more than its share of the CTAs
+  const int64_t sums = 6 * (int64_t)rows * hq + 257 * ctas;
   auto round = [](int64_t n) { return (n + 7) / 8 * 8; };
-  p.head = 0;
-  p.segs = 8;
+  p.begin = 0;
+  p.segs = ctas * 4;
   p.rows = p.segs + segs * 16;
   p.gseg = p.rows + (int64_t)rows * 4;
   p.ml = round(p.gseg + groups);
@@ -1109,7 +1201,7 @@ template <typename T> int run_typed(SpArgs &s, const SpPlan &p, float *scratch, 
   }
   s.box = p.box;
   s.ctas = sm_count();
-  s.head = reinterpret_cast<SpPlanHead *>(scratch);
+  s.begin = reinterpret_cast<SpBegin *>(scratch + p.begin);
   s.segs = reinterpret_cast<SpSeg *>(scratch + p.segs);
   s.rows = reinterpret_cast<SpRow *>(scratch + p.rows);
   s.gseg = reinterpret_cast<int32_t *>(scratch + p.gseg);
@@ -1125,7 +1217,13 @@ template <typename T> int run_typed(SpArgs &s, const SpPlan &p, float *scratch, 
   if (int e = check_launch("shared_prefix_plan_kernel")) return e;
   launch_kernel(kern, dim3(s.ctas), dim3(kSpThreads), kSpSmem, st, tk, tv, s);
   if (int e = check_launch("shared_prefix_kernel")) return e;
-  launch_kernel(shared_prefix_merge_kernel<T>, dim3((unsigned)rh), dim3(kMergeWarps * 32), 0, st, s);
+  if (rh < 8L * s.ctas)
+    launch_kernel(shared_prefix_merge_kernel<T, true>, dim3((unsigned)rh), dim3(kMergeWarps * 32), 0,
+                  st, s);
+  else
+    launch_kernel(shared_prefix_merge_kernel<T, false>,
+                  dim3((unsigned)((rh + kMergeWarps - 1) / kMergeWarps)), dim3(kMergeWarps * 32), 0,
+                  st, s);
   return check_launch("shared_prefix_merge_kernel");
 }
 
