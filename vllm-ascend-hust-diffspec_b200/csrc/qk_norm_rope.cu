@@ -69,8 +69,11 @@ __device__ __forceinline__ int64_t dest_row(const QkArgs &a, int t, int pos, boo
   return page * a.bs + pos % a.bs;
 }
 
-// One warp per (token, head), heads in the order q, k, v.  Element pairs that
-// rotate together are read and written by one lane, so q_out may be q.
+// ---------------------------------------------------------------- any head
+// One warp per (token, head), heads in the order q, k, v, for head sizes,
+// partial rotations and alignments that the kernel below does not take.
+// Element pairs that rotate together are read and written by one lane, so
+// q_out may be q.
 template <typename T, typename CS>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkArgs a) {
   pdl_begin();
@@ -139,18 +142,184 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkArgs a) {
   }
 }
 
+// ------------------------------------------------------------- whole heads
+// Heads of D = 64, 128 or 256 rotated in full, 16-byte aligned rows: D / 16
+// lanes a head, a lane 16 of its elements in two 16-byte pieces that rotate
+// with each other (NeoX: elements 8 l .. and D / 2 + 8 l ..; pairs: 16 l ..),
+// so the rotation needs no exchange and the norm a few shuffles.  A thread
+// takes kQkHeads heads of one token at once: its loads are all on their way
+// before the first is used, and one row of cosines and sines serves them.
+constexpr int kQkHeads = 4;
+
+template <typename T> __device__ __forceinline__ void qk_unpack(const uint4 &w, float (&v)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<T>(u[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+template <typename T> __device__ __forceinline__ uint4 qk_pack(const float (&v)[8]) {
+  return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
+                    pack2<T>(v[6], v[7]));
+}
+// 8 consecutive entries of the table
+template <typename CS> __device__ __forceinline__ void qk_table(const CS *p, float (&v)[8]) {
+  qk_unpack<CS>(*reinterpret_cast<const uint4 *>(p), v);
+}
+template <> __device__ __forceinline__ void qk_table<float>(const float *p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
+template <typename T, typename CS, int D, bool NEOX>
+__global__ void __launch_bounds__(256) qk_norm_rope_heads_kernel(const QkArgs a) {
+  constexpr int kLanes = D / 16, kGroups = 32 / kLanes;  // heads that a warp has side by side
+  constexpr int kPer = kGroups * kQkHeads;               // heads of one token a warp takes
+  pdl_begin();
+  const int64_t warp = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31, l = lane % kLanes;
+  const int heads = a.hq + 2 * a.hk, chunks = (heads + kPer - 1) / kPer;
+  if (warp >= (int64_t)a.tokens * chunks) return;
+  const int t = (int)(warp / chunks), h0 = (int)(warp % chunks) * kPer + lane / kLanes;
+  const int e1 = NEOX ? 8 * l : 16 * l, e2 = NEOX ? D / 2 + 8 * l : 16 * l + 8;
+  // every load first
+  uint4 x1[kQkHeads], x2[kQkHeads];
+#pragma unroll
+  for (int i = 0; i < kQkHeads; ++i) {
+    const int h = h0 + i * kGroups;
+    x1[i] = x2[i] = make_uint4(0, 0, 0, 0);
+    if (h >= heads) continue;
+    const T *src = h < a.hq ? static_cast<const T *>(a.q) + t * a.q_stride + (int64_t)h * D
+                   : h < a.hq + a.hk
+                       ? static_cast<const T *>(a.k) + t * a.k_stride + (int64_t)(h - a.hq) * D
+                       : static_cast<const T *>(a.v) + t * a.v_stride + (int64_t)(h - a.hq - a.hk) * D;
+    x1[i] = *reinterpret_cast<const uint4 *>(src + e1);
+    x2[i] = *reinterpret_cast<const uint4 *>(src + e2);
+  }
+  const int pos = a.positions[t] + a.pos_offset;
+  const bool turn = pos >= 0 && pos < a.rotary_rows;  // else: normed, not rotated
+  if (!turn && lane == 0 && h0 == 0) flag_error(a.err, DSB_FLAG_POSITION);
+  const CS *cs = static_cast<const CS *>(a.cos_sin) + (turn ? pos : 0) * a.cs_stride;
+  float co[8], si[8];
+  qk_table<CS>(cs + 8 * l, co);
+  qk_table<CS>(cs + D / 2 + 8 * l, si);
+  int64_t row = -1;
+  const bool keys = (int)(warp % chunks) * kPer + kPer > a.hq;  // the warp has keys or values
+  if (keys && a.dest != kDestNone) row = dest_row(a, t, pos, lane == 0);
+#pragma unroll
+  for (int i = 0; i < kQkHeads; ++i) {
+    const int h = h0 + i * kGroups;
+    // (lanes past the last head join the shuffles below)
+    const bool in = h < heads, value = h >= a.hq + a.hk, is_q = h < a.hq;
+    const int kh = is_q ? 0 : value ? h - a.hq - a.hk : h - a.hq;
+    float v1[8], v2[8];
+    qk_unpack<T>(x1[i], v1);
+    qk_unpack<T>(x2[i], v2);
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss = fmaf(v1[j], v1[j], fmaf(v2[j], v2[j], ss));
+#pragma unroll
+    for (int o = kLanes / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (!in) continue;
+    uint4 r1 = x1[i], r2 = x2[i], y1 = x1[i], y2 = x2[i];
+    if (!value) {
+      const float inv = rsqrtf(ss * (1.f / D) + a.eps);
+      const T *w = static_cast<const T *>(is_q ? a.qw : a.kw);
+      float w1[8], w2[8];
+      qk_unpack<T>(*reinterpret_cast<const uint4 *>(w + e1), w1);
+      qk_unpack<T>(*reinterpret_cast<const uint4 *>(w + e2), w2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v1[j] *= inv * w1[j];
+        v2[j] *= inv * w2[j];
+      }
+      if (a.dest == kDestRaw && !is_q) y1 = qk_pack<T>(v1), y2 = qk_pack<T>(v2);
+      if (turn) {
+        float o1[8], o2[8];
+        if (NEOX) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            o1[j] = v1[j] * co[j] - v2[j] * si[j];
+            o2[j] = v2[j] * co[j] + v1[j] * si[j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            o1[j] = v1[j] * co[j / 2] - v1[j + 1] * si[j / 2];
+            o1[j + 1] = v1[j + 1] * co[j / 2] + v1[j] * si[j / 2];
+            o2[j] = v2[j] * co[4 + j / 2] - v2[j + 1] * si[4 + j / 2];
+            o2[j + 1] = v2[j + 1] * co[4 + j / 2] + v2[j] * si[4 + j / 2];
+          }
+        }
+        r1 = qk_pack<T>(o1), r2 = qk_pack<T>(o2);
+      } else {
+        r1 = qk_pack<T>(v1), r2 = qk_pack<T>(v2);
+      }
+    }
+    const int64_t out_row = ((int64_t)t * a.hk + kh) * D;
+    T *out = is_q ? static_cast<T *>(a.q_out) + t * a.qo_stride + (int64_t)h * D
+             : value ? (a.v_out != nullptr ? static_cast<T *>(a.v_out) + out_row : nullptr)
+                     : (a.k_out != nullptr ? static_cast<T *>(a.k_out) + out_row : nullptr);
+    if (out != nullptr) {
+      *reinterpret_cast<uint4 *>(out + e1) = r1;
+      *reinterpret_cast<uint4 *>(out + e2) = r2;
+    }
+    if (!is_q && row >= 0) {
+      T *dst = static_cast<T *>(value ? a.dst_v : a.dst_k) + (row * a.hk + kh) * D;
+      const bool raw = a.dest == kDestRaw;
+      *reinterpret_cast<uint4 *>(dst + e1) = raw ? y1 : r1;
+      *reinterpret_cast<uint4 *>(dst + e2) = raw ? y2 : r2;
+    }
+  }
+}
+
+// Whether the whole-head kernel takes the call: its pieces are 16 bytes.
+bool whole_heads(const QkArgs &a, int cos_sin_dtype) {
+  auto ok = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  const int64_t cs_step = cos_sin_dtype == DSB_F32 ? 4 : 8;
+  return (a.d == 64 || a.d == 128 || a.d == 256) && a.rot == a.d && ok(a.q) && ok(a.q_out) &&
+         ok(a.k) && ok(a.v) && ok(a.k_out) && ok(a.v_out) && ok(a.dst_k) && ok(a.dst_v) && ok(a.qw) &&
+         ok(a.kw) && ok(a.cos_sin) && a.q_stride % 8 == 0 && a.qo_stride % 8 == 0 &&
+         a.k_stride % 8 == 0 && a.v_stride % 8 == 0 && a.cs_stride % cs_step == 0;
+}
+
+template <typename T, typename CS, int D> void launch_heads(const QkArgs &a, cudaStream_t st) {
+  const int per = 32 / (D / 16) * kQkHeads;
+  const int64_t warps = (int64_t)a.tokens * ((a.hq + 2 * a.hk + per - 1) / per);
+  const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
+  if (a.neox)
+    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, true>, grid, block, 0, st, a);
+  else
+    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, false>, grid, block, 0, st, a);
+}
+
 int launch(const QkArgs &a, int cos_sin_dtype, int dtype, cudaStream_t st) {
   const int64_t warps = (int64_t)a.tokens * (a.hq + 2 * a.hk);
   if ((warps + 7) / 8 > INT32_MAX) return fail(DSB_ERR_UNSUPPORTED, "grid too large");
   const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
-  auto go = [&](auto tag) {
+  const bool whole = whole_heads(a, cos_sin_dtype);
+  auto with = [&](auto tag, auto table) {
     using T = decltype(tag);
-    if (cos_sin_dtype == DSB_F32)
-      launch_kernel(qk_norm_rope_kernel<T, float>, grid, block, 0, st, a);
-    else if (cos_sin_dtype == DSB_BF16)
-      launch_kernel(qk_norm_rope_kernel<T, __nv_bfloat16>, grid, block, 0, st, a);
+    using CS = decltype(table);
+    if (!whole)
+      launch_kernel(qk_norm_rope_kernel<T, CS>, grid, block, 0, st, a);
+    else if (a.d == 64)
+      launch_heads<T, CS, 64>(a, st);
+    else if (a.d == 128)
+      launch_heads<T, CS, 128>(a, st);
     else
-      launch_kernel(qk_norm_rope_kernel<T, __half>, grid, block, 0, st, a);
+      launch_heads<T, CS, 256>(a, st);
+  };
+  auto go = [&](auto tag) {
+    if (cos_sin_dtype == DSB_F32)
+      with(tag, 0.f);
+    else if (cos_sin_dtype == DSB_BF16)
+      with(tag, __nv_bfloat16());
+    else
+      with(tag, __half());
   };
   if (dtype == DSB_BF16)
     go(__nv_bfloat16());
