@@ -174,101 +174,178 @@ template <> __device__ __forceinline__ void qk_table<float>(const float *p, floa
   v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
+// 16 bytes that no other thread reads, kept out of L1 (not through the
+// read-only path: the queries may be rotated in place).
+__device__ __forceinline__ uint4 qk_load(const void *p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+// A lane's two pieces of a head: the mean of the head's squares.
+template <int D>
+__device__ __forceinline__ float qk_mean_square(const float (&v1)[8], const float (&v2)[8]) {
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ss = fmaf(v1[j], v1[j], fmaf(v2[j], v2[j], ss));
+#pragma unroll
+  for (int o = D / 32; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  return ss * (1.f / D);
+}
+
+// What turns a head's pieces: out = inv * (v1 * c1 - v2' * s2 ...), the weight
+// and the cosines and sines of the token in one factor each, shared by the
+// heads that a thread takes.  A lane's 16 elements make 8 pairs (x, y):
+// NeoX (v1[j], v2[j]), else neighbours.
+struct QkTurn {
+  float xc[8], ys[8], yc[8], xs[8];  // wx c, wy s, wy c, wx s
+};
+
 template <typename T, typename CS, int D, bool NEOX>
-__global__ void __launch_bounds__(256) qk_norm_rope_heads_kernel(const QkArgs a) {
+__device__ __forceinline__ void qk_factors(QkTurn &f, const T *w, const CS *cs, int l, bool turn) {
+  float c[8], n[8], w1[8], w2[8];
+  qk_table<CS>(cs + 8 * l, c);
+  qk_table<CS>(cs + D / 2 + 8 * l, n);
+  qk_unpack<T>(*reinterpret_cast<const uint4 *>(w + (NEOX ? 8 * l : 16 * l)), w1);
+  qk_unpack<T>(*reinterpret_cast<const uint4 *>(w + (NEOX ? D / 2 + 8 * l : 16 * l + 8)), w2);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float wx = NEOX ? w1[j] : (j < 4 ? w1[2 * j] : w2[2 * j - 8]);
+    const float wy = NEOX ? w2[j] : (j < 4 ? w1[2 * j + 1] : w2[2 * j - 7]);
+    const float cj = turn ? c[j] : 1.f, sj = turn ? n[j] : 0.f;
+    f.xc[j] = wx * cj, f.ys[j] = wy * sj;
+    f.yc[j] = wy * cj, f.xs[j] = wx * sj;
+  }
+}
+
+template <bool NEOX>
+__device__ __forceinline__ void qk_turn(const QkTurn &f, float inv, const float (&v1)[8],
+                                        const float (&v2)[8], float (&o1)[8], float (&o2)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = NEOX ? v1[j] : (j < 4 ? v1[2 * j] : v2[2 * j - 8]);
+    const float y = NEOX ? v2[j] : (j < 4 ? v1[2 * j + 1] : v2[2 * j - 7]);
+    const float a = inv * (x * f.xc[j] - y * f.ys[j]), b = inv * (y * f.yc[j] + x * f.xs[j]);
+    if (NEOX) {
+      o1[j] = a, o2[j] = b;
+    } else if (j < 4) {
+      o1[2 * j] = a, o1[2 * j + 1] = b;
+    } else {
+      o2[2 * j - 8] = a, o2[2 * j - 7] = b;
+    }
+  }
+}
+
+// A warp takes kPer query heads of one token, or kPer of its key and value
+// heads.  `ahead`: tokens between a warp's and the one whose rows it asks into
+// L2, about what the GPU has resident, so that the loads of a later warp hit
+// there (0: none).
+template <typename T, typename CS, int D, bool NEOX>
+__global__ void __launch_bounds__(256, 2) qk_norm_rope_heads_kernel(const QkArgs a, int ahead) {
   constexpr int kLanes = D / 16, kGroups = 32 / kLanes;  // heads that a warp has side by side
   constexpr int kPer = kGroups * kQkHeads;               // heads of one token a warp takes
   pdl_begin();
   const int64_t warp = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31, l = lane % kLanes;
-  const int heads = a.hq + 2 * a.hk, chunks = (heads + kPer - 1) / kPer;
-  if (warp >= (int64_t)a.tokens * chunks) return;
-  const int t = (int)(warp / chunks), h0 = (int)(warp % chunks) * kPer + lane / kLanes;
+  const int qchunks = (a.hq + kPer - 1) / kPer, chunks = qchunks + (2 * a.hk + kPer - 1) / kPer;
+  const int t = (int)(warp / chunks), chunk = (int)(warp - (int64_t)t * chunks);
+  if (t >= a.tokens) return;
   const int e1 = NEOX ? 8 * l : 16 * l, e2 = NEOX ? D / 2 + 8 * l : 16 * l + 8;
-  // every load first
-  uint4 x1[kQkHeads], x2[kQkHeads];
-#pragma unroll
-  for (int i = 0; i < kQkHeads; ++i) {
-    const int h = h0 + i * kGroups;
-    x1[i] = x2[i] = make_uint4(0, 0, 0, 0);
-    if (h >= heads) continue;
-    const T *src = h < a.hq ? static_cast<const T *>(a.q) + t * a.q_stride + (int64_t)h * D
-                   : h < a.hq + a.hk
-                       ? static_cast<const T *>(a.k) + t * a.k_stride + (int64_t)(h - a.hq) * D
-                       : static_cast<const T *>(a.v) + t * a.v_stride + (int64_t)(h - a.hq - a.hk) * D;
-    x1[i] = *reinterpret_cast<const uint4 *>(src + e1);
-    x2[i] = *reinterpret_cast<const uint4 *>(src + e2);
-  }
   const int pos = a.positions[t] + a.pos_offset;
   const bool turn = pos >= 0 && pos < a.rotary_rows;  // else: normed, not rotated
-  if (!turn && lane == 0 && h0 == 0) flag_error(a.err, DSB_FLAG_POSITION);
   const CS *cs = static_cast<const CS *>(a.cos_sin) + (turn ? pos : 0) * a.cs_stride;
-  float co[8], si[8];
-  qk_table<CS>(cs + 8 * l, co);
-  qk_table<CS>(cs + D / 2 + 8 * l, si);
-  int64_t row = -1;
-  const bool keys = (int)(warp % chunks) * kPer + kPer > a.hq;  // the warp has keys or values
-  if (keys && a.dest != kDestNone) row = dest_row(a, t, pos, lane == 0);
+  const bool later = ahead > 0 && lane == 0 && t + ahead < a.tokens;
+  uint4 x1[kQkHeads], x2[kQkHeads];
+  QkTurn f;
+
+  if (chunk < qchunks) {
+    const int h0 = chunk * kPer + lane / kLanes;
+    const T *src = static_cast<const T *>(a.q) + t * a.q_stride + (int64_t)h0 * D;
+    if (later)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + ahead * a.q_stride),
+                   "r"(min(kPer, a.hq - chunk * kPer) * D * 2)
+                   : "memory");
+#pragma unroll
+    for (int i = 0; i < kQkHeads; ++i) {  // (a head past the last: zeros, not stored)
+      const bool in = h0 + i * kGroups < a.hq;
+      x1[i] = in ? qk_load(src + i * kGroups * D + e1) : make_uint4(0, 0, 0, 0);
+      x2[i] = in ? qk_load(src + i * kGroups * D + e2) : make_uint4(0, 0, 0, 0);
+    }
+    if (!turn && lane == 0 && chunk == 0) flag_error(a.err, DSB_FLAG_POSITION);
+    qk_factors<T, CS, D, NEOX>(f, static_cast<const T *>(a.qw), cs, l, turn);
+    T *out = static_cast<T *>(a.q_out) + t * a.qo_stride + (int64_t)h0 * D;
+#pragma unroll
+    for (int i = 0; i < kQkHeads; ++i) {
+      float v1[8], v2[8], o1[8], o2[8];
+      qk_unpack<T>(x1[i], v1);
+      qk_unpack<T>(x2[i], v2);
+      const float inv = rsqrtf(qk_mean_square<D>(v1, v2) + a.eps);
+      qk_turn<NEOX>(f, inv, v1, v2, o1, o2);
+      if (h0 + i * kGroups < a.hq) {
+        *reinterpret_cast<uint4 *>(out + i * kGroups * D + e1) = qk_pack<T>(o1);
+        *reinterpret_cast<uint4 *>(out + i * kGroups * D + e2) = qk_pack<T>(o2);
+      }
+    }
+    return;
+  }
+
+  const int k0 = (chunk - qchunks) * kPer, h0 = k0 + lane / kLanes;  // keys, then values
+  const T *key = static_cast<const T *>(a.k) + t * a.k_stride;
+  const T *value = static_cast<const T *>(a.v) + t * a.v_stride;
+  if (later && k0 == 0) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(key + ahead * a.k_stride),
+                 "r"(a.hk * D * 2)
+                 : "memory");
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(value + ahead * a.v_stride),
+                 "r"(a.hk * D * 2)
+                 : "memory");
+  }
 #pragma unroll
   for (int i = 0; i < kQkHeads; ++i) {
     const int h = h0 + i * kGroups;
-    // (lanes past the last head join the shuffles below)
-    const bool in = h < heads, value = h >= a.hq + a.hk, is_q = h < a.hq;
-    const int kh = is_q ? 0 : value ? h - a.hq - a.hk : h - a.hq;
-    float v1[8], v2[8];
-    qk_unpack<T>(x1[i], v1);
-    qk_unpack<T>(x2[i], v2);
-    float ss = 0.f;
+    const T *src = h < a.hk ? key + h * D : value + (h - a.hk) * D;
+    const bool in = h < 2 * a.hk;
+    x1[i] = in ? qk_load(src + e1) : make_uint4(0, 0, 0, 0);
+    x2[i] = in ? qk_load(src + e2) : make_uint4(0, 0, 0, 0);
+  }
+  const int64_t row = a.dest != kDestNone ? dest_row(a, t, pos, lane == 0) : -1;
+  if (k0 < a.hk) qk_factors<T, CS, D, NEOX>(f, static_cast<const T *>(a.kw), cs, l, turn);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(v1[j], v1[j], fmaf(v2[j], v2[j], ss));
-#pragma unroll
-    for (int o = kLanes / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!in) continue;
+  for (int i = 0; i < kQkHeads; ++i) {
+    const int h = h0 + i * kGroups;
     uint4 r1 = x1[i], r2 = x2[i], y1 = x1[i], y2 = x2[i];
-    if (!value) {
-      const float inv = rsqrtf(ss * (1.f / D) + a.eps);
-      const T *w = static_cast<const T *>(is_q ? a.qw : a.kw);
-      float w1[8], w2[8];
-      qk_unpack<T>(*reinterpret_cast<const uint4 *>(w + e1), w1);
-      qk_unpack<T>(*reinterpret_cast<const uint4 *>(w + e2), w2);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v1[j] *= inv * w1[j];
-        v2[j] *= inv * w2[j];
-      }
-      if (a.dest == kDestRaw && !is_q) y1 = qk_pack<T>(v1), y2 = qk_pack<T>(v2);
-      if (turn) {
-        float o1[8], o2[8];
-        if (NEOX) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            o1[j] = v1[j] * co[j] - v2[j] * si[j];
-            o2[j] = v2[j] * co[j] + v1[j] * si[j];
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            o1[j] = v1[j] * co[j / 2] - v1[j + 1] * si[j / 2];
-            o1[j + 1] = v1[j + 1] * co[j / 2] + v1[j] * si[j / 2];
-            o2[j] = v2[j] * co[4 + j / 2] - v2[j + 1] * si[4 + j / 2];
-            o2[j + 1] = v2[j + 1] * co[4 + j / 2] + v2[j] * si[4 + j / 2];
-          }
-        }
+    if (k0 + i * kGroups < a.hk) {  // some of the warp's heads are keys
+      float v1[8], v2[8], o1[8], o2[8];
+      qk_unpack<T>(x1[i], v1);
+      qk_unpack<T>(x2[i], v2);
+      const float inv = rsqrtf(qk_mean_square<D>(v1, v2) + a.eps);
+      if (h < a.hk) {
+        qk_turn<NEOX>(f, inv, v1, v2, o1, o2);
         r1 = qk_pack<T>(o1), r2 = qk_pack<T>(o2);
-      } else {
-        r1 = qk_pack<T>(v1), r2 = qk_pack<T>(v2);
+        if (a.dest == kDestRaw) {  // the raw cache holds them before the rotation
+          float w1[8], w2[8];
+          const T *w = static_cast<const T *>(a.kw);
+          qk_unpack<T>(*reinterpret_cast<const uint4 *>(w + e1), w1);
+          qk_unpack<T>(*reinterpret_cast<const uint4 *>(w + e2), w2);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v1[j] *= inv * w1[j], v2[j] *= inv * w2[j];
+          y1 = qk_pack<T>(v1), y2 = qk_pack<T>(v2);
+        }
       }
     }
-    const int64_t out_row = ((int64_t)t * a.hk + kh) * D;
-    T *out = is_q ? static_cast<T *>(a.q_out) + t * a.qo_stride + (int64_t)h * D
-             : value ? (a.v_out != nullptr ? static_cast<T *>(a.v_out) + out_row : nullptr)
-                     : (a.k_out != nullptr ? static_cast<T *>(a.k_out) + out_row : nullptr);
+    if (h >= 2 * a.hk) continue;
+    const bool is_key = h < a.hk;
+    const int kh = is_key ? h : h - a.hk;
+    T *out = static_cast<T *>(is_key ? a.k_out : a.v_out);
     if (out != nullptr) {
+      out += ((int64_t)t * a.hk + kh) * D;
       *reinterpret_cast<uint4 *>(out + e1) = r1;
       *reinterpret_cast<uint4 *>(out + e2) = r2;
     }
-    if (!is_q && row >= 0) {
-      T *dst = static_cast<T *>(value ? a.dst_v : a.dst_k) + (row * a.hk + kh) * D;
+    if (row >= 0) {
+      T *dst = static_cast<T *>(is_key ? a.dst_k : a.dst_v) + (row * a.hk + kh) * D;
       const bool raw = a.dest == kDestRaw;
       *reinterpret_cast<uint4 *>(dst + e1) = raw ? y1 : r1;
       *reinterpret_cast<uint4 *>(dst + e2) = raw ? y2 : r2;
@@ -288,12 +365,14 @@ bool whole_heads(const QkArgs &a, int cos_sin_dtype) {
 
 template <typename T, typename CS, int D> void launch_heads(const QkArgs &a, cudaStream_t st) {
   const int per = 32 / (D / 16) * kQkHeads;
-  const int64_t warps = (int64_t)a.tokens * ((a.hq + 2 * a.hk + per - 1) / per);
+  const int64_t chunks = (a.hq + per - 1) / per + (2 * a.hk + per - 1) / per;
+  const int64_t warps = (int64_t)a.tokens * chunks;
   const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
+  const int ahead = (int)(16L * sm_count() / chunks);  // two CTAs of 8 warps an SM
   if (a.neox)
-    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, true>, grid, block, 0, st, a);
+    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, true>, grid, block, 0, st, a, ahead);
   else
-    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, false>, grid, block, 0, st, a);
+    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, false>, grid, block, 0, st, a, ahead);
 }
 
 int launch(const QkArgs &a, int cos_sin_dtype, int dtype, cudaStream_t st) {
