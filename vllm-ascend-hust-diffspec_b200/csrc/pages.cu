@@ -14,9 +14,14 @@
 namespace dsb {
 namespace {
 
-constexpr int kPgThreads = 1024;
+constexpr int kPgThreads = 512;     // of the planning CTA
+constexpr int kPgPages = 8;         // pages a thread looks at in a turn (in a row)
 constexpr int kPgMaxRows = 4096;    // rows of one call
 constexpr int kPgMaxCaches = 128;   // caches of one launch
+// Rows x table columns up to which one CTA lets the pages go by itself; beyond
+// it a kernel over the GPU does first (524288 entries of 64 rows: 497 us by
+// one CTA; 8192 entries of 8 rows: one launch less is worth 2 us).
+constexpr int64_t kPgAlone = 16384;
 
 struct Pool {
   int32_t *refs;
@@ -34,30 +39,26 @@ struct Caches {
   int n;
 };
 
-// Inclusive prefix sum over the block's threads; `total` gets the sum.
+// Inclusive prefix sum over the planning CTA; `total` gets the sum.
 __device__ int block_scan(int v, int32_t *warp_tot, int &total) {
+  constexpr int kWarps = kPgThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
+    const int x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
   }
+  if (lane == 31) warp_tot[warp] = v;
   __syncthreads();
-  if (lane == 31) warp_tot[warp] = incl;
-  __syncthreads();
-  if (warp == 0) {
-    int w = warp_tot[lane];
+  int before = 0;
+  total = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += x;
-    }
-    warp_tot[lane] = w;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) before = total;
+    total += warp_tot[w];
   }
   __syncthreads();
-  total = warp_tot[31];
-  return incl + (warp > 0 ? warp_tot[warp - 1] : 0);
+  return before + v;
 }
 
 // a[0..n) in shared memory becomes its inclusive prefix sum.
@@ -76,22 +77,59 @@ __device__ int scan_rows(int32_t *a, int n, int32_t *warp_tot) {
 
 __device__ int free_pages(const Pool &p, int32_t *warp_tot) {
   int mine = 0, total;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < p.pages; i += kPgThreads) mine += __ldcg(p.refs + i) == 0;
   block_scan(mine, warp_tot, total);
   return total;
 }
 
-// Drop one reference to `page`; a page that nothing holds is flagged.
-__device__ __forceinline__ void release(const Pool &p, int page) {
+// Drop `n` references to `page`; more than there are is flagged.
+__device__ __forceinline__ void release(const Pool &p, int page, int n) {
   if (page < 0 || page >= p.pages) {
     flag_error(p.err, DSB_FLAG_BLOCK);
     return;
   }
-  if (atomicSub(p.refs + page, 1) <= 0) {
-    atomicAdd(p.refs + page, 1);
+  const int old = atomicSub(p.refs + page, n);
+  if (old < n) {
+    atomicAdd(p.refs + page, n - max(old, 0));
     flag_error(p.err, DSB_FLAG_BLOCK);
   }
 }
+
+// Changes of reference counts that a thread meets one after another, joined
+// while they name one of the last four pages: the rows of a call share most
+// of their pages, and an atomic a page is what they cost.
+struct PageCounts {
+  int page[4], n[4], next;
+  __device__ PageCounts() : next(0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) page[i] = -1, n[i] = 0;
+  }
+  template <typename F> __device__ void add(int x, F flush) {
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n[i] > 0 && page[i] == x) {
+        ++n[i];
+        found = true;
+        break;
+      }
+    if (found) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i == next) {
+        if (n[i] > 0) flush(page[i], n[i]);
+        page[i] = x;
+        n[i] = 1;
+      }
+    next = (next + 1) & 3;
+  }
+  template <typename F> __device__ void finish(F flush) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n[i] > 0) flush(page[i], n[i]);
+  }
+};
 
 // Hand the lowest free pages out: want[] is the inclusive prefix sum of the
 // rows' needs, `granted` the pages given in all; give(i, k, page) stores row
@@ -100,20 +138,28 @@ template <typename F>
 __device__ void allot(const Pool &p, const int32_t *want, int n, int granted, int32_t *warp_tot,
                       F give) {
   int run = 0;
-  for (int64_t base = 0; base < p.pages && run < granted; base += kPgThreads) {
-    const int64_t page = base + threadIdx.x;
-    const bool is_free = page < p.pages && __ldcg(p.refs + page) == 0;
-    int total;
-    const int rank = run + block_scan(is_free, warp_tot, total) - 1;
-    if (is_free && rank < granted) {
+  for (int64_t base = 0; base < p.pages && run < granted; base += kPgThreads * kPgPages) {
+    const int64_t first = base + (int64_t)threadIdx.x * kPgPages;
+    bool is_free[kPgPages];
+    int mine = 0, total;
+#pragma unroll
+    for (int j = 0; j < kPgPages; ++j) {
+      is_free[j] = first + j < p.pages && __ldcg(p.refs + first + j) == 0;
+      mine += is_free[j];
+    }
+    int rank = run + block_scan(mine, warp_tot, total) - mine;
+#pragma unroll
+    for (int j = 0; j < kPgPages; ++j) {
+      if (!is_free[j] || rank >= granted) continue;
       int lo = 0, hi = n - 1;  // first row whose prefix sum passes the rank
       while (lo < hi) {
         const int mid = (lo + hi) / 2;
         if (want[mid] > rank) hi = mid;
         else lo = mid + 1;
       }
-      p.refs[page] = 1;
-      give(lo, rank - (lo > 0 ? want[lo - 1] : 0), (int)page);
+      p.refs[first + j] = 1;
+      give(lo, rank - (lo > 0 ? want[lo - 1] : 0), (int)(first + j));
+      ++rank;
     }
     run += total;
   }
@@ -126,44 +172,93 @@ __device__ bool repeated(const int32_t *rows, int i) {
   return false;
 }
 
+// Pages of row r: those it has, and those `len` tokens need (-1: the table
+// cannot hold them).
+__device__ __forceinline__ int pages_held(const Pool &p, int r) {
+  return min(max(p.held[r], 0), (int)min(p.cols, (int64_t)INT32_MAX));
+}
+__device__ __forceinline__ int pages_needed(const Pool &p, int len) {
+  const int64_t need = ((int64_t)len + p.bs - 1) / p.bs;
+  return len < 0 || need > p.cols ? -1 : (int)need;
+}
+
+// The surplus pages of 16 rows of the call in 256 table columns: a thread has
+// a column, so that a warp reads a row's entries side by side.
+constexpr int kPgRows = 16;
+__global__ void __launch_bounds__(256)
+    release_kernel(const Pool p, const int32_t *__restrict__ rows, const int32_t *__restrict__ lens,
+                   int n) {
+  __shared__ int32_t s_row[kPgRows], s_keep[kPgRows], s_held[kPgRows];
+  pdl_begin();
+  const int i0 = blockIdx.y * kPgRows, m = min(kPgRows, n - i0);
+  if (threadIdx.x < kPgRows) {
+    int r = -1, keep = 0, held = 0;
+    if (threadIdx.x < m) {
+      r = rows[i0 + threadIdx.x];
+      if (r < 0 || r >= p.rows) r = -1;
+      if (r >= 0) {
+        held = pages_held(p, r);
+        keep = pages_needed(p, lens[i0 + threadIdx.x]);
+        if (keep < 0 || keep >= held) r = -1;  // nothing to let go
+      }
+    }
+    s_row[threadIdx.x] = r, s_keep[threadIdx.x] = keep, s_held[threadIdx.x] = held;
+  }
+  __syncthreads();
+  // a row named before in the call is not this one's to change
+  for (int j = threadIdx.x; j < i0 + m; j += 256) {
+    const int r = rows[j];
+#pragma unroll
+    for (int k = 0; k < kPgRows; ++k)
+      if (k < m && j < i0 + k && r == rows[i0 + k]) s_row[k] = -1;
+  }
+  __syncthreads();
+  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  auto flush = [&](int page, int count) { release(p, page, count); };
+  PageCounts counts;
+#pragma unroll 4
+  for (int k = 0; k < m; ++k) {
+    if (s_row[k] < 0 || j < s_keep[k] || j >= s_held[k]) continue;
+    int32_t *entry = p.tables + (int64_t)s_row[k] * p.stride + j;
+    counts.add(*entry, flush);
+    *entry = -1;
+  }
+  counts.finish(flush);
+}
+
 __global__ void __launch_bounds__(kPgThreads)
     resize_kernel(const Pool p, const int32_t *__restrict__ rows, const int32_t *__restrict__ lens,
-                  int n) {
+                  int n, int alone) {
   extern __shared__ int32_t pg_smem[];
   int32_t *want = pg_smem, *row = want + n, *has = row + n, *target = has + n;
   __shared__ int32_t warp_tot[32];
-  __shared__ int lacking;
+  __shared__ int lacking, granted;
   pdl_begin();
   const int tid = threadIdx.x;
-  if (tid == 0) lacking = 0;
+  if (tid == 0) lacking = granted = 0;
   for (int i = tid; i < n; i += kPgThreads) row[i] = rows[i];
   __syncthreads();
   for (int i = tid; i < n; i += kPgThreads) {
-    const int r = row[i], len = lens[i];
-    int have = 0, need = 0;
-    bool ok = true;
+    const int r = row[i];
+    int have = 0, need = -1;
     if (r < 0 || r >= p.rows || repeated(row, i)) {
-      ok = false;
       flag_error(p.err, DSB_FLAG_SLOT);
     } else {
-      have = min(max(p.held[r], 0), (int)min(p.cols, (int64_t)INT32_MAX));
-      need = len < 0 ? -1 : (int)(((int64_t)len + p.bs - 1) / p.bs);
-      if (need < 0 || need > p.cols) {
-        ok = false;
-        flag_error(p.err, DSB_FLAG_POSITION);
-      }
+      have = pages_held(p, r);
+      need = pages_needed(p, lens[i]);
+      if (need < 0) flag_error(p.err, DSB_FLAG_POSITION);
     }
     has[i] = have;
-    target[i] = ok ? need : -1;
-    want[i] = ok ? max(0, need - have) : 0;
+    target[i] = need;
+    want[i] = max(0, need - have);
   }
   __syncthreads();
-  // releases first: a warp a row
+  // releases first: a warp a row (or release_kernel's, before)
   for (int i = tid >> 5; i < n; i += kPgThreads / 32) {
     if (target[i] < 0 || target[i] >= has[i]) continue;
     int32_t *t = p.tables + (int64_t)row[i] * p.stride;
-    for (int j = target[i] + (tid & 31); j < has[i]; j += 32) {
-      release(p, t[j]);
+    for (int j = target[i] + (tid & 31); alone && j < has[i]; j += 32) {
+      release(p, t[j], 1);
       t[j] = -1;
     }
     if ((tid & 31) == 0) p.held[row[i]] = target[i];
@@ -171,9 +266,6 @@ __global__ void __launch_bounds__(kPgThreads)
   __syncthreads();
   const int nfree = free_pages(p, warp_tot);
   scan_rows(want, n, warp_tot);
-  __shared__ int granted;
-  if (tid == 0) granted = 0;
-  __syncthreads();
   // rows in order until the first that does not fit
   for (int i = tid; i < n; i += kPgThreads) {
     const int need = want[i] - (i > 0 ? want[i - 1] : 0);
@@ -263,34 +355,61 @@ __global__ void __launch_bounds__(kPgThreads)
   }
 }
 
-// blockIdx.y: child.  The first blocks along x rename its whole pages (each a
-// reference more), the others copy the started page's tokens of the caches.
+// `bytes` (a multiple of 16) from src to dst by a CTA of 256 threads, four
+// pieces of a thread on their way at once.
+__device__ __forceinline__ void copy_bytes(char *dst, const char *src, int64_t bytes) {
+  const int64_t n = bytes / 16;
+  const uint4 *from = reinterpret_cast<const uint4 *>(src);
+  uint4 *to = reinterpret_cast<uint4 *>(dst);
+  for (int64_t i = threadIdx.x; i < n; i += 4 * 256) {
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + 256 * j < n) v[j] = from[i + 256 * j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + 256 * j < n) to[i + 256 * j] = v[j];
+  }
+}
+
+// blockIdx.y: 16 children.  The first blocks along x name their whole pages (a
+// reference more for each), 256 table columns a block; the others copy the
+// started pages' tokens, a (child, cache) at a time.
 __global__ void __launch_bounds__(256)
-    fork_apply_kernel(const Pool p, const ForkPlan *__restrict__ plan, const Caches caches,
+    fork_apply_kernel(const Pool p, const ForkPlan *__restrict__ plan, int n, const Caches caches,
                       int64_t token_bytes, int table_blocks) {
+  __shared__ ForkPlan s_plan[kPgRows];
   pdl_begin();
-  const ForkPlan f = plan[blockIdx.y];
-  if (f.child < 0) return;
+  const int i0 = blockIdx.y * kPgRows, m = min(kPgRows, n - i0);
+  if (threadIdx.x < m) s_plan[threadIdx.x] = plan[i0 + threadIdx.x];
+  __syncthreads();
   if ((int)blockIdx.x < table_blocks) {
-    const int32_t *up = p.tables + (int64_t)f.parent * p.stride;
-    int32_t *to = p.tables + (int64_t)f.child * p.stride;
-    for (int j = blockIdx.x * 256 + threadIdx.x; j < f.full; j += table_blocks * 256) {
-      const int page = up[j];
-      to[j] = page;
+    auto flush = [&](int page, int count) {
       if (page >= 0 && page < p.pages)
-        atomicAdd(p.refs + page, 1);
+        atomicAdd(p.refs + page, count);
       else
         flag_error(p.err, DSB_FLAG_BLOCK);
+    };
+    for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < p.cols; j += table_blocks * 256) {
+      PageCounts counts;
+#pragma unroll 4
+      for (int k = 0; k < m; ++k) {
+        const ForkPlan &f = s_plan[k];
+        if (f.child < 0 || j >= f.full) continue;
+        const int page = p.tables[(int64_t)f.parent * p.stride + j];
+        p.tables[(int64_t)f.child * p.stride + j] = page;
+        counts.add(page, flush);
+      }
+      counts.finish(flush);
     }
     return;
   }
-  if (f.tokens <= 0) return;
-  const int64_t bytes = f.tokens * token_bytes, page_bytes = p.bs * token_bytes;
-  for (int c = blockIdx.x - table_blocks; c < caches.n; c += gridDim.x - table_blocks) {
-    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const char *>(caches.p[c]) +
-                                                       f.src * page_bytes);
-    uint4 *dst = reinterpret_cast<uint4 *>(static_cast<char *>(caches.p[c]) + f.dst * page_bytes);
-    for (int64_t i = threadIdx.x; i < bytes / 16; i += 256) dst[i] = src[i];
+  const int64_t page_bytes = p.bs * token_bytes;
+  for (int u = blockIdx.x - table_blocks; u < m * caches.n; u += gridDim.x - table_blocks) {
+    const ForkPlan &f = s_plan[u / caches.n];
+    if (f.child < 0 || f.tokens <= 0) continue;
+    char *base = static_cast<char *>(caches.p[u % caches.n]);
+    copy_bytes(base + f.dst * page_bytes, base + f.src * page_bytes, f.tokens * token_bytes);
   }
 }
 
@@ -304,21 +423,31 @@ __global__ void __launch_bounds__(kPgThreads)
   const int64_t live = p.pages - nfree;
   int32_t *src = scratch + 1, *dst = src + p.pages, *name = dst + p.pages;
   int holes = 0, moved = 0;
-  for (int64_t base = 0; base < p.pages; base += kPgThreads) {
-    const int64_t page = base + tid;
-    const bool in = page < p.pages;
-    const bool used = in && p.refs[page] != 0;
-    const bool hole = in && !used && page < live, move = used && page >= live;
-    int total;
-    const int h = holes + block_scan(hole, warp_tot, total) - 1;
-    holes += total;
-    const int m = moved + block_scan(move, warp_tot, total) - 1;
-    moved += total;
-    if (hole) dst[h] = (int)page;
-    if (move) src[m] = (int)page;
-    if (in && !used && page >= live) name[page] = -1;  // no row holds it
+  for (int64_t base = 0; base < p.pages; base += kPgThreads * kPgPages) {
+    const int64_t first = base + (int64_t)tid * kPgPages;
+    bool hole[kPgPages], move[kPgPages];
+    int mine = 0, total;  // holes, and pages to move, in 16 bits each
+#pragma unroll
+    for (int j = 0; j < kPgPages; ++j) {
+      const int64_t page = first + j;
+      const bool in = page < p.pages, used = in && p.refs[page] != 0;
+      hole[j] = in && !used && page < live;
+      move[j] = used && page >= live;
+      mine += (hole[j] ? 1 : 0) + (move[j] ? 1 << 16 : 0);
+      if (in && !used && page >= live) name[page] = -1;  // no row holds it
+    }
+    const int before = block_scan(mine, warp_tot, total) - mine;
+    int h = holes + (before & 0xffff), m = moved + (before >> 16);
+#pragma unroll
+    for (int j = 0; j < kPgPages; ++j) {
+      if (hole[j]) dst[h++] = (int)(first + j);
+      if (move[j]) src[m++] = (int)(first + j);
+    }
+    holes += total & 0xffff;
+    moved += total >> 16;
   }
   __syncthreads();
+#pragma unroll 4
   for (int k = tid; k < moved; k += kPgThreads) {
     const int s = src[k], t = dst[k];
     name[s] = t;
@@ -327,52 +456,63 @@ __global__ void __launch_bounds__(kPgThreads)
   }
   if (tid == 0) {
     scratch[0] = moved;
-    if (p.status != nullptr) {
-      p.status[0] = 0;
-      p.status[1] = nfree;
-    }
-  }
-}
-
-__global__ void __launch_bounds__(256)
-    rename_kernel(const Pool p, const int32_t *__restrict__ scratch) {
-  pdl_begin();
-  const int32_t *name = scratch + 1 + 2 * p.pages;
-  const int row = blockIdx.y;
-  const int held = min(max(p.held[row], 0), (int)min(p.cols, (int64_t)INT32_MAX));
-  int32_t *t = p.tables + (int64_t)row * p.stride;
-  // live pages are in front now: an entry that points behind them was moved
-  const int64_t live = p.pages - p.status[1];
-  for (int j = blockIdx.x * 256 + threadIdx.x; j < held; j += gridDim.x * 256) {
-    const int page = t[j];
-    if (page < 0 || page >= p.pages)
-      flag_error(p.err, DSB_FLAG_BLOCK);
-    else if (page >= live)
-      t[j] = name[page];
+    p.status[0] = 0;
+    p.status[1] = nfree;
   }
 }
 
 // Pages src[k] -> dst[k] of every cache, k < *count (or `n` when null);
-// negative entries are skipped, bad ones flagged.
-__global__ void __launch_bounds__(256)
-    copy_pages_kernel(const Caches caches, int64_t page_bytes, int64_t pages,
-                      const int32_t *__restrict__ src, const int32_t *__restrict__ dst,
-                      const int32_t *__restrict__ count, int n, int32_t *err) {
-  pdl_begin();
-  const int64_t total = (int64_t)(count != nullptr ? *count : n) * caches.n;
-  for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
+// negative entries are skipped, bad ones flagged.  A CTA takes one page of one
+// cache at a time.
+__device__ void copy_pairs(const Caches &caches, int64_t page_bytes, int64_t pages,
+                           const int32_t *__restrict__ src, const int32_t *__restrict__ dst,
+                           int64_t count, int32_t *err, int64_t first, int64_t step) {
+  for (int64_t u = first; u < count * caches.n; u += step) {
     const int64_t k = u / caches.n;
-    const int c = (int)(u % caches.n);
     const int s = src[k], t = dst[k];
     if (s < 0 || t < 0) continue;
     if (s >= pages || t >= pages) {
       if (threadIdx.x == 0) flag_error(err, DSB_FLAG_BLOCK);
       continue;
     }
-    const uint4 *from = reinterpret_cast<const uint4 *>(static_cast<const char *>(caches.p[c]) +
-                                                        s * page_bytes);
-    uint4 *to = reinterpret_cast<uint4 *>(static_cast<char *>(caches.p[c]) + t * page_bytes);
-    for (int64_t i = threadIdx.x; i < page_bytes / 16; i += 256) to[i] = from[i];
+    char *base = static_cast<char *>(caches.p[u % caches.n]);
+    copy_bytes(base + t * page_bytes, base + s * page_bytes, page_bytes);
+  }
+}
+
+__global__ void __launch_bounds__(256)
+    copy_pages_kernel(const Caches caches, int64_t page_bytes, int64_t pages,
+                      const int32_t *__restrict__ src, const int32_t *__restrict__ dst, int n,
+                      int32_t *err) {
+  pdl_begin();
+  copy_pairs(caches, page_bytes, pages, src, dst, n, err, blockIdx.x, gridDim.x);
+}
+
+// The first `rename_blocks` blocks name the moved pages' new places in the
+// rows' tables, the others move the pages.
+__global__ void __launch_bounds__(256)
+    compact_apply_kernel(const Pool p, const Caches caches, int64_t page_bytes,
+                         const int32_t *__restrict__ scratch, int rename_blocks) {
+  pdl_begin();
+  if ((int)blockIdx.x >= rename_blocks) {
+    copy_pairs(caches, page_bytes, p.pages, scratch + 1, scratch + 1 + p.pages, scratch[0], p.err,
+               blockIdx.x - rename_blocks, gridDim.x - rename_blocks);
+    return;
+  }
+  const int32_t *name = scratch + 1 + 2 * p.pages;
+  // live pages are in front now: an entry that points behind them was moved
+  const int64_t live = p.pages - p.status[1];
+  for (int64_t row = blockIdx.x; row < p.rows; row += rename_blocks) {
+    const int held = pages_held(p, (int)row);
+    int32_t *t = p.tables + row * p.stride;
+#pragma unroll 4
+    for (int j = threadIdx.x; j < held; j += 256) {
+      const int page = t[j];
+      if (page < 0 || page >= p.pages)
+        flag_error(p.err, DSB_FLAG_BLOCK);
+      else if (page >= live)
+        t[j] = name[page];
+    }
   }
 }
 
@@ -422,10 +562,18 @@ extern "C" int dsb_resize_requests(int32_t *ref_counts, int64_t num_pages, int32
                held,       block_size, status,      error_flag};
   if (int e = check_pool(p, n)) return e;
   if (n > 0 && (!rows || !lens)) return fail(DSB_ERR_INVALID, "null pointer argument");
+  const cudaStream_t st = as_stream(stream);
+  const bool alone = (int64_t)n * table_cols <= kPgAlone;
+  if (!alone) {
+    launch_kernel(release_kernel,
+                  dim3((unsigned)((table_cols + 255) / 256), (unsigned)((n + kPgRows - 1) / kPgRows)),
+                  dim3(256), 0, st, p, rows, lens, (int)n);
+    if (int e = check_launch("release_kernel")) return e;
+  }
   const size_t smem = (size_t)n * 4 * sizeof(int32_t);
   if (int e = ensure_smem((const void *)resize_kernel, smem)) return e;
-  launch_kernel(resize_kernel, dim3(1), dim3(kPgThreads), smem, as_stream(stream), p, rows, lens,
-                (int)n);
+  launch_kernel(resize_kernel, dim3(1), dim3(kPgThreads), smem, st, p, rows, lens, (int)n,
+                alone ? 1 : 0);
   return check_launch("resize_kernel");
 }
 
@@ -454,14 +602,14 @@ extern "C" int dsb_fork_requests(int32_t *ref_counts, int64_t num_pages, int32_t
                 (int)n, plan);
   if (int e = check_launch("fork_plan_kernel")) return e;
   if (n == 0) return DSB_OK;
-  const int table_blocks = (int)std::min<int64_t>(32, (table_cols + 255) / 256);
+  const int table_blocks = (int)std::min<int64_t>(64, (table_cols + 255) / 256);
+  const unsigned gy = (unsigned)((n + kPgRows - 1) / kPgRows);
   bool first = true;
   auto apply = [&](const Caches &part) {
     const int tb = first ? table_blocks : 0;  // the tables once
     first = false;
-    if (tb + part.n > 0)
-      launch_kernel(fork_apply_kernel, dim3(tb + part.n, n), dim3(256), 0, st, p,
-                    (const ForkPlan *)plan, part, token_bytes, tb);
+    launch_kernel(fork_apply_kernel, dim3(tb + std::min(kPgRows * part.n, 128), gy), dim3(256), 0, st,
+                  p, (const ForkPlan *)plan, (int)n, part, token_bytes, tb);
   };
   each_part(caches, num_caches, apply);
   if (num_caches == 0) apply(Caches{});
@@ -485,22 +633,21 @@ extern "C" int dsb_compact_pages(int32_t *ref_counts, int64_t num_pages, int32_t
   if (!status || !scratch) return fail(DSB_ERR_INVALID, "null pointer argument");
   if (scratch_ints < dsb_compact_scratch_ints(num_pages))
     return fail(DSB_ERR_INVALID, "scratch smaller than dsb_compact_scratch_ints");
-  if (table_rows > 65535) return fail(DSB_ERR_UNSUPPORTED, "grid too large");
   const cudaStream_t st = as_stream(stream);
   launch_kernel(compact_plan_kernel, dim3(1), dim3(kPgThreads), 0, st, p, scratch);
   if (int e = check_launch("compact_plan_kernel")) return e;
-  const unsigned gx = (unsigned)std::min<int64_t>(32, (table_cols + 255) / 256);
-  launch_kernel(rename_kernel, dim3(gx, (unsigned)table_rows), dim3(256), 0, st, p,
-                (const int32_t *)scratch);
-  if (int e = check_launch("rename_kernel")) return e;
-  each_part(caches, num_caches, [&](const Caches &part) {
+  bool first = true;
+  auto apply = [&](const Caches &part) {
+    const int rb = first ? (int)std::min<int64_t>(table_rows, 64) : 0;  // the tables once
+    first = false;
     const int64_t units = (num_pages / 2 + 1) * part.n;  // at most half of the pages move
-    launch_kernel(copy_pages_kernel, dim3((unsigned)std::min<int64_t>(units, 8L * sm_count())),
-                  dim3(256), 0, st, part, token_bytes * block_size, num_pages,
-                  (const int32_t *)(scratch + 1), (const int32_t *)(scratch + 1 + num_pages),
-                  (const int32_t *)scratch, 0, error_flag);
-  });
-  return check_launch("copy_pages_kernel");
+    const unsigned cb = (unsigned)std::min<int64_t>(units, 8L * sm_count());
+    launch_kernel(compact_apply_kernel, dim3(rb + cb), dim3(256), 0, st, p, part,
+                  token_bytes * block_size, (const int32_t *)scratch, rb);
+  };
+  each_part(caches, num_caches, apply);
+  if (num_caches == 0) apply(Caches{});
+  return check_launch("compact_apply_kernel");
 }
 
 extern "C" int dsb_copy_pages(void *const *caches, int32_t num_caches, int64_t num_pages,
@@ -514,8 +661,8 @@ extern "C" int dsb_copy_pages(void *const *caches, int32_t num_caches, int64_t n
   each_part(caches, num_caches, [&](const Caches &part) {
     const int64_t units = (int64_t)n * part.n;
     launch_kernel(copy_pages_kernel, dim3((unsigned)std::min<int64_t>(units, 8L * sm_count())),
-                  dim3(256), 0, as_stream(stream), part, page_bytes, num_pages, src, dst,
-                  (const int32_t *)nullptr, (int)n, error_flag);
+                  dim3(256), 0, as_stream(stream), part, page_bytes, num_pages, src, dst, (int)n,
+                  error_flag);
   });
   return check_launch("copy_pages_kernel");
 }
