@@ -9,13 +9,18 @@
 // call's result depends on its arguments alone.
 #include <algorithm>
 
-#include "common.cuh"
+#include "tma_umma.cuh"
 
 namespace dsb {
 namespace {
 
-constexpr int kPgThreads = 512;     // of the planning CTA
-constexpr int kPgPages = 8;         // pages a thread looks at in a turn (in a row)
+constexpr int kPgThreads = 512;     // of a planning CTA
+constexpr int kPgPages = 8;         // pages a thread looks at in a turn
+constexpr int kPgTurn = kPgThreads * kPgPages;
+// The planning CTAs are a cluster, each with a stretch of the pool: one for
+// pools of up to two turns, else eight (40000 pages, one CTA: 21 us to resize
+// and 28 to fork, most of it reading the counts; a cluster barrier is ~1 us).
+constexpr int kPgCluster = 8;
 constexpr int kPgMaxRows = 4096;    // rows of one call
 constexpr int kPgMaxCaches = 128;   // caches of one launch
 // Rows x table columns up to which one CTA lets the pages go by itself; beyond
@@ -39,26 +44,31 @@ struct Caches {
   int n;
 };
 
-// Inclusive prefix sum over the planning CTA; `total` gets the sum.
-__device__ int block_scan(int v, int32_t *warp_tot, int &total) {
+// Sum of the warps' values before this warp's; `total` gets the sum of all.
+__device__ int warps_before(int mine, int32_t *warp_tot, int &total) {
   constexpr int kWarps = kPgThreads / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += x;
-  }
-  if (lane == 31) warp_tot[warp] = v;
+  if ((threadIdx.x & 31) == 0) warp_tot[threadIdx.x >> 5] = mine;
   __syncthreads();
   int before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w == warp) before = total;
+    if (w == (int)(threadIdx.x >> 5)) before = total;
     total += warp_tot[w];
   }
   __syncthreads();
-  return before + v;
+  return before;
+}
+
+// Inclusive prefix sum over the CTA's threads.
+__device__ int block_scan(int v, int32_t *warp_tot, int &total) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return warps_before(__shfl_sync(0xffffffffu, v, 31), warp_tot, total) + v;
 }
 
 // a[0..n) in shared memory becomes its inclusive prefix sum.
@@ -75,10 +85,60 @@ __device__ int scan_rows(int32_t *a, int n, int32_t *warp_tot) {
   return run;
 }
 
-__device__ int free_pages(const Pool &p, int32_t *warp_tot) {
+// This CTA's stretch of the pool, and what the CTAs of the cluster tell each
+// other (every CTA of it calls these together).
+struct Stretch {
+  int64_t from, till;
+  int rank, ranks;
+  int32_t *told;  // [kPgCluster] in shared memory
+  __device__ Stretch(int64_t pages, int ranks_, int32_t *told_) : ranks(ranks_), told(told_) {
+    rank = ranks > 1 ? (int)cluster_rank() : 0;
+    const int64_t per = (pages + ranks - 1) / ranks;
+    from = min(pages, rank * per);
+    till = min(pages, from + per);
+  }
+  __device__ void sync() const {
+    __syncthreads();
+    if (ranks > 1) cluster_sync_all();
+  }
+  // Sum of `mine` over the CTAs, and over those before this one.
+  __device__ int gather(int mine, int &before) const {
+    if (ranks == 1) {
+      before = 0;
+      return mine;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < ranks)
+      st_cluster(cluster_map(smem_u32(told + rank), threadIdx.x), __int_as_float(mine));
+    cluster_sync_all();
+    int total = 0;
+    before = 0;
+    for (int r = 0; r < ranks; ++r) {
+      if (r == rank) before = total;
+      total += told[r];
+    }
+    cluster_sync_all();  // (the places are written again by the next gather)
+    return total;
+  }
+};
+
+// The CTA's stretch in turns of kPgTurn pages: look(page, count) for each page
+// of a thread, side by side in a warp (a warp has 256 pages in a row, a thread
+// every 32nd of them), with the loads of a turn all on their way at once.
+template <typename F> __device__ __forceinline__ void read_turn(const Pool &p, int64_t base, int64_t till, F look) {
+  int v[kPgPages];
+  const int64_t first = base + (int64_t)(threadIdx.x >> 5) * 32 * kPgPages + (threadIdx.x & 31);
+#pragma unroll
+  for (int j = 0; j < kPgPages; ++j) v[j] = first + 32 * j < till ? __ldcg(p.refs + first + 32 * j) : -1;
+#pragma unroll
+  for (int j = 0; j < kPgPages; ++j) look(j, first + 32 * j, v[j]);  // (behind `till`: -1)
+}
+
+// Free pages of the CTA's stretch.
+__device__ int free_pages(const Pool &p, const Stretch &s, int32_t *warp_tot) {
   int mine = 0, total;
-#pragma unroll 8
-  for (int64_t i = threadIdx.x; i < p.pages; i += kPgThreads) mine += __ldcg(p.refs + i) == 0;
+  for (int64_t base = s.from; base < s.till; base += kPgTurn)
+    read_turn(p, base, s.till, [&](int, int64_t, int v) { mine += v == 0; });
   block_scan(mine, warp_tot, total);
   return total;
 }
@@ -132,34 +192,34 @@ struct PageCounts {
 };
 
 // Hand the lowest free pages out: want[] is the inclusive prefix sum of the
-// rows' needs, `granted` the pages given in all; give(i, k, page) stores row
-// i's k-th new page.
+// rows' needs, `granted` the pages given in all, `run` the free pages before
+// this CTA's stretch; give(i, k, page) stores row i's k-th new page.
 template <typename F>
-__device__ void allot(const Pool &p, const int32_t *want, int n, int granted, int32_t *warp_tot,
-                      F give) {
-  int run = 0;
-  for (int64_t base = 0; base < p.pages && run < granted; base += kPgThreads * kPgPages) {
-    const int64_t first = base + (int64_t)threadIdx.x * kPgPages;
-    bool is_free[kPgPages];
+__device__ void allot(const Pool &p, const Stretch &s, const int32_t *want, int n, int granted, int run,
+                      int32_t *warp_tot, F give) {
+  const unsigned below = (1u << (threadIdx.x & 31)) - 1;
+  for (int64_t base = s.from; base < s.till && run < granted; base += kPgTurn) {
+    unsigned mask[kPgPages];
     int mine = 0, total;
+    read_turn(p, base, s.till, [&](int j, int64_t, int v) {
+      mask[j] = __ballot_sync(0xffffffffu, v == 0);
+      mine += __popc(mask[j]);
+    });
+    int rank = run + warps_before(mine, warp_tot, total);
+    const int64_t first = base + (int64_t)(threadIdx.x >> 5) * 32 * kPgPages + (threadIdx.x & 31);
 #pragma unroll
     for (int j = 0; j < kPgPages; ++j) {
-      is_free[j] = first + j < p.pages && __ldcg(p.refs + first + j) == 0;
-      mine += is_free[j];
-    }
-    int rank = run + block_scan(mine, warp_tot, total) - mine;
-#pragma unroll
-    for (int j = 0; j < kPgPages; ++j) {
-      if (!is_free[j] || rank >= granted) continue;
+      const int k = rank + __popc(mask[j] & below);
+      rank += __popc(mask[j]);
+      if (!(mask[j] >> (threadIdx.x & 31) & 1) || k >= granted) continue;
       int lo = 0, hi = n - 1;  // first row whose prefix sum passes the rank
       while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (want[mid] > rank) hi = mid;
+        if (want[mid] > k) hi = mid;
         else lo = mid + 1;
       }
-      p.refs[first + j] = 1;
-      give(lo, rank - (lo > 0 ? want[lo - 1] : 0), (int)(first + j));
-      ++rank;
+      p.refs[first + 32 * j] = 1;
+      give(lo, k - (lo > 0 ? want[lo - 1] : 0), (int)(first + 32 * j));
     }
     run += total;
   }
@@ -226,14 +286,17 @@ __global__ void __launch_bounds__(256)
   counts.finish(flush);
 }
 
+// Every CTA of the cluster has the rows' needs; the first one changes what
+// they hold and reports.
 __global__ void __launch_bounds__(kPgThreads)
     resize_kernel(const Pool p, const int32_t *__restrict__ rows, const int32_t *__restrict__ lens,
-                  int n, int alone) {
+                  int n, int alone, int ranks) {
   extern __shared__ int32_t pg_smem[];
   int32_t *want = pg_smem, *row = want + n, *has = row + n, *target = has + n;
-  __shared__ int32_t warp_tot[32];
+  __shared__ int32_t warp_tot[kPgThreads / 32], told[kPgCluster];
   __shared__ int lacking, granted;
   pdl_begin();
+  const Stretch s(p.pages, ranks, told);
   const int tid = threadIdx.x;
   if (tid == 0) lacking = granted = 0;
   for (int i = tid; i < n; i += kPgThreads) row[i] = rows[i];
@@ -242,49 +305,52 @@ __global__ void __launch_bounds__(kPgThreads)
     const int r = row[i];
     int have = 0, need = -1;
     if (r < 0 || r >= p.rows || repeated(row, i)) {
-      flag_error(p.err, DSB_FLAG_SLOT);
+      if (s.rank == 0) flag_error(p.err, DSB_FLAG_SLOT);
     } else {
       have = pages_held(p, r);
       need = pages_needed(p, lens[i]);
-      if (need < 0) flag_error(p.err, DSB_FLAG_POSITION);
+      if (need < 0 && s.rank == 0) flag_error(p.err, DSB_FLAG_POSITION);
     }
     has[i] = have;
     target[i] = need;
     want[i] = max(0, need - have);
   }
   __syncthreads();
-  // releases first: a warp a row (or release_kernel's, before)
-  for (int i = tid >> 5; i < n; i += kPgThreads / 32) {
-    if (target[i] < 0 || target[i] >= has[i]) continue;
-    int32_t *t = p.tables + (int64_t)row[i] * p.stride;
-    for (int j = target[i] + (tid & 31); alone && j < has[i]; j += 32) {
-      release(p, t[j], 1);
-      t[j] = -1;
+  // releases first, a warp a row (unless release_kernel has let them go)
+  if (alone) {
+    for (int i = tid >> 5; i < n && s.rank == 0; i += kPgThreads / 32) {
+      if (target[i] < 0) continue;
+      int32_t *t = p.tables + (int64_t)row[i] * p.stride;
+      for (int j = target[i] + (tid & 31); j < has[i]; j += 32) {
+        release(p, t[j], 1);
+        t[j] = -1;
+      }
     }
-    if ((tid & 31) == 0) p.held[row[i]] = target[i];
+    s.sync();
   }
-  __syncthreads();
-  const int nfree = free_pages(p, warp_tot);
+  int before;
+  const int nfree = s.gather(free_pages(p, s, warp_tot), before);
   scan_rows(want, n, warp_tot);
   // rows in order until the first that does not fit
   for (int i = tid; i < n; i += kPgThreads) {
     const int need = want[i] - (i > 0 ? want[i - 1] : 0);
-    if (need == 0) continue;
     if (want[i] <= nfree) {
-      atomicMax(&granted, want[i]);
-      p.held[row[i]] = target[i];
-    } else {
+      if (need > 0) atomicMax(&granted, want[i]);
+    } else if (need > 0) {
       atomicAdd(&lacking, 1);
+      continue;
     }
+    if (s.rank == 0 && target[i] >= 0) p.held[row[i]] = target[i];
   }
   __syncthreads();
-  allot(p, want, n, granted, warp_tot, [&](int i, int k, int page) {
+  allot(p, s, want, n, granted, before, warp_tot, [&](int i, int k, int page) {
     p.tables[(int64_t)row[i] * p.stride + has[i] + k] = page;
   });
-  if (tid == 0 && p.status != nullptr) {
+  if (tid == 0 && s.rank == 0 && p.status != nullptr) {
     p.status[0] = lacking;
     p.status[1] = nfree - granted;
   }
+  s.sync();  // (held has been read by every CTA before one of them ends)
 }
 
 // Per child: parent row, child row (-1: not forked), whole pages, the started
@@ -293,27 +359,31 @@ struct ForkPlan {
   int32_t parent, child, full, src, dst, tokens;
 };
 
+// As in resize_kernel, every CTA has the children's needs, the first one
+// writes the plan.
 __global__ void __launch_bounds__(kPgThreads)
     fork_plan_kernel(const Pool p, const int32_t *__restrict__ parents,
                      const int32_t *__restrict__ children, const int32_t *__restrict__ lens, int n,
-                     ForkPlan *__restrict__ plan) {
+                     ForkPlan *__restrict__ plan, int ranks) {
   extern __shared__ int32_t pg_smem[];
-  int32_t *want = pg_smem, *kid = want + n;
-  __shared__ int32_t warp_tot[32];
+  int32_t *want = pg_smem, *kid = want + n, *full = kid + n;  // full: -1 not forked
+  __shared__ int32_t warp_tot[kPgThreads / 32], told[kPgCluster];
   __shared__ int lacking, granted;
   pdl_begin();
+  const Stretch s(p.pages, ranks, told);
   const int tid = threadIdx.x;
   if (tid == 0) lacking = granted = 0;
   for (int i = tid; i < n; i += kPgThreads) kid[i] = children[i];
   __syncthreads();
   for (int i = tid; i < n; i += kPgThreads) {
     const int up = parents[i], c = kid[i], len = lens[i];
-    ForkPlan f{up, -1, 0, -1, -1, 0};
+    ForkPlan f{up, -1, -1, -1, -1, 0};
+    int flag = 0;
     if (up < 0 || up >= p.rows || c < 0 || c >= p.rows || repeated(kid, i) || p.held[c] != 0) {
-      flag_error(p.err, DSB_FLAG_SLOT);
+      flag = DSB_FLAG_SLOT;
     } else if (len < 0 || (int64_t)len > (int64_t)p.held[up] * p.bs ||
                (int64_t)len > p.cols * p.bs) {
-      flag_error(p.err, DSB_FLAG_POSITION);
+      flag = DSB_FLAG_POSITION;
     } else {
       f.child = c;
       f.full = len / p.bs;
@@ -321,38 +391,43 @@ __global__ void __launch_bounds__(kPgThreads)
       if (f.tokens > 0) {
         f.src = p.tables[(int64_t)up * p.stride + f.full];
         if (f.src < 0 || f.src >= p.pages) {
-          flag_error(p.err, DSB_FLAG_BLOCK);
-          f.child = -1;
+          flag = DSB_FLAG_BLOCK;
+          f.child = f.full = -1;
           f.tokens = 0;
         }
       }
     }
     want[i] = f.tokens > 0;
-    plan[i] = f;
-  }
-  __syncthreads();
-  const int nfree = free_pages(p, warp_tot);
-  scan_rows(want, n, warp_tot);
-  for (int i = tid; i < n; i += kPgThreads) {
-    ForkPlan &f = plan[i];
-    if (f.tokens > 0 && want[i] > nfree) {  // no page for it: not forked
-      atomicAdd(&lacking, 1);
-      f.child = -1;
-      f.tokens = 0;
-    } else if (f.child >= 0) {
-      if (f.tokens > 0) atomicMax(&granted, want[i]);
-      p.held[f.child] = f.full + (f.tokens > 0);
+    full[i] = f.full;
+    if (s.rank == 0) {
+      plan[i] = f;
+      if (flag != 0) flag_error(p.err, flag);
     }
   }
   __syncthreads();
-  allot(p, want, n, granted, warp_tot, [&](int i, int, int page) {
+  int before;
+  const int nfree = s.gather(free_pages(p, s, warp_tot), before);
+  scan_rows(want, n, warp_tot);
+  for (int i = tid; i < n; i += kPgThreads) {
+    const bool started = want[i] > (i > 0 ? want[i - 1] : 0);
+    if (started && want[i] > nfree) {  // no page for it: not forked
+      atomicAdd(&lacking, 1);
+      if (s.rank == 0) plan[i].child = -1;
+    } else if (full[i] >= 0) {
+      if (started) atomicMax(&granted, want[i]);
+      if (s.rank == 0) p.held[kid[i]] = full[i] + (started ? 1 : 0);
+    }
+  }
+  __syncthreads();
+  allot(p, s, want, n, granted, before, warp_tot, [&](int i, int, int page) {
     plan[i].dst = page;
-    p.tables[(int64_t)kid[i] * p.stride + plan[i].full] = page;
+    p.tables[(int64_t)kid[i] * p.stride + full[i]] = page;
   });
-  if (tid == 0 && p.status != nullptr) {
+  if (tid == 0 && s.rank == 0 && p.status != nullptr) {
     p.status[0] = lacking;
     p.status[1] = nfree - granted;
   }
+  s.sync();
 }
 
 // `bytes` (a multiple of 16) from src to dst by a CTA of 256 threads, four
@@ -415,46 +490,61 @@ __global__ void __launch_bounds__(256)
 
 // scratch: [0] pages to move, then sources[N], targets[N], new names[N]
 __global__ void __launch_bounds__(kPgThreads)
-    compact_plan_kernel(const Pool p, int32_t *__restrict__ scratch) {
-  __shared__ int32_t warp_tot[32];
+    compact_plan_kernel(const Pool p, int32_t *__restrict__ scratch, int ranks) {
+  __shared__ int32_t warp_tot[kPgThreads / 32], told[kPgCluster];
   pdl_begin();
+  const Stretch s(p.pages, ranks, told);
   const int tid = threadIdx.x;
-  const int nfree = free_pages(p, warp_tot);
+  const unsigned below = (1u << (tid & 31)) - 1;
+  int before;
+  const int nfree = s.gather(free_pages(p, s, warp_tot), before);
   const int64_t live = p.pages - nfree;
   int32_t *src = scratch + 1, *dst = src + p.pages, *name = dst + p.pages;
-  int holes = 0, moved = 0;
-  for (int64_t base = 0; base < p.pages; base += kPgThreads * kPgPages) {
-    const int64_t first = base + (int64_t)tid * kPgPages;
-    bool hole[kPgPages], move[kPgPages];
+  // Holes are the free pages below `live`: before this stretch as many as
+  // pages free before it, or all of them; pages to move likewise.
+  int holes, moved;
+  {
+    int h = 0, total;  // free pages of the stretch below `live`
+    for (int64_t base = s.from; base < min(s.till, live); base += kPgTurn)
+      read_turn(p, base, min(s.till, live), [&](int, int64_t, int v) { h += v == 0; });
+    block_scan(h, warp_tot, total);
+    moved = s.gather(total, holes);  // as many pages move as there are holes
+  }
+  // live pages at or behind `live` and before this stretch: those before the
+  // stretch less those before `live`
+  int at = s.from <= live ? 0 : (int)(s.from - before) - (int)(live - moved);
+  int hole_at = holes;
+  for (int64_t base = s.from; base < s.till; base += kPgTurn) {
+    unsigned hm[kPgPages], mm[kPgPages];
     int mine = 0, total;  // holes, and pages to move, in 16 bits each
+    read_turn(p, base, s.till, [&](int j, int64_t page, int v) {
+      hm[j] = __ballot_sync(0xffffffffu, v == 0 && page < live);
+      mm[j] = __ballot_sync(0xffffffffu, v != 0 && page >= live && page < s.till);
+      mine += __popc(hm[j]) + (__popc(mm[j]) << 16);
+      if (v == 0 && page >= live) name[page] = -1;  // no row holds it
+    });
+    const int b = warps_before(mine, warp_tot, total);
+    int h = hole_at + (b & 0xffff), m = at + (b >> 16);
+    const int64_t page0 = base + (int64_t)(tid >> 5) * 32 * kPgPages + (tid & 31);
 #pragma unroll
     for (int j = 0; j < kPgPages; ++j) {
-      const int64_t page = first + j;
-      const bool in = page < p.pages, used = in && p.refs[page] != 0;
-      hole[j] = in && !used && page < live;
-      move[j] = used && page >= live;
-      mine += (hole[j] ? 1 : 0) + (move[j] ? 1 << 16 : 0);
-      if (in && !used && page >= live) name[page] = -1;  // no row holds it
+      if (hm[j] >> (tid & 31) & 1) dst[h + __popc(hm[j] & below)] = (int)(page0 + 32 * j);
+      if (mm[j] >> (tid & 31) & 1) src[m + __popc(mm[j] & below)] = (int)(page0 + 32 * j);
+      h += __popc(hm[j]);
+      m += __popc(mm[j]);
     }
-    const int before = block_scan(mine, warp_tot, total) - mine;
-    int h = holes + (before & 0xffff), m = moved + (before >> 16);
-#pragma unroll
-    for (int j = 0; j < kPgPages; ++j) {
-      if (hole[j]) dst[h++] = (int)(first + j);
-      if (move[j]) src[m++] = (int)(first + j);
-    }
-    holes += total & 0xffff;
-    moved += total >> 16;
+    hole_at += total & 0xffff;
+    at += total >> 16;
   }
-  __syncthreads();
+  s.sync();
 #pragma unroll 4
-  for (int k = tid; k < moved; k += kPgThreads) {
-    const int s = src[k], t = dst[k];
-    name[s] = t;
-    p.refs[t] = p.refs[s];
-    p.refs[s] = 0;
+  for (int k = s.rank * kPgThreads + tid; k < moved; k += ranks * kPgThreads) {
+    const int a = __ldcg(src + k), t = __ldcg(dst + k);
+    name[a] = t;
+    p.refs[t] = p.refs[a];
+    p.refs[a] = 0;
   }
-  if (tid == 0) {
+  if (tid == 0 && s.rank == 0) {
     scratch[0] = moved;
     p.status[0] = 0;
     p.status[1] = nfree;
@@ -516,6 +606,8 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+int planners(int64_t pages) { return pages <= 2 * kPgTurn ? 1 : kPgCluster; }
+
 int check_pool(const Pool &p, int n) {
   if (p.pages <= 0 || p.pages > INT32_MAX || p.rows <= 0 || p.rows > INT32_MAX || p.cols <= 0 ||
       p.stride < p.cols)
@@ -572,8 +664,9 @@ extern "C" int dsb_resize_requests(int32_t *ref_counts, int64_t num_pages, int32
   }
   const size_t smem = (size_t)n * 4 * sizeof(int32_t);
   if (int e = ensure_smem((const void *)resize_kernel, smem)) return e;
-  launch_kernel(resize_kernel, dim3(1), dim3(kPgThreads), smem, st, p, rows, lens, (int)n,
-                alone ? 1 : 0);
+  const int ranks = planners(num_pages);
+  launch_kernel_cluster(resize_kernel, dim3(ranks), dim3(kPgThreads), smem, st, ranks, p, rows, lens,
+                        (int)n, alone ? 1 : 0, ranks);
   return check_launch("resize_kernel");
 }
 
@@ -596,10 +689,11 @@ extern "C" int dsb_fork_requests(int32_t *ref_counts, int64_t num_pages, int32_t
     return fail(DSB_ERR_INVALID, "scratch smaller than dsb_fork_scratch_ints");
   const cudaStream_t st = as_stream(stream);
   ForkPlan *plan = reinterpret_cast<ForkPlan *>(scratch);
-  const size_t smem = (size_t)n * 2 * sizeof(int32_t);
+  const size_t smem = (size_t)n * 3 * sizeof(int32_t);
   if (int e = ensure_smem((const void *)fork_plan_kernel, smem)) return e;
-  launch_kernel(fork_plan_kernel, dim3(1), dim3(kPgThreads), smem, st, p, parents, children, lens,
-                (int)n, plan);
+  const int ranks = planners(num_pages);
+  launch_kernel_cluster(fork_plan_kernel, dim3(ranks), dim3(kPgThreads), smem, st, ranks, p, parents,
+                        children, lens, (int)n, plan, ranks);
   if (int e = check_launch("fork_plan_kernel")) return e;
   if (n == 0) return DSB_OK;
   const int table_blocks = (int)std::min<int64_t>(64, (table_cols + 255) / 256);
@@ -634,7 +728,9 @@ extern "C" int dsb_compact_pages(int32_t *ref_counts, int64_t num_pages, int32_t
   if (scratch_ints < dsb_compact_scratch_ints(num_pages))
     return fail(DSB_ERR_INVALID, "scratch smaller than dsb_compact_scratch_ints");
   const cudaStream_t st = as_stream(stream);
-  launch_kernel(compact_plan_kernel, dim3(1), dim3(kPgThreads), 0, st, p, scratch);
+  const int ranks = planners(num_pages);
+  launch_kernel_cluster(compact_plan_kernel, dim3(ranks), dim3(kPgThreads), 0, st, ranks, p, scratch,
+                        ranks);
   if (int e = check_launch("compact_plan_kernel")) return e;
   bool first = true;
   auto apply = [&](const Caches &part) {
