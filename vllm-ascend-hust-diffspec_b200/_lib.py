@@ -268,11 +268,14 @@ def call(name: str, *args) -> None:
 def call_on(device: torch.device, name: str, *args) -> None:
     """:func:`call` with ``device`` current (the kernels of tensors on another
     device than the current one)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        check(getattr(load(), name)(*args), name)
-        return
-    with torch.cuda.device(device):
-        check(getattr(load(), name)(*args), name)
+    fn = getattr(_lib or load(), name)
+    if device.index == torch.cuda.current_device():
+        status = fn(*args)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args)
+    if status != DSB_OK:
+        check(status, name)
 
 
 _error_flags: dict[int, torch.Tensor] = {}
@@ -307,6 +310,29 @@ def sm_count(device: torch.device) -> int:
         n = torch.cuda.get_device_properties(idx).multi_processor_count
         _sm_counts[idx] = n
     return n
+
+
+_devices: dict[int, torch.device] = {}
+
+
+def device_of(*tensors: torch.Tensor | None) -> torch.device:
+    """:func:`require_cuda` by device numbers alone (a few tens of ns a tensor)."""
+    index = -1
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if i < 0:
+                raise ValueError("DiffSpec B200 ops need CUDA tensors (there is no CPU path)")
+            if i != index:
+                if index >= 0:
+                    raise ValueError("all tensors must share one CUDA device")
+                index = i
+    device = _devices.get(index)
+    if device is None:
+        if index < 0:
+            raise ValueError("no tensor arguments")
+        device = _devices.setdefault(index, torch.device("cuda", index))
+    return device
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:

@@ -267,43 +267,44 @@ def qk_norm_rope(query: torch.Tensor, kv: torch.Tensor, positions: torch.Tensor,
     :func:`kernels.qkv_projection_write_raw` writes for keys without a norm.
     A position outside the table is flagged and leaves the rows normed but
     unrotated.  Returns ``(query_out, key_out, value_out)``."""
-    d, rot, query_out, q_weight, k_weight = _qk_norm_inputs(
+    d, rot, query_out, q_weight, k_weight, head, value = _qk_norm_inputs(
         query, kv, positions, cos_sin, num_kv_heads, q_weight, k_weight, rotary_dim, query_out)
-    tokens, hk = query.shape[0], num_kv_heads
-    raw_key, raw_value, slots, abs_positions = (None,) * 4 if raw is None else raw
-    num_slots = max_len = 0
-    if raw is not None:
-        if raw_key.ndim != 4 or raw_key.shape != raw_value.shape or raw_key.shape[2:] != (hk, d):
+    tokens, dtype = query.shape[0], query.dtype
+    shape = (tokens, num_kv_heads, d)
+    if raw is None:
+        raw_key = raw_value = slots = abs_positions = None
+        places = (None, None, None, None, 0, 0)
+    else:
+        raw_key, raw_value, slots, abs_positions = raw
+        raw_shape = raw_key.shape
+        if raw_key.ndim != 4 or raw_shape != raw_value.shape or raw_shape[2:] != shape[1:]:
             raise ValueError("raw key/value must have matching [S, max_model_len, Hk, D] shapes")
-        if not (raw_key.dtype == raw_value.dtype == kv.dtype):
+        if raw_key.dtype is not dtype or raw_value.dtype is not dtype:
             raise ValueError("raw caches must have the keys' dtype")
         if not (raw_key.is_contiguous() and raw_value.is_contiguous()):
             raise ValueError("raw caches must be contiguous")
-        if slots.dtype != torch.int32 or abs_positions.dtype != torch.int64:
+        if slots.dtype is not torch.int32 or abs_positions.dtype is not torch.int64:
             raise ValueError("slots must be int32 and positions int64")
         if slots.numel() < tokens or abs_positions.numel() < tokens or not (
                 slots.is_contiguous() and abs_positions.is_contiguous()):
             raise ValueError("slots/positions must cover every token, contiguously")
-        num_slots, max_len = raw_key.shape[:2]
-    device = _lib.require_cuda(query, kv, positions, cos_sin, q_weight, k_weight, query_out, key_out,
-                               value_out, raw_key, raw_value, slots, abs_positions)
-    shape = (tokens, hk, d)
+        places = (raw_key.data_ptr(), raw_value.data_ptr(), slots.data_ptr(),
+                  abs_positions.data_ptr(), raw_shape[0], raw_shape[1])
+    device = _lib.device_of(query, kv, positions, cos_sin, q_weight, k_weight, query_out, key_out,
+                            value_out, raw_key, raw_value, slots, abs_positions)
     for name, t in (("key_out", key_out), ("value_out", value_out)):
-        if t is not None and (t.shape != shape or t.dtype != kv.dtype or not t.is_contiguous()):
+        if t is not None and (t.shape != shape or t.dtype is not dtype or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous [T, Hk, D] in the kv dtype")
     if key_out is None:
-        key_out = torch.empty(shape, dtype=kv.dtype, device=device)
+        key_out = kv.new_empty(shape)
     if value_out is None:
-        value_out = torch.empty(shape, dtype=kv.dtype, device=device)
+        value_out = kv.new_empty(shape)
     _lib.call_on(
-        device, "dsb_qk_norm_rope", _lib.ptr(query), query.stride(0), _lib.ptr(query_out),
-        query_out.stride(0), query.shape[1] // d, _lib.ptr(kv), kv.stride(0), _lib.ptr(key_out),
-        kv.data_ptr() + hk * d * kv.element_size(), kv.stride(0), _lib.ptr(value_out), hk, d, rot,
-        int(bool(is_neox_style)), _lib.ptr(q_weight), _lib.ptr(k_weight),
-        float(eps), _lib.ptr(positions), int(position_offset), tokens, _lib.ptr(cos_sin),
-        cos_sin.stride(0), cos_sin.shape[0], _lib.dtype_code(cos_sin.dtype),
-        _lib.dtype_code(kv.dtype), _lib.ptr(raw_key), _lib.ptr(raw_value), _lib.ptr(slots),
-        _lib.ptr(abs_positions), num_slots, max_len, _lib.ptr(_lib.error_flag(device)),
+        device, "dsb_qk_norm_rope", *head, key_out.data_ptr(), value, head[-1],
+        value_out.data_ptr(), num_kv_heads, d, rot, 1 if is_neox_style else 0, q_weight.data_ptr(),
+        k_weight.data_ptr(), eps, positions.data_ptr(), position_offset, tokens,
+        cos_sin.data_ptr(), cos_sin.stride(0), cos_sin.shape[0], _lib.dtype_code(cos_sin.dtype),
+        _lib.dtype_code(dtype), *places, _lib.error_flag(device).data_ptr(),
         _lib.stream_ptr(device))
     return query_out, key_out, value_out
 

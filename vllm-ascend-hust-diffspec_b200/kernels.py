@@ -7,6 +7,8 @@ work runs in hand-written sm_100a kernels behind ``libdiffspec_b200.so``.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -613,34 +615,37 @@ def shared_prefix_attention_lse(
     ``(out [rows, Hq, 128], lse [rows, Hq] fp32)``."""
     if query.ndim != 3 or key_cache.ndim != 4 or key_cache.shape != value_cache.shape:
         raise ValueError("query must be [rows, Hq, D] and the caches matching [blocks, bs, Hk, D]")
-    rows, hq, d = query.shape
+    rows, hq, d = shape = query.shape
     num_blocks, block_size, hk, kd = key_cache.shape
+    dtype = query.dtype
     if d != kd or hq % hk:
         raise ValueError("head dims must match and Hq must be a multiple of Hk")
-    if not (query.dtype == key_cache.dtype == value_cache.dtype):
+    if key_cache.dtype is not dtype or value_cache.dtype is not dtype:
         raise ValueError("query and caches must share a dtype")
     if block_table.ndim != 2 or seq_lens.numel() < rows:
         raise ValueError("block_table must be 2-D and seq_lens cover every row")
-    if table_rows is None and block_table.shape[0] < rows:
-        raise ValueError("block_table must have one row per query row without table_rows")
-    if table_rows is not None and table_rows.numel() < rows:
+    if table_rows is None:
+        if block_table.shape[0] < rows:
+            raise ValueError("block_table must have one row per query row without table_rows")
+    elif table_rows.numel() < rows:
         raise ValueError("table_rows must map every query row")
     groups = prefix_lens.numel()
-    if group_starts is None and groups != 1:
-        raise ValueError("prefix_lens must have one entry without group_starts")
-    if group_starts is not None and group_starts.numel() != groups + 1:
+    if group_starts is None:
+        if groups != 1:
+            raise ValueError("prefix_lens must have one entry without group_starts")
+    elif group_starts.numel() != groups + 1:
         raise ValueError("group_starts must have one entry more than prefix_lens")
     if max_prefix_len < 0 or max_suffix_len < 0:
         raise ValueError("max_prefix_len and max_suffix_len must be >= 0")
-    device = _lib.require_cuda(query, key_cache, value_cache, block_table, seq_lens, prefix_lens,
-                               group_starts, table_rows, out, lse)
+    device = _lib.device_of(query, key_cache, value_cache, block_table, seq_lens, prefix_lens,
+                            group_starts, table_rows, out, lse)
     if out is None:
-        out = torch.empty((rows, hq, d), dtype=query.dtype, device=device)
-    elif out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
+        out = query.new_empty(shape)
+    elif out.shape != shape or out.dtype is not dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous and shaped like query")
     if lse is None:
-        lse = torch.empty((rows, hq), dtype=torch.float32, device=device)
-    elif lse.shape != (rows, hq) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        lse = query.new_empty((rows, hq), dtype=torch.float32)
+    elif lse.shape != (rows, hq) or lse.dtype is not torch.float32 or not lse.is_contiguous():
         raise ValueError("lse must be contiguous fp32 [rows, Hq]")
     if rows == 0:
         return out, lse
@@ -654,52 +659,68 @@ def shared_prefix_attention_lse(
     prefix = _prep_index(prefix_lens).contiguous()
     starts = None if group_starts is None else _prep_index(group_starts).contiguous()
     trows = None if table_rows is None else _prep_index(table_rows).contiguous()
-    sizes = (int(max_prefix_len), int(max_suffix_len))
-    floats = _lib.load().dsb_shared_prefix_scratch_floats(rows, hq, hk, groups, block_size, *sizes)
-    scratch = torch.empty(max(floats, 1), dtype=torch.float32, device=device)
+    table_shape = table.shape
+    floats = _shared_prefix_floats(rows, hq, hk, groups, block_size, max_prefix_len, max_suffix_len)
+    scratch = lse.new_empty(floats)
     _lib.call_on(
         device, "dsb_shared_prefix_attention_lse",
-        _lib.ptr(query), rows, hq, hk, d, _lib.ptr(key_cache), _lib.ptr(value_cache), num_blocks,
-        block_size, _lib.ptr(table), table.stride(0), table.shape[0], table.shape[1],
-        _lib.ptr(seq), _lib.ptr(trows), _lib.ptr(prefix), _lib.ptr(starts), groups, *sizes,
-        float(scale), _lib.dtype_code(query.dtype), _lib.ptr(out), _lib.ptr(lse),
-        _lib.ptr(scratch), scratch.numel(), _lib.ptr(_lib.error_flag(device)),
-        _lib.stream_ptr(device),
+        query.data_ptr(), rows, hq, hk, d, key_cache.data_ptr(), value_cache.data_ptr(), num_blocks,
+        block_size, table.data_ptr(), table.stride(0), table_shape[0], table_shape[1],
+        seq.data_ptr(), None if trows is None else trows.data_ptr(), prefix.data_ptr(),
+        None if starts is None else starts.data_ptr(), groups, max_prefix_len, max_suffix_len, scale,
+        _lib.dtype_code(dtype), out.data_ptr(), lse.data_ptr(), scratch.data_ptr(), floats,
+        _lib.error_flag(device).data_ptr(), _lib.stream_ptr(device),
     )
     return out, lse
+
+
+@functools.lru_cache(maxsize=256)
+def _shared_prefix_floats(*sizes: int) -> int:
+    """dsb_shared_prefix_scratch_floats, at least 1."""
+    return max(_lib.load().dsb_shared_prefix_scratch_floats(*sizes), 1)
 
 
 def _qk_norm_inputs(query, kv, positions, cos_sin, num_kv_heads, q_weight, k_weight, rotary_dim,
                     query_out):
     """What the two query/key norm calls check alike; returns head_dim,
-    rotary_dim, query_out and the contiguous weights."""
-    tokens = query.shape[0]
-    if query.ndim != 2 or kv.ndim != 2 or kv.shape[0] != tokens:
+    rotary_dim, query_out, the contiguous weights, the first arguments of the C
+    calls (through the key's row stride) and the value's address."""
+    if query.ndim != 2 or kv.ndim != 2:
         raise ValueError("query must be [T, Hq * D] and kv [T, 2 * Hk * D]")
-    if num_kv_heads <= 0 or kv.shape[1] % (2 * num_kv_heads):
-        raise ValueError("kv must hold num_kv_heads keys, then as many values")
-    d = kv.shape[1] // (2 * num_kv_heads)
-    if d == 0 or query.shape[1] == 0 or query.shape[1] % d:
+    (tokens, q_cols), (kv_rows, kv_cols) = shape, kv_shape = query.shape, kv.shape
+    if kv_rows != tokens or num_kv_heads <= 0 or kv_cols % (2 * num_kv_heads):
         raise ValueError("query must be [T, Hq * D] and kv [T, 2 * Hk * D]")
-    if query.stride(1) != 1 or kv.stride(1) != 1:
+    d = kv_cols // (2 * num_kv_heads)
+    if d == 0 or q_cols == 0 or q_cols % d:
+        raise ValueError("query must be [T, Hq * D] and kv [T, 2 * Hk * D]")
+    (q_stride, q_step), (kv_stride, kv_step) = query.stride(), kv.stride()
+    if q_step != 1 or kv_step != 1:
         raise ValueError("query and kv must have contiguous rows")
     if q_weight.shape != (d,) or k_weight.shape != (d,):
         raise ValueError("q_weight and k_weight must be [head_dim]")
-    if not (query.dtype == kv.dtype == q_weight.dtype == k_weight.dtype):
+    dtype = query.dtype
+    if kv.dtype is not dtype or q_weight.dtype is not dtype or k_weight.dtype is not dtype:
         raise ValueError("query, kv and the weights must share a dtype")
-    rotary_dim = d if rotary_dim is None else int(rotary_dim)
-    if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > d:
+    if rotary_dim is None:
+        rotary_dim = d
+    elif rotary_dim < 0 or rotary_dim % 2 or rotary_dim > d:
+        raise ValueError("rotary_dim must be even and between zero and head_dim")
+    if rotary_dim % 2:
         raise ValueError("rotary_dim must be even and between zero and head_dim")
     if cos_sin.ndim != 2 or cos_sin.shape[1] < rotary_dim or cos_sin.stride(1) != 1:
         raise ValueError("cos_sin must be a [rows, cos | sin] table of rotary_dim columns")
-    if positions.dtype != torch.int32 or positions.numel() < tokens or not positions.is_contiguous():
+    if (positions.dtype is not torch.int32 or positions.numel() < tokens
+            or not positions.is_contiguous()):
         raise ValueError("positions must be contiguous int32 with one entry per token")
     if query_out is None:
         query_out = query
-    elif (query_out.shape != query.shape or query_out.dtype != query.dtype
-          or query_out.stride(1) != 1):
+    elif query_out.shape != shape or query_out.dtype is not dtype or query_out.stride(1) != 1:
         raise ValueError("query_out must be shaped like query, in contiguous rows")
-    return d, rotary_dim, query_out, q_weight.contiguous(), k_weight.contiguous()
+    # query, query_out, heads, key: the arguments both calls begin with
+    head = (query.data_ptr(), q_stride, query_out.data_ptr(), query_out.stride(0), q_cols // d,
+            kv.data_ptr(), kv_stride)
+    value = kv.data_ptr() + num_kv_heads * d * kv.element_size()
+    return d, rotary_dim, query_out, q_weight.contiguous(), k_weight.contiguous(), head, value
 
 
 def qk_norm_rope_write_paged(
@@ -735,10 +756,10 @@ def qk_norm_rope_write_paged(
     if key_cache.ndim != 4 or key_cache.shape != value_cache.shape:
         raise ValueError("the caches must be matching [blocks, bs, Hk, D]")
     num_blocks, block_size, hk, kd = key_cache.shape
-    d, rot, query_out, q_weight, k_weight = _qk_norm_inputs(
+    d, rot, query_out, q_weight, k_weight, head, value = _qk_norm_inputs(
         query, kv, positions, cos_sin, hk, q_weight, k_weight, rotary_dim, query_out)
-    tokens = query.shape[0]
-    if kd != d or not (key_cache.dtype == value_cache.dtype == query.dtype):
+    tokens, dtype = query.shape[0], query.dtype
+    if kd != d or key_cache.dtype is not dtype or value_cache.dtype is not dtype:
         raise ValueError("the caches must have the keys' head_dim and dtype")
     if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
         raise ValueError("caches must be contiguous")
@@ -746,22 +767,20 @@ def qk_norm_rope_write_paged(
         raise ValueError("block_table must be 2-D with a row for every token")
     if table_rows is not None and table_rows.numel() < tokens:
         raise ValueError("table_rows must map every token")
-    device = _lib.require_cuda(query, kv, positions, cos_sin, key_cache, value_cache, block_table,
-                               q_weight, k_weight, table_rows, query_out)
+    device = _lib.device_of(query, kv, positions, cos_sin, key_cache, value_cache, block_table,
+                            q_weight, k_weight, table_rows, query_out)
     table = _prep_index(block_table)
     if table.stride(1) != 1:
         table = table.contiguous()
     trows = None if table_rows is None else _prep_index(table_rows).contiguous()
-    item = kv.element_size()
+    table_shape = table.shape
     _lib.call_on(
-        device, "dsb_qk_norm_rope_paged",
-        _lib.ptr(query), query.stride(0), _lib.ptr(query_out), query_out.stride(0),
-        query.shape[1] // d, _lib.ptr(kv), kv.stride(0), kv.data_ptr() + hk * d * item,
-        kv.stride(0), hk, d, rot, int(bool(is_neox_style)), _lib.ptr(q_weight),
-        _lib.ptr(k_weight), float(eps), _lib.ptr(positions), tokens,
-        _lib.ptr(cos_sin), cos_sin.stride(0), cos_sin.shape[0], _lib.dtype_code(cos_sin.dtype),
-        _lib.dtype_code(query.dtype), _lib.ptr(key_cache), _lib.ptr(value_cache), num_blocks,
-        block_size, _lib.ptr(table), table.stride(0), table.shape[0], table.shape[1],
-        _lib.ptr(trows), _lib.ptr(_lib.error_flag(device)), _lib.stream_ptr(device),
+        device, "dsb_qk_norm_rope_paged", *head, value, head[-1], hk, d, rot,
+        1 if is_neox_style else 0, q_weight.data_ptr(), k_weight.data_ptr(), eps,
+        positions.data_ptr(), tokens, cos_sin.data_ptr(), cos_sin.stride(0), cos_sin.shape[0],
+        _lib.dtype_code(cos_sin.dtype), _lib.dtype_code(dtype), key_cache.data_ptr(),
+        value_cache.data_ptr(), num_blocks, block_size, table.data_ptr(), table.stride(0),
+        table_shape[0], table_shape[1], None if trows is None else trows.data_ptr(),
+        _lib.error_flag(device).data_ptr(), _lib.stream_ptr(device),
     )
     return query_out

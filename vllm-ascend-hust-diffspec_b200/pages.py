@@ -23,64 +23,67 @@ The tables are the ``block_table`` of the paged kernels
 
 from __future__ import annotations
 
-import ctypes
+from array import array
 from collections.abc import Sequence
 
 import torch
 
 from . import _lib
-from .kernels import _prep_index
 
 __all__ = ["resize_requests", "fork_requests", "compact_pages", "copy_pages"]
+
+
+_INT32 = torch.int32
 
 
 def _pool(ref_counts, block_tables, held):
     """The pool's arguments of every call."""
     if ref_counts.ndim != 1 or block_tables.ndim != 2 or held.ndim != 1:
         raise ValueError("ref_counts must be [pages], block_tables [rows, cols] and held [rows]")
-    if held.shape[0] != block_tables.shape[0]:
+    rows, cols = block_tables.shape
+    if held.shape[0] != rows:
         raise ValueError("held must have one entry per block-table row")
-    if not (ref_counts.dtype == block_tables.dtype == held.dtype == torch.int32):
+    if not (ref_counts.dtype is _INT32 and block_tables.dtype is _INT32 and held.dtype is _INT32):
         raise ValueError("ref_counts, block_tables and held must be int32")
-    if not (ref_counts.is_contiguous() and held.is_contiguous()) or block_tables.stride(1) != 1:
+    stride, step = block_tables.stride()
+    if step != 1 or not (ref_counts.is_contiguous() and held.is_contiguous()):
         raise ValueError("ref_counts and held must be contiguous, block_tables in contiguous rows")
-    return (_lib.ptr(ref_counts), ref_counts.shape[0], _lib.ptr(block_tables), block_tables.shape[0],
-            block_tables.stride(0), block_tables.shape[1], _lib.ptr(held))
+    return (ref_counts.data_ptr(), ref_counts.shape[0], block_tables.data_ptr(), rows, stride, cols,
+            held.data_ptr())
 
 
 def _caches(caches: Sequence[torch.Tensor], pages: int):
-    """Pointers of the caches, their page size (tokens) and a token's bytes."""
-    caches = list(caches)
-    if not caches:
+    """Addresses of the caches (an array to keep), their page size (tokens) and
+    a token's bytes."""
+    if not len(caches):
         raise ValueError("caches must name at least one tensor")
     first = caches[0]
     if first.ndim < 3:
         raise ValueError("caches must be [pages, block_size, ...]")
+    shape, dtype = first.shape, first.dtype
     for t in caches:
-        if t.shape != first.shape or t.dtype != first.dtype or not t.is_contiguous():
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
             raise ValueError("caches must be contiguous tensors of one shape and dtype")
-    if first.shape[0] != pages:
+    if shape[0] != pages:
         raise ValueError("caches must have one page per reference count")
-    token_bytes = first[0, 0].numel() * first.element_size()
-    array = (ctypes.c_void_p * len(caches))(*(t.data_ptr() for t in caches))
-    return caches, array, first.shape[1], token_bytes
+    addresses = array("Q", [t.data_ptr() for t in caches])
+    return addresses, shape[1], first.stride(1) * first.element_size()
 
 
-def _rows(n: int, **named):
-    out = []
-    for name, t in named.items():
-        if t.ndim != 1 or t.shape[0] != n:
-            raise ValueError(f"{name} must have one entry per request of the call")
+def _row(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
+    if t.ndim != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must have one entry per request of the call")
+    if t.dtype is not _INT32:
         if t.is_floating_point() or t.dtype == torch.bool:
             raise ValueError(f"{name} must be whole numbers")
-        out.append(_prep_index(t).contiguous())
-    return out
+        t = t.to(_INT32)
+    return t.contiguous()
 
 
-def _status(status, device):
+def _status(status, like):
     if status is None:
-        return torch.empty(2, dtype=torch.int32, device=device)
-    if status.shape != (2,) or status.dtype != torch.int32 or not status.is_contiguous():
+        return like.new_empty(2)
+    if status.shape != (2,) or status.dtype is not _INT32 or not status.is_contiguous():
         raise ValueError("status must be int32 [2]")
     return status
 
@@ -101,11 +104,11 @@ def resize_requests(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: 
         raise ValueError("block_size must be positive")
     pool = _pool(ref_counts, block_tables, held)
     n = rows.shape[0] if rows.ndim == 1 else -1
-    rows, lens = _rows(n, rows=rows, lens=lens)
-    device = _lib.require_cuda(ref_counts, block_tables, held, rows, lens, status)
-    status = _status(status, device)
-    _lib.call_on(device, "dsb_resize_requests", *pool, _lib.ptr(rows), _lib.ptr(lens), n,
-                 int(block_size), _lib.ptr(status), _lib.ptr(_lib.error_flag(device)),
+    rows, lens = _row(rows, n, "rows"), _row(lens, n, "lens")
+    device = _lib.device_of(ref_counts, block_tables, held, rows, lens, status)
+    status = _status(status, ref_counts)
+    _lib.call_on(device, "dsb_resize_requests", *pool, rows.data_ptr(), lens.data_ptr(), n,
+                 block_size, status.data_ptr(), _lib.error_flag(device).data_ptr(),
                  _lib.stream_ptr(device))
     return status
 
@@ -127,16 +130,17 @@ def fork_requests(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: to
     find no page for their started one are not forked and counted in
     ``status[0]``.  Returns ``status``."""
     pool = _pool(ref_counts, block_tables, held)
-    caches, array, block_size, token_bytes = _caches(caches, ref_counts.shape[0])
+    addresses, block_size, token_bytes = _caches(caches, pool[1])
     n = parents.shape[0] if parents.ndim == 1 else -1
-    parents, children, lens = _rows(n, parents=parents, children=children, lens=lens)
-    device = _lib.require_cuda(ref_counts, block_tables, held, parents, children, lens, status, *caches)
-    status = _status(status, device)
-    scratch = torch.empty(6 * n, dtype=torch.int32, device=device)
-    _lib.call_on(device, "dsb_fork_requests", *pool, _lib.ptr(parents), _lib.ptr(children),
-                 _lib.ptr(lens), n, block_size, array, len(caches), token_bytes, _lib.ptr(status),
-                 _lib.ptr(scratch), scratch.numel(), _lib.ptr(_lib.error_flag(device)),
-                 _lib.stream_ptr(device))
+    parents, children = _row(parents, n, "parents"), _row(children, n, "children")
+    lens = _row(lens, n, "lens")
+    device = _lib.device_of(ref_counts, block_tables, held, parents, children, lens, status, *caches)
+    status = _status(status, ref_counts)
+    scratch = ref_counts.new_empty(6 * n)  # dsb_fork_scratch_ints
+    _lib.call_on(device, "dsb_fork_requests", *pool, parents.data_ptr(), children.data_ptr(),
+                 lens.data_ptr(), n, block_size, addresses.buffer_info()[0], len(addresses),
+                 token_bytes, status.data_ptr(), scratch.data_ptr(), 6 * n,
+                 _lib.error_flag(device).data_ptr(), _lib.stream_ptr(device))
     return status
 
 
@@ -151,14 +155,14 @@ def compact_pages(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: to
     below ``n`` stay where they are.  Returns ``status`` (``status[1]``: the
     free pages, now the last ones)."""
     pool = _pool(ref_counts, block_tables, held)
-    caches, array, block_size, token_bytes = _caches(caches, ref_counts.shape[0])
-    device = _lib.require_cuda(ref_counts, block_tables, held, status, *caches)
-    status = _status(status, device)
-    ints = _lib.load().dsb_compact_scratch_ints(ref_counts.shape[0])
-    scratch = torch.empty(ints, dtype=torch.int32, device=device)
-    _lib.call_on(device, "dsb_compact_pages", *pool, block_size, array, len(caches), token_bytes,
-                 _lib.ptr(status), _lib.ptr(scratch), scratch.numel(),
-                 _lib.ptr(_lib.error_flag(device)), _lib.stream_ptr(device))
+    addresses, block_size, token_bytes = _caches(caches, pool[1])
+    device = _lib.device_of(ref_counts, block_tables, held, status, *caches)
+    status = _status(status, ref_counts)
+    ints = 1 + 3 * pool[1]  # dsb_compact_scratch_ints
+    scratch = ref_counts.new_empty(ints)
+    _lib.call_on(device, "dsb_compact_pages", *pool, block_size, addresses.buffer_info()[0],
+                 len(addresses), token_bytes, status.data_ptr(), scratch.data_ptr(), ints,
+                 _lib.error_flag(device).data_ptr(), _lib.stream_ptr(device))
     return status
 
 
@@ -171,10 +175,11 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
     first = caches[0] if len(caches) else None
     if first is None or first.ndim < 3:
         raise ValueError("caches must be [pages, block_size, ...] tensors")
-    caches, array, block_size, token_bytes = _caches(caches, first.shape[0])
+    pages = first.shape[0]
+    addresses, block_size, token_bytes = _caches(caches, pages)
     n = src.shape[0] if src.ndim == 1 else -1
-    src, dst = _rows(n, src=src, dst=dst)
-    device = _lib.require_cuda(src, dst, *caches)
-    _lib.call_on(device, "dsb_copy_pages", array, len(caches), first.shape[0],
-                 block_size * token_bytes, _lib.ptr(src), _lib.ptr(dst), n,
-                 _lib.ptr(_lib.error_flag(device)), _lib.stream_ptr(device))
+    src, dst = _row(src, n, "src"), _row(dst, n, "dst")
+    device = _lib.device_of(src, dst, *caches)
+    _lib.call_on(device, "dsb_copy_pages", addresses.buffer_info()[0], len(addresses), pages,
+                 block_size * token_bytes, src.data_ptr(), dst.data_ptr(), n,
+                 _lib.error_flag(device).data_ptr(), _lib.stream_ptr(device))
