@@ -83,7 +83,8 @@ class _Pool:
     (3000, 40, 100, 5, 1, torch.float32),  # several passes over the pool, odd pages
     (1, 2, 1, 16, 1, torch.bfloat16),      # a single page
     (9000, 16, 700, 8, 3, torch.bfloat16),
-    (20011, 24, 900, 2, 1, torch.bfloat16),  # several CTAs plan
+    (20011, 24, 900, 2, 1, torch.bfloat16),
+    (70001, 24, 3500, 1, 1, torch.bfloat16),  # several CTAs plan
 ])
 def test_random_histories(dsb, cuda, pages, rows, cols, bs, layers, dtype):
     rng = random.Random(pages)

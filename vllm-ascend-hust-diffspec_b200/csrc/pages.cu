@@ -14,12 +14,12 @@
 namespace dsb {
 namespace {
 
-constexpr int kPgThreads = 512;     // of a planning CTA
-constexpr int kPgPages = 8;         // pages a thread looks at in a turn
+constexpr int kPgThreads = 1024;    // of a planning CTA
+constexpr int kPgPages = 16;        // pages a thread looks at in a turn
 constexpr int kPgTurn = kPgThreads * kPgPages;
 // The planning CTAs are a cluster, each with a stretch of the pool: one for
-// pools of up to two turns, else eight (40000 pages, one CTA: 21 us to resize
-// and 28 to fork, most of it reading the counts; a cluster barrier is ~1 us).
+// pools of up to four turns, whose counts it reads in ~2 us, else eight (a
+// cluster's barriers cost about as much).
 constexpr int kPgCluster = 8;
 constexpr int kPgMaxRows = 4096;    // rows of one call
 constexpr int kPgMaxCaches = 128;   // caches of one launch
@@ -134,26 +134,31 @@ template <typename F> __device__ __forceinline__ void read_turn(const Pool &p, i
   for (int j = 0; j < kPgPages; ++j) look(j, first + 32 * j, v[j]);  // (behind `till`: -1)
 }
 
-// Free pages of the CTA's stretch.
+// Free pages of the CTA's stretch; counts below zero (pages let go more often
+// than they were held) are flagged and cleared.
 __device__ int free_pages(const Pool &p, const Stretch &s, int32_t *warp_tot) {
   int mine = 0, total;
   for (int64_t base = s.from; base < s.till; base += kPgTurn)
-    read_turn(p, base, s.till, [&](int, int64_t, int v) { mine += v == 0; });
+    read_turn(p, base, s.till, [&](int, int64_t page, int v) {
+      if (v < 0 && page < s.till) {
+        p.refs[page] = 0;
+        flag_error(p.err, DSB_FLAG_BLOCK);
+        v = 0;
+      }
+      mine += v == 0;
+    });
   block_scan(mine, warp_tot, total);
   return total;
 }
 
-// Drop `n` references to `page`; more than there are is flagged.
+// Drop `n` references to `page`.  More than there are leave a negative count,
+// which the pass over the pool that follows flags and clears: an atomic that
+// returns nothing is half the time of one that tells.
 __device__ __forceinline__ void release(const Pool &p, int page, int n) {
-  if (page < 0 || page >= p.pages) {
+  if (page < 0 || page >= p.pages)
     flag_error(p.err, DSB_FLAG_BLOCK);
-    return;
-  }
-  const int old = atomicSub(p.refs + page, n);
-  if (old < n) {
-    atomicAdd(p.refs + page, n - max(old, 0));
-    flag_error(p.err, DSB_FLAG_BLOCK);
-  }
+  else
+    atomicSub(p.refs + page, n);
 }
 
 // Changes of reference counts that a thread meets one after another, joined
@@ -169,10 +174,9 @@ struct PageCounts {
     bool found = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (n[i] > 0 && page[i] == x) {
+      if (!found && n[i] > 0 && page[i] == x) {
         ++n[i];
         found = true;
-        break;
       }
     if (found) return;
 #pragma unroll
@@ -183,11 +187,6 @@ struct PageCounts {
         n[i] = 1;
       }
     next = (next + 1) & 3;
-  }
-  template <typename F> __device__ void finish(F flush) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n[i] > 0) flush(page[i], n[i]);
   }
 };
 
@@ -226,10 +225,14 @@ __device__ void allot(const Pool &p, const Stretch &s, const int32_t *want, int 
 }
 
 // Rows given twice in one call: the first counts, the others are flagged.
-__device__ bool repeated(const int32_t *rows, int i) {
-  for (int j = 0; j < i; ++j)
-    if (rows[j] == rows[i]) return true;
-  return false;
+// again[i] for rows[0..n) in shared memory, a warp a row.
+__device__ void find_repeats(const int32_t *rows, int32_t *again, int n) {
+  for (int i = threadIdx.x >> 5; i < n; i += kPgThreads / 32) {
+    bool hit = false;
+    for (int j = threadIdx.x & 31; j < i; j += 32) hit |= rows[j] == rows[i];
+    hit = __any_sync(0xffffffffu, hit);
+    if ((threadIdx.x & 31) == 0) again[i] = hit;
+  }
 }
 
 // Pages of row r: those it has, and those `len` tokens need (-1: the table
@@ -274,16 +277,24 @@ __global__ void __launch_bounds__(256)
   }
   __syncthreads();
   const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  auto flush = [&](int page, int count) { release(p, page, count); };
+  int entry[kPgRows];  // (every read on its way before the first is used)
+  unsigned mine = 0;
+#pragma unroll
+  for (int k = 0; k < kPgRows; ++k)
+    if (k < m && s_row[k] >= 0 && j >= s_keep[k] && j < s_held[k]) {
+      mine |= 1u << k;
+      entry[k] = p.tables[(int64_t)s_row[k] * p.stride + j];
+    }
   PageCounts counts;
-#pragma unroll 4
-  for (int k = 0; k < m; ++k) {
-    if (s_row[k] < 0 || j < s_keep[k] || j >= s_held[k]) continue;
-    int32_t *entry = p.tables + (int64_t)s_row[k] * p.stride + j;
-    counts.add(*entry, flush);
-    *entry = -1;
-  }
-  counts.finish(flush);
+#pragma unroll
+  for (int k = 0; k < kPgRows; ++k)
+    if (mine >> k & 1) {
+      p.tables[(int64_t)s_row[k] * p.stride + j] = -1;
+      counts.add(entry[k], [&](int page, int count) { release(p, page, count); });
+    }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (counts.n[i] > 0) release(p, counts.page[i], counts.n[i]);
 }
 
 // Every CTA of the cluster has the rows' needs; the first one changes what
@@ -301,10 +312,12 @@ __global__ void __launch_bounds__(kPgThreads)
   if (tid == 0) lacking = granted = 0;
   for (int i = tid; i < n; i += kPgThreads) row[i] = rows[i];
   __syncthreads();
+  find_repeats(row, want, n);
+  __syncthreads();
   for (int i = tid; i < n; i += kPgThreads) {
     const int r = row[i];
     int have = 0, need = -1;
-    if (r < 0 || r >= p.rows || repeated(row, i)) {
+    if (r < 0 || r >= p.rows || want[i]) {
       if (s.rank == 0) flag_error(p.err, DSB_FLAG_SLOT);
     } else {
       have = pages_held(p, r);
@@ -375,11 +388,13 @@ __global__ void __launch_bounds__(kPgThreads)
   if (tid == 0) lacking = granted = 0;
   for (int i = tid; i < n; i += kPgThreads) kid[i] = children[i];
   __syncthreads();
+  find_repeats(kid, want, n);
+  __syncthreads();
   for (int i = tid; i < n; i += kPgThreads) {
     const int up = parents[i], c = kid[i], len = lens[i];
     ForkPlan f{up, -1, -1, -1, -1, 0};
     int flag = 0;
-    if (up < 0 || up >= p.rows || c < 0 || c >= p.rows || repeated(kid, i) || p.held[c] != 0) {
+    if (up < 0 || up >= p.rows || c < 0 || c >= p.rows || want[i] || p.held[c] != 0) {
       flag = DSB_FLAG_SLOT;
     } else if (len < 0 || (int64_t)len > (int64_t)p.held[up] * p.bs ||
                (int64_t)len > p.cols * p.bs) {
@@ -466,16 +481,24 @@ __global__ void __launch_bounds__(256)
         flag_error(p.err, DSB_FLAG_BLOCK);
     };
     for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < p.cols; j += table_blocks * 256) {
+      int page[kPgRows];  // (every read on its way before the first is used)
+      unsigned mine = 0;
+#pragma unroll
+      for (int k = 0; k < kPgRows; ++k)
+        if (k < m && s_plan[k].child >= 0 && j < s_plan[k].full) {
+          mine |= 1u << k;
+          page[k] = p.tables[(int64_t)s_plan[k].parent * p.stride + j];
+        }
       PageCounts counts;
-#pragma unroll 4
-      for (int k = 0; k < m; ++k) {
-        const ForkPlan &f = s_plan[k];
-        if (f.child < 0 || j >= f.full) continue;
-        const int page = p.tables[(int64_t)f.parent * p.stride + j];
-        p.tables[(int64_t)f.child * p.stride + j] = page;
-        counts.add(page, flush);
-      }
-      counts.finish(flush);
+#pragma unroll
+      for (int k = 0; k < kPgRows; ++k)
+        if (mine >> k & 1) {
+          p.tables[(int64_t)s_plan[k].child * p.stride + j] = page[k];
+          counts.add(page[k], flush);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (counts.n[i] > 0) flush(counts.page[i], counts.n[i]);
     }
     return;
   }
@@ -606,7 +629,9 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-int planners(int64_t pages) { return pages <= 2 * kPgTurn ? 1 : kPgCluster; }
+// (three passes over the counts to compact: a cluster from a second turn on,
+// 96 us against 110 for 32768 pages)
+int planners(int64_t pages, int turns) { return pages <= (int64_t)turns * kPgTurn ? 1 : kPgCluster; }
 
 int check_pool(const Pool &p, int n) {
   if (p.pages <= 0 || p.pages > INT32_MAX || p.rows <= 0 || p.rows > INT32_MAX || p.cols <= 0 ||
@@ -664,7 +689,7 @@ extern "C" int dsb_resize_requests(int32_t *ref_counts, int64_t num_pages, int32
   }
   const size_t smem = (size_t)n * 4 * sizeof(int32_t);
   if (int e = ensure_smem((const void *)resize_kernel, smem)) return e;
-  const int ranks = planners(num_pages);
+  const int ranks = planners(num_pages, 4);
   launch_kernel_cluster(resize_kernel, dim3(ranks), dim3(kPgThreads), smem, st, ranks, p, rows, lens,
                         (int)n, alone ? 1 : 0, ranks);
   return check_launch("resize_kernel");
@@ -691,7 +716,7 @@ extern "C" int dsb_fork_requests(int32_t *ref_counts, int64_t num_pages, int32_t
   ForkPlan *plan = reinterpret_cast<ForkPlan *>(scratch);
   const size_t smem = (size_t)n * 3 * sizeof(int32_t);
   if (int e = ensure_smem((const void *)fork_plan_kernel, smem)) return e;
-  const int ranks = planners(num_pages);
+  const int ranks = planners(num_pages, 4);
   launch_kernel_cluster(fork_plan_kernel, dim3(ranks), dim3(kPgThreads), smem, st, ranks, p, parents,
                         children, lens, (int)n, plan, ranks);
   if (int e = check_launch("fork_plan_kernel")) return e;
@@ -728,7 +753,7 @@ extern "C" int dsb_compact_pages(int32_t *ref_counts, int64_t num_pages, int32_t
   if (scratch_ints < dsb_compact_scratch_ints(num_pages))
     return fail(DSB_ERR_INVALID, "scratch smaller than dsb_compact_scratch_ints");
   const cudaStream_t st = as_stream(stream);
-  const int ranks = planners(num_pages);
+  const int ranks = planners(num_pages, 1);
   launch_kernel_cluster(compact_plan_kernel, dim3(ranks), dim3(kPgThreads), 0, st, ranks, p, scratch,
                         ranks);
   if (int e = check_launch("compact_plan_kernel")) return e;

@@ -239,11 +239,17 @@ __device__ __forceinline__ void qk_turn(const QkTurn &f, float inv, const float 
 }
 
 // A warp takes kPer query heads of one token, or kPer of its key and value
-// heads.  `ahead`: tokens between a warp's and the one whose rows it asks into
-// L2, about what the GPU has resident, so that the loads of a later warp hit
-// there (0: none).
+// heads.  Bound by memory, by way of the loads in flight and of how soon a
+// finished warp's place is taken: 65536 tokens of 32/4 heads of 128 into
+// pages (1.35 GB) take 281 us with 16 warps of 123 registers an SM in CTAs of
+// 256 threads, 247 with 24 warps of 80 (a few spills), 235 with stores that
+// do not stay in the way in L2, 227 (5.9 TB/s, 0.90 of the measured copy) in
+// CTAs of 64.  Two or six heads a thread are slower (268 and 286), and so is
+// asking later rows into L2 ahead of their warps (243 for 235).
+constexpr int kQkThreads = 64;
+
 template <typename T, typename CS, int D, bool NEOX>
-__global__ void __launch_bounds__(256, 2) qk_norm_rope_heads_kernel(const QkArgs a, int ahead) {
+__global__ void __launch_bounds__(kQkThreads, 12) qk_norm_rope_heads_kernel(const QkArgs a) {
   constexpr int kLanes = D / 16, kGroups = 32 / kLanes;  // heads that a warp has side by side
   constexpr int kPer = kGroups * kQkHeads;               // heads of one token a warp takes
   pdl_begin();
@@ -256,17 +262,12 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_heads_kernel(const QkArgs
   const int pos = a.positions[t] + a.pos_offset;
   const bool turn = pos >= 0 && pos < a.rotary_rows;  // else: normed, not rotated
   const CS *cs = static_cast<const CS *>(a.cos_sin) + (turn ? pos : 0) * a.cs_stride;
-  const bool later = ahead > 0 && lane == 0 && t + ahead < a.tokens;
   uint4 x1[kQkHeads], x2[kQkHeads];
   QkTurn f;
 
   if (chunk < qchunks) {
     const int h0 = chunk * kPer + lane / kLanes;
     const T *src = static_cast<const T *>(a.q) + t * a.q_stride + (int64_t)h0 * D;
-    if (later)
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + ahead * a.q_stride),
-                   "r"(min(kPer, a.hq - chunk * kPer) * D * 2)
-                   : "memory");
 #pragma unroll
     for (int i = 0; i < kQkHeads; ++i) {  // (a head past the last: zeros, not stored)
       const bool in = h0 + i * kGroups < a.hq;
@@ -284,8 +285,8 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_heads_kernel(const QkArgs
       const float inv = rsqrtf(qk_mean_square<D>(v1, v2) + a.eps);
       qk_turn<NEOX>(f, inv, v1, v2, o1, o2);
       if (h0 + i * kGroups < a.hq) {
-        *reinterpret_cast<uint4 *>(out + i * kGroups * D + e1) = qk_pack<T>(o1);
-        *reinterpret_cast<uint4 *>(out + i * kGroups * D + e2) = qk_pack<T>(o2);
+        __stcs(reinterpret_cast<uint4 *>(out + i * kGroups * D + e1), qk_pack<T>(o1));
+        __stcs(reinterpret_cast<uint4 *>(out + i * kGroups * D + e2), qk_pack<T>(o2));
       }
     }
     return;
@@ -294,14 +295,6 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_heads_kernel(const QkArgs
   const int k0 = (chunk - qchunks) * kPer, h0 = k0 + lane / kLanes;  // keys, then values
   const T *key = static_cast<const T *>(a.k) + t * a.k_stride;
   const T *value = static_cast<const T *>(a.v) + t * a.v_stride;
-  if (later && k0 == 0) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(key + ahead * a.k_stride),
-                 "r"(a.hk * D * 2)
-                 : "memory");
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(value + ahead * a.v_stride),
-                 "r"(a.hk * D * 2)
-                 : "memory");
-  }
 #pragma unroll
   for (int i = 0; i < kQkHeads; ++i) {
     const int h = h0 + i * kGroups;
@@ -341,14 +334,14 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_heads_kernel(const QkArgs
     T *out = static_cast<T *>(is_key ? a.k_out : a.v_out);
     if (out != nullptr) {
       out += ((int64_t)t * a.hk + kh) * D;
-      *reinterpret_cast<uint4 *>(out + e1) = r1;
-      *reinterpret_cast<uint4 *>(out + e2) = r2;
+      __stcs(reinterpret_cast<uint4 *>(out + e1), r1);
+      __stcs(reinterpret_cast<uint4 *>(out + e2), r2);
     }
     if (row >= 0) {
       T *dst = static_cast<T *>(is_key ? a.dst_k : a.dst_v) + (row * a.hk + kh) * D;
       const bool raw = a.dest == kDestRaw;
-      *reinterpret_cast<uint4 *>(dst + e1) = raw ? y1 : r1;
-      *reinterpret_cast<uint4 *>(dst + e2) = raw ? y2 : r2;
+      __stcs(reinterpret_cast<uint4 *>(dst + e1), raw ? y1 : r1);
+      __stcs(reinterpret_cast<uint4 *>(dst + e2), raw ? y2 : r2);
     }
   }
 }
@@ -367,12 +360,12 @@ template <typename T, typename CS, int D> void launch_heads(const QkArgs &a, cud
   const int per = 32 / (D / 16) * kQkHeads;
   const int64_t chunks = (a.hq + per - 1) / per + (2 * a.hk + per - 1) / per;
   const int64_t warps = (int64_t)a.tokens * chunks;
-  const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
-  const int ahead = (int)(16L * sm_count() / chunks);  // two CTAs of 8 warps an SM
+  constexpr int kWarps = kQkThreads / 32;
+  const dim3 grid((unsigned)((warps + kWarps - 1) / kWarps)), block(kQkThreads);
   if (a.neox)
-    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, true>, grid, block, 0, st, a, ahead);
+    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, true>, grid, block, 0, st, a);
   else
-    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, false>, grid, block, 0, st, a, ahead);
+    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, false>, grid, block, 0, st, a);
 }
 
 int launch(const QkArgs &a, int cos_sin_dtype, int dtype, cudaStream_t st) {
