@@ -200,3 +200,14 @@ def test_abi_rejects_before_any_launch(dsb):
               dict(rk=fake, rv=fake, slots=fake, abs=fake)):
         assert norm(**k) == P.DSB_ERR_INVALID, k
     assert norm(tokens=0) == P.DSB_OK
+
+
+def test_prefix_groups(dsb):
+    f = dsb.runtime.prefix_groups
+    assert f([300], [4], [3, 6, 9, 12], [340, 301, 333, 420]) == ([300], [0, 12], 120)
+    assert f([300, 0, 130], [2, 2, 4], [1, 2, 3, 4], [340, 301, 200, 131]) == (
+        [300, 0, 130], [0, 2, 2, 4], 70)
+    assert f([7], [0], [], []) == ([7], [0, 0], 0)
+    for lens, ends in (([], []), ([1], [3, 4]), ([-1], [4]), ([1, 1], [3, 2]), ([1], [5]), ([1], [3])):
+        with pytest.raises(ValueError, match="shared_prefix"):
+            f(lens, ends, [1, 2, 3, 4], [5, 5, 5, 5])

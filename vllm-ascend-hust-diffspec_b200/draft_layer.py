@@ -326,12 +326,39 @@ def silu_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Te
     return out
 
 
+def _queries_keys_values(layer, h, *, slots, abs_positions, local_positions, raw_key, raw_value,
+                         cos_sin, position_offset, prefetch_l2=False):
+    """The attention's rotated queries and contiguous keys and values of one
+    step, with the raw-cache write: the fused projection and :func:`rope_qk`,
+    or, for a layer whose queries and keys are normed, the plain projection
+    and :func:`qk_norm_rope` (the raw cache then holds normed keys, so that
+    the working-cache rebuild rotates them as they are)."""
+    n = h.shape[0]
+    if layer.q_norm is None:
+        q, kv = qkv_projection_write_raw(h, layer.p_qkv, layer.hq * layer.d, slots, abs_positions,
+                                         raw_key, raw_value, prefetch_weight=True,
+                                         packed_weight=True, prefetch_l2=prefetch_l2)
+        k, v = rope_qk(q, kv, local_positions, cos_sin, layer.hk, position_offset=position_offset)
+    else:
+        qkv = draft_linear(h, layer.p_qkv, packed=True, prefetch_l2=prefetch_l2)
+        split = layer.hq * layer.d
+        q = torch.empty((n, split), dtype=h.dtype, device=h.device)
+        _, k, v = qk_norm_rope(qkv[:, :split], qkv[:, split:], local_positions, cos_sin, layer.hk,
+                               layer.q_norm, layer.k_norm, layer.eps, query_out=q,
+                               position_offset=position_offset,
+                               raw=(raw_key, raw_value, slots, abs_positions))
+    return q.view(n, layer.hq, layer.d), k, v
+
+
 class Eagle3DraftLayer:
     """Random-init weights of one draft layer (bf16): hidden 2048, qkv input
-    4096 (embedding + hidden), 32 query / 4 kv heads of 128, SwiGLU 6144."""
+    4096 (embedding + hidden), 32 query / 4 kv heads of 128, SwiGLU 6144.
+    ``qk_norm``: every query and key head is normed before the rotation
+    (weights ``q_norm`` / ``k_norm [head_dim]``)."""
 
     def __init__(self, device, *, hidden=2048, qkv_in=4096, num_heads=32, num_kv_heads=4,
-                 head_dim=128, intermediate=6144, dtype=torch.bfloat16, seed=0, eps=1e-6):
+                 head_dim=128, intermediate=6144, dtype=torch.bfloat16, seed=0, eps=1e-6,
+                 qk_norm=False):
         g = torch.Generator(device=device).manual_seed(seed)
 
         def w(rows, cols):
@@ -357,6 +384,8 @@ class Eagle3DraftLayer:
         self.p_down = pack_linear_weight(self.w_down)
         self.in_norm = torch.ones(qkv_in, dtype=dtype, device=device)
         self.post_norm = torch.ones(hidden, dtype=dtype, device=device)
+        self.q_norm = torch.ones(head_dim, dtype=dtype, device=device) if qk_norm else None
+        self.k_norm = torch.ones(head_dim, dtype=dtype, device=device) if qk_norm else None
         self.workspace = AttentionWorkspace(device)
         # linears ("qkv", "o_proj", "gate_up", "down_proj") whose whole weight
         # is requested into L2 while the kernel before them runs
@@ -377,11 +406,11 @@ class Eagle3DraftLayer:
         n = x_in.shape[0]
         h = rms_norm(x_in, self.in_norm, self.eps)
         l2 = self.l2_prefetch
-        q, kv = qkv_projection_write_raw(h, self.p_qkv, self.hq * self.d, slots, abs_positions,
-                                         raw_key, raw_value, prefetch_weight=True,
-                                         packed_weight=True, prefetch_l2="qkv" in l2)
-        k, v = rope_qk(q, kv, local_positions, cos_sin, self.hk, position_offset=position_offset)
-        attn = draft_decode_attention(q.view(n, self.hq, self.d), k, v, working_key, working_value,
+        q, k, v = _queries_keys_values(
+            self, h, slots=slots, abs_positions=abs_positions, local_positions=local_positions,
+            raw_key=raw_key, raw_value=raw_value, cos_sin=cos_sin, position_offset=position_offset,
+            prefetch_l2="qkv" in l2)
+        attn = draft_decode_attention(q, k, v, working_key, working_value,
                                       slots, local_positions, self.d ** -0.5,
                                       position_offset=position_offset, workspace=self.workspace)
         x = draft_linear(attn.view(n, self.hq * self.d), self.p_o, "residual", residual,
@@ -456,6 +485,7 @@ class Eagle3DraftLayerTP:
         self.p_gate_up = pack_linear_weight(interleave_gate_up(self.w_gate_up))
         self.p_down = pack_linear_weight(self.w_down)
         self.in_norm, self.post_norm = full.in_norm, full.post_norm
+        self.q_norm, self.k_norm = full.q_norm, full.k_norm  # of one head: whole on every rank
         self.workspace = AttentionWorkspace(full.w_o.device)
         if all_reduce is None:
             def all_reduce(t):
@@ -475,11 +505,10 @@ class Eagle3DraftLayerTP:
         the draft attention over its heads and its fp32 o_proj partial."""
         n = x_in.shape[0]
         h = rms_norm(x_in, self.in_norm, self.eps)
-        q, kv = qkv_projection_write_raw(h, self.p_qkv, self.hq * self.d, slots, abs_positions,
-                                         raw_key, raw_value, prefetch_weight=True,
-                                         packed_weight=True)
-        k, v = rope_qk(q, kv, local_positions, cos_sin, self.hk, position_offset=position_offset)
-        attn = draft_decode_attention(q.view(n, self.hq, self.d), k, v, working_key, working_value,
+        q, k, v = _queries_keys_values(
+            self, h, slots=slots, abs_positions=abs_positions, local_positions=local_positions,
+            raw_key=raw_key, raw_value=raw_value, cos_sin=cos_sin, position_offset=position_offset)
+        attn = draft_decode_attention(q, k, v, working_key, working_value,
                                       slots, local_positions, self.d ** -0.5,
                                       position_offset=position_offset, workspace=self.workspace)
         return draft_linear(attn.view(n, self.hq * self.d), self.p_o, "partial", out=partial,
@@ -521,11 +550,10 @@ class Eagle3DraftLayerTP:
         every rank's buffer of the o_proj site (fused all-reduce)."""
         n = x_in.shape[0]
         h = rms_norm(x_in, self.in_norm, self.eps)
-        q, kv = qkv_projection_write_raw(h, self.p_qkv, self.hq * self.d, slots, abs_positions,
-                                         raw_key, raw_value, prefetch_weight=True,
-                                         packed_weight=True)
-        k, v = rope_qk(q, kv, local_positions, cos_sin, self.hk, position_offset=position_offset)
-        attn = draft_decode_attention(q.view(n, self.hq, self.d), k, v, working_key, working_value,
+        q, k, v = _queries_keys_values(
+            self, h, slots=slots, abs_positions=abs_positions, local_positions=local_positions,
+            raw_key=raw_key, raw_value=raw_value, cos_sin=cos_sin, position_offset=position_offset)
+        attn = draft_decode_attention(q, k, v, working_key, working_value,
                                       slots, local_positions, self.d ** -0.5,
                                       position_offset=position_offset, workspace=self.workspace)
         draft_linear_peer(attn.view(n, self.hq * self.d), self.p_o, self.peer[0], packed=True)

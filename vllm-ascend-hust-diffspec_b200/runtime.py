@@ -37,7 +37,12 @@ import torch
 from . import _lib
 from .attention import AttentionWorkspace, draft_decode_attention
 from .compact_kv import rebuild_working_cache
-from .kernels import kv_projection_write_raw, paged_chunk_head_scores, paged_decode_attention_lse
+from .kernels import (
+    kv_projection_write_raw,
+    paged_chunk_head_scores,
+    paged_decode_attention_lse,
+    shared_prefix_attention_lse,
+)
 from .parallel import gather_head_scores
 from .selection import (
     DiffSpecSelection,
@@ -195,6 +200,26 @@ def causal_row_lengths(query_ends: list[int], seq_lens: list[int]) -> tuple[list
             table_rows.append(i)
         start = end
     return visible, table_rows
+
+
+def prefix_groups(prefix_lens: list[int], request_ends: list[int], query_ends: list[int],
+                  seq_lens: list[int]) -> tuple[list[int], list[int], int]:
+    """Query rows of groups of requests that share a prefix: ``(prefix lengths,
+    first row of each group and the row count, most tokens that a request has
+    behind its group's prefix)``."""
+    prefix_lens, request_ends = [int(p) for p in prefix_lens], [int(e) for e in request_ends]
+    if not prefix_lens or len(prefix_lens) != len(request_ends):
+        raise ValueError("shared_prefix needs one prefix length and one end for every group")
+    starts, longest, begin = [0], 0, 0
+    for prefix, end in zip(prefix_lens, request_ends):
+        if prefix < 0 or end < begin or end > len(query_ends):
+            raise ValueError("shared_prefix ends must ascend within the requests, lengths be >= 0")
+        longest = max([longest, *(n - prefix for n in seq_lens[begin:end])])
+        starts.append(query_ends[end - 1] if end else 0)
+        begin = end
+    if begin != len(query_ends):
+        raise ValueError("shared_prefix groups must cover every request")
+    return prefix_lens, starts, longest
 
 
 class DiffSpecDraftCache:
@@ -417,6 +442,8 @@ class DiffSpecDraftCache:
         value_cache: torch.Tensor,
         metadata: Any,
         scale: float,
+        *,
+        shared_prefix: tuple[list[int], list[int]] | None = None,
     ) -> torch.Tensor:
         """The target verifier's attention with its softmax LSE, captured for
         retrieval: the B200 counterpart of the FIA call with softmax_lse_flag
@@ -430,6 +457,12 @@ class DiffSpecDraftCache:
         alike).  Runs ``paged_decode_attention_lse`` once, stores the query,
         LSE, cache and table through :meth:`capture_target_attention`, and
         returns the attention output ``[n, Hq, D]``.
+
+        ``shared_prefix = (prefix_lens, request_ends)`` names runs of requests
+        that hold the same first tokens: group i's requests end before
+        ``request_ends[i]`` (cumulative, the last one the request count) and
+        share ``prefix_lens[i]`` tokens (0: none).  Those are then read once a
+        group (``shared_prefix_attention_lse``); the results are the same.
         """
         query_ends = [int(e) for e in metadata.actual_seq_lengths_q]
         seq_lens = [int(x) for x in metadata.seq_lens_list]
@@ -438,10 +471,20 @@ class DiffSpecDraftCache:
         visible, table_rows = causal_row_lengths(query_ends, seq_lens)
         lens = torch.tensor(visible, dtype=torch.int32).to(self.device)
         rows = torch.tensor(table_rows, dtype=torch.int32).to(self.device)
-        out, lse = paged_decode_attention_lse(
-            query, key_cache, value_cache, metadata.block_tables, lens, scale=scale,
-            max_seq_len=max(seq_lens, default=0), table_rows=rows,
-        )
+        if shared_prefix is None:
+            out, lse = paged_decode_attention_lse(
+                query, key_cache, value_cache, metadata.block_tables, lens, scale=scale,
+                max_seq_len=max(seq_lens, default=0), table_rows=rows,
+            )
+        else:
+            prefix_lens, starts, longest = prefix_groups(*shared_prefix, query_ends, seq_lens)
+            out, lse = shared_prefix_attention_lse(
+                query, key_cache, value_cache, metadata.block_tables, lens,
+                torch.tensor(prefix_lens, dtype=torch.int32).to(self.device), scale=scale,
+                max_prefix_len=max(prefix_lens), max_suffix_len=longest,
+                group_starts=torch.tensor(starts, dtype=torch.int32).to(self.device),
+                table_rows=rows,
+            )
         self.capture_target_attention(query, lse, key_cache, metadata, scale)
         return out
 
