@@ -46,10 +46,11 @@ struct alignas(16) SpSeg {
 };
 static_assert(sizeof(SpSeg) == 64, "one segment per 64 bytes");
 
-// Where a CTA begins: all the units, and the segment its first one is in.
+// The units' even shares, floor and remainder of units / CTAs, and the segment
+// that a CTA's first unit is in.
 struct alignas(16) SpBegin {
-  int64_t units;
-  int32_t seg, pad;
+  int64_t share;
+  int32_t rest, seg;
 };
 
 // Where a row's partial sums are: its group's first prefix segment and row,
@@ -72,20 +73,18 @@ struct SpArgs {
   float2 *ml;          // [rows of partial sums]: maximum (log2), sum
 };
 
-// floor(x / y) of whole numbers below 2^52 without a 64-bit division: the
-// rounded quotient, put right by at most one.
-__device__ __forceinline__ int64_t sp_div(int64_t x, int64_t y) {
-  int64_t q = (int64_t)((double)x / (double)y);
-  if (q * y > x) --q;
-  if ((q + 1) * y <= x) ++q;
-  return q;
+// A CTA's first unit, floor(cta * units / ctas), and the CTA that owns unit u
+// (64-bit divisions cost more than the loads they wait for).
+__device__ __forceinline__ int64_t sp_first(int cta, const SpBegin &x, int ctas) {
+  return cta * x.share + (unsigned)(cta * x.rest) / (unsigned)ctas;
 }
-// The CTA that owns unit u of `units`, and a CTA's first unit.
-__device__ __forceinline__ int sp_owner(int64_t u, int64_t units, int ctas) {
-  return (int)sp_div((u + 1) * ctas - 1, units);
-}
-__device__ __forceinline__ int64_t sp_first(int64_t cta, int64_t units, int ctas) {
-  return sp_div(cta * units, ctas);
+__device__ __forceinline__ int sp_owner(int64_t u, const SpBegin &x, int ctas) {
+  const float units = (float)x.share * (float)ctas + (float)x.rest;
+  // floor(((u + 1) * ctas - 1) / units), right to one
+  int b = min((int)(((float)(u + 1) * (float)ctas - 1.f) / units), ctas - 1);
+  while (b > 0 && sp_first(b, x, ctas) > u) --b;
+  while (b + 1 < ctas && sp_first(b + 1, x, ctas) <= u) ++b;
+  return b;
 }
 
 // Tokens that row r may see, 0 for a row without a valid table row.
@@ -345,15 +344,17 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
   }
   // where each CTA begins: the last segment that starts at or before its first
   // unit (an empty one starts where the next does)
+  SpBegin shares{units / s.ctas, (int)(units % s.ctas), 0};
   for (int b = tid; b < s.ctas; b += kPlanThreads) {
-    const int64_t u = sp_first(b, units, s.ctas);
+    const int64_t u = sp_first(b, shares, s.ctas);
     int x = 0, y = nseg;
     while (x < y) {
       const int mid = (x + y) / 2;
       if ((mid < kPlanKeep ? s_unit0[mid] : s.segs[mid].unit0) <= u) x = mid + 1;
       else y = mid;
     }
-    s.begin[b] = SpBegin{units, max(x - 1, 0), 0};
+    shares.seg = max(x - 1, 0);
+    s.begin[b] = shares;
   }
 }
 
@@ -447,27 +448,6 @@ __device__ __forceinline__ float sp_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// pairs of fp32 in one 64-bit register
-__device__ __forceinline__ uint64_t sp_pair(float x, float y) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
-  return d;
-}
-__device__ __forceinline__ float2 sp_unpair(uint64_t d) {
-  float2 v;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(d));
-  return v;
-}
-__device__ __forceinline__ uint64_t sp_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t sp_add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // 32 bytes of a row (32-byte aligned)
 __device__ __forceinline__ void sp_st_global8(float *p, const float (&v)[8]) {
   asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]),
@@ -483,14 +463,14 @@ struct SpPiece {
 
 // The pieces of this CTA, in order; every role walks them for itself.
 struct SpWalk {
-  int64_t u, end, units;
+  int64_t u, end;
+  SpBegin share;
   int seg;
   __device__ void begin(const SpArgs &s) {
-    const SpBegin x = s.begin[blockIdx.x];
-    units = x.units;
-    seg = x.seg;
-    u = sp_first(blockIdx.x, units, s.ctas);
-    end = sp_first(blockIdx.x + 1, units, s.ctas);
+    share = s.begin[blockIdx.x];
+    seg = share.seg;
+    u = sp_first(blockIdx.x, share, s.ctas);
+    end = sp_first(blockIdx.x + 1, share, s.ctas);
   }
   __device__ bool next(const SpArgs &s, SpPiece &p) {
     while (u < end) {
@@ -500,7 +480,9 @@ struct SpWalk {
         continue;
       }
       const int64_t off = u - p.g.unit0;
-      p.h = (int)sp_div(off, p.g.len);
+      p.h = (int)((float)off / (float)p.g.len);  // right to one
+      if (p.h * (int64_t)p.g.len > off) --p.h;
+      if ((p.h + 1) * (int64_t)p.g.len <= off) ++p.h;
       const int a = (int)(off - (int64_t)p.h * p.g.len);
       const int b = (int)min((int64_t)p.g.len, a + (end - u));
       u += b - a;
@@ -508,7 +490,7 @@ struct SpWalk {
       p.n = max(b - kSpStart, 0) - p.t0;
       if (p.n <= 0) continue;
       p.index = (int)blockIdx.x -
-                sp_owner(p.g.unit0 + (int64_t)p.h * p.g.len, units, s.ctas);
+                sp_owner(p.g.unit0 + (int64_t)p.h * p.g.len, share, s.ctas);
       return true;
     }
     return false;
@@ -732,8 +714,6 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     const int stream = warp >> 2, m128 = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + lanes + stream * 128, to = ts + 256;
-    const uint64_t scale2 = sp_pair(a.scale_log2, a.scale_log2);
-    const uint64_t neg1 = sp_pair(-1.f, -1.f);
     int i0 = 0, kt = 0;  // loads and this stream's tiles of the pieces before
     int joints = 0;
     bool ok = true;
@@ -826,10 +806,15 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         if (works) {
           const int from = p.g.tok0 - T0, till = (rehearsal ? kSpTok : lim - T0);  // columns seen
           const bool whole = __all_sync(0xffffffffu, from <= 0 && till >= kSpTok);
+          // Columns that the row does not see become -inf, here and in the
+          // tensor memory that the weights are made from.
           auto hide = [&](uint32_t(&x)[32], int c) {
+            const int lo = min(max(from - c, 0), 32), hi = min(max(till - c, 0), 32);
+            const uint32_t seen = (uint32_t)((1ull << hi) - 1) & ~(uint32_t)((1ull << lo) - 1);
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (c + i < from || c + i >= till) x[i] = __float_as_uint(-INFINITY);
+              if (!(seen >> i & 1)) x[i] = __float_as_uint(-INFINITY);
+            sp_st32(ts + c, x);
           };
           // the tile's maximum, 32 columns at a time, the next ones on their way
           float top = -INFINITY;
@@ -854,6 +839,11 @@ __global__ void __launch_bounds__(kSpThreads, 1)
             sp_ld32(ts + ((c + 64) & 127), x0);  // (at the end the first again, for the weights)
             maximum(x1, c + 32);
           }
+          if (!whole) {
+            sp_wait_st();
+            sp_wait_ld(x0);
+            sp_ld32(ts, x0);
+          }
           top *= a.scale_log2;
           if (__any_sync(0xffffffffu, top > m_ref + kSpGrow)) {
             const float now = fmaxf(m_ref, top);
@@ -873,23 +863,16 @@ __global__ void __launch_bounds__(kSpThreads, 1)
             }
           }
           const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
-          const uint64_t neg2 = sp_pair(neg, neg);
-          uint64_t sum0 = 0, sum1 = 0;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
           auto weights = [&](uint32_t(&x)[32], int c) {
-            if (!whole) hide(x, c);
             uint32_t w[32];  // 16 pairs of hi terms, 16 of lo terms
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float2 e = sp_unpair(
-                  sp_fma2(sp_pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, neg2));
-              const float p0 = sp_exp2(e.x), p1 = sp_exp2(e.y);
-              const uint64_t pp = sp_pair(p0, p1);
-              if (i & 1) sum1 = sp_add2(sum1, pp);
-              else sum0 = sp_add2(sum0, pp);
-              w[i] = pack2<T>(p0, p1);
-              const float2 h = unpack2<T>(w[i]);
-              const float2 r = sp_unpair(sp_fma2(sp_pair(h.x, h.y), neg1, pp));
-              w[16 + i] = pack2<T>(r.x, r.y);
+              const float p0 = sp_exp2(fmaf(__uint_as_float(x[2 * i]), a.scale_log2, neg));
+              const float p1 = sp_exp2(fmaf(__uint_as_float(x[2 * i + 1]), a.scale_log2, neg));
+              sum[(2 * i) & 3] += p0;
+              sum[(2 * i + 1) & 3] += p1;
+              pack2_split<T>(p0, p1, w[i], w[16 + i]);
             }
             sp_st32(ts + c, w);
           };
@@ -907,8 +890,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
               mbar_arrive(p_ready + 16 * stream);
             }
           }
-          const float2 t = sp_unpair(sp_add2(sum0, sum1));
-          l += t.x + t.y;
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           sp_wait_st();
         } else if (!rehearsal) {
           mbar_arrive(p_ready + 16 * stream);
@@ -1033,7 +1015,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(c
   const int64_t rh = SPREAD ? blockIdx.x : (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
   if (rh >= (int64_t)a.rows * a.hq) return;  // (whole warps, none of SPREAD's)
   const int row = (int)(rh / a.hq), head = (int)(rh % a.hq), h = head / G;
-  const int64_t units = s.begin[0].units;
+  const SpBegin share = s.begin[0];
   const SpRow at = s.rows[row];
   const int m = (row - at.row0) * G + head % G;  // query row in the group
   // the two segments: pieces, first owner, first place, places between pieces
@@ -1047,8 +1029,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(c
     len[part] = g.len;
     if (g.len == 0) continue;
     A[part] = g.unit0 + (int64_t)h * g.len;
-    b0[part] = sp_owner(A[part], units, s.ctas);
-    count[part] = sp_owner(A[part] + g.len - 1, units, s.ctas) - b0[part] + 1;
+    b0[part] = sp_owner(A[part], share, s.ctas);
+    count[part] = sp_owner(A[part] + g.len - 1, share, s.ctas) - b0[part] + 1;
     stride[part] = g.nq;
     place[part] = g.acc + (int64_t)h * g.maxp * g.nq + (part == 0 ? m % 256 : at.srow * G + head % G);
   }
@@ -1064,8 +1046,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(c
       const int k = own ? i - count[0] : i;
       const int64_t u0 = own ? A[1] : A[0];
       const int b = (own ? b0[1] : b0[0]) + k;
-      const int from = (int)max(sp_first(b, units, s.ctas) - u0, (int64_t)0);
-      const int till = (int)min(sp_first(b + 1, units, s.ctas) - u0, (int64_t)(own ? len[1] : len[0]));
+      const int from = (int)max(sp_first(b, share, s.ctas) - u0, (int64_t)0);
+      const int till = (int)min(sp_first(b + 1, share, s.ctas) - u0, (int64_t)(own ? len[1] : len[0]));
       src = (own ? place[1] : place[0]) + (int64_t)k * (own ? stride[1] : stride[0]);
       if (max(till - kSpStart, 0) > max(from - kSpStart, 0)) x = s.ml[src];  // (else nothing was written)
     }
