@@ -408,6 +408,23 @@ __device__ __forceinline__ void sp_wait_ld(uint32_t *r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : SP_M8(r, 0), SP_M8(r, 8), SP_M8(r, 16), SP_M8(r, 24)::"memory");
 }
+__device__ __forceinline__ void sp_ld16(uint32_t addr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15}, [%16];"
+      : SP_R8(r, 0), SP_R8(r, 8)
+      : "r"(addr));
+}
+__device__ __forceinline__ void sp_st16(uint32_t addr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15};" ::SP_U8(r, 0),
+      SP_U8(r, 8), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void sp_wait_ld16(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : SP_M8(r, 0), SP_M8(r, 8)::"memory");
+}
 __device__ __forceinline__ void sp_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -422,24 +439,49 @@ __device__ __forceinline__ void sp_load(uint32_t dst, const CUtensorMap *map, in
       "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row8), "r"(head), "r"(bar)
       : "memory");
 }
-// D[tmem] (+)= A[smem] . B[smem], and A[tmem] . B[smem]; descriptors as words
-__device__ __forceinline__ void sp_umma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
-                                           uint32_t b_hi, uint32_t idesc, bool accumulate) {
+// D[tmem] (+)= A[smem] . B[smem], and A[tmem] . B[smem], by the one thread
+// whose `one` is set; descriptors as words.  The whole warp comes here with the
+// same values, so they stay in the registers that the products are issued from:
+// under a branch on the lane a tile's products were issued in 1180 clocks, in
+// 955 this way.
+__device__ __forceinline__ void sp_umma_ss(uint32_t one, uint32_t d, uint32_t a_lo, uint32_t a_hi,
+                                           uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                           bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %6, 0;\n"
+      "{\n .reg .pred p, e;\n .reg .b64 a, b;\n setp.ne.b32 p, %6, 0;\n setp.ne.b32 e, %7, 0;\n"
       " mov.b64 a, {%1, %2};\n mov.b64 b, {%3, %4};\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}" ::"r"(d),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(one)
       : "memory");
 }
-__device__ __forceinline__ void sp_umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
-                                           uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void sp_umma_ts(uint32_t one, uint32_t d, uint32_t a, uint32_t b_lo,
+                                           uint32_t b_hi, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n"
+      "{\n .reg .pred p, e;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 e, %6, 0;\n"
       " mov.b64 b, {%2, %3};\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(one)
       : "memory");
+}
+__device__ __forceinline__ void sp_commit(uint32_t one, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar),
+      "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void sp_arrive(uint32_t one, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n @e mbarrier.arrive.shared::cta.b64 _, [%0];\n}" ::"r"(
+          bar),
+      "r"(one)
+      : "memory");
+}
+// one lane of a warp
+__device__ __forceinline__ uint32_t sp_elect() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}" : "=r"(one));
+  return one;
 }
 
 // d = max(a, b, c)
@@ -499,10 +541,15 @@ struct SpWalk {
 
 // Warps 0-3 and 4-7 are two softmax streams; warps 8 and 10 load keys and
 // values, warps 9 and 11 issue the products of a stream each (the waits of one
-// pass beside the products of the other).  Per 128-token tile of a stream:
-//   S[128 x 128] = Q . K^T                (tensor memory, fp32)
+// pass beside the products of the other).  A stream takes a 128-token tile in
+// two halves, which alternate between two places of its tensor memory:
+//   S[128 x 64] = Q . K^T                 (tensor memory, fp32)
 //   P = exp2(scale S - m), m the row's running maximum; a thread has a row
 //   O[128 x 128] += P . V                 (A = P from tensor memory)
+// While the exponentials of one half are taken, the other half's P . V and
+// next Q . K^T run, so a stream's softmax hardly waits for its own products
+// (4700 clocks for a tile of each stream; whole tiles, whose products take a
+// quarter less of the tensor pipe, 4900, two fifths of it that wait).
 // P takes S's place as two 16-bit terms, hi + lo (the weights keep ~16 bits;
 // one term alone costs the output half a step more), so P . V is two
 // products.  O is rescaled only when a row's maximum has grown by more than
@@ -523,12 +570,12 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   const uint32_t s_q = smem_u32(smem), s_kv = s_q + 2 * kSpTile;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + kSpSlots) * kSpTile);
   const uint32_t full = smem_u32(bars), empty = full + 8 * kSpSlots, s_full = empty + 8 * kSpSlots,
-                 p_ready = s_full + 16, o_done = p_ready + 32, q_ready = o_done + 8,
+                 p_ready = s_full + 32, o_done = p_ready + 32, q_ready = o_done + 8,
                  joint = q_ready + 8, drain = joint + 8,
-                 turn_of = drain + 8;
+                 pv_done = drain + 8;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_issued[2];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int G = a.hq / a.hk;
 
   if (tid == 0) {
@@ -538,13 +585,13 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       mbar_init(full + 8 * i);
       mbar_init_count(empty + 8 * i, 2);  // both streams, or one of them twice
     }
-    for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i);
+    for (int i = 0; i < 4; ++i) mbar_init(s_full + 8 * i);  // [stream][half]
     for (int i = 0; i < 4; ++i) mbar_init_count(p_ready + 8 * i, 128);
     mbar_init_count(o_done, 2);
     mbar_init_count(q_ready, 256);
     mbar_init_count(joint, 256);
     mbar_init_count(drain, 2);
-    for (int i = 0; i < 2; ++i) mbar_init(turn_of + 8 * i);
+    for (int i = 0; i < 4; ++i) mbar_init(pv_done + 8 * i);  // [stream][half]
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_abort = s_issued[0] = s_issued[1] = 0;
   }
@@ -612,104 +659,100 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       s_issued[is_v] = last;
     }
   } else if (warp == 9 || warp == 11) {
-    const uint32_t qk = umma_idesc<T, 128>(false), pv = qk | (1u << 16);  // V is dim-contiguous
+    const int st = warp == 11;
+    const uint32_t qk = umma_idesc<T, 64>(false);
+    const uint32_t pv = umma_idesc<T, 128>(false) | (1u << 16);  // V is dim-contiguous
     // Operand descriptors as two words; only the address (16-byte units, in
     // the low word) changes, so a product costs two additions to issue.
     constexpr uint32_t kHi = (1u << 14) | (2u << 29);  // version, 128-byte swizzle
     constexpr uint32_t kHiQ = kHi | 1024 / 16, kHiKv = kHi | 2048 / 16;
-    const int st = warp == 11;
-    const uint32_t ts = tmem + st * 128;
+    const uint32_t one = sp_elect(), ts = __reduce_max_sync(0xffffffffu, tmem) + st * 128;
     int i0 = 0, tiles = 0;  // loads, and this stream's tiles, of the pieces before
-    int turns = 0;
     bool ok = true, rehearsal = true;
-    // S of the stream's first tile, then O and the next S in turn.  `e` counts
-    // the tiles of both streams, this one's are those of its parity.  The
-    // second half of O with the next S is issued in the order of `e`: the
-    // streams then work half a period apart, one's products beside the other's
-    // exponentials (left alone they fall into step and wait for each other).
-    while (lane == 0 && ok) {  // one thread issues them
+    // S of the halves of a stream's first tile, then O of a half and S of the
+    // same half of its next tile in turn, the streams taking turns.  `e` counts
+    // the tiles of both, a stream's are those of its parity.
+    while (ok) {
       bool two = false;
       int n = 2;
       if (!rehearsal) {
-        if (!walk.next(s, p)) break;
-        n = p.n;
-        two = p.g.nq > 128;
-        ok = sp_wait(q_ready, (uint32_t)pieces & 1u);
+        if (!__any_sync(0xffffffffu, walk.next(s, p))) break;
+        n = __reduce_max_sync(0xffffffffu, p.n);
+        two = __reduce_max_sync(0xffffffffu, p.g.nq) > 128;
+        ok = __all_sync(0xffffffffu, sp_wait(q_ready, (uint32_t)pieces & 1u));
         if (!ok) break;
       }
-      // one query tile alternates between the two places
-      const uint32_t q0 = s_q + (two ? st : pieces & 1) * kSpTile;
-      const uint32_t a0 = (q0 >> 4) | 1u << 16;
       const int all = two ? 2 * n : n;
-      for (int e = st - 2; e < all; e += 2) {
-        if (e >= 0) {
+      for (int u = 0; ok && u < 2 * ((all - st + 1) / 2 + 1); ++u) {
+        const int half = u & 1, k = (u >> 1) - 1, e = 2 * k + st;
+        const uint32_t th = ts + half * 64;
+        if (k >= 0) {  // O, this half of the stream's tile k
           const int v = i0 + (two ? e | 1 : min(2 * e + 2, 2 * n - 1));  // the load of its V
           const uint32_t slot = (uint32_t)v % kSpSlots, turn = (uint32_t)v / kSpSlots;
-          const uint32_t b0 = ((s_kv + slot * kSpTile) >> 4) | (1024 / 16) << 16;
+          const uint32_t b0 =
+              ((s_kv + slot * kSpTile + half * (kSpTile / 2)) >> 4) | (1024 / 16) << 16;
           if (!rehearsal) {
-            ok = sp_wait(full + 8 * slot, turn & 1u);
+            ok = (half == 1 || sp_wait(full + 8 * slot, turn & 1u)) &&
+                 sp_wait(p_ready + 16 * st + 8 * half, (uint32_t)(tiles + k) & 1u);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
           }
+          tc_fence_after();
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {  // 64 tokens, as their weights come
-            if (!rehearsal) {
-              ok = sp_wait(p_ready + 16 * st + 8 * part, (uint32_t)tiles & 1u) &&
-                   (part == 0 || e == 0 || sp_wait(turn_of + 8 * st, (uint32_t)turns++ & 1u));
-              if (!ok) break;
-            }
-            tc_fence_after();
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {  // 16 tokens, the hi terms, then the lo ones
-              const int c = part * 4 + (x >> 1);
-              sp_umma_ts(ts + 256, ts + (c >> 1) * 32 + (c & 1) * 8 + (x & 1) * 16,
-                         b0 + c * (4096 / 16), kHiKv, pv, part + x > 0 || e >= 2);
-            }
+          for (int x = 0; x < 8; ++x) {  // 16 tokens, the hi terms, then the lo ones
+            const int c = x >> 1;
+            sp_umma_ts(one, ts + 256, th + (c >> 1) * 32 + (c & 1) * 8 + (x & 1) * 16,
+                       b0 + c * (4096 / 16), kHiKv, pv, x + half + k > 0);
           }
-          if (!ok) break;
-          ++tiles;
           if (!rehearsal) {
-            umma_commit(empty + 8 * slot);
-            if (!two) mbar_arrive(empty + 8 * slot);
+            sp_commit(one, pv_done + 16 * st + 8 * half);
+            if (half == 1) {
+              sp_commit(one, empty + 8 * slot);
+              if (!two) sp_arrive(one, empty + 8 * slot);
+            }
           }
         }
-        if (e + 2 < all) {
-          const int k = i0 + (two ? (e + 2) & ~1 : (e < 0 ? e + 2 : 2 * e + 3));  // of its K
-          const uint32_t slot = (uint32_t)k % kSpSlots, turn = (uint32_t)k / kSpSlots;
-          const uint32_t b0 = ((s_kv + slot * kSpTile) >> 4) | 1u << 16;
+        if (e + 2 < all) {  // S, this half of its next tile
+          const int kl = i0 + (two ? (e + 2) & ~1 : (k < 0 ? e + 2 : 2 * e + 3));  // the load of its K
+          const uint32_t slot = (uint32_t)kl % kSpSlots, turn = (uint32_t)kl / kSpSlots;
+          const uint32_t b0 = ((s_kv + slot * kSpTile + half * (kSpTile / 2)) >> 4) | 1u << 16;
+          // one query tile alternates between the two places
+          const uint32_t a0 = ((s_q + (two ? st : pieces & 1) * kSpTile) >> 4) | 1u << 16;
           if (!rehearsal) {
-            ok = sp_wait(full + 8 * slot, turn & 1u);
+            ok = __all_sync(0xffffffffu, half == 1 || sp_wait(full + 8 * slot, turn & 1u));
             if (!ok) break;
           }
           tc_fence_after();
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
             const uint32_t d = (x & 3) * (32 / 16);
-            sp_umma_ss(ts, a0 + (x >> 2) * (kSpHalf / 16) + d, kHiQ,
+            sp_umma_ss(one, th, a0 + (x >> 2) * (kSpHalf / 16) + d, kHiQ,
                        b0 + (x >> 2) * (1024 / 16) + d, kHiKv, qk, x > 0);
           }
           if (!rehearsal) {
-            umma_commit(s_full + 8 * st);
-            umma_commit(empty + 8 * slot);
-            if (!two) mbar_arrive(empty + 8 * slot);
+            sp_commit(one, s_full + 16 * st + 8 * half);
+            if (half == 1) {
+              sp_commit(one, empty + 8 * slot);
+              if (!two) sp_arrive(one, empty + 8 * slot);
+            }
           }
         }
-        if (!rehearsal && e >= 0 && e + 1 < all) mbar_arrive(turn_of + 8 * (st ^ 1));
       }
       if (!ok) break;
       if (rehearsal) {  // (on whatever shared memory holds; the sums are not used)
         rehearsal = false;
-        tiles = 0;
-        umma_commit(drain);
-        ok = sp_wait(drain, 0);
+        sp_commit(one, drain);
+        ok = __all_sync(0xffffffffu, sp_wait(drain, 0));
         pdl_begin();
         walk.begin(s);
         continue;
       }
       i0 += 2 * n;
-      umma_commit(o_done);
+      tiles += (all - st + 1) / 2;
+      sp_commit(one, o_done);
       ++pieces;
     }
-    if (!ok) stop();
+    if (!ok && lane == 0) stop();
   } else if (warp < 8) {
     const int stream = warp >> 2, m128 = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -779,16 +822,19 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       const bool works = __any_sync(0xffffffffu, mine);
       const int count = rehearsal ? 1 : two ? n : (n - stream + 1) / 2;
       float m_ref = -INFINITY, l = 0.f;
-      for (int k = 0; k < count; ++k) {
-        const int j = two ? k : 2 * k + stream;
+#pragma unroll 1
+      for (int u = 0; u < 2 * count; ++u) {
+        const int k = u >> 1, half = u & 1, j = two ? k : 2 * k + stream;
         const int T0 = p.g.base + (p.t0 + j) * kSpTok;
+        const uint32_t th = ts + half * 64;
         if (!rehearsal) {
-          ok = __all_sync(0xffffffffu, sp_wait(s_full + 8 * stream, (uint32_t)(kt + k) & 1u));
+          ok = __all_sync(0xffffffffu, sp_wait(s_full + 16 * stream + 8 * half, (uint32_t)(kt + k) & 1u));
           if (!ok) break;
           tc_fence_after();
           // What a page holds behind the segment's end has weights of zero, but
-          // zero times what lies there may not be: those values become zeros.
-          if (T0 + kSpTok > p.g.tok1 && (!two || stream == 0)) {
+          // zero times what lies there may not be: those values become zeros
+          // (two streams write theirs both, each before its own products).
+          if (half == 0 && T0 + kSpTok > p.g.tok1) {
             const int i = i0 + (two ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1));
             ok = __all_sync(0xffffffffu, sp_wait(full + 8 * (i % kSpSlots),
                                                  (uint32_t)(i / kSpSlots) & 1u));
@@ -804,67 +850,58 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           }
         }
         if (works) {
-          const int from = p.g.tok0 - T0, till = (rehearsal ? kSpTok : lim - T0);  // columns seen
-          const bool whole = __all_sync(0xffffffffu, from <= 0 && till >= kSpTok);
-          // Columns that the row does not see become -inf, here and in the
-          // tensor memory that the weights are made from.
-          auto hide = [&](uint32_t(&x)[32], int c) {
-            const int lo = min(max(from - c, 0), 32), hi = min(max(till - c, 0), 32);
-            const uint32_t seen = (uint32_t)((1ull << hi) - 1) & ~(uint32_t)((1ull << lo) - 1);
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(seen >> i & 1)) x[i] = __float_as_uint(-INFINITY);
-            sp_st32(ts + c, x);
-          };
-          // the tile's maximum, 32 columns at a time, the next ones on their way
-          float top = -INFINITY;
           uint32_t x0[32], x1[32];
-          auto maximum = [&](uint32_t(&x)[32], int c) {
-            if (!whole) hide(x, c);
-            float t0 = -INFINITY, t1 = -INFINITY;
+          sp_ld32(th, x0);
+          sp_ld32(th + 32, x1);
+          // columns of this half that the row sees
+          const int from = min(max(p.g.tok0 - T0 - half * 64, 0), 64);
+          const int till = min(max((rehearsal ? kSpTok : lim - T0) - half * 64, 0), 64);
+          sp_wait_ld(x0);
+          sp_wait_ld(x1);
+          if (!__all_sync(0xffffffffu, from <= 0 && till >= 64)) {
+            const uint64_t seen = (till < 64 ? (1ull << till) - 1 : ~0ull) &
+                                  (from < 64 ? ~((1ull << from) - 1) : 0ull);
+            const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              t0 = sp_max3(t0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-              t1 = sp_max3(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+            for (int i = 0; i < 32; ++i) {
+              if (!(s0 >> i & 1)) x0[i] = __float_as_uint(-INFINITY);
+              if (!(s1 >> i & 1)) x1[i] = __float_as_uint(-INFINITY);
             }
-            top = sp_max3(top, t0, t1);
-          };
-          sp_ld32(ts, x0);
-#pragma unroll 1
-          for (int c = 0; c < 128; c += 64) {
-            sp_wait_ld(x0);
-            sp_ld32(ts + c + 32, x1);
-            maximum(x0, c);
-            sp_wait_ld(x1);
-            sp_ld32(ts + ((c + 64) & 127), x0);  // (at the end the first again, for the weights)
-            maximum(x1, c + 32);
           }
-          if (!whole) {
-            sp_wait_st();
-            sp_wait_ld(x0);
-            sp_ld32(ts, x0);
+          float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            t0 = sp_max3(t0, __uint_as_float(x0[i]), __uint_as_float(x0[i + 1]));
+            t1 = sp_max3(t1, __uint_as_float(x0[i + 2]), __uint_as_float(x0[i + 3]));
+            t2 = sp_max3(t2, __uint_as_float(x1[i]), __uint_as_float(x1[i + 1]));
+            t3 = sp_max3(t3, __uint_as_float(x1[i + 2]), __uint_as_float(x1[i + 3]));
           }
-          top *= a.scale_log2;
+          const float top = fmaxf(sp_max3(t0, t1, t2), t3) * a.scale_log2;
           if (__any_sync(0xffffffffu, top > m_ref + kSpGrow)) {
             const float now = fmaxf(m_ref, top);
             const float f = now == -INFINITY ? 1.f : sp_exp2(m_ref - now);
             m_ref = now;
             l *= f;
-            if (k > 0) {
+            if (u > 0 && !rehearsal) {
+              // O is whole once the half before this one has been added
+              ok = __all_sync(0xffffffffu, sp_wait(pv_done + 16 * stream + 8 * (half ^ 1),
+                                                   (uint32_t)(kt + ((u - 1) >> 1)) & 1u));
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < 128; c += 32) {
-                uint32_t o[32];
-                sp_ld32(to + c, o);
-                sp_wait_ld(o);
+              for (int c = 0; c < 128; c += 16) {
+                uint32_t o[16];
+                sp_ld16(to + c, o);
+                sp_wait_ld16(o);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                sp_st32(to + c, o);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                sp_st16(to + c, o);
               }
             }
           }
           const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          auto weights = [&](uint32_t(&x)[32], int c) {
+          auto weights = [&](const uint32_t(&x)[32], int c) {
             uint32_t w[32];  // 16 pairs of hi terms, 16 of lo terms
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -874,29 +911,15 @@ __global__ void __launch_bounds__(kSpThreads, 1)
               sum[(2 * i + 1) & 3] += p1;
               pack2_split<T>(p0, p1, w[i], w[16 + i]);
             }
-            sp_st32(ts + c, w);
+            sp_st32(th + c, w);
           };
-#pragma unroll 1
-          for (int c = 0; c < 128; c += 64) {
-            sp_wait_ld(x0);
-            sp_ld32(ts + c + 32, x1);
-            weights(x0, c);
-            sp_wait_ld(x1);
-            if (c == 0) sp_ld32(ts + 64, x0);
-            weights(x1, c + 32);
-            if (c == 0 && !rehearsal) {  // half of the tile's weights are there
-              sp_wait_st();
-              tc_fence_before();
-              mbar_arrive(p_ready + 16 * stream);
-            }
-          }
+          weights(x0, 0);
+          weights(x1, 32);
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           sp_wait_st();
-        } else if (!rehearsal) {
-          mbar_arrive(p_ready + 16 * stream);
         }
         tc_fence_before();
-        if (!rehearsal) mbar_arrive(p_ready + 16 * stream + 8);
+        if (!rehearsal) mbar_arrive(p_ready + 16 * stream + 8 * half);
       }
       if (!ok) break;
       if (rehearsal) {
@@ -985,8 +1008,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     if (tid < 2)  // (of the keys, and of the values: no more than the ring holds)
       for (int i = max(0, s_issued[tid] - kSpSlots); i < s_issued[tid]; ++i)
         mbar_wait(full + 8 * (i % kSpSlots), (uint32_t)(i / kSpSlots) & 1u);
-    if (tid == 9 * 32 || tid == 11 * 32) {
-      umma_commit(drain);
+    if (warp == 9 || warp == 11) {
+      sp_commit(sp_elect(), drain);
       mbar_wait(drain, 1);
     }
     __syncthreads();
