@@ -69,6 +69,7 @@ struct SpArgs {
   SpSeg *segs;
   SpRow *rows;
   int32_t *gseg;       // [groups] first prefix segment of each
+  int32_t *pieces;     // [segs, kv heads] pieces of a segment with tokens
   float *acc;          // [rows of partial sums, D]
   float2 *ml;          // [rows of partial sums]: maximum (log2), sum
 };
@@ -497,10 +498,11 @@ __device__ __forceinline__ void sp_st_global8(float *p, const float (&v)[8]) {
                : "memory");
 }
 
-// A CTA's share of a segment's kv head: tiles [t0, t0 + n) from `base`.
+// A CTA's share of a segment's kv head: tiles [t0, t0 + n) from `base`, the
+// index-th of the shares that have tiles.
 struct SpPiece {
   SpSeg g;
-  int h, t0, n, index;
+  int seg, h, t0, n, index;
 };
 
 // The pieces of this CTA, in order; every role walks them for itself.
@@ -531,8 +533,11 @@ struct SpWalk {
       p.t0 = max(a - kSpStart, 0);
       p.n = max(b - kSpStart, 0) - p.t0;
       if (p.n <= 0) continue;
-      p.index = (int)blockIdx.x -
-                sp_owner(p.g.unit0 + (int64_t)p.h * p.g.len, share, s.ctas);
+      p.seg = seg;
+      // (fewer units than CTAs: every tile is a piece)
+      p.index = share.share == 0
+                    ? a - kSpStart
+                    : (int)blockIdx.x - sp_owner(p.g.unit0 + (int64_t)p.h * p.g.len + kSpStart, share, s.ctas);
       return true;
     }
     return false;
@@ -939,6 +944,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       tc_fence_after();
       const int64_t at = p.g.acc + ((int64_t)p.h * p.g.maxp + p.index) * nq + m;
       float *part = s.acc + at * kTaD;
+      if (tid == 0 && p.t0 + n == p.g.len - kSpStart) s.pieces[(int64_t)p.seg * a.hk + p.h] = p.index + 1;
       if (two) {
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
@@ -1022,10 +1028,10 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 constexpr int kMergeWarps = 4;
 
 // A CTA a (row, query head), a lane four of its dims: warp w takes pieces w,
-// w + 4, ... of the prefix and, behind them, of the row's own tokens, and the
-// warps' sums are joined in order.  One warp a (row, head) instead (SPREAD
-// false) when they alone fill the GPU: 2560 of a few pieces each, 11.8 us
-// against 19.8.
+// w + 4, ... of the prefix and, behind them, of the row's own tokens, eight
+// loads on their way, and the warps' sums are joined in order.  One warp a
+// (row, head) instead (SPREAD false) when they alone fill the GPU: 2560 of a
+// few pieces each, 11.8 us against 19.8.
 template <typename T, bool SPREAD>
 __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(const SpArgs s) {
   __shared__ float4 s_acc[kMergeWarps][32];
@@ -1037,65 +1043,59 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(c
   const int warp = SPREAD ? threadIdx.x >> 5 : 0;
   const int64_t rh = SPREAD ? blockIdx.x : (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
   if (rh >= (int64_t)a.rows * a.hq) return;  // (whole warps, none of SPREAD's)
-  const int row = (int)(rh / a.hq), head = (int)(rh % a.hq), h = head / G;
-  const SpBegin share = s.begin[0];
+  const int row = (int)(rh / a.hq), head = (int)(rh - (int64_t)row * a.hq), h = head / G;
   const SpRow at = s.rows[row];
   const int m = (row - at.row0) * G + head % G;  // query row in the group
-  // the two segments: pieces, first owner, first place, places between pieces
-  int count[2] = {0, 0}, b0[2] = {0, 0}, len[2] = {0, 0}, stride[2] = {0, 0};
-  int64_t A[2] = {0, 0}, place[2] = {0, 0};
+  // the two segments: pieces, first place, places between pieces
+  int count[2] = {0, 0}, stride[2] = {0, 0};
+  int64_t place[2] = {0, 0};
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     const int seg = part == 0 ? (at.pseg < 0 ? -1 : at.pseg + m / 256) : at.sseg;
     if (seg < 0) continue;
     const SpSeg &g = s.segs[seg];
-    len[part] = g.len;
-    if (g.len == 0) continue;
-    A[part] = g.unit0 + (int64_t)h * g.len;
-    b0[part] = sp_owner(A[part], share, s.ctas);
-    count[part] = sp_owner(A[part] + g.len - 1, share, s.ctas) - b0[part] + 1;
+    const int pieces = s.pieces[(int64_t)seg * a.hk + h];
+    if (g.len == 0) continue;  // (and `pieces` was never written)
+    count[part] = pieces;
     stride[part] = g.nq;
     place[part] = g.acc + (int64_t)h * g.maxp * g.nq + (part == 0 ? m % 256 : at.srow * G + head % G);
   }
   const int all = count[0] + count[1];
   float M = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int base = warp; base < all; base += 32 * kStep) {
-    const int i = base + lane * kStep;
-    float2 x = make_float2(-INFINITY, 0.f);
-    int64_t src = 0;
-    if (i < all) {
-      const bool own = i >= count[0];
-      const int k = own ? i - count[0] : i;
-      const int64_t u0 = own ? A[1] : A[0];
-      const int b = (own ? b0[1] : b0[0]) + k;
-      const int from = (int)max(sp_first(b, share, s.ctas) - u0, (int64_t)0);
-      const int till = (int)min(sp_first(b + 1, share, s.ctas) - u0, (int64_t)(own ? len[1] : len[0]));
-      src = (own ? place[1] : place[0]) + (int64_t)k * (own ? stride[1] : stride[0]);
-      if (max(till - kSpStart, 0) > max(from - kSpStart, 0)) x = s.ml[src];  // (else nothing was written)
-    }
-    float top = x.x;
+#pragma unroll 1
+  for (int base = warp; base < all; base += 8 * kStep) {
+    float4 v[8];
+    float2 x[8];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float now = fmaxf(M, top);
+    for (int j = 0; j < 8; ++j) {
+      const int i = base + j * kStep;
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      x[j] = make_float2(-INFINITY, 0.f);
+      if (i < all) {
+        const bool own = i >= count[0];
+        const int64_t src = (own ? place[1] : place[0]) +
+                            (int64_t)(own ? i - count[0] : i) * (own ? stride[1] : stride[0]);
+        x[j] = s.ml[src];
+        v[j] = *reinterpret_cast<const float4 *>(s.acc + src * kTaD + 4 * lane);
+      }
+    }
+    float now = M;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) now = fmaxf(now, x[j].x);
     if (now == -INFINITY) continue;
-    const float f = exp2f(M - now);
+    const float f = sp_exp2(M - now);
     M = now;
-    acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-    const float w = x.x == -INFINITY ? 0.f : exp2f(x.x - now);
-    sum = fmaf(sum, f, warp_sum(w * x.y));
-    const int n = min(32, (all - 1 - base) / kStep + 1);
-    const unsigned live = __ballot_sync(0xffffffffu, x.x != -INFINITY);
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      const int64_t sj = __shfl_sync(0xffffffffu, src, j);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (live >> j & 1) v = *reinterpret_cast<const float4 *>(s.acc + sj * kTaD + 4 * lane);
-      acc.x = fmaf(v.x, wj, acc.x);
-      acc.y = fmaf(v.y, wj, acc.y);
-      acc.z = fmaf(v.z, wj, acc.z);
-      acc.w = fmaf(v.w, wj, acc.w);
+    sum *= f, acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (x[j].x == -INFINITY) continue;  // (nothing seen: its sums are nothing, too)
+      const float w = sp_exp2(x[j].x - now);
+      sum = fmaf(x[j].y, w, sum);
+      acc.x = fmaf(v[j].x, w, acc.x);
+      acc.y = fmaf(v[j].y, w, acc.y);
+      acc.z = fmaf(v[j].z, w, acc.z);
+      acc.w = fmaf(v[j].w, w, acc.w);
     }
   }
   float top = M;
@@ -1112,7 +1112,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(c
 #pragma unroll
     for (int w = 0; w < kMergeWarps; ++w) {
       if (s_ml[w].x == -INFINITY) continue;
-      const float f = exp2f(s_ml[w].x - top);
+      const float f = sp_exp2(s_ml[w].x - top);
       const float4 v = s_acc[w][lane];
       sum = fmaf(s_ml[w].y, f, sum);
       acc.x = fmaf(v.x, f, acc.x);
@@ -1153,7 +1153,7 @@ struct SpPlan {
   int box;             // 0: pages that no TMA box fits (every row for itself)
   int64_t splits;      // of a row, without boxes
   // scratch, in floats (every part a multiple of 16 bytes)
-  int64_t begin, segs, rows, gseg, acc, ml, total;
+  int64_t begin, segs, rows, gseg, pieces, acc, ml, total;
 };
 
 SpPlan plan_for(int rows, int hq, int hk, int groups, int bs, int max_prefix, int max_suffix) {
@@ -1183,7 +1183,8 @@ SpPlan plan_for(int rows, int hq, int hk, int groups, int bs, int max_prefix, in
   p.segs = ctas * 4;
   p.rows = p.segs + segs * 16;
   p.gseg = p.rows + (int64_t)rows * 4;
-  p.ml = round(p.gseg + groups);
+  p.pieces = round(p.gseg + groups);
+  p.ml = round(p.pieces + segs * hk);
   p.acc = round(p.ml + 2 * sums);
   p.total = p.acc + sums * kTaD;
   return p;
@@ -1210,6 +1211,7 @@ template <typename T> int run_typed(SpArgs &s, const SpPlan &p, float *scratch, 
   s.segs = reinterpret_cast<SpSeg *>(scratch + p.segs);
   s.rows = reinterpret_cast<SpRow *>(scratch + p.rows);
   s.gseg = reinterpret_cast<int32_t *>(scratch + p.gseg);
+  s.pieces = reinterpret_cast<int32_t *>(scratch + p.pieces);
   s.ml = reinterpret_cast<float2 *>(scratch + p.ml);
   s.acc = scratch + p.acc;
   auto kern = shared_prefix_kernel<T>;
