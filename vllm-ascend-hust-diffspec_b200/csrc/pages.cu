@@ -14,12 +14,17 @@
 namespace dsb {
 namespace {
 
-constexpr int kPgThreads = 1024;    // of a planning CTA
+// A planning CTA has 256 threads when they see its pages in one turn (and the
+// call's rows are few), else 1024: what such a call takes is the latency of its
+// barriers and dependent reads (512 pages to compact: 13 us with 1024 threads,
+// 6.5 with 256).
+constexpr int kPgThreads = 1024, kPgFew = 256;
 constexpr int kPgPages = 16;        // pages a thread looks at in a turn
 constexpr int kPgTurn = kPgThreads * kPgPages;
-// The planning CTAs are a cluster, each with a stretch of the pool: one for
-// pools of up to four turns, whose counts it reads in ~2 us, else eight (a
-// cluster's barriers cost about as much).
+// The planning CTAs are a cluster, each with a stretch of the pool: one CTA as
+// long as it sees the pool in one turn, else eight (40000 pages, 64 children:
+// 19 us by one, 15 by eight; a turn's masks are kept in registers from the
+// count to the pages handed out).
 constexpr int kPgCluster = 8;
 constexpr int kPgMaxRows = 4096;    // rows of one call
 constexpr int kPgMaxCaches = 128;   // caches of one launch
@@ -45,14 +50,13 @@ struct Caches {
 };
 
 // Sum of the warps' values before this warp's; `total` gets the sum of all.
-__device__ int warps_before(int mine, int32_t *warp_tot, int &total) {
-  constexpr int kWarps = kPgThreads / 32;
+template <int T> __device__ int warps_before(int mine, int32_t *warp_tot, int &total) {
   if ((threadIdx.x & 31) == 0) warp_tot[threadIdx.x >> 5] = mine;
   __syncthreads();
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < T / 32; ++w) {
     if (w == (int)(threadIdx.x >> 5)) before = total;
     total += warp_tot[w];
   }
@@ -61,23 +65,23 @@ __device__ int warps_before(int mine, int32_t *warp_tot, int &total) {
 }
 
 // Inclusive prefix sum over the CTA's threads.
-__device__ int block_scan(int v, int32_t *warp_tot, int &total) {
+template <int T> __device__ int block_scan(int v, int32_t *warp_tot, int &total) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += x;
   }
-  return warps_before(__shfl_sync(0xffffffffu, v, 31), warp_tot, total) + v;
+  return warps_before<T>(__shfl_sync(0xffffffffu, v, 31), warp_tot, total) + v;
 }
 
 // a[0..n) in shared memory becomes its inclusive prefix sum.
-__device__ int scan_rows(int32_t *a, int n, int32_t *warp_tot) {
+template <int T> __device__ int scan_rows(int32_t *a, int n, int32_t *warp_tot) {
   int run = 0;
-  for (int base = 0; base < n; base += kPgThreads) {
+  for (int base = 0; base < n; base += T) {
     const int i = base + threadIdx.x;
     int total;
-    const int s = block_scan(i < n ? a[i] : 0, warp_tot, total) + run;
+    const int s = block_scan<T>(i < n ? a[i] : 0, warp_tot, total) + run;
     if (i < n) a[i] = s;
     run += total;
   }
@@ -122,33 +126,60 @@ struct Stretch {
   }
 };
 
-// The CTA's stretch in turns of kPgTurn pages: look(page, count) for each page
-// of a thread, side by side in a warp (a warp has 256 pages in a row, a thread
-// every 32nd of them), with the loads of a turn all on their way at once.
+// The CTA's stretch in turns of 16 pages a thread: look(j, page, count) for
+// each page of a thread, side by side in a warp (a warp has 512 pages in a row,
+// a thread every 32nd of them), with the loads of a turn all on their way at
+// once.
+__device__ __forceinline__ int64_t warp_page(int64_t base, int j) {
+  return base + (int64_t)(threadIdx.x >> 5) * 32 * kPgPages + 32 * j;
+}
 template <typename F> __device__ __forceinline__ void read_turn(const Pool &p, int64_t base, int64_t till, F look) {
   int v[kPgPages];
-  const int64_t first = base + (int64_t)(threadIdx.x >> 5) * 32 * kPgPages + (threadIdx.x & 31);
+  const int64_t first = warp_page(base, 0) + (threadIdx.x & 31);
 #pragma unroll
   for (int j = 0; j < kPgPages; ++j) v[j] = first + 32 * j < till ? __ldcg(p.refs + first + 32 * j) : -1;
 #pragma unroll
   for (int j = 0; j < kPgPages; ++j) look(j, first + 32 * j, v[j]);  // (behind `till`: -1)
 }
 
-// Free pages of the CTA's stretch; counts below zero (pages let go more often
-// than they were held) are flagged and cleared.
-__device__ int free_pages(const Pool &p, const Stretch &s, int32_t *warp_tot) {
-  int mine = 0, total;
-  for (int64_t base = s.from; base < s.till; base += kPgTurn)
-    read_turn(p, base, s.till, [&](int, int64_t page, int v) {
-      if (v < 0 && page < s.till) {
-        p.refs[page] = 0;
-        flag_error(p.err, DSB_FLAG_BLOCK);
-        v = 0;
-      }
-      mine += v == 0;
+// The free pages of the CTA's stretch: their number, and of its last turn
+// (`whole`: its only one) a mask for each 32 pages of the warp and the free
+// ones before the warp.
+template <int T> struct Free {
+  unsigned mask[kPgPages];
+  int before, total;
+  bool whole;
+  __device__ __forceinline__ int read(const Pool &p, const Stretch &s, int64_t base) {
+    int mine = 0;
+    read_turn(p, base, s.till, [&](int j, int64_t, int v) {
+      mask[j] = __ballot_sync(0xffffffffu, v == 0);
+      mine += __popc(mask[j]);
     });
-  block_scan(mine, warp_tot, total);
-  return total;
+    return mine;
+  }
+  // Counts below zero (pages let go more often than they were held) are
+  // flagged and cleared.
+  __device__ __forceinline__ void count(const Pool &p, const Stretch &s, int32_t *warp_tot) {
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < kPgPages; ++j) mask[j] = 0;
+    for (int64_t base = s.from; base < s.till; base += T * kPgPages)
+      read_turn(p, base, s.till, [&](int j, int64_t page, int v) {
+        if (v < 0 && page < s.till) {
+          p.refs[page] = 0;
+          flag_error(p.err, DSB_FLAG_BLOCK);
+          v = 0;
+        }
+        mask[j] = __ballot_sync(0xffffffffu, v == 0);
+        mine += __popc(mask[j]);
+      });
+    before = warps_before<T>(mine, warp_tot, total);
+    whole = s.till - s.from <= T * kPgPages;
+  }
+};
+// The lowest x of 32 bits.
+__device__ __forceinline__ unsigned low_bits(int x) {
+  return x <= 0 ? 0u : x >= 32 ? ~0u : (1u << x) - 1;
 }
 
 // Drop `n` references to `page`.  More than there are leave a negative count,
@@ -193,41 +224,37 @@ struct PageCounts {
 // Hand the lowest free pages out: want[] is the inclusive prefix sum of the
 // rows' needs, `granted` the pages given in all, `run` the free pages before
 // this CTA's stretch; give(i, k, page) stores row i's k-th new page.
-template <typename F>
-__device__ void allot(const Pool &p, const Stretch &s, const int32_t *want, int n, int granted, int run,
-                      int32_t *warp_tot, F give) {
-  const unsigned below = (1u << (threadIdx.x & 31)) - 1;
-  for (int64_t base = s.from; base < s.till && run < granted; base += kPgTurn) {
-    unsigned mask[kPgPages];
-    int mine = 0, total;
-    read_turn(p, base, s.till, [&](int j, int64_t, int v) {
-      mask[j] = __ballot_sync(0xffffffffu, v == 0);
-      mine += __popc(mask[j]);
-    });
-    int rank = run + warps_before(mine, warp_tot, total);
-    const int64_t first = base + (int64_t)(threadIdx.x >> 5) * 32 * kPgPages + (threadIdx.x & 31);
+template <int T, typename F>
+__device__ void allot(const Pool &p, const Stretch &s, Free<T> &free, const int32_t *want, int n, int granted,
+                      int run, int32_t *warp_tot, F give) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t base = s.from; base < s.till && run < granted; base += T * kPgPages) {
+    if (!free.whole) free.before = warps_before<T>(free.read(p, s, base), warp_tot, free.total);
+    int rank = run + free.before;
 #pragma unroll
     for (int j = 0; j < kPgPages; ++j) {
-      const int k = rank + __popc(mask[j] & below);
-      rank += __popc(mask[j]);
-      if (!(mask[j] >> (threadIdx.x & 31) & 1) || k >= granted) continue;
+      const unsigned mask = free.mask[j];
+      const int k = rank + __popc(mask & ((1u << lane) - 1));
+      rank += __popc(mask);
+      if (!(mask >> lane & 1) || k >= granted) continue;
       int lo = 0, hi = n - 1;  // first row whose prefix sum passes the rank
       while (lo < hi) {
         const int mid = (lo + hi) / 2;
         if (want[mid] > k) hi = mid;
         else lo = mid + 1;
       }
-      p.refs[first + 32 * j] = 1;
-      give(lo, k - (lo > 0 ? want[lo - 1] : 0), (int)(first + 32 * j));
+      const int page = (int)warp_page(base, j) + lane;
+      p.refs[page] = 1;
+      give(lo, k - (lo > 0 ? want[lo - 1] : 0), page);
     }
-    run += total;
+    run += free.total;
   }
 }
 
 // Rows given twice in one call: the first counts, the others are flagged.
 // again[i] for rows[0..n) in shared memory, a warp a row.
-__device__ void find_repeats(const int32_t *rows, int32_t *again, int n) {
-  for (int i = threadIdx.x >> 5; i < n; i += kPgThreads / 32) {
+template <int T> __device__ void find_repeats(const int32_t *rows, int32_t *again, int n) {
+  for (int i = threadIdx.x >> 5; i < n; i += T / 32) {
     bool hit = false;
     for (int j = threadIdx.x & 31; j < i; j += 32) hit |= rows[j] == rows[i];
     hit = __any_sync(0xffffffffu, hit);
@@ -299,29 +326,29 @@ __global__ void __launch_bounds__(256)
 
 // Every CTA of the cluster has the rows' needs; the first one changes what
 // they hold and reports.
-__global__ void __launch_bounds__(kPgThreads)
+template <int T> __global__ void __launch_bounds__(T)
     resize_kernel(const Pool p, const int32_t *__restrict__ rows, const int32_t *__restrict__ lens,
                   int n, int alone, int ranks) {
   extern __shared__ int32_t pg_smem[];
   int32_t *want = pg_smem, *row = want + n, *has = row + n, *target = has + n;
-  __shared__ int32_t warp_tot[kPgThreads / 32], told[kPgCluster];
+  __shared__ int32_t warp_tot[T / 32], told[kPgCluster];
   __shared__ int lacking, granted;
   pdl_begin();
   const Stretch s(p.pages, ranks, told);
   const int tid = threadIdx.x;
   if (tid == 0) lacking = granted = 0;
-  for (int i = tid; i < n; i += kPgThreads) row[i] = rows[i];
+  for (int i = tid; i < n; i += T) row[i] = rows[i], target[i] = lens[i];
   __syncthreads();
-  find_repeats(row, want, n);
+  find_repeats<T>(row, want, n);
   __syncthreads();
-  for (int i = tid; i < n; i += kPgThreads) {
+  for (int i = tid; i < n; i += T) {
     const int r = row[i];
     int have = 0, need = -1;
     if (r < 0 || r >= p.rows || want[i]) {
       if (s.rank == 0) flag_error(p.err, DSB_FLAG_SLOT);
     } else {
       have = pages_held(p, r);
-      need = pages_needed(p, lens[i]);
+      need = pages_needed(p, target[i]);
       if (need < 0 && s.rank == 0) flag_error(p.err, DSB_FLAG_POSITION);
     }
     has[i] = have;
@@ -331,7 +358,7 @@ __global__ void __launch_bounds__(kPgThreads)
   __syncthreads();
   // releases first, a warp a row (unless release_kernel has let them go)
   if (alone) {
-    for (int i = tid >> 5; i < n && s.rank == 0; i += kPgThreads / 32) {
+    for (int i = tid >> 5; i < n && s.rank == 0; i += T / 32) {
       if (target[i] < 0) continue;
       int32_t *t = p.tables + (int64_t)row[i] * p.stride;
       for (int j = target[i] + (tid & 31); j < has[i]; j += 32) {
@@ -341,11 +368,13 @@ __global__ void __launch_bounds__(kPgThreads)
     }
     s.sync();
   }
+  Free<T> free;
+  free.count(p, s, warp_tot);
   int before;
-  const int nfree = s.gather(free_pages(p, s, warp_tot), before);
-  scan_rows(want, n, warp_tot);
+  const int nfree = s.gather(free.total, before);
+  scan_rows<T>(want, n, warp_tot);
   // rows in order until the first that does not fit
-  for (int i = tid; i < n; i += kPgThreads) {
+  for (int i = tid; i < n; i += T) {
     const int need = want[i] - (i > 0 ? want[i - 1] : 0);
     if (want[i] <= nfree) {
       if (need > 0) atomicMax(&granted, want[i]);
@@ -356,7 +385,7 @@ __global__ void __launch_bounds__(kPgThreads)
     if (s.rank == 0 && target[i] >= 0) p.held[row[i]] = target[i];
   }
   __syncthreads();
-  allot(p, s, want, n, granted, before, warp_tot, [&](int i, int k, int page) {
+  allot(p, s, free, want, n, granted, before, warp_tot, [&](int i, int k, int page) {
     p.tables[(int64_t)row[i] * p.stride + has[i] + k] = page;
   });
   if (tid == 0 && s.rank == 0 && p.status != nullptr) {
@@ -374,29 +403,41 @@ struct ForkPlan {
 
 // As in resize_kernel, every CTA has the children's needs, the first one
 // writes the plan.
-__global__ void __launch_bounds__(kPgThreads)
+template <int T> __global__ void __launch_bounds__(T)
     fork_plan_kernel(const Pool p, const int32_t *__restrict__ parents,
                      const int32_t *__restrict__ children, const int32_t *__restrict__ lens, int n,
                      ForkPlan *__restrict__ plan, int ranks) {
   extern __shared__ int32_t pg_smem[];
-  int32_t *want = pg_smem, *kid = want + n, *full = kid + n;  // full: -1 not forked
-  __shared__ int32_t warp_tot[kPgThreads / 32], told[kPgCluster];
+  int32_t *want = pg_smem, *kid = want + n, *par = kid + n;
+  int32_t *full = par + n;  // the length, then the whole pages, -1 not forked
+  __shared__ int32_t warp_tot[T / 32], told[kPgCluster];
   __shared__ int lacking, granted;
   pdl_begin();
   const Stretch s(p.pages, ranks, told);
   const int tid = threadIdx.x;
   if (tid == 0) lacking = granted = 0;
-  for (int i = tid; i < n; i += kPgThreads) kid[i] = children[i];
+  // (the first T children and the pool are read at the same time)
+  const int c0 = tid < n ? children[tid] : 0, up0 = tid < n ? parents[tid] : 0;
+  const int len0 = tid < n ? lens[tid] : 0;
+  Free<T> free;
+  free.count(p, s, warp_tot);
+  for (int i = tid; i < n; i += T) {
+    kid[i] = i < T ? c0 : children[i];
+    par[i] = i < T ? up0 : parents[i];
+    full[i] = i < T ? len0 : lens[i];
+  }
   __syncthreads();
-  find_repeats(kid, want, n);
+  find_repeats<T>(kid, want, n);
   __syncthreads();
-  for (int i = tid; i < n; i += kPgThreads) {
-    const int up = parents[i], c = kid[i], len = lens[i];
+  for (int i = tid; i < n; i += T) {
+    const int up = par[i], c = kid[i], len = full[i];
+    const bool inside = up >= 0 && up < p.rows && c >= 0 && c < p.rows;
+    const int parent_has = inside ? p.held[up] : 0, child_has = inside ? p.held[c] : 0;
     ForkPlan f{up, -1, -1, -1, -1, 0};
     int flag = 0;
-    if (up < 0 || up >= p.rows || c < 0 || c >= p.rows || want[i] || p.held[c] != 0) {
+    if (!inside || want[i] || child_has != 0) {
       flag = DSB_FLAG_SLOT;
-    } else if (len < 0 || (int64_t)len > (int64_t)p.held[up] * p.bs ||
+    } else if (len < 0 || (int64_t)len > (int64_t)parent_has * p.bs ||
                (int64_t)len > p.cols * p.bs) {
       flag = DSB_FLAG_POSITION;
     } else {
@@ -421,9 +462,9 @@ __global__ void __launch_bounds__(kPgThreads)
   }
   __syncthreads();
   int before;
-  const int nfree = s.gather(free_pages(p, s, warp_tot), before);
-  scan_rows(want, n, warp_tot);
-  for (int i = tid; i < n; i += kPgThreads) {
+  const int nfree = s.gather(free.total, before);
+  scan_rows<T>(want, n, warp_tot);
+  for (int i = tid; i < n; i += T) {
     const bool started = want[i] > (i > 0 ? want[i - 1] : 0);
     if (started && want[i] > nfree) {  // no page for it: not forked
       atomicAdd(&lacking, 1);
@@ -434,7 +475,7 @@ __global__ void __launch_bounds__(kPgThreads)
     }
   }
   __syncthreads();
-  allot(p, s, want, n, granted, before, warp_tot, [&](int i, int, int page) {
+  allot(p, s, free, want, n, granted, before, warp_tot, [&](int i, int, int page) {
     plan[i].dst = page;
     p.tables[(int64_t)kid[i] * p.stride + full[i]] = page;
   });
@@ -512,56 +553,67 @@ __global__ void __launch_bounds__(256)
 }
 
 // scratch: [0] pages to move, then sources[N], targets[N], new names[N]
-__global__ void __launch_bounds__(kPgThreads)
+template <int T> __global__ void __launch_bounds__(T)
     compact_plan_kernel(const Pool p, int32_t *__restrict__ scratch, int ranks) {
-  __shared__ int32_t warp_tot[kPgThreads / 32], told[kPgCluster];
+  __shared__ int32_t warp_tot[T / 32], told[kPgCluster];
   pdl_begin();
   const Stretch s(p.pages, ranks, told);
-  const int tid = threadIdx.x;
-  const unsigned below = (1u << (tid & 31)) - 1;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const unsigned below = (1u << lane) - 1;
+  Free<T> free;
+  free.count(p, s, warp_tot);
   int before;
-  const int nfree = s.gather(free_pages(p, s, warp_tot), before);
+  const int nfree = s.gather(free.total, before);
   const int64_t live = p.pages - nfree;
   int32_t *src = scratch + 1, *dst = src + p.pages, *name = dst + p.pages;
-  // Holes are the free pages below `live`: before this stretch as many as
-  // pages free before it, or all of them; pages to move likewise.
-  int holes, moved;
-  {
+  // Holes are the free pages below `live`, and as many pages move: in all, and
+  // before this stretch.  (One CTA with one turn finds them in its masks.)
+  int holes = 0, moved = 0;
+  const bool once = ranks == 1 && free.whole;
+  if (!once) {
     int h = 0, total;  // free pages of the stretch below `live`
-    for (int64_t base = s.from; base < min(s.till, live); base += kPgTurn)
+    for (int64_t base = s.from; base < min(s.till, live); base += T * kPgPages)
       read_turn(p, base, min(s.till, live), [&](int, int64_t, int v) { h += v == 0; });
-    block_scan(h, warp_tot, total);
-    moved = s.gather(total, holes);  // as many pages move as there are holes
+    block_scan<T>(h, warp_tot, total);
+    moved = s.gather(total, holes);
   }
   // live pages at or behind `live` and before this stretch: those before the
   // stretch less those before `live`
   int at = s.from <= live ? 0 : (int)(s.from - before) - (int)(live - moved);
   int hole_at = holes;
-  for (int64_t base = s.from; base < s.till; base += kPgTurn) {
-    unsigned hm[kPgPages], mm[kPgPages];
+  for (int64_t base = s.from; base < s.till; base += T * kPgPages) {
+    if (!free.whole) free.read(p, s, base);
     int mine = 0, total;  // holes, and pages to move, in 16 bits each
-    read_turn(p, base, s.till, [&](int j, int64_t page, int v) {
-      hm[j] = __ballot_sync(0xffffffffu, v == 0 && page < live);
-      mm[j] = __ballot_sync(0xffffffffu, v != 0 && page >= live && page < s.till);
-      mine += __popc(hm[j]) + (__popc(mm[j]) << 16);
-      if (v == 0 && page >= live) name[page] = -1;  // no row holds it
-    });
-    const int b = warps_before(mine, warp_tot, total);
+    // pages of the warp below `live`, and within the stretch
+    auto ahead = [&](int64_t x) {
+      return (int)max((int64_t)0, min((int64_t)32 * kPgPages, x - warp_page(base, 0)));
+    };
+    const int front = ahead(live), all = ahead(s.till);
+    auto hole = [&](int j) { return free.mask[j] & low_bits(front - 32 * j); };
+    auto move = [&](int j) {
+      return ~free.mask[j] & ~low_bits(front - 32 * j) & low_bits(all - 32 * j);
+    };
+#pragma unroll
+    for (int j = 0; j < kPgPages; ++j) mine += __popc(hole(j)) + (__popc(move(j)) << 16);
+    const int b = warps_before<T>(mine, warp_tot, total);
     int h = hole_at + (b & 0xffff), m = at + (b >> 16);
-    const int64_t page0 = base + (int64_t)(tid >> 5) * 32 * kPgPages + (tid & 31);
 #pragma unroll
     for (int j = 0; j < kPgPages; ++j) {
-      if (hm[j] >> (tid & 31) & 1) dst[h + __popc(hm[j] & below)] = (int)(page0 + 32 * j);
-      if (mm[j] >> (tid & 31) & 1) src[m + __popc(mm[j] & below)] = (int)(page0 + 32 * j);
-      h += __popc(hm[j]);
-      m += __popc(mm[j]);
+      const unsigned hm = hole(j), mm = move(j);
+      const int page = (int)warp_page(base, j) + lane;
+      if (hm >> lane & 1) dst[h + __popc(hm & below)] = page;
+      else if (mm >> lane & 1) src[m + __popc(mm & below)] = page;
+      else if (free.mask[j] >> lane & 1) name[page] = -1;  // no row holds it
+      h += __popc(hm);
+      m += __popc(mm);
     }
     hole_at += total & 0xffff;
     at += total >> 16;
+    if (once) moved = total & 0xffff;
   }
   s.sync();
 #pragma unroll 4
-  for (int k = s.rank * kPgThreads + tid; k < moved; k += ranks * kPgThreads) {
+  for (int k = s.rank * T + tid; k < moved; k += ranks * T) {
     const int a = __ldcg(src + k), t = __ldcg(dst + k);
     name[a] = t;
     p.refs[t] = p.refs[a];
@@ -629,9 +681,14 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// (three passes over the counts to compact: a cluster from a second turn on,
-// 96 us against 110 for 32768 pages)
-int planners(int64_t pages, int turns) { return pages <= (int64_t)turns * kPgTurn ? 1 : kPgCluster; }
+// f(threads, CTAs) with the planners of a pool: the variant's threads as a type.
+template <typename F> void with_planners(int64_t pages, int n, F f) {
+  const int ranks = pages <= kPgFew * kPgPages ? 1 : kPgCluster;
+  if (pages <= (int64_t)ranks * kPgFew * kPgPages && n <= kPgFew)
+    f(std::integral_constant<int, kPgFew>{}, ranks);
+  else
+    f(std::integral_constant<int, kPgThreads>{}, pages <= kPgTurn ? 1 : kPgCluster);
+}
 
 int check_pool(const Pool &p, int n) {
   if (p.pages <= 0 || p.pages > INT32_MAX || p.rows <= 0 || p.rows > INT32_MAX || p.cols <= 0 ||
@@ -688,11 +745,14 @@ extern "C" int dsb_resize_requests(int32_t *ref_counts, int64_t num_pages, int32
     if (int e = check_launch("release_kernel")) return e;
   }
   const size_t smem = (size_t)n * 4 * sizeof(int32_t);
-  if (int e = ensure_smem((const void *)resize_kernel, smem)) return e;
-  const int ranks = planners(num_pages, 4);
-  launch_kernel_cluster(resize_kernel, dim3(ranks), dim3(kPgThreads), smem, st, ranks, p, rows, lens,
-                        (int)n, alone ? 1 : 0, ranks);
-  return check_launch("resize_kernel");
+  int e = DSB_OK;
+  with_planners(num_pages, n, [&](auto threads, int ranks) {
+    auto kern = resize_kernel<threads()>;
+    if ((e = ensure_smem((const void *)kern, smem)) != DSB_OK) return;
+    launch_kernel_cluster(kern, dim3(ranks), dim3(threads()), smem, st, ranks, p, rows, lens, (int)n,
+                          alone ? 1 : 0, ranks);
+  });
+  return e != DSB_OK ? e : check_launch("resize_kernel");
 }
 
 extern "C" int64_t dsb_fork_scratch_ints(int32_t n) { return n > 0 ? 6 * (int64_t)n : 0; }
@@ -714,12 +774,16 @@ extern "C" int dsb_fork_requests(int32_t *ref_counts, int64_t num_pages, int32_t
     return fail(DSB_ERR_INVALID, "scratch smaller than dsb_fork_scratch_ints");
   const cudaStream_t st = as_stream(stream);
   ForkPlan *plan = reinterpret_cast<ForkPlan *>(scratch);
-  const size_t smem = (size_t)n * 3 * sizeof(int32_t);
-  if (int e = ensure_smem((const void *)fork_plan_kernel, smem)) return e;
-  const int ranks = planners(num_pages, 4);
-  launch_kernel_cluster(fork_plan_kernel, dim3(ranks), dim3(kPgThreads), smem, st, ranks, p, parents,
-                        children, lens, (int)n, plan, ranks);
-  if (int e = check_launch("fork_plan_kernel")) return e;
+  const size_t smem = (size_t)n * 4 * sizeof(int32_t);
+  int e = DSB_OK;
+  with_planners(num_pages, n, [&](auto threads, int ranks) {
+    auto kern = fork_plan_kernel<threads()>;
+    if ((e = ensure_smem((const void *)kern, smem)) != DSB_OK) return;
+    launch_kernel_cluster(kern, dim3(ranks), dim3(threads()), smem, st, ranks, p, parents, children, lens,
+                          (int)n, plan, ranks);
+  });
+  if (e != DSB_OK) return e;
+  if (int err = check_launch("fork_plan_kernel")) return err;
   if (n == 0) return DSB_OK;
   const int table_blocks = (int)std::min<int64_t>(64, (table_cols + 255) / 256);
   const unsigned gy = (unsigned)((n + kPgRows - 1) / kPgRows);
@@ -753,9 +817,10 @@ extern "C" int dsb_compact_pages(int32_t *ref_counts, int64_t num_pages, int32_t
   if (scratch_ints < dsb_compact_scratch_ints(num_pages))
     return fail(DSB_ERR_INVALID, "scratch smaller than dsb_compact_scratch_ints");
   const cudaStream_t st = as_stream(stream);
-  const int ranks = planners(num_pages, 1);
-  launch_kernel_cluster(compact_plan_kernel, dim3(ranks), dim3(kPgThreads), 0, st, ranks, p, scratch,
-                        ranks);
+  with_planners(num_pages, 0, [&](auto threads, int ranks) {
+    launch_kernel_cluster(compact_plan_kernel<threads()>, dim3(ranks), dim3(threads()), 0, st, ranks, p,
+                          scratch, ranks);
+  });
   if (int e = check_launch("compact_plan_kernel")) return e;
   bool first = true;
   auto apply = [&](const Caches &part) {
