@@ -88,10 +88,9 @@ __device__ __forceinline__ int sp_owner(int64_t u, const SpBegin &x, int ctas) {
   return b;
 }
 
-// Tokens that row r may see, 0 for a row without a valid table row.
-__device__ __forceinline__ int sp_visible(const TaArgs &a, int r, int64_t &trow, bool report) {
-  const int L = a.seq[r];
-  trow = a.trows != nullptr ? a.trows[r] : r;
+// Tokens that a row of L tokens on table row `trow` may see, 0 for a row
+// without a valid table row.
+__device__ __forceinline__ int sp_sees(const TaArgs &a, int L, int64_t trow, bool report) {
   if (L <= 0) return 0;
   if (trow < 0 || trow >= a.bt_rows) {
     if (report) flag_error(a.err, DSB_FLAG_SLOT);
@@ -103,6 +102,9 @@ __device__ __forceinline__ int sp_visible(const TaArgs &a, int r, int64_t &trow,
     return (int)cap;
   }
   return L;
+}
+__device__ __forceinline__ int64_t sp_table_row(const TaArgs &a, int r) {
+  return a.trows != nullptr ? a.trows[r] : r;
 }
 
 // ------------------------------------------------------------------- plan
@@ -150,23 +152,30 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
 
   // The rows of a turn: what each sees, and its table row (-1: none).  A run
   // may reach into the rows of the next turn.
-  auto read_rows = [&](int base) {
+  auto read_rows = [&](int base, int L, int64_t t) {  // (of the thread's first row)
     for (int i = tid; i < kPlanThreads + run_rows && base + i < a.rows; i += kPlanThreads) {
-      int64_t t;
-      s_seen[i] = sp_visible(a, base + i, t, i < kPlanThreads);
-      t = a.trows != nullptr ? a.trows[base + i] : base + i;
+      if (i >= kPlanThreads) L = a.seq[base + i], t = sp_table_row(a, base + i);
+      s_seen[i] = sp_sees(a, L, t, i < kPlanThreads);
       s_trow[i] = t >= 0 && t < a.bt_rows ? (int)t : -1;
     }
   };
-  read_rows(0);
+  // what the first turns need is read at the same time
+  const int L0 = tid < a.rows ? a.seq[tid] : 0;
+  const int64_t t0 = tid < a.rows ? sp_table_row(a, tid) : -1;
+  const bool first_groups = tid <= s.groups, starts_given = s.group_starts != nullptr;
+  const int at0 = first_groups && starts_given ? s.group_starts[tid] : 0;
+  const int before0 = first_groups && starts_given && tid > 0 ? s.group_starts[tid - 1] : 0;
+  const int prefix0 = tid < s.groups ? s.prefix_lens[tid] : 0;
+  read_rows(0, L0, t0);
   // the groups; if they do not ascend within the rows, nothing is shared
   bool bad = false;
   for (int i = tid; i <= s.groups; i += kPlanThreads) {
-    const int at = s.group_starts != nullptr ? s.group_starts[i] : (i == 0 ? 0 : a.rows);
+    const bool mine = i == tid;
+    const int at = !starts_given ? (i == 0 ? 0 : a.rows) : mine ? at0 : s.group_starts[i];
     if (i <= kPlanKeep) s_start[i] = at;
-    if (i < s.groups && i < kPlanKeep) s_prefix[i] = s.prefix_lens[i];
+    if (i < s.groups && i < kPlanKeep) s_prefix[i] = mine ? prefix0 : s.prefix_lens[i];
     bad |= at < 0 || at > a.rows ||
-           (i > 0 && s.group_starts != nullptr && s.group_starts[i - 1] > at);
+           (i > 0 && starts_given && (mine ? before0 : s.group_starts[i - 1]) > at);
   }
   for (int r = tid; r < a.rows; r += kPlanThreads) s.rows[r] = SpRow{0, -1, -1, 0};
   bad = __syncthreads_or(bad);
@@ -203,8 +212,9 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
   }
   __syncthreads();
 
-  // the prefix segments, a warp each: as far as any of their rows sees
-  for (int p = warp; p < nprefix; p += kPlanThreads / 32) {
+  // the prefix segments, a warp each (the last ones first: the first warps have
+  // the rows): as far as any of their rows sees
+  for (int p = kPlanThreads / 32 - 1 - warp; p < nprefix; p += kPlanThreads / 32) {
     int x = 0, y = groups;
     while (x < y) {
       const int mid = (x + y) / 2;
@@ -225,7 +235,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
         if (r < kPlanThreads) {
           L = s_seen[r], t = s_trow[r];
         } else {
-          L = sp_visible(a, r, t, false);
+          t = sp_table_row(a, r);
+          L = sp_sees(a, a.seq[r], t, false);
         }
         L = min(L, prefix);
       }
@@ -246,7 +257,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
   for (int base = 0; base < a.rows; base += kPlanThreads) {
     if (base > 0) {
       __syncthreads();
-      read_rows(base);
+      const bool mine = base + tid < a.rows;
+      read_rows(base, mine ? a.seq[base + tid] : 0, mine ? sp_table_row(a, base + tid) : -1);
       __syncthreads();
     }
     const int r = base + tid;
@@ -279,7 +291,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
         if (tid > 0) {
           before = s_trow[tid - 1];
         } else {
-          const int64_t t = a.trows != nullptr ? a.trows[r - 1] : r - 1;
+          const int64_t t = sp_table_row(a, r - 1);
           before = t >= 0 && t < a.bt_rows ? (int)t : -1;
         }
       }
@@ -820,8 +832,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         if (early) fetch(after, pieces + 1);
         lim = 0;
         if (mine) {
-          int64_t t;
-          lim = min(sp_visible(a, p.g.row0 + (p.g.q0 + m) / G, t, false), p.g.tok1);
+          const int row = p.g.row0 + (p.g.q0 + m) / G;
+          lim = min(sp_sees(a, a.seq[row], sp_table_row(a, row), false), p.g.tok1);
         }
       }
       const bool works = __any_sync(0xffffffffu, mine);
