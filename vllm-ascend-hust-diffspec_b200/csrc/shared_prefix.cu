@@ -30,15 +30,24 @@ constexpr int kSpSlots = 5;         // K / V tiles in flight
 constexpr int kSpThreads = 384;
 constexpr int kSpSmem = 1024 + (2 + kSpSlots) * kSpTile + 256;  // queries, ring, barriers
 constexpr float kSpGrow = 8.f;      // log2 of the growth that rescales O
-// A piece costs about two tiles beside its tiles (its queries, first loads
-// and sums), so each segment counts two units more than its tiles.
-constexpr int kSpStart = 2;
+// The shares are counted in units of 2300 clocks: a tile is one of them, or two
+// when both streams take it, and what a piece costs beside its tiles (its
+// queries, first loads and sums) is START1 of them, or START2.  (80 x 8 query
+// rows are tiles of both kinds, TIME0 with a unit for each; 64 rows with 512
+// tokens of their own behind two prefixes TIME1.)
+struct SpCost {
+  int tile, start;
+  __device__ explicit SpCost(int nq) : tile(nq > 128 ? 2 : 1), start(nq > 128 ? 4 : 3) {}
+  __device__ int units(int tiles) const { return tiles * tile + start; }
+  // tiles that begin before unit x of a segment's kv head
+  __device__ int before(int x) const { return (max(x - start, 0) + tile - 1) >> (tile - 1); }
+};
 
 // Tokens [tok0, tok1) for query rows m < nq: (row0 + (q0 + m) / G, head
 // (q0 + m) % G).  Tiles start at `base`, tok0 rounded down to a TMA box.
 struct alignas(16) SpSeg {
   int32_t row0, q0, nq, trow, tok0, tok1, base;
-  int32_t len;     // units of one kv head: tiles + kSpStart, 0: nothing to do
+  int32_t len;     // units of one kv head, 0: nothing to do
   int64_t unit0;   // units before this segment
   int64_t acc;     // first row of its partial sums
   int32_t maxp;    // pieces that one kv head may be cut into
@@ -248,7 +257,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
     most = __reduce_max_sync(0xffffffffu, most);
     g.trow = max(trow, 0);
     g.tok1 = most;
-    g.len = most > 0 ? (most + kSpTok - 1) / kSpTok + kSpStart : 0;
+    g.len = most > 0 ? SpCost(g.nq).units((most + kSpTok - 1) / kSpTok) : 0;
     if (lane == 0) keep(p, g);
   }
 
@@ -314,7 +323,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
       g.row0 = r, g.q0 = 0, g.nq = nrows * G, g.trow = trow;
       g.tok0 = prefix, g.tok1 = most;
       g.base = prefix / s.box * s.box;
-      g.len = (most - g.base + kSpTok - 1) / kSpTok + kSpStart;
+      g.len = SpCost(g.nq).units((most - g.base + kSpTok - 1) / kSpTok);
       keep(at, g);
       for (int j = 0; j < nrows; ++j) {
         s.rows[r + j].sseg = at;
@@ -510,8 +519,8 @@ __device__ __forceinline__ void sp_st_global8(float *p, const float (&v)[8]) {
                : "memory");
 }
 
-// A CTA's share of a segment's kv head: tiles [t0, t0 + n) from `base`, the
-// index-th of the shares that have tiles.
+// A CTA's share of a segment's kv head: tiles [t0, t0 + n) from `base`, those
+// whose first units it has, and the index-th of the shares that have tiles.
 struct SpPiece {
   SpSeg g;
   int seg, h, t0, n, index;
@@ -542,14 +551,17 @@ struct SpWalk {
       const int a = (int)(off - (int64_t)p.h * p.g.len);
       const int b = (int)min((int64_t)p.g.len, a + (end - u));
       u += b - a;
-      p.t0 = max(a - kSpStart, 0);
-      p.n = max(b - kSpStart, 0) - p.t0;
+      const SpCost cost(p.g.nq);
+      p.t0 = cost.before(a);
+      p.n = cost.before(b) - p.t0;
       if (p.n <= 0) continue;
       p.seg = seg;
-      // (fewer units than CTAs: every tile is a piece)
-      p.index = share.share == 0
-                    ? a - kSpStart
-                    : (int)blockIdx.x - sp_owner(p.g.unit0 + (int64_t)p.h * p.g.len + kSpStart, share, s.ctas);
+      // (shares below a tile: every tile is a piece; else every share between
+      // the first and the last that have tiles has some)
+      p.index = share.share < cost.tile
+                    ? p.t0
+                    : (int)blockIdx.x -
+                          sp_owner(p.g.unit0 + (int64_t)p.h * p.g.len + cost.start, share, s.ctas);
       return true;
     }
     return false;
@@ -781,24 +793,26 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       mbar_arrive(joint);
       ok = __all_sync(0xffffffffu, sp_wait(joint, (uint32_t)joints++ & 1u));
     };
-    // A piece's queries, swizzled as the operand wants them (places behind nq
-    // hold anything: a query row meets only its own sums).  One query tile
-    // alternates between the two places.
+    // A piece's queries, swizzled as the operand wants them, 16 rows at a time
+    // (places behind nq keep what they hold: a query row meets only its own
+    // sums).  One query tile alternates between the two places.
+    const int step_row = 16 / G, step_head = 16 - step_row * G;
     auto fetch = [&](const SpPiece &x, int place) {
-      for (int b = 0; b < (x.g.nq > 128 ? 2 : 1); ++b) {
-        const uint32_t dst = s_q + (x.g.nq > 128 ? b : place & 1) * kSpTile;
-        const int c = tid & 15;
-#pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          const int r = y * 16 + (tid >> 4);
-          const int mm = x.g.q0 + min(b * 128 + r, x.g.nq - 1);
-          const T *src = static_cast<const T *>(a.q) +
-                         ((int64_t)(x.g.row0 + mm / G) * a.hq + x.h * G + mm % G) * kTaD + c * 8;
+      const bool pair = x.g.nq > 128;
+      const int c = tid & 15, first = x.g.q0 + (tid >> 4);
+      int row = first / G, head = first - row * G;
+#pragma unroll 1
+      for (int r = tid >> 4; r - (tid >> 4) < x.g.nq; r += 16) {
+        const uint32_t dst = s_q + (pair ? r >> 7 : place & 1) * kSpTile;
+        const T *src = static_cast<const T *>(a.q) +
+                       ((int64_t)(x.g.row0 + row) * a.hq + x.h * G + head) * kTaD + c * 8;
+        if (r < x.g.nq)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                           dst + (c >> 3) * kSpHalf + r * 128 + (((c & 7) ^ (r & 7)) * 16)),
+                           dst + (c >> 3) * kSpHalf + (r & 127) * 128 + (((c & 7) ^ (r & 7)) * 16)),
                        "l"(src)
                        : "memory");
-        }
+        row += step_row, head += step_head;
+        if (head >= G) head -= G, ++row;
       }
       cp_async_commit();
     };
@@ -816,25 +830,22 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     p.g.tok0 = p.g.base = p.t0 = 0;
     p.g.nq = 128;
     p.g.tok1 = kSpTok;
+    // this thread's query row of a piece; the tokens [tok0, sees) are what it sees
+    auto query_row = [&](const SpPiece &x) { return (x.g.nq > 128 ? stream * 128 : 0) + m128; };
+    auto sees = [&](const SpPiece &x) {
+      if (query_row(x) >= x.g.nq) return 0;
+      const int row = x.g.row0 + (x.g.q0 + query_row(x)) / G;
+      return min(sp_sees(a, a.seq[row], sp_table_row(a, row), false), x.g.tok1);
+    };
+    int lim = kSpTok;
     while (ok) {
       const int n = p.n, nq = p.g.nq;
       const bool two = nq > 128;
-      const int m = (two ? stream * 128 : 0) + m128;  // this thread's query row
+      const int m = query_row(p);
       const bool mine = m < nq;
-      int lim = kSpTok;  // the tokens [tok0, lim) are what it sees
-      if (!rehearsal) {
-        if (!early) {
-          fetch(p, pieces);
-          fetched();
-        }
-        has_next = walk.next(s, after);
-        early = has_next && !two && after.g.nq <= 128;
-        if (early) fetch(after, pieces + 1);
-        lim = 0;
-        if (mine) {
-          const int row = p.g.row0 + (p.g.q0 + m) / G;
-          lim = min(sp_sees(a, a.seq[row], sp_table_row(a, row), false), p.g.tok1);
-        }
+      if (!rehearsal && !early) {
+        fetch(p, pieces);
+        fetched();
       }
       const bool works = __any_sync(0xffffffffu, mine);
       const int count = rehearsal ? 1 : two ? n : (n - stream + 1) / 2;
@@ -944,19 +955,27 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         pdl_begin();
         walk.begin(s);
         if (!walk.next(s, p)) break;
+        lim = sees(p);
         continue;
       }
       kt += count;
       i0 += 2 * n;
-      if (early) fetched();  // the next piece's first products run beside the sums
+      // the next piece's queries, while the last products run; its first ones
+      // run beside the sums
+      has_next = walk.next(s, after);
+      early = has_next && !two && after.g.nq <= 128;
+      if (early) fetch(after, pieces + 1);
+      if (has_next) lim = sees(after);
 
       // the piece's sums (its products are done): [nq][D], and (maximum, sum)
       ok = __all_sync(0xffffffffu, sp_wait(o_done, (uint32_t)pieces & 1u));
       if (!ok) break;
+      if (early) fetched();
       tc_fence_after();
       const int64_t at = p.g.acc + ((int64_t)p.h * p.g.maxp + p.index) * nq + m;
       float *part = s.acc + at * kTaD;
-      if (tid == 0 && p.t0 + n == p.g.len - kSpStart) s.pieces[(int64_t)p.seg * a.hk + p.h] = p.index + 1;
+      if (tid == 0 && p.t0 + n == SpCost(nq).before(p.g.len))
+        s.pieces[(int64_t)p.seg * a.hk + p.h] = p.index + 1;
       if (two) {
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
