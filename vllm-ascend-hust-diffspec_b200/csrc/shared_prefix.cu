@@ -29,15 +29,17 @@ constexpr int kSpTok = 128;
 constexpr int kSpSlots = 5;         // K / V tiles in flight
 constexpr int kSpThreads = 384;
 constexpr int kSpSmem = 1024 + (2 + kSpSlots) * kSpTile + 256;  // queries, ring, barriers
+constexpr int kSpStage = 144;       // bytes: 32 columns of a row, and 16 more for the banks
 constexpr float kSpGrow = 8.f;      // log2 of the growth that rescales O
 // The shares are counted in units of 2300 clocks: a tile is one of them, or two
-// when both streams take it, and what a piece costs beside its tiles (its
-// queries, first loads and sums) is START1 of them, or START2.  (80 x 8 query
-// rows are tiles of both kinds, TIME0 with a unit for each; 64 rows with 512
-// tokens of their own behind two prefixes TIME1.)
+// when both streams take it, and a piece's queries, first loads and sums are
+// five.  (640 query rows of a kv head are tiles of both kinds: 88 us against
+// 98 with a unit for every tile; 64 rows with 512 tokens of their own behind
+// two prefixes of 65536: 191 us with five, 214 with three.)
 struct SpCost {
-  int tile, start;
-  __device__ explicit SpCost(int nq) : tile(nq > 128 ? 2 : 1), start(nq > 128 ? 4 : 3) {}
+  static constexpr int start = 5;
+  int tile;
+  __device__ explicit SpCost(int nq) : tile(nq > 128 ? 2 : 1) {}
   __device__ int units(int tiles) const { return tiles * tile + start; }
   // tiles that begin before unit x of a segment's kv head
   __device__ int before(int x) const { return (max(x - start, 0) + tile - 1) >> (tile - 1); }
@@ -977,21 +979,37 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       if (tid == 0 && p.t0 + n == SpCost(nq).before(p.g.len))
         s.pieces[(int64_t)p.seg * a.hk + p.h] = p.index + 1;
       if (two) {
+        // 32 columns of the warp's rows at a time pass through where the
+        // queries were, so that a store writes 128 bytes of four rows (each
+        // lane its own row: 8000 clocks for the sums of 256 rows)
+        const uint32_t stage = s_q + warp * (32 * kSpStage);
+        float *rows = part - (int64_t)lane * kTaD;
+        const int left = nq - (m - lane);  // rows of this warp that there are
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
           uint32_t o[32];
           sp_ld32(to + c, o);
           sp_wait_ld(o);
-          if (mine)
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              float y[8];
+          for (int i = 0; i < 32; i += 4)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * kSpStage + i * 4),
+                         "r"(o[i]), "r"(o[i + 1]), "r"(o[i + 2]), "r"(o[i + 3])
+                         : "memory");
+          __syncwarp();
 #pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[i + e]);
-              sp_st_global8(part + c + i, y);
-            }
+          for (int r = lane >> 3; r < 32; r += 4) {
+            float4 v;
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                         : "r"(stage + r * kSpStage + (lane & 7) * 16)
+                         : "memory");
+            if (r < left) *reinterpret_cast<float4 *>(rows + (int64_t)r * kTaD + c + (lane & 7) * 4) = v;
+          }
+          __syncwarp();
         }
         if (mine) s.ml[at] = make_float2(l != l ? 0.f : m_ref, l);  // (NaN is no empty sum)
+        tc_fence_before();
+        both();  // all of it is read before the next piece's queries
       } else {
         // both streams' sums of a row lie in the same lane: each stream joins
         // half of the columns (maxima and sums pass where the queries were)
