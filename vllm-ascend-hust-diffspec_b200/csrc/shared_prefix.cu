@@ -824,12 +824,12 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       mbar_arrive(q_ready);
     };
     // The first turn of the loop is a rehearsal on whatever the tensor memory
-    // holds: it brings the instructions in (~7000 clocks of misses) while the
-    // plan is still being made.
+    // holds, stores nothing and brings the instructions in (~7000 clocks of
+    // misses) while the plan is still being made.
     bool rehearsal = true, has_next = false, early = false;
     SpPiece after;
+    p = SpPiece{};
     p.n = 1;
-    p.g.tok0 = p.g.base = p.t0 = 0;
     p.g.nq = 128;
     p.g.tok1 = kSpTok;
     // this thread's query row of a piece; the tokens [tok0, sees) are what it sees
@@ -844,12 +844,12 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       const int n = p.n, nq = p.g.nq;
       const bool two = nq > 128;
       const int m = query_row(p);
-      const bool mine = m < nq;
+      const bool mine = m < nq && !rehearsal;
       if (!rehearsal && !early) {
         fetch(p, pieces);
         fetched();
       }
-      const bool works = __any_sync(0xffffffffu, mine);
+      const bool works = __any_sync(0xffffffffu, m < nq);
       const int count = rehearsal ? 1 : two ? n : (n - stream + 1) / 2;
       float m_ref = -INFINITY, l = 0.f;
 #pragma unroll 1
@@ -952,31 +952,25 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         if (!rehearsal) mbar_arrive(p_ready + 16 * stream + 8 * half);
       }
       if (!ok) break;
-      if (rehearsal) {
-        rehearsal = false;
-        pdl_begin();
-        walk.begin(s);
-        if (!walk.next(s, p)) break;
-        lim = sees(p);
-        continue;
-      }
-      kt += count;
-      i0 += 2 * n;
-      // the next piece's queries, while the last products run; its first ones
-      // run beside the sums
-      has_next = walk.next(s, after);
-      early = has_next && !two && after.g.nq <= 128;
-      if (early) fetch(after, pieces + 1);
-      if (has_next) lim = sees(after);
+      if (!rehearsal) {
+        kt += count;
+        i0 += 2 * n;
+        // the next piece's queries, while the last products run; its first ones
+        // run beside the sums
+        has_next = walk.next(s, after);
+        early = has_next && !two && after.g.nq <= 128;
+        if (early) fetch(after, pieces + 1);
+        if (has_next) lim = sees(after);
 
-      // the piece's sums (its products are done): [nq][D], and (maximum, sum)
-      ok = __all_sync(0xffffffffu, sp_wait(o_done, (uint32_t)pieces & 1u));
-      if (!ok) break;
-      if (early) fetched();
+        // the piece's sums (its products are done): [nq][D], and (maximum, sum)
+        ok = __all_sync(0xffffffffu, sp_wait(o_done, (uint32_t)pieces & 1u));
+        if (!ok) break;
+        if (early) fetched();
+      }
       tc_fence_after();
       const int64_t at = p.g.acc + ((int64_t)p.h * p.g.maxp + p.index) * nq + m;
       float *part = s.acc + at * kTaD;
-      if (tid == 0 && p.t0 + n == SpCost(nq).before(p.g.len))
+      if (tid == 0 && mine && p.t0 + n == SpCost(nq).before(p.g.len))
         s.pieces[(int64_t)p.seg * a.hk + p.h] = p.index + 1;
       if (two) {
         // 32 columns of the warp's rows at a time pass through where the
@@ -1047,6 +1041,14 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         // all of it is read before the next piece's queries and products
         tc_fence_before();
         both();
+      }
+      if (rehearsal) {
+        rehearsal = false;
+        pdl_begin();
+        walk.begin(s);
+        if (!walk.next(s, p)) break;
+        lim = sees(p);
+        continue;
       }
       ++pieces;
       if (!has_next) break;
