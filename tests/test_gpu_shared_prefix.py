@@ -299,3 +299,36 @@ def test_a_cache_past_32_bits(dsb, cuda):
     torch.cuda.synchronize()
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
     _check(c, out, lse)
+
+
+@pytest.mark.parametrize("own", [0, 1, 150])
+@pytest.mark.parametrize("prefix", [127, 1000, 9000, 12000, 19000, 38000])
+def test_shares_of_a_few_units(dsb, cuda, prefix, own):
+    """160 query rows of one kv head on a prefix whose tiles are fewer, as many
+    and a few times as many as the CTAs: shares below a tile, of one and of
+    several."""
+    c = _case(cuda, [(prefix, [prefix + own * (i % 3 > 0) for i in range(20)], 1)], 8, 1, 16, "bf16",
+              prefix + own)
+    out, lse = _run(dsb, c)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+    _check(c, out, lse)
+    again, lse2 = _run(dsb, c)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def test_what_lies_behind_many_rows_is_not_read(dsb, cuda):
+    """The same with more query rows than one operand holds (two streams read
+    the tile that the prefix ends inside), and with row counts on both sides."""
+    for requests, hq, hk, prefix in ((20, 8, 1, 203), (33, 16, 2, 75), (17, 8, 1, 129)):
+        c = _case(cuda, [(prefix, [prefix + i % 4 for i in range(requests)], 1)], hq, hk, 16, "bf16",
+                  requests)
+        seen = torch.zeros(c["key"].shape[:2], dtype=torch.bool, device=cuda)
+        for r in range(requests):
+            t = torch.arange(int(c["seq"][r]), device=cuda)
+            seen[c["table"][c["trow"][r].long(), t // 16].long(), t % 16] = True
+        c["key"][~seen] = float("inf")
+        c["value"][~seen] = float("nan")
+        for _ in range(5):
+            out, lse = _run(dsb, c)
+            _check(c, out, lse)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
