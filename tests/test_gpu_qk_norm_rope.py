@@ -238,3 +238,34 @@ def test_captured_and_on_another_stream(dsb, cuda):
     torch.cuda.synchronize()
     for o in outs[1:]:
         assert torch.equal(o, outs[0])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq,hk", [(1, 1), (2, 1), (3, 3), (4, 2), (5, 1), (8, 1), (8, 8), (16, 2), (17, 9)])
+def test_heads_on_both_sides_of_a_warp(dsb, cuda, hq, hk, d):
+    """Head counts around what a warp takes (tokens side by side, the last ones
+    of a run missing), raw and paged; a bad slot in a run harms no neighbour."""
+    for tokens, neox in ((1, True), (13, False), (38, True)):
+        test_rows_and_raw_caches(dsb, cuda, tokens, hq, hk, d, d, "bf16", torch.float32, neox)
+        test_pages(dsb, cuda, tokens, hq, hk, d, d, "f16", torch.bfloat16, neox, 16)
+    tokens, n = 11, 6
+    qkv, w, cs, pos = _inputs(cuda, tokens, hq, hk, d, d, "bf16", torch.float32, 50, d + hq)
+    flat = qkv.view(tokens, -1)
+    slots = torch.arange(tokens, device=cuda).int()
+    at = torch.zeros(tokens, dtype=torch.int64, device=cuda)
+    raw = [torch.full((tokens, 2, hk, d), 7.0, dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    slots[n], pos[n + 2] = tokens, 50  # a slot and a position outside
+    out = torch.empty((tokens, hq * d), dtype=torch.bfloat16, device=cuda)
+    q, k, v = dsb.draft_layer.qk_norm_rope(
+        flat[:, : hq * d], flat[:, hq * d:], pos, cs, hk, w[0], w[1], 1e-6, query_out=out,
+        raw=(*raw, slots, at))
+    assert dsb._lib.read_and_clear_error_flag(cuda) == dsb._lib.DSB_FLAG_SLOT | dsb._lib.DSB_FLAG_POSITION
+    pos[n + 2] = 0
+    (qy, qr), (ky, kr) = _expect(qkv, w, cs, pos, hq, hk, d, True, 1e-6)
+    qr[n + 2], kr[n + 2] = qy[n + 2], ky[n + 2]  # normed, not rotated
+    _close(q.view(tokens, hq, d), qr, _both(qy), d, "bf16")
+    _close(k, kr, _both(ky), d, "bf16")
+    keep = [i for i in range(tokens) if i != n]
+    _close(raw[0][keep, 0], ky[keep], _both(ky[keep]), d, "bf16")
+    assert torch.equal(raw[1][keep, 0], v[keep])
+    assert (raw[0][n] == 7.0).all() and (raw[0][:, 1] == 7.0).all()

@@ -248,16 +248,57 @@ __device__ __forceinline__ void qk_turn(const QkTurn &f, float inv, const float 
 // asking later rows into L2 ahead of their warps (243 for 235).
 constexpr int kQkThreads = 64;
 
-template <typename T, typename CS, int D, bool NEOX>
+// With fewer query heads (keys and values) than half of what a warp takes, it
+// takes 2, 4 or 8 tokens side by side (QSIDE, KSIDE).  400000 tokens of 8/1
+// heads of 64: 705 us with one token a warp, 234 so; 60000 of 32/4 heads of 64:
+// 135 and 123.  Not the keys and values of D = 256, two of whose heads are a
+// warp's width (47725 tokens of 12/2 heads: 174 and 186).
+__host__ __device__ __forceinline__ int qk_side(int heads, int per, int groups) {
+  int n = 1;
+  while (2 * n <= groups && per / (2 * n) >= heads) n *= 2;
+  return n;
+}
+// The warps of a run of tokens: those of the query heads, then those of the
+// keys and values.
+struct QkWarps {
+  int qside, kside, tokens, qchunks, kchunks, q, all;
+  __host__ __device__ QkWarps(int hq, int hk, int groups, bool qs, bool ks) {
+    const int per = groups * kQkHeads;
+    qside = qs ? qk_side(hq, per, groups) : 1;
+    kside = ks ? qk_side(2 * hk, per, groups) : 1;
+    tokens = qside > kside ? qside : kside;
+    qchunks = (hq + per / qside - 1) / (per / qside);
+    kchunks = (2 * hk + per / kside - 1) / (per / kside);
+    q = tokens / qside * qchunks;
+    all = q + tokens / kside * kchunks;
+  }
+};
+
+template <typename T, typename CS, int D, bool NEOX, bool QSIDE, bool KSIDE>
 __global__ void __launch_bounds__(kQkThreads, 12) qk_norm_rope_heads_kernel(const QkArgs a) {
-  constexpr int kLanes = D / 16, kGroups = 32 / kLanes;  // heads that a warp has side by side
-  constexpr int kPer = kGroups * kQkHeads;               // heads of one token a warp takes
+  constexpr int kLanes = D / 16;  // of a head
   pdl_begin();
+  const QkWarps w(a.hq, a.hk, 32 / kLanes, QSIDE, KSIDE);
   const int64_t warp = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31, l = lane % kLanes;
-  const int qchunks = (a.hq + kPer - 1) / kPer, chunks = qchunks + (2 * a.hk + kPer - 1) / kPer;
-  const int t = (int)(warp / chunks), chunk = (int)(warp - (int64_t)t * chunks);
-  if (t >= a.tokens) return;
+  const int64_t run = warp / w.all;
+  const int of_run = (int)(warp - run * w.all);
+  const bool queries = of_run < w.q;
+  const int u = queries ? of_run : of_run - w.q, chunks = queries ? w.qchunks : w.kchunks;
+  const int side = queries ? (QSIDE ? w.qside : 1) : (KSIDE ? w.kside : 1);
+  const int kGroups = 32 / kLanes / side;  // heads of a token that a warp has side by side
+  const int group = lane / kLanes % kGroups;
+  int chunk = u, turn_of = 0;  // of the run's tokens
+  if (QSIDE || KSIDE) {
+    turn_of = chunks == 1 ? u : u / chunks;
+    chunk = u - turn_of * chunks;
+  }
+  const int64_t token0 = run * w.tokens + turn_of * side;
+  if (token0 >= a.tokens) return;
+  const int64_t mine = token0 + (QSIDE || KSIDE ? lane / kLanes / kGroups : 0);
+  const bool live = !(QSIDE || KSIDE) || mine < a.tokens;  // (else its lanes only take part)
+  const int t = (int)(live ? mine : a.tokens - 1);
+  const bool first = QSIDE || KSIDE ? live && lane % (kLanes * kGroups) == 0 : lane == 0;
   const int e1 = NEOX ? 8 * l : 16 * l, e2 = NEOX ? D / 2 + 8 * l : 16 * l + 8;
   const int pos = a.positions[t] + a.pos_offset;
   const bool turn = pos >= 0 && pos < a.rotary_rows;  // else: normed, not rotated
@@ -265,16 +306,16 @@ __global__ void __launch_bounds__(kQkThreads, 12) qk_norm_rope_heads_kernel(cons
   uint4 x1[kQkHeads], x2[kQkHeads];
   QkTurn f;
 
-  if (chunk < qchunks) {
-    const int h0 = chunk * kPer + lane / kLanes;
+  if (queries) {
+    const int h0 = chunk * kGroups * kQkHeads + group;
     const T *src = static_cast<const T *>(a.q) + t * a.q_stride + (int64_t)h0 * D;
 #pragma unroll
     for (int i = 0; i < kQkHeads; ++i) {  // (a head past the last: zeros, not stored)
-      const bool in = h0 + i * kGroups < a.hq;
+      const bool in = live && h0 + i * kGroups < a.hq;
       x1[i] = in ? qk_load(src + i * kGroups * D + e1) : make_uint4(0, 0, 0, 0);
       x2[i] = in ? qk_load(src + i * kGroups * D + e2) : make_uint4(0, 0, 0, 0);
     }
-    if (!turn && lane == 0 && chunk == 0) flag_error(a.err, DSB_FLAG_POSITION);
+    if (!turn && first && chunk == 0) flag_error(a.err, DSB_FLAG_POSITION);
     qk_factors<T, CS, D, NEOX>(f, static_cast<const T *>(a.qw), cs, l, turn);
     T *out = static_cast<T *>(a.q_out) + t * a.qo_stride + (int64_t)h0 * D;
 #pragma unroll
@@ -284,7 +325,7 @@ __global__ void __launch_bounds__(kQkThreads, 12) qk_norm_rope_heads_kernel(cons
       qk_unpack<T>(x2[i], v2);
       const float inv = rsqrtf(qk_mean_square<D>(v1, v2) + a.eps);
       qk_turn<NEOX>(f, inv, v1, v2, o1, o2);
-      if (h0 + i * kGroups < a.hq) {
+      if (live && h0 + i * kGroups < a.hq) {
         __stcs(reinterpret_cast<uint4 *>(out + i * kGroups * D + e1), qk_pack<T>(o1));
         __stcs(reinterpret_cast<uint4 *>(out + i * kGroups * D + e2), qk_pack<T>(o2));
       }
@@ -292,18 +333,18 @@ __global__ void __launch_bounds__(kQkThreads, 12) qk_norm_rope_heads_kernel(cons
     return;
   }
 
-  const int k0 = (chunk - qchunks) * kPer, h0 = k0 + lane / kLanes;  // keys, then values
+  const int k0 = chunk * kGroups * kQkHeads, h0 = k0 + group;  // keys, then values
   const T *key = static_cast<const T *>(a.k) + t * a.k_stride;
   const T *value = static_cast<const T *>(a.v) + t * a.v_stride;
 #pragma unroll
   for (int i = 0; i < kQkHeads; ++i) {
     const int h = h0 + i * kGroups;
     const T *src = h < a.hk ? key + h * D : value + (h - a.hk) * D;
-    const bool in = h < 2 * a.hk;
+    const bool in = live && h < 2 * a.hk;
     x1[i] = in ? qk_load(src + e1) : make_uint4(0, 0, 0, 0);
     x2[i] = in ? qk_load(src + e2) : make_uint4(0, 0, 0, 0);
   }
-  const int64_t row = a.dest != kDestNone ? dest_row(a, t, pos, lane == 0) : -1;
+  const int64_t row = a.dest != kDestNone ? dest_row(a, t, pos, first) : -1;
   if (k0 < a.hk) qk_factors<T, CS, D, NEOX>(f, static_cast<const T *>(a.kw), cs, l, turn);
 #pragma unroll
   for (int i = 0; i < kQkHeads; ++i) {
@@ -328,7 +369,7 @@ __global__ void __launch_bounds__(kQkThreads, 12) qk_norm_rope_heads_kernel(cons
         }
       }
     }
-    if (h >= 2 * a.hk) continue;
+    if (!live || h >= 2 * a.hk) continue;
     const bool is_key = h < a.hk;
     const int kh = is_key ? h : h - a.hk;
     T *out = static_cast<T *>(is_key ? a.k_out : a.v_out);
@@ -357,15 +398,22 @@ bool whole_heads(const QkArgs &a, int cos_sin_dtype) {
 }
 
 template <typename T, typename CS, int D> void launch_heads(const QkArgs &a, cudaStream_t st) {
-  const int per = 32 / (D / 16) * kQkHeads;
-  const int64_t chunks = (a.hq + per - 1) / per + (2 * a.hk + per - 1) / per;
-  const int64_t warps = (int64_t)a.tokens * chunks;
+  const QkWarps w(a.hq, a.hk, 32 / (D / 16), true, D < 256);
+  const int64_t warps = ((int64_t)a.tokens + w.tokens - 1) / w.tokens * w.all;
   constexpr int kWarps = kQkThreads / 32;
   const dim3 grid((unsigned)((warps + kWarps - 1) / kWarps)), block(kQkThreads);
-  if (a.neox)
-    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, true>, grid, block, 0, st, a);
-  else
-    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, false>, grid, block, 0, st, a);
+  auto with = [&](auto neox, auto qside, auto kside) {
+    launch_kernel(qk_norm_rope_heads_kernel<T, CS, D, neox(), qside(), kside()>, grid, block, 0, st, a);
+  };
+  auto sides = [&](auto neox) {
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if constexpr (D < 256) {
+      if (w.kside > 1) return w.qside > 1 ? with(neox, Yes(), Yes()) : with(neox, No(), Yes());
+    }
+    w.qside > 1 ? with(neox, Yes(), No()) : with(neox, No(), No());
+  };
+  a.neox ? sides(std::true_type()) : sides(std::false_type());
 }
 
 int launch(const QkArgs &a, int cos_sin_dtype, int dtype, cudaStream_t st) {
