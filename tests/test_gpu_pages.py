@@ -222,3 +222,35 @@ def test_captured(dsb, cuda):
     for x, y in zip((*a.state, *a.caches), (*b.state, *b.caches)):
         assert torch.equal(x, y)
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+@pytest.mark.parametrize("pages", [1900, 4096, 4097, 30000])
+def test_many_rows_in_a_call(dsb, cuda, pages):
+    """More rows than a small planner has threads, pools on both sides of what
+    it sees in one turn."""
+    rows = 700
+    p = _Pool(dsb, cuda, pages, rows, 9, 4)
+    rng = random.Random(pages)
+    who = rng.sample(range(rows), 300)
+    p.resize(who, [rng.randint(0, 20) for _ in who])
+    kids = [r for r in range(rows) if not p.ref.held[r]][:390]
+    ups = [rng.choice(who) for _ in kids]
+    p.fork(ups, kids, [rng.randint(0, p.ref.held[u] * 4) for u in ups])
+    p.resize(who + kids, [rng.choice([0, 3, 36]) for _ in who + kids])
+    p.compact()
+    p.resize(kids, [rng.randint(0, 36) for _ in kids])
+
+
+def test_pools_beyond_a_turn_of_the_planners(dsb, cuda):
+    """More pages than the planning CTAs hold in registers."""
+    pages, cols = 300001, 40000
+    p = _Pool(dsb, cuda, pages, 12, cols, 1, hk=1)
+    p.resize([3, 1, 7], [30000, 39999, 12345])
+    p.fork([1, 3, 1], [0, 2, 9], [39999, 29999, 77])
+    p.resize([5, 6, 8, 10, 11], [40000] * 5)
+    p.resize([3, 2, 5], [0, 17, 100])
+    p.resize([4], [40000])
+    p.compact()
+    p.resize([1, 6], [0, 0])
+    p.compact()
+    p.resize([1, 3, 6], [39000, 5, 40000])

@@ -618,7 +618,7 @@ def shared_prefix_attention_lse(
     rows, hq, d = shape = query.shape
     num_blocks, block_size, hk, kd = key_cache.shape
     dtype = query.dtype
-    if d != kd or hq % hk:
+    if d != kd or hk == 0 or hq % hk:
         raise ValueError("head dims must match and Hq must be a multiple of Hk")
     if key_cache.dtype is not dtype or value_cache.dtype is not dtype:
         raise ValueError("query and caches must share a dtype")

@@ -12,7 +12,8 @@ all int32 on the device and owned by the caller; a fresh pool is zeros, -1
 and zeros.  The calls are kernels on the current stream and read nothing
 back: a bad index is skipped and flagged in the error word, and ``status [2]``
 (int32) receives the rows that found no page and the free pages left.  Pages
-are handed out lowest id first, rows in call order.  The calls change the
+are handed out lowest id first, rows in call order.  A call names at most 4096
+rows; a token's bytes in a cache are a multiple of 16.  The calls change the
 pool in place, so two of them on one pool belong on one stream.
 
 The tables are the ``block_table`` of the paged kernels
