@@ -241,6 +241,7 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def stream_ptr(device: torch.device) -> int:
@@ -269,7 +270,7 @@ def call_on(device: torch.device, name: str, *args) -> None:
     """:func:`call` with ``device`` current (the kernels of tensors on another
     device than the current one)."""
     fn = getattr(_lib or load(), name)
-    if device.index == torch.cuda.current_device():
+    if device.index == _raw_device():
         status = fn(*args)
     else:
         with torch.cuda.device(device):
@@ -279,6 +280,7 @@ def call_on(device: torch.device, name: str, *args) -> None:
 
 
 _error_flags: dict[int, torch.Tensor] = {}
+_error_flag_ptrs: dict[int, int] = {}
 _sm_counts: dict[int, int] = {}
 
 
@@ -290,6 +292,15 @@ def error_flag(device: torch.device) -> torch.Tensor:
         flag = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
         _error_flags[idx] = flag
     return flag
+
+
+def error_flag_ptr(device: torch.device) -> int:
+    """Address of :func:`error_flag` of a device with an index (the word is
+    there for as long as the process)."""
+    address = _error_flag_ptrs.get(device.index)
+    if address is None:
+        address = _error_flag_ptrs[device.index] = error_flag(device).data_ptr()
+    return address
 
 
 def read_and_clear_error_flag(device: torch.device) -> int:

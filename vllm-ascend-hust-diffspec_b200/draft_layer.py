@@ -267,7 +267,7 @@ def qk_norm_rope(query: torch.Tensor, kv: torch.Tensor, positions: torch.Tensor,
     :func:`kernels.qkv_projection_write_raw` writes for keys without a norm.
     A position outside the table is flagged and leaves the rows normed but
     unrotated.  Returns ``(query_out, key_out, value_out)``."""
-    d, rot, query_out, q_weight, k_weight, head, value = _qk_norm_inputs(
+    d, rot, query_out, q_weight, k_weight, head, value, table = _qk_norm_inputs(
         query, kv, positions, cos_sin, num_kv_heads, q_weight, k_weight, rotary_dim, query_out)
     tokens, dtype = query.shape[0], query.dtype
     shape = (tokens, num_kv_heads, d)
@@ -277,7 +277,10 @@ def qk_norm_rope(query: torch.Tensor, kv: torch.Tensor, positions: torch.Tensor,
     else:
         raw_key, raw_value, slots, abs_positions = raw
         raw_shape = raw_key.shape
-        if raw_key.ndim != 4 or raw_shape != raw_value.shape or raw_shape[2:] != shape[1:]:
+        if len(raw_shape) != 4 or raw_shape != raw_value.shape:
+            raise ValueError("raw key/value must have matching [S, max_model_len, Hk, D] shapes")
+        raw_slots, max_len, raw_heads, raw_dim = raw_shape
+        if raw_heads != num_kv_heads or raw_dim != d:
             raise ValueError("raw key/value must have matching [S, max_model_len, Hk, D] shapes")
         if raw_key.dtype is not dtype or raw_value.dtype is not dtype:
             raise ValueError("raw caches must have the keys' dtype")
@@ -289,23 +292,22 @@ def qk_norm_rope(query: torch.Tensor, kv: torch.Tensor, positions: torch.Tensor,
                 slots.is_contiguous() and abs_positions.is_contiguous()):
             raise ValueError("slots/positions must cover every token, contiguously")
         places = (raw_key.data_ptr(), raw_value.data_ptr(), slots.data_ptr(),
-                  abs_positions.data_ptr(), raw_shape[0], raw_shape[1])
+                  abs_positions.data_ptr(), raw_slots, max_len)
     device = _lib.device_of(query, kv, positions, cos_sin, q_weight, k_weight, query_out, key_out,
                             value_out, raw_key, raw_value, slots, abs_positions)
-    for name, t in (("key_out", key_out), ("value_out", value_out)):
-        if t is not None and (t.shape != shape or t.dtype is not dtype or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous [T, Hk, D] in the kv dtype")
     if key_out is None:
         key_out = kv.new_empty(shape)
+    elif key_out.dtype is not dtype or key_out.shape != shape or not key_out.is_contiguous():
+        raise ValueError("key_out must be contiguous [T, Hk, D] in the kv dtype")
     if value_out is None:
         value_out = kv.new_empty(shape)
+    elif value_out.dtype is not dtype or value_out.shape != shape or not value_out.is_contiguous():
+        raise ValueError("value_out must be contiguous [T, Hk, D] in the kv dtype")
     _lib.call_on(
         device, "dsb_qk_norm_rope", *head, key_out.data_ptr(), value, head[-1],
         value_out.data_ptr(), num_kv_heads, d, rot, 1 if is_neox_style else 0, q_weight.data_ptr(),
-        k_weight.data_ptr(), eps, positions.data_ptr(), position_offset, tokens,
-        cos_sin.data_ptr(), cos_sin.stride(0), cos_sin.shape[0], _lib.dtype_code(cos_sin.dtype),
-        _lib.dtype_code(dtype), *places, _lib.error_flag(device).data_ptr(),
-        _lib.stream_ptr(device))
+        k_weight.data_ptr(), eps, positions.data_ptr(), position_offset, tokens, *table, *places,
+        _lib.error_flag_ptr(device), _lib.stream_ptr(device))
     return query_out, key_out, value_out
 
 

@@ -669,7 +669,7 @@ def shared_prefix_attention_lse(
         seq.data_ptr(), None if trows is None else trows.data_ptr(), prefix.data_ptr(),
         None if starts is None else starts.data_ptr(), groups, max_prefix_len, max_suffix_len, scale,
         _lib.dtype_code(dtype), out.data_ptr(), lse.data_ptr(), scratch.data_ptr(), floats,
-        _lib.error_flag(device).data_ptr(), _lib.stream_ptr(device),
+        _lib.error_flag_ptr(device), _lib.stream_ptr(device),
     )
     return out, lse
 
@@ -684,7 +684,8 @@ def _qk_norm_inputs(query, kv, positions, cos_sin, num_kv_heads, q_weight, k_wei
                     query_out):
     """What the two query/key norm calls check alike; returns head_dim,
     rotary_dim, query_out, the contiguous weights, the first arguments of the C
-    calls (through the key's row stride) and the value's address."""
+    calls (through the key's row stride), the value's address and the
+    arguments from the table's address through the dtype."""
     if query.ndim != 2 or kv.ndim != 2:
         raise ValueError("query must be [T, Hq * D] and kv [T, 2 * Hk * D]")
     (tokens, q_cols), (kv_rows, kv_cols) = shape, kv_shape = query.shape, kv.shape
@@ -707,20 +708,30 @@ def _qk_norm_inputs(query, kv, positions, cos_sin, num_kv_heads, q_weight, k_wei
         raise ValueError("rotary_dim must be even and between zero and head_dim")
     if rotary_dim % 2:
         raise ValueError("rotary_dim must be even and between zero and head_dim")
-    if cos_sin.ndim != 2 or cos_sin.shape[1] < rotary_dim or cos_sin.stride(1) != 1:
+    if cos_sin.ndim != 2:
+        raise ValueError("cos_sin must be a [rows, cos | sin] table of rotary_dim columns")
+    (cs_rows, cs_cols), (cs_stride, cs_step) = cos_sin.shape, cos_sin.stride()
+    if cs_cols < rotary_dim or cs_step != 1:
         raise ValueError("cos_sin must be a [rows, cos | sin] table of rotary_dim columns")
     if (positions.dtype is not torch.int32 or positions.numel() < tokens
             or not positions.is_contiguous()):
         raise ValueError("positions must be contiguous int32 with one entry per token")
     if query_out is None:
-        query_out = query
-    elif query_out.shape != shape or query_out.dtype is not dtype or query_out.stride(1) != 1:
-        raise ValueError("query_out must be shaped like query, in contiguous rows")
+        query_out, out_stride = query, q_stride
+    else:
+        if query_out.dtype is not dtype or query_out.shape != shape:
+            raise ValueError("query_out must be shaped like query, in contiguous rows")
+        out_stride, out_step = query_out.stride()
+        if out_step != 1:
+            raise ValueError("query_out must be shaped like query, in contiguous rows")
     # query, query_out, heads, key: the arguments both calls begin with
-    head = (query.data_ptr(), q_stride, query_out.data_ptr(), query_out.stride(0), q_cols // d,
-            kv.data_ptr(), kv_stride)
-    value = kv.data_ptr() + num_kv_heads * d * kv.element_size()
-    return d, rotary_dim, query_out, q_weight.contiguous(), k_weight.contiguous(), head, value
+    key = kv.data_ptr()
+    head = (query.data_ptr(), q_stride, query_out.data_ptr(), out_stride, q_cols // d, key, kv_stride)
+    # the table's, and the type's: cos_sin, its row stride, rows and type, the type
+    table = (cos_sin.data_ptr(), cs_stride, cs_rows, _lib.dtype_code(cos_sin.dtype),
+             _lib.dtype_code(dtype))
+    return (d, rotary_dim, query_out, q_weight.contiguous(), k_weight.contiguous(), head,
+            key + num_kv_heads * d * kv.element_size(), table)
 
 
 def qk_norm_rope_write_paged(
@@ -756,7 +767,7 @@ def qk_norm_rope_write_paged(
     if key_cache.ndim != 4 or key_cache.shape != value_cache.shape:
         raise ValueError("the caches must be matching [blocks, bs, Hk, D]")
     num_blocks, block_size, hk, kd = key_cache.shape
-    d, rot, query_out, q_weight, k_weight, head, value = _qk_norm_inputs(
+    d, rot, query_out, q_weight, k_weight, head, value, cos_args = _qk_norm_inputs(
         query, kv, positions, cos_sin, hk, q_weight, k_weight, rotary_dim, query_out)
     tokens, dtype = query.shape[0], query.dtype
     if kd != d or key_cache.dtype is not dtype or value_cache.dtype is not dtype:
@@ -777,10 +788,9 @@ def qk_norm_rope_write_paged(
     _lib.call_on(
         device, "dsb_qk_norm_rope_paged", *head, value, head[-1], hk, d, rot,
         1 if is_neox_style else 0, q_weight.data_ptr(), k_weight.data_ptr(), eps,
-        positions.data_ptr(), tokens, cos_sin.data_ptr(), cos_sin.stride(0), cos_sin.shape[0],
-        _lib.dtype_code(cos_sin.dtype), _lib.dtype_code(dtype), key_cache.data_ptr(),
-        value_cache.data_ptr(), num_blocks, block_size, table.data_ptr(), table.stride(0),
-        table_shape[0], table_shape[1], None if trows is None else trows.data_ptr(),
-        _lib.error_flag(device).data_ptr(), _lib.stream_ptr(device),
+        positions.data_ptr(), tokens, *cos_args, key_cache.data_ptr(), value_cache.data_ptr(),
+        num_blocks, block_size, table.data_ptr(), table.stride(0), table_shape[0], table_shape[1],
+        None if trows is None else trows.data_ptr(), _lib.error_flag_ptr(device),
+        _lib.stream_ptr(device),
     )
     return query_out

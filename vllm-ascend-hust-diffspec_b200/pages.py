@@ -42,14 +42,14 @@ def _pool(ref_counts, block_tables, held):
     if ref_counts.ndim != 1 or block_tables.ndim != 2 or held.ndim != 1:
         raise ValueError("ref_counts must be [pages], block_tables [rows, cols] and held [rows]")
     rows, cols = block_tables.shape
-    if held.shape[0] != rows:
+    if held.numel() != rows:
         raise ValueError("held must have one entry per block-table row")
     if not (ref_counts.dtype is _INT32 and block_tables.dtype is _INT32 and held.dtype is _INT32):
         raise ValueError("ref_counts, block_tables and held must be int32")
     stride, step = block_tables.stride()
     if step != 1 or not (ref_counts.is_contiguous() and held.is_contiguous()):
         raise ValueError("ref_counts and held must be contiguous, block_tables in contiguous rows")
-    return (ref_counts.data_ptr(), ref_counts.shape[0], block_tables.data_ptr(), rows, stride, cols,
+    return (ref_counts.data_ptr(), ref_counts.numel(), block_tables.data_ptr(), rows, stride, cols,
             held.data_ptr())
 
 
@@ -72,7 +72,7 @@ def _caches(caches: Sequence[torch.Tensor], pages: int):
 
 
 def _row(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
-    if t.ndim != 1 or t.shape[0] != n:
+    if t.ndim != 1 or t.numel() != n:
         raise ValueError(f"{name} must have one entry per request of the call")
     if t.dtype is not _INT32:
         if t.is_floating_point() or t.dtype == torch.bool:
@@ -104,12 +104,12 @@ def resize_requests(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: 
     if block_size <= 0:
         raise ValueError("block_size must be positive")
     pool = _pool(ref_counts, block_tables, held)
-    n = rows.shape[0] if rows.ndim == 1 else -1
+    n = rows.numel() if rows.ndim == 1 else -1
     rows, lens = _row(rows, n, "rows"), _row(lens, n, "lens")
     device = _lib.device_of(ref_counts, block_tables, held, rows, lens, status)
     status = _status(status, ref_counts)
     _lib.call_on(device, "dsb_resize_requests", *pool, rows.data_ptr(), lens.data_ptr(), n,
-                 block_size, status.data_ptr(), _lib.error_flag(device).data_ptr(),
+                 block_size, status.data_ptr(), _lib.error_flag_ptr(device),
                  _lib.stream_ptr(device))
     return status
 
@@ -132,7 +132,7 @@ def fork_requests(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: to
     ``status[0]``.  Returns ``status``."""
     pool = _pool(ref_counts, block_tables, held)
     addresses, block_size, token_bytes = _caches(caches, pool[1])
-    n = parents.shape[0] if parents.ndim == 1 else -1
+    n = parents.numel() if parents.ndim == 1 else -1
     parents, children = _row(parents, n, "parents"), _row(children, n, "children")
     lens = _row(lens, n, "lens")
     device = _lib.device_of(ref_counts, block_tables, held, parents, children, lens, status, *caches)
@@ -141,7 +141,7 @@ def fork_requests(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: to
     _lib.call_on(device, "dsb_fork_requests", *pool, parents.data_ptr(), children.data_ptr(),
                  lens.data_ptr(), n, block_size, addresses.buffer_info()[0], len(addresses),
                  token_bytes, status.data_ptr(), scratch.data_ptr(), 6 * n,
-                 _lib.error_flag(device).data_ptr(), _lib.stream_ptr(device))
+                 _lib.error_flag_ptr(device), _lib.stream_ptr(device))
     return status
 
 
@@ -163,7 +163,7 @@ def compact_pages(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: to
     scratch = ref_counts.new_empty(ints)
     _lib.call_on(device, "dsb_compact_pages", *pool, block_size, addresses.buffer_info()[0],
                  len(addresses), token_bytes, status.data_ptr(), scratch.data_ptr(), ints,
-                 _lib.error_flag(device).data_ptr(), _lib.stream_ptr(device))
+                 _lib.error_flag_ptr(device), _lib.stream_ptr(device))
     return status
 
 
@@ -178,9 +178,9 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
         raise ValueError("caches must be [pages, block_size, ...] tensors")
     pages = first.shape[0]
     addresses, block_size, token_bytes = _caches(caches, pages)
-    n = src.shape[0] if src.ndim == 1 else -1
+    n = src.numel() if src.ndim == 1 else -1
     src, dst = _row(src, n, "src"), _row(dst, n, "dst")
     device = _lib.device_of(src, dst, *caches)
     _lib.call_on(device, "dsb_copy_pages", addresses.buffer_info()[0], len(addresses), pages,
                  block_size * token_bytes, src.data_ptr(), dst.data_ptr(), n,
-                 _lib.error_flag(device).data_ptr(), _lib.stream_ptr(device))
+                 _lib.error_flag_ptr(device), _lib.stream_ptr(device))
