@@ -332,3 +332,29 @@ def test_what_lies_behind_many_rows_is_not_read(dsb, cuda):
             out, lse = _run(dsb, c)
             _check(c, out, lse)
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+def test_loads_that_arrive_out_of_order(dsb, cuda):
+    """Pages scattered over a cache of several GB, each read for the first time:
+    some loads then take microseconds longer than the ones behind them.  The
+    cold run gives what the warm one does."""
+    page, hk, rows, tokens, n = 32, 8, 4, 45718, 24
+    per = -(-(tokens + 100) // page)
+    key, value = (torch.empty((n * per, page, hk, _D), dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    for cache in (key, value):
+        for part in cache.chunk(n):
+            part.normal_()
+    g = torch.Generator(device=cuda).manual_seed(1)
+    order = torch.randperm(n * per, generator=g, device=cuda).int()
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    query = torch.randn((rows, 32, _D), generator=g, device=cuda).bfloat16()
+    trow, prefix, seq = ints(*[0] * rows), ints(tokens), ints(*[tokens + 10 + i for i in range(rows)])
+    for i in range(n):
+        call = lambda: dsb.kernels.shared_prefix_attention_lse(  # noqa: E731
+            query, key, value, order[i * per:(i + 1) * per].view(1, per), seq, prefix, scale=_D ** -0.5,
+            max_prefix_len=tokens, max_suffix_len=100, table_rows=trow)
+        cold, cold_lse = call()
+        for _ in range(2):
+            warm, warm_lse = call()
+        assert torch.equal(cold, warm) and torch.equal(cold_lse, warm_lse), i
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0

@@ -399,6 +399,32 @@ __device__ __forceinline__ bool sp_wait(uint32_t bar, uint32_t parity) {
   return mbar_wait(bar, parity);
 }
 
+// Slots of the ring are taken in turn by both loaders and used by both streams,
+// so one of them may come to a slot before the turn ahead of its own has ended,
+// or even begun, and a wait on a parity alone would be satisfied by the turn
+// before that.  `turns[slot]` counts the loads that were asked for; whoever
+// needs load i waits for it first.
+__device__ __forceinline__ bool sp_wait_turn(const volatile int *turns, int i, int count) {
+  uint64_t t0 = 0;
+  for (int k = 0; turns[i % kSpSlots] < count; ++k) {  // (bounded as mbar_wait)
+    if ((k & 63) == 63) {
+      const uint64_t now = global_ns();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > kWaitNs) return false;
+    }
+  }
+  return true;
+}
+// Load i has landed; its slot may be filled with load i.
+__device__ __forceinline__ bool sp_wait_load(const volatile int *turns, uint32_t full, int i) {
+  return sp_wait_turn(turns, i, i / kSpSlots + 1) &&
+         sp_wait(full + 8 * (i % kSpSlots), (uint32_t)(i / kSpSlots) & 1u);
+}
+__device__ __forceinline__ bool sp_wait_slot(const volatile int *turns, uint32_t empty, int i) {
+  return i < kSpSlots || (sp_wait_turn(turns, i, i / kSpSlots) &&
+                          sp_wait(empty + 8 * (i % kSpSlots), (uint32_t)(i / kSpSlots - 1) & 1u));
+}
+
 __device__ __forceinline__ float sp_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -605,7 +631,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
                  joint = q_ready + 8, drain = joint + 8,
                  pv_done = drain + 8;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_issued[2];
+  __shared__ int s_abort, s_turns[kSpSlots];
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int G = a.hq / a.hk;
 
@@ -624,7 +650,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     mbar_init_count(drain, 2);
     for (int i = 0; i < 4; ++i) mbar_init(pv_done + 8 * i);  // [stream][half]
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    s_abort = s_issued[0] = s_issued[1] = 0;
+    s_abort = 0;
+    for (int i = 0; i < kSpSlots; ++i) s_turns[i] = 0;
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
@@ -650,7 +677,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     const bool is_v = warp == 10;
     const CUtensorMap *map = is_v ? &tv : &tk;
     const int boxes = kSpTok / s.box;  // of a tile, at most 16: a lane each
-    int i0 = 0, last = 0;  // loads of the pieces before; this warp's last load + 1
+    int i0 = 0;  // loads of the pieces before
     bool bad = false, ok = true;
     while (ok && walk.next(s, p)) {
       const int32_t *bt = a.bt + (int64_t)p.g.trow * a.bt_stride;
@@ -672,23 +699,22 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         const int i = i0 + (is_v ? (two ? 2 * j + 1 : min(2 * j + 2, 2 * p.n - 1))
                                  : (two ? 2 * j : (j < 2 ? j : 2 * j - 1)));
         const int slot = i % kSpSlots;
-        if (i >= kSpSlots) ok = sp_wait(empty + 8 * slot, (uint32_t)(i / kSpSlots - 1) & 1u);
+        ok = sp_wait_slot(s_turns, empty, i);
         ok = __all_sync(0xffffffffu, ok && !*reinterpret_cast<volatile int *>(&s_abort));
         if (!ok) break;
         const uint32_t bar = full + 8 * slot;
-        if (lane == 0) mbar_expect_tx(bar, kSpTile);
+        if (lane == 0) {
+          mbar_expect_tx(bar, kSpTile);
+          *reinterpret_cast<volatile int *>(s_turns + slot) = i / kSpSlots + 1;
+        }
         __syncwarp();
         if (lane < boxes) sp_load(s_kv + slot * kSpTile + lane * s.box * 256, map, at, p.h, bar);
-        last = i + 1;
         if (j + 1 < p.n) at = place(j + 1);
       }
       i0 += 2 * p.n;
     }
     if (bad) flag_error(a.err, DSB_FLAG_BLOCK);
-    if (lane == 0) {
-      if (!ok) stop();
-      s_issued[is_v] = last;
-    }
+    if (!ok && lane == 0) stop();
   } else if (warp == 9 || warp == 11) {
     const int st = warp == 11;
     const uint32_t qk = umma_idesc<T, 64>(false);
@@ -719,11 +745,11 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         const uint32_t th = ts + half * 64;
         if (k >= 0) {  // O, this half of the stream's tile k
           const int v = i0 + (two ? e | 1 : min(2 * e + 2, 2 * n - 1));  // the load of its V
-          const uint32_t slot = (uint32_t)v % kSpSlots, turn = (uint32_t)v / kSpSlots;
+          const uint32_t slot = (uint32_t)v % kSpSlots;
           const uint32_t b0 =
               ((s_kv + slot * kSpTile + half * (kSpTile / 2)) >> 4) | (1024 / 16) << 16;
           if (!rehearsal) {
-            ok = (half == 1 || sp_wait(full + 8 * slot, turn & 1u)) &&
+            ok = (half == 1 || sp_wait_load(s_turns, full, v)) &&
                  sp_wait(p_ready + 16 * st + 8 * half, (uint32_t)(tiles + k) & 1u);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -745,12 +771,12 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         }
         if (e + 2 < all) {  // S, this half of its next tile
           const int kl = i0 + (two ? (e + 2) & ~1 : (k < 0 ? e + 2 : 2 * e + 3));  // the load of its K
-          const uint32_t slot = (uint32_t)kl % kSpSlots, turn = (uint32_t)kl / kSpSlots;
+          const uint32_t slot = (uint32_t)kl % kSpSlots;
           const uint32_t b0 = ((s_kv + slot * kSpTile + half * (kSpTile / 2)) >> 4) | 1u << 16;
           // one query tile alternates between the two places
           const uint32_t a0 = ((s_q + (two ? st : pieces & 1) * kSpTile) >> 4) | 1u << 16;
           if (!rehearsal) {
-            ok = __all_sync(0xffffffffu, half == 1 || sp_wait(full + 8 * slot, turn & 1u));
+            ok = __all_sync(0xffffffffu, half == 1 || sp_wait_load(s_turns, full, kl));
             if (!ok) break;
           }
           tc_fence_after();
@@ -866,8 +892,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           // (two streams write theirs both, each before its own products).
           if (half == 0 && T0 + kSpTok > p.g.tok1) {
             const int i = i0 + (two ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1));
-            ok = __all_sync(0xffffffffu, sp_wait(full + 8 * (i % kSpSlots),
-                                                 (uint32_t)(i / kSpSlots) & 1u));
+            ok = __all_sync(0xffffffffu, sp_wait_load(s_turns, full, i));
             if (!ok) break;
             const uint32_t v = s_kv + (i % kSpSlots) * kSpTile;
             for (int z = (p.g.tok1 - T0) * 8 + m128; z < kSpTok * 8; z += 128) {
@@ -1062,9 +1087,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   if (s_abort) {
     // A wait ran out: let the copies land and the products end before the
     // shared and tensor memory go.
-    if (tid < 2)  // (of the keys, and of the values: no more than the ring holds)
-      for (int i = max(0, s_issued[tid] - kSpSlots); i < s_issued[tid]; ++i)
-        mbar_wait(full + 8 * (i % kSpSlots), (uint32_t)(i / kSpSlots) & 1u);
+    if (tid < kSpSlots && s_turns[tid] > 0)  // (the last load of each slot)
+      mbar_wait(full + 8 * tid, (uint32_t)(s_turns[tid] - 1) & 1u);
     if (warp == 9 || warp == 11) {
       sp_commit(sp_elect(), drain);
       mbar_wait(drain, 1);
