@@ -334,11 +334,12 @@ def test_what_lies_behind_many_rows_is_not_read(dsb, cuda):
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
 
 
-def test_loads_that_arrive_out_of_order(dsb, cuda):
+@pytest.mark.parametrize("rows", [4, 40])
+def test_loads_that_arrive_out_of_order(dsb, cuda, rows):
     """Pages scattered over a cache of several GB, each read for the first time:
     some loads then take microseconds longer than the ones behind them.  The
     cold run gives what the warm one does."""
-    page, hk, rows, tokens, n = 32, 8, 4, 45718, 24
+    page, hk, tokens, n = 32, 8, 45718, 24
     per = -(-(tokens + 100) // page)
     key, value = (torch.empty((n * per, page, hk, _D), dtype=torch.bfloat16, device=cuda) for _ in range(2))
     for cache in (key, value):

@@ -407,6 +407,7 @@ __device__ __forceinline__ bool sp_wait(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ bool sp_wait_turn(const volatile int *turns, int i, int count) {
   uint64_t t0 = 0;
   for (int k = 0; turns[i % kSpSlots] < count; ++k) {  // (bounded as mbar_wait)
+    if (k == kWaitSpins) return false;
     if ((k & 63) == 63) {
       const uint64_t now = global_ns();
       if (t0 == 0) t0 = now;
