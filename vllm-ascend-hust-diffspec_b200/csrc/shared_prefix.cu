@@ -1106,8 +1106,8 @@ constexpr int kMergeWarps = 4;
 // A CTA a (row, query head), a lane four of its dims: warp w takes pieces w,
 // w + 4, ... of the prefix and, behind them, of the row's own tokens, eight
 // loads on their way, and the warps' sums are joined in order.  One warp a
-// (row, head) instead (SPREAD false) when they alone fill the GPU: 2560 of a
-// few pieces each, 11.8 us against 19.8.
+// (row, head) instead (SPREAD false) when they alone fill the GPU (a call with
+// 7680 of a few pieces each: 54 us against 67; 512 of 38 pieces: 50 against 46).
 template <typename T, bool SPREAD>
 __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(const SpArgs s) {
   __shared__ float4 s_acc[kMergeWarps][32];
