@@ -874,6 +874,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       const bool mine = m < nq && !rehearsal;
       if (!rehearsal && !early) {
         fetch(p, pieces);
+        lim = sees(p);  // (beside the copies)
         fetched();
       }
       const bool works = __any_sync(0xffffffffu, m < nq);
@@ -985,8 +986,10 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         // run beside the sums
         has_next = walk.next(s, after);
         early = has_next && !two && after.g.nq <= 128;
-        if (early) fetch(after, pieces + 1);
-        if (has_next) lim = sees(after);
+        if (early) {
+          fetch(after, pieces + 1);
+          lim = sees(after);
+        }
 
         // the piece's sums (its products are done): [nq][D], and (maximum, sum)
         ok = __all_sync(0xffffffffu, sp_wait(o_done, (uint32_t)pieces & 1u));
@@ -1073,7 +1076,6 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         pdl_begin();
         walk.begin(s);
         if (!walk.next(s, p)) break;
-        lim = sees(p);
         continue;
       }
       ++pieces;
