@@ -359,3 +359,27 @@ def test_loads_that_arrive_out_of_order(dsb, cuda, rows):
             warm, warm_lse = call()
         assert torch.equal(cold, warm) and torch.equal(cold_lse, warm_lse), i
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+def test_scratch_that_holds_other_numbers(dsb, cuda):
+    """The merge walks as many pieces as the scratch says.  The counts of
+    segments that no CTA writes (without tokens here; those of a CTA whose wait
+    ran out) are zeros after the call, whatever the scratch held."""
+    lens, hq, hk, page, groups = [33, 1, 200], 32, 4, 16, 1
+    c = _case(cuda, [(0, lens, 1)], hq, hk, page, "bf16", 1)
+    rows, P = len(lens), dsb._lib
+    floats = P.load().dsb_shared_prefix_scratch_floats(rows, hq, hk, groups, page, 0, 200)
+    scratch = torch.full((floats,), 0x7f7f7f7f, dtype=torch.int32, device=cuda)
+    out, lse = torch.empty_like(c["query"]), torch.empty((rows, hq), device=cuda)
+    P.call("dsb_shared_prefix_attention_lse", P.ptr(c["query"]), rows, hq, hk, _D, P.ptr(c["key"]),
+           P.ptr(c["value"]), c["key"].shape[0], page, P.ptr(c["table"]), c["table"].stride(0),
+           *c["table"].shape, P.ptr(c["seq"]), P.ptr(c["trow"]), P.ptr(c["prefix"]),
+           P.ptr(c["starts"]), groups, 0, 200, _D ** -0.5, P.dtype_code(torch.bfloat16), P.ptr(out),
+           P.ptr(lse), P.ptr(scratch), floats, P.ptr(P.error_flag(cuda)), P.stream_ptr(cuda))
+    _check(c, out, lse)
+    # scratch: 4 words a CTA, 16 a segment, 4 a row, 1 a group, then the counts [segments, kv heads]
+    segments = -(-rows * (hq // hk) // 256) + groups + rows
+    at = -(-(P.sm_count(cuda) * 4 + segments * 16 + rows * 4 + groups) // 8) * 8
+    counts = scratch[at: at + (1 + rows) * hk].view(-1, hk)
+    assert counts.tolist() == [[0] * hk, [1] * hk, [1] * hk, [2] * hk]
+    assert P.read_and_clear_error_flag(cuda) == 0

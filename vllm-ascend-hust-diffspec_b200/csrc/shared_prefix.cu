@@ -82,7 +82,7 @@ struct SpArgs {
   SpSeg *segs;
   SpRow *rows;
   int32_t *gseg;       // [groups] first prefix segment of each
-  int32_t *pieces;     // [segs, kv heads] pieces of a segment with tokens
+  int32_t *pieces;     // [segs, kv heads] pieces of a segment, 0 until its last one is there
   float *acc;          // [rows of partial sums, D]
   float2 *ml;          // [rows of partial sums]: maximum (log2), sum
 };
@@ -368,6 +368,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
       s.segs[i].maxp = maxp;
     }
   }
+  // no pieces yet: a CTA that gives up on a wait leaves its segments without
+  for (int64_t i = tid; i < (int64_t)nseg * a.hk; i += kPlanThreads) s.pieces[i] = 0;
   // where each CTA begins: the last segment that starts at or before its first
   // unit (an empty one starts where the next does)
   SpBegin shares{units / s.ctas, (int)(units % s.ctas), 0};
@@ -1134,9 +1136,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(c
     const int seg = part == 0 ? (at.pseg < 0 ? -1 : at.pseg + m / 256) : at.sseg;
     if (seg < 0) continue;
     const SpSeg &g = s.segs[seg];
-    const int pieces = s.pieces[(int64_t)seg * a.hk + h];
-    if (g.len == 0) continue;  // (and `pieces` was never written)
-    count[part] = pieces;
+    count[part] = min(s.pieces[(int64_t)seg * a.hk + h], g.maxp);  // (0 of 0 without tokens)
     stride[part] = g.nq;
     place[part] = g.acc + (int64_t)h * g.maxp * g.nq + (part == 0 ? m % 256 : at.srow * G + head % G);
   }
