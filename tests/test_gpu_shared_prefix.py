@@ -383,3 +383,23 @@ def test_scratch_that_holds_other_numbers(dsb, cuda):
     counts = scratch[at: at + (1 + rows) * hk].view(-1, hk)
     assert counts.tolist() == [[0] * hk, [1] * hk, [1] * hk, [2] * hk]
     assert P.read_and_clear_error_flag(cuda) == 0
+
+
+@pytest.mark.parametrize("requests,page", [(3, 16), (40, 16), (3, 5)])
+@pytest.mark.parametrize("shift", [1, 2, 6])
+def test_outputs_at_an_offset(dsb, cuda, requests, page, shift):
+    """``out`` and ``lse`` that are views into wider buffers, at any element."""
+    c = _case(cuda, [(100, [101 + i for i in range(requests)], 1)], 32, 4, page, "bf16", shift)
+    rows, hq = c["query"].shape[:2]
+    wide = torch.full((rows * hq * _D + 16,), 7.0, dtype=torch.bfloat16, device=cuda)
+    wide_lse = torch.full((rows * hq + 16,), 7.0, device=cuda)
+    out = wide[shift: shift + rows * hq * _D].view(rows, hq, _D)
+    lse = wide_lse[shift: shift + rows * hq].view(rows, hq)
+    got = _run(dsb, c, out=out, lse=lse)
+    assert got[0] is out and got[1] is lse
+    _check(c, out, lse)
+    plain, plain_lse = _run(dsb, c)
+    assert torch.equal(out, plain) and torch.equal(lse, plain_lse)
+    for w, n in ((wide, rows * hq * _D), (wide_lse, rows * hq)):
+        assert (w[:shift] == 7).all() and (w[shift + n:] == 7).all()
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0

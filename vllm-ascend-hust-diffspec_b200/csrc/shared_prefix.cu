@@ -1207,7 +1207,14 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_prefix_merge_kernel(c
   uint2 out;
   out.x = pack2<T>(acc.x * inv, acc.y * inv);
   out.y = pack2<T>(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + rh * kTaD + 4 * lane) = out;
+  T *dst = static_cast<T *>(a.out) + rh * kTaD + 4 * lane;
+  if (reinterpret_cast<uintptr_t>(dst) % 8 == 0) {
+    *reinterpret_cast<uint2 *>(dst) = out;
+  } else {  // rows that begin off an 8-byte boundary (a view of a wider buffer)
+    const T *y = reinterpret_cast<const T *>(&out);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = y[i];
+  }
   if (lane == 0) a.lse[rh] = none ? -INFINITY : (top + log2f(sum)) * kTaLn2;
 }
 
