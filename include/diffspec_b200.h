@@ -595,7 +595,7 @@ int dsb_qk_norm_rope_paged(
  * [group_starts[i], group_starts[i + 1]) (num_groups + 1 entries, ascending;
  * null: one group of every row) hold the same tokens at positions
  * [0, prefix_lens[i]), which are read once for the group, through the table
- * row of the first row that sees any; the tokens behind it, up to
+ * row of a row that sees as much of them as any; the tokens behind it, up to
  * seq_lens[r], through the row's own, once for consecutive rows on one table
  * row.  Groups that do not ascend within the rows are flagged
  * (DSB_FLAG_SLOT) and share nothing.  max_prefix_len and max_suffix_len size

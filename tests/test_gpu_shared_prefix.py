@@ -403,3 +403,25 @@ def test_outputs_at_an_offset(dsb, cuda, requests, page, shift):
     for w, n in ((wide, rows * hq * _D), (wide_lse, rows * hq)):
         assert (w[:shift] == 7).all() and (w[shift + n:] == 7).all()
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+@pytest.mark.parametrize("behind", ["none", "others"])
+@pytest.mark.parametrize("page", [16, 128, 5])
+def test_a_short_row_in_front(dsb, cuda, behind, page):
+    """Rows that see less of the prefix than the ones behind them, in one
+    segment and in several, whose table rows have no pages, or pages of
+    something else, behind their own lengths."""
+    for lens, hq, hk in (([120, 0, 300, 310], 16, 2), ([0, 1, 299, 300], 8, 1),
+                         ([7, *[290] * 8, 300, 301] * 8, 16, 1), ([33, 120], 8, 1)):
+        c = _case(cuda, [(300, lens, 1)], hq, hk, page, "bf16", page + len(lens))
+        c["prefix"].fill_(max(min(300, n) for n in lens))
+        other = c["table"].max() if behind == "others" else -1
+        for r, n in enumerate(lens):
+            c["table"][r, -(-n // page):] = other
+        out, lse = _run(dsb, c)
+        assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+        _check(c, out, lse)
+    # a prefix beyond the table is cut to it, and no row's missing pages are read
+    c["prefix"].fill_(10 ** 6)
+    _run(dsb, c)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0

@@ -226,7 +226,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
   __syncthreads();
 
   // the prefix segments, a warp each (the last ones first: the first warps have
-  // the rows): as far as any of their rows sees
+  // the rows): as far as any of their rows sees, through the table row of one
+  // that sees as far (a shorter one's need not name the pages behind it)
   for (int p = kPlanThreads / 32 - 1 - warp; p < nprefix; p += kPlanThreads / 32) {
     int x = 0, y = groups;
     while (x < y) {
@@ -240,26 +241,24 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
     g.row0 = lo, g.q0 = (p - gseg_of(gi)) * 256;
     g.nq = (int)min((int64_t)256, (int64_t)(start_of(gi + 1) - lo) * G - g.q0);
     const int r0 = lo + g.q0 / G, r1 = lo + (g.q0 + g.nq - 1) / G;
-    int most = 0, trow = -1;
-    for (int r = r0 + lane; r - lane <= r1; r += 32) {
-      int64_t t = -1;
-      int L = 0;
-      if (r <= r1) {
-        if (r < kPlanThreads) {
-          L = s_seen[r], t = s_trow[r];
-        } else {
-          t = sp_table_row(a, r);
-          L = sp_sees(a, a.seq[r], t, false);
-        }
-        L = min(L, prefix);
+    int most = 0, trow = 0;  // of the lane's rows, its first that sees most
+    for (int r = r0 + lane; r <= r1; r += 32) {
+      int64_t t;
+      int L;
+      if (r < kPlanThreads) {
+        L = s_seen[r], t = s_trow[r];
+      } else {
+        t = sp_table_row(a, r);
+        L = sp_sees(a, a.seq[r], t, false);
       }
-      most = max(most, L);
-      const unsigned sees = __ballot_sync(0xffffffffu, L > 0);
-      const int tr = __shfl_sync(0xffffffffu, (int)t, sees ? __ffs(sees) - 1 : 0);
-      if (trow < 0 && sees) trow = tr;
+      L = min(L, prefix);
+      if (L > most) most = L, trow = (int)t;
     }
+    const int lane_most = most;
     most = __reduce_max_sync(0xffffffffu, most);
-    g.trow = max(trow, 0);
+    const unsigned whole = __ballot_sync(0xffffffffu, lane_most == most);
+    trow = __shfl_sync(0xffffffffu, trow, __ffs(whole) - 1);
+    g.trow = trow;
     g.tok1 = most;
     g.len = most > 0 ? SpCost(g.nq).units((most + kSpTok - 1) / kSpTok) : 0;
     if (lane == 0) keep(p, g);

@@ -603,9 +603,10 @@ def shared_prefix_attention_lse(
     are flagged and share nothing): requests forked from one
     prompt (:func:`pages.fork_requests`), or verify rows of theirs.  Row ``r``
     sees the first ``seq_lens[r]`` tokens of block-table row ``table_rows[r]``
-    (default ``r``); the prefix is read through the table row of the first row
-    that sees any of it.  A row may see less than its prefix, or nothing
-    (zeros, and an LSE of -inf); what the rows of a group see must be finite.
+    (default ``r``); the prefix is read through the table row of a row that
+    sees as much of it as any.  A row may see less than its prefix (and its
+    table row hold no pages behind that), or nothing (zeros, and an LSE of
+    -inf); what the rows of a group see must be finite.
 
     ``max_prefix_len`` and ``max_suffix_len`` (the most tokens that a row has
     behind its prefix) size the launches; longer ones are read all the same.
