@@ -425,3 +425,46 @@ def test_a_short_row_in_front(dsb, cuda, behind, page):
     c["prefix"].fill_(10 ** 6)
     _run(dsb, c)
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("span", [1, 30])
+def test_weights_far_below_the_largest(dsb, cuda, dtype, page, span):
+    """One token takes nearly all of the weight and has a value of zero; 7000
+    others, 15 to 18 nats below it, make the output by themselves.  With one
+    product a logit, dS is the rounding of the scale, of the logit times it and
+    of the difference from the maximum (4 u of 26 bits); the rest as above, of
+    the output itself, as all of its terms are of one sign.  A weight is off by
+    2^-32 of the largest at most in fp16, and never by more than 2^-17 of itself
+    in bf16."""
+    n, requests = 7000, 20
+    lens = [n - i for i in range(requests)]
+    c = _case(cuda, [(0, lens, span)], 8, 8, page, dtype, 3)  # each request reads its own tokens
+    low = torch.tensor([12.375, 10.75, 11.5, 12.0, 12.75, 10.625, 11.0, 12.625], device=cuda)
+    c["query"].zero_()
+    c["query"][..., 0] = 16
+    c["key"].zero_()
+    c["key"][..., 0] = -low.to(_T[dtype])
+    c["value"].fill_(1.0)
+    for r in range(requests):
+        first = c["table"][r, 0].long()
+        c["key"][first, 0, :, 0] = 0
+        c["value"][first, 0] = 0
+    scale = _D ** -0.5
+    out, lse = _run(dsb, c, max_prefix_len=0, max_suffix_len=0)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+    u, step = 2.0 ** -24, torch.finfo(_T[dtype]).eps / 2
+    far = torch.exp(-16 * low.to(_T[dtype]).double() * scale)
+    for r, seen in enumerate(c["seq"].tolist()):
+        w = far * (seen - 1)
+        ref = (w / (1 + w))[:, None]
+        chain = (seen / 32 + 256) * u
+        e = ref * (4 * 26 * u + 2.0 ** -17 + 2.0 ** -22 + chain)
+        if dtype == "f16":
+            e = e + (seen - 1) * 2.0 ** -32
+        tol = step * (ref + e) + e + torch.finfo(_T[dtype]).smallest_normal * step
+        off = (out[r].double() - ref).abs()
+        assert bool((off <= tol).all()), (r, float((off / tol).max()))
+        tol = 4 * 26 * u + 2.0 ** -22 + chain + u
+        assert bool(((lse[r].double() - torch.log1p(w)).abs() <= tol).all()), r

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -79,11 +80,14 @@ __device__ __forceinline__ void ta_ldsm_x4_trans(uint32_t (&r)[4], uint32_t addr
 // Rows past the split (or past seq_lens) are zero-filled and masked; a page
 // entry outside the cache is flagged and its tokens read as zeros.
 // ANY: a group of any size up to GMAX query heads, and the row's tokens split
-// evenly over the launch's splits whatever its length.
+// evenly over the launch's splits whatever its length.  A split may then be
+// long, so fp16 weights, which have no steps below 2^-24, are taken 2^15 times
+// (they are at most 1): off by 2^-40 of the largest, not by 2^-25, each.
 template <typename T, int GMAX, bool ANY>
 __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(const TaArgs a) {
   static_assert(GMAX <= 16, "at most 16 query heads per kv head");
   const int G = ANY ? a.hq / a.hk : GMAX;
+  constexpr float kUp = ANY && std::is_same<T, __half>::value ? 32768.f : 1.f;
   extern __shared__ __align__(128) uint8_t s_raw[];  // rings, then the warps' states
   pdl_begin();
   // kv head fastest: the Hk CTAs of one (split, row) read the quarters of
@@ -232,10 +236,10 @@ __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(co
     float p[2][4];
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
-      p[nt][0] = exp2f(sc[nt][0] - mn_lo);
-      p[nt][1] = exp2f(sc[nt][1] - mn_lo);
-      p[nt][2] = exp2f(sc[nt][2] - mn_hi);
-      p[nt][3] = exp2f(sc[nt][3] - mn_hi);
+      p[nt][0] = exp2f(sc[nt][0] - mn_lo) * kUp;
+      p[nt][1] = exp2f(sc[nt][1] - mn_lo) * kUp;
+      p[nt][2] = exp2f(sc[nt][2] - mn_hi) * kUp;
+      p[nt][3] = exp2f(sc[nt][3] - mn_hi) * kUp;
     }
     l_lo = l_lo * c_lo + (p[0][0] + p[0][1] + p[1][0] + p[1][1]);  // this lane's share
     l_hi = l_hi * c_hi + (p[0][2] + p[0][3] + p[1][2] + p[1][3]);
@@ -306,10 +310,10 @@ __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(co
       }
     }
     float *pp = a.part + (((int64_t)r * a.hq + h * G + hh) * a.splits + split) * (kTaD + 2);
-    pp[d] = ac;
+    pp[d] = ac * (1.f / kUp);
     if (d == 0) {
       pp[kTaD] = M;
-      pp[kTaD + 1] = sum;
+      pp[kTaD + 1] = sum * (1.f / kUp);
     }
   }
 }

@@ -19,6 +19,8 @@
 // same bits.  Back to back: 16 rows on one prefix of 40800 tokens (32/4 heads)
 // 37 us, 80 on 32777 90, 64 on two of 65536 (64/8 heads) 244 (0.34 of the
 // measured bf16 rate before the second term of the weights is counted).
+#include <type_traits>
+
 #include "paged_split.cuh"
 #include "tma_umma.cuh"
 
@@ -33,6 +35,9 @@ constexpr int kSpThreads = 384;
 constexpr int kSpSmem = 1024 + (2 + kSpSlots) * kSpTile + 256;  // queries, ring, barriers
 constexpr int kSpStage = 144;       // bytes: 32 columns of a row, and 16 more for the banks
 constexpr float kSpGrow = 8.f;      // log2 of the growth that rescales O
+// log2 of what the weights are multiplied by: fp16 has no steps below 2^-24, and
+// with the growth above this takes the weights to its upper end, 2^15.
+template <typename T> constexpr float kSpUp = std::is_same<T, __half>::value ? 7.f : 0.f;
 // The shares are counted in units of 2300 clocks: a tile is one of them, or two
 // when both streams take it, and a piece's queries, first loads and sums are
 // five.  (640 query rows of a kv head are tiles of both kinds: 88 us against
@@ -614,7 +619,11 @@ struct SpWalk {
 // P takes S's place as two 16-bit terms, hi + lo (the weights keep ~16 bits;
 // one term alone costs the output half a step more), so P . V is two
 // products.  O is rescaled only when a row's maximum has grown by more than
-// 2^8 since the last time: until then P stays below 2^8, in fp32 sums.
+// 2^8 since the last time: until then P stays below 2^8, in fp32 sums.  In fp16,
+// whose steps end at 2^-24, P is 2^7 times that: a weight is then off by at most
+// 2^-17 of itself or 2^-32 of the row's largest (without, 2^-25 of it, and the
+// tokens 17 nats below one that dominates a piece were lost to the output and
+// not to the sum: 4e-5 of 1.7e-4 for 7000 such tokens).
 //   up to 128 query rows in the segment: the streams take its even and odd
 //   tiles, and their sums are joined at the piece's end;
 //   more: each stream has 128 of the query rows, and takes every tile.
@@ -959,7 +968,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
               }
             }
           }
-          const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+          const float neg = (m_ref == -INFINITY ? 0.f : -m_ref) + kSpUp<T>;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
           auto weights = [&](const uint32_t(&x)[32], int c) {
             uint32_t w[32];  // 16 pairs of hi terms, 16 of lo terms
@@ -1033,7 +1042,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           }
           __syncwarp();
         }
-        if (mine) s.ml[at] = make_float2(l != l ? 0.f : m_ref, l);  // (NaN is no empty sum)
+        if (mine) s.ml[at] = make_float2(l != l ? 0.f : m_ref - kSpUp<T>, l);  // (NaN is no empty sum)
         tc_fence_before();
         both();  // all of it is read before the next piece's queries
       } else {
@@ -1069,7 +1078,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
               }
           }
         const float sum = x0.y * f0 + x1.y * f1;
-        if (mine && stream == 0) s.ml[at] = make_float2(sum != sum ? 0.f : M, sum);
+        if (mine && stream == 0) s.ml[at] = make_float2(sum != sum ? 0.f : M - kSpUp<T>, sum);
         // all of it is read before the next piece's queries and products
         tc_fence_before();
         both();
