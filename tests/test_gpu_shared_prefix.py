@@ -468,3 +468,39 @@ def test_weights_far_below_the_largest(dsb, cuda, dtype, page, span):
         assert bool((off <= tol).all()), (r, float((off / tol).max()))
         tol = 4 * 26 * u + 2.0 ** -22 + chain + u
         assert bool(((lse[r].double() - torch.log1p(w)).abs() <= tol).all()), r
+
+
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_nan_among_what_a_row_sees(dsb, cuda, page, dtype):
+    """A key that is not a number among a request's own tokens, every key of a
+    request, a value: the rows that see it say so, whatever the page size, and
+    the others are right."""
+    def case():
+        return _case(cuda, [(90, [100, 95, 97], 2)], 8, 1, page, dtype, 5)
+
+    def alone(c, rows, out, lse):
+        part = {**c, "query": c["query"][rows], "trow": c["trow"][rows]}
+        _check(part, out[rows], lse[rows], seq=[c["seq"].tolist()[r] for r in rows])
+
+    c = case()
+    at = c["table"][0, 98 // page].long(), 98 % page
+    c["key"][at] = float("nan")  # behind all that the others see
+    out, lse = _run(dsb, c)
+    for r in (0, 1):
+        assert torch.isnan(out[r]).all() and torch.isnan(lse[r]).all(), r
+    alone(c, [2, 3, 4, 5], out, lse)
+    c = case()
+    c["value"][at[0], at[1], 0, 3] = float("nan")
+    out, lse = _run(dsb, c)
+    assert torch.isnan(out[:2, :, 3]).all() and not torch.isnan(out[:2, :, 4:]).any()
+    assert torch.isfinite(lse).all()
+    alone(c, [2, 3, 4, 5], out, lse)
+    c = case()
+    c["key"].fill_(float("nan"))
+    c["seq"][4] = 0
+    out, lse = _run(dsb, c)
+    for r in (0, 1, 2, 3, 5):
+        assert torch.isnan(out[r]).all() and torch.isnan(lse[r]).all(), r
+    assert (out[4] == 0).all() and torch.isneginf(lse[4]).all()
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0

@@ -289,9 +289,10 @@ __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(co
       if (row < G) s_acc[(warp * GMAX + row) * kTaD + d] = o[dn][j];
     }
   if (t == 0) {
-    s_ml[(warp * 16 + g) * 2] = m_lo;
+    // (ANY: a sum that is NaN is no empty one, although its maximum may be -inf)
+    s_ml[(warp * 16 + g) * 2] = ANY && l_lo != l_lo ? 0.f : m_lo;
     s_ml[(warp * 16 + g) * 2 + 1] = l_lo;
-    s_ml[(warp * 16 + g + 8) * 2] = m_hi;
+    s_ml[(warp * 16 + g + 8) * 2] = ANY && l_hi != l_hi ? 0.f : m_hi;
     s_ml[(warp * 16 + g + 8) * 2 + 1] = l_hi;
   }
   __syncthreads();
@@ -319,8 +320,8 @@ __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(co
 }
 
 // One CTA per (row, query head), thread = output element: merge the splits
-// in order.
-template <typename T>
+// in order.  ANY: rows whose sum is NaN are NaN (else zeros, and -inf).
+template <typename T, bool ANY>
 __global__ void __launch_bounds__(kTaD) paged_decode_merge_kernel(const TaArgs a) {
   pdl_begin();
   const int64_t rh = blockIdx.x;  // r * hq + head
@@ -337,9 +338,10 @@ __global__ void __launch_bounds__(kTaD) paged_decode_merge_kernel(const TaArgs a
       ac = fmaf(q[d], f, ac);
     }
   }
-  const float y = sum > 0.f ? ac / sum : 0.f;
+  const bool some = ANY ? M != -INFINITY : sum > 0.f;
+  const float y = some ? ac / sum : 0.f;
   static_cast<T *>(a.out)[rh * kTaD + d] = Elem<T>::from_f(y);
-  if (d == 0) a.lse[rh] = sum > 0.f ? (M + log2f(sum)) * kTaLn2 : -INFINITY;
+  if (d == 0) a.lse[rh] = some ? (M + log2f(sum)) * kTaLn2 : -INFINITY;
 }
 
 }  // namespace

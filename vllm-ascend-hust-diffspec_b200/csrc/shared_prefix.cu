@@ -1297,7 +1297,7 @@ template <typename T> int run_typed(SpArgs &s, const SpPlan &p, float *scratch, 
     if (int e = ensure_smem((const void *)kern, smem); e != DSB_OK) return e;
     launch_kernel(kern, dim3(a.hk, a.splits, a.rows), dim3(kTaWarps * 32), smem, st, a);
     if (int e = check_launch("paged_decode_split_kernel")) return e;
-    launch_kernel(paged_decode_merge_kernel<T>, dim3((unsigned)rh), dim3(kTaD), 0, st, a);
+    launch_kernel(paged_decode_merge_kernel<T, true>, dim3((unsigned)rh), dim3(kTaD), 0, st, a);
     return check_launch("paged_decode_merge_kernel");
   }
   s.box = p.box;

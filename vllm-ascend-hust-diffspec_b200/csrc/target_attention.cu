@@ -45,7 +45,7 @@ template <typename T> int launch_typed(const TaArgs &a, int group, cudaStream_t 
   }
   if (e != DSB_OK) return e;
   if (int e2 = check_launch("paged_decode_split_kernel")) return e2;
-  launch_kernel(paged_decode_merge_kernel<T>, dim3((unsigned)(a.rows * a.hq)), dim3(kTaD), 0, st,
+  launch_kernel(paged_decode_merge_kernel<T, false>, dim3((unsigned)(a.rows * a.hq)), dim3(kTaD), 0, st,
                 a);
   return check_launch("paged_decode_merge_kernel");
 }
