@@ -592,9 +592,10 @@ int dsb_qk_norm_rope_paged(
     int32_t *error_flag, void *stream);
 
 /* dsb_paged_decode_attention_lse for rows that share a prefix: rows
- * [group_starts[i], group_starts[i + 1]) (num_groups + 1 entries, ascending;
- * null: one group of every row) hold the same tokens at positions
- * [0, prefix_lens[i]), which are read once for the group, through the table
+ * [group_starts[i], group_starts[i + 1]) (num_groups + 1 entries, ascending,
+ * at most query_rows groups; null: one group of every row) hold the same
+ * tokens at positions [0, prefix_lens[i]), which are read once for the group,
+ * through the table
  * row of a row that sees as much of them as any; the tokens behind it, up to
  * seq_lens[r], through the row's own, once for consecutive rows on one table
  * row.  Groups that do not ascend within the rows are flagged

@@ -159,6 +159,33 @@ def test_runtime_target_attention_with_shared_prefixes(dsb, cuda, groups):
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
 
 
+@pytest.mark.parametrize("query_ends", [[1, 1, 2, 3], [0, 0, 2, 2], [3, 3, 3, 3], [0, 0, 0, 0]])
+def test_runtime_groups_without_query_rows(dsb, cuda, query_ends):
+    """Requests without query rows this step, each a group of its own (more
+    groups than rows): the plain call's outputs and LSE."""
+    g = torch.Generator(device=cuda).manual_seed(sum(query_ends))
+    hq, hk, d, page = 8, 2, 128, 16
+    cache = [torch.randn((40, page, hk, d), generator=g, device=cuda).to(_BF) for _ in range(2)]
+    query = torch.randn((query_ends[-1], hq, d), generator=g, device=cuda).to(_BF)
+    meta = SimpleNamespace(actual_seq_lengths_q=query_ends, seq_lens_list=[30, 40, 50, 60],
+                           block_tables=torch.arange(40, device=cuda, dtype=torch.int32).view(4, 10),
+                           num_prefills=0)
+    got = []
+    for kw in ({}, dict(shared_prefix=([10, 0, 5, 7], [1, 2, 3, 4])), dict(shared_prefix=([0, 9], [3, 4]))):
+        state = dsb.runtime.DiffSpecDraftCache(
+            dsb.runtime.DiffSpecSettings(16, 128, 1, 4, 3, 0.7, False), max_num_reqs=4,
+            max_model_len=512, num_kv_heads=hk, head_dim=d, target_num_layers=2, dtype=_BF,
+            device=cuda, cos_sin_cache=torch.zeros((128, d), device=cuda).to(_BF))
+        state.begin_target_forward(["a", "b", "c", "d"])
+        got.append((state.run_target_attention(query, *cache, meta, d ** -0.5, **kw),
+                    state._target["lse"].clone()))
+    for out, lse in got[1:]:
+        assert out.shape == got[0][0].shape
+        close_bf16(out.float().cpu().numpy(), got[0][0].float().cpu().numpy(), max_rel=2.0 ** -7)
+        np.testing.assert_allclose(lse.cpu().numpy(), got[0][1].cpu().numpy(), atol=2e-5)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
 def test_draft_layer_with_head_norms(dsb, cuda):
     """Eagle3DraftLayer(qk_norm=True): the pieces of its step against the layer
     computed from the projection by hand, the raw cache's keys normed and not

@@ -599,8 +599,8 @@ def shared_prefix_attention_lse(
     Rows ``[group_starts[i], group_starts[i + 1])`` (int32 ``[groups + 1]``,
     ascending from 0 to the row count; one group of every row when omitted)
     hold the same tokens at positions ``[0, prefix_lens[i])`` (int32
-    ``[groups]``; any length, whole pages or not; groups that do not ascend
-    are flagged and share nothing): requests forked from one
+    ``[groups]``; any length, whole pages or not; no more groups than rows;
+    groups that do not ascend are flagged and share nothing): requests forked from one
     prompt (:func:`pages.fork_requests`), or verify rows of theirs.  Row ``r``
     sees the first ``seq_lens[r]`` tokens of block-table row ``table_rows[r]``
     (default ``r``); the prefix is read through the table row of a row that

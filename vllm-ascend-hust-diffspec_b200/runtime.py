@@ -478,10 +478,13 @@ class DiffSpecDraftCache:
             )
         else:
             prefix_lens, starts, longest = prefix_groups(*shared_prefix, query_ends, seq_lens)
+            # (requests without query rows this step may leave groups without any)
+            some = [i for i, first in enumerate(starts[:-1]) if starts[i + 1] > first]
+            prefix_lens, starts = [prefix_lens[i] for i in some], [starts[i] for i in some] + starts[-1:]
             out, lse = shared_prefix_attention_lse(
                 query, key_cache, value_cache, metadata.block_tables, lens,
                 torch.tensor(prefix_lens, dtype=torch.int32).to(self.device), scale=scale,
-                max_prefix_len=max(prefix_lens), max_suffix_len=longest,
+                max_prefix_len=max(prefix_lens, default=0), max_suffix_len=longest,
                 group_starts=torch.tensor(starts, dtype=torch.int32).to(self.device),
                 table_rows=rows,
             )
