@@ -602,7 +602,7 @@ int dsb_qk_norm_rope_paged(
  * (DSB_FLAG_SLOT) and share nothing.  max_prefix_len and max_suffix_len size
  * the launches alone.  Block sizes that are no multiple of 8 share nothing.
  * Any group of up to 16 query heads per kv head, head_dim 128; scratch is
- * 32-byte aligned. */
+ * 32-byte aligned, of the size for the device that is current, the call's. */
 int64_t dsb_shared_prefix_scratch_floats(int32_t query_rows, int32_t num_query_heads,
                                          int32_t num_kv_heads, int32_t num_groups,
                                          int32_t block_size, int32_t max_prefix_len,

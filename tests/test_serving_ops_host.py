@@ -211,3 +211,41 @@ def test_prefix_groups(dsb):
     for lens, ends in (([], []), ([1], [3, 4]), ([-1], [4]), ([1, 1], [3, 2]), ([1], [5]), ([1], [3])):
         with pytest.raises(ValueError, match="shared_prefix"):
             f(lens, ends, [1, 2, 3, 4], [5, 5, 5, 5])
+
+
+def test_scratch_is_sized_on_the_tensors_device(dsb, monkeypatch):
+    """Two devices of other SM counts: each call's scratch has the size that
+    the device of its tensors needs, whatever is current and whatever came
+    before."""
+    kernels, lib = dsb.kernels, dsb._lib
+    current, sizes, asked = [0], {0: 1000, 1: 3000}, []
+
+    class Device:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Library:
+        @staticmethod
+        def dsb_shared_prefix_scratch_floats(*sizes_):
+            return sizes[current[0]]
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(lib, "load", Library)
+    monkeypatch.setattr(lib, "error_flag_ptr", lambda device: 0)
+    monkeypatch.setattr(lib, "stream_ptr", lambda device: 0)
+    monkeypatch.setattr(lib, "call_on", lambda device, name, *a: asked.append((device.index, a[-3])))
+    q = torch.zeros((3, 8, 128), dtype=torch.bfloat16)
+    kc = torch.zeros((4, 16, 2, 128), dtype=torch.bfloat16)
+    kernels._shared_prefix_floats.cache_clear()
+    for index in (1, 0, 1, 0):
+        monkeypatch.setattr(lib, "device_of", lambda *_: torch.device("cuda", index))
+        kernels.shared_prefix_attention_lse(q, kc, kc, _i(3, 4), _i(3), _i(1), scale=0.1,
+                                            max_prefix_len=16, max_suffix_len=16)
+    kernels._shared_prefix_floats.cache_clear()
+    assert asked == [(1, 3000), (0, 1000), (1, 3000), (0, 1000)]

@@ -661,7 +661,8 @@ def shared_prefix_attention_lse(
     starts = None if group_starts is None else _prep_index(group_starts).contiguous()
     trows = None if table_rows is None else _prep_index(table_rows).contiguous()
     table_shape = table.shape
-    floats = _shared_prefix_floats(rows, hq, hk, groups, block_size, max_prefix_len, max_suffix_len)
+    floats = _shared_prefix_floats(device, rows, hq, hk, groups, block_size, max_prefix_len,
+                                   max_suffix_len)
     scratch = lse.new_empty(floats)
     _lib.call_on(
         device, "dsb_shared_prefix_attention_lse",
@@ -676,9 +677,10 @@ def shared_prefix_attention_lse(
 
 
 @functools.lru_cache(maxsize=256)
-def _shared_prefix_floats(*sizes: int) -> int:
-    """dsb_shared_prefix_scratch_floats, at least 1."""
-    return max(_lib.load().dsb_shared_prefix_scratch_floats(*sizes), 1)
+def _shared_prefix_floats(device: torch.device, *sizes: int) -> int:
+    """dsb_shared_prefix_scratch_floats on a device (its SMs count), at least 1."""
+    with torch.cuda.device(device):
+        return max(_lib.load().dsb_shared_prefix_scratch_floats(*sizes), 1)
 
 
 def _qk_norm_inputs(query, kv, positions, cos_sin, num_kv_heads, q_weight, k_weight, rotary_dim,
