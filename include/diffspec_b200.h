@@ -627,7 +627,9 @@ int dsb_shared_prefix_attention_lse(
  * resize: row rows[i] gets the pages of lens[i] tokens.  Surplus pages go
  * back first; the first row that does not fit and the later ones that need
  * pages keep what they had (status[0] counts them).  Rows outside the table
- * or named again, and lengths beyond it, are flagged and left alone. */
+ * or named again, and lengths beyond it, are flagged and left alone.  A row
+ * cut back to inside a page that other rows hold keeps it, shared, and is
+ * flagged (DSB_FLAG_POSITION): it must not write there. */
 int dsb_resize_requests(int32_t *ref_counts, int64_t num_pages, int32_t *block_tables,
                         int64_t table_rows, int64_t table_stride, int64_t table_cols,
                         int32_t *held, const int32_t *rows, const int32_t *lens, int32_t n,

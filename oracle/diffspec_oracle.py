@@ -652,14 +652,17 @@ class PagePool:
             if n < 0 or need > self.cols:
                 self.flags.add("position")
                 continue
-            todo.append((r, need))
-        for r, need in todo:
+            todo.append((r, need, n))
+        for r, need, _ in todo:
             for j in range(need, self.held[r]):
                 self.refs[self.tables[r][j]] -= 1
                 self.tables[r][j] = -1
             self.held[r] = min(self.held[r], need)
+        for r, need, n in todo:  # the next token's page is other rows', too
+            if n % self.bs and need == self.held[r] and self.refs[self.tables[r][need - 1]] > 1:
+                self.flags.add("position")
         free, full = self.free(), False
-        for r, need in todo:
+        for r, need, _ in todo:
             k = need - self.held[r]
             if k <= 0:
                 continue

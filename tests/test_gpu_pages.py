@@ -254,3 +254,33 @@ def test_pools_beyond_a_turn_of_the_planners(dsb, cuda):
     p.resize([1, 6], [0, 0])
     p.compact()
     p.resize([1, 3, 6], [39000, 5, 40000])
+
+
+@pytest.mark.parametrize("pages,cols", [(64, 9), (64, 9000), (5000, 9), (40000, 9000)])
+def test_a_row_cut_back_into_a_shared_page_is_flagged(dsb, cuda, pages, cols):
+    """What the row would write next is in a page of its siblings.  Cut to a
+    page's end, into a page of its own, or as the others leave, it is not
+    (tables on both sides of what one CTA lets go by itself; one planner and
+    several)."""
+    def take():
+        return dsb._lib.read_and_clear_error_flag(cuda)
+
+    def resize(rows, lens):
+        dsb.pages.resize_requests(*p.state, p.ints(rows), p.ints(lens), block_size=4)
+        flag = take()
+        p.ref.resize(rows, lens)
+        p.ref.flags.clear()
+        p.check(p.ints([p.ref.lacking, len(p.ref.free())]))
+        return flag
+
+    p = _Pool(dsb, cuda, pages, 5, cols, 4)
+    p.resize([0], [18])
+    p.fork([0, 0], [1, 2], [16, 18])  # four shared pages, and two tokens of its own for row 2
+    assert resize([1], [15]) == dsb._lib.DSB_FLAG_POSITION
+    assert resize([1], [15]) == dsb._lib.DSB_FLAG_POSITION  # still so
+    assert resize([1, 2, 0], [12, 17, 17]) == 0  # whole pages, pages of their own
+    assert resize([0, 1, 2], [3, 4, 20]) == dsb._lib.DSB_FLAG_POSITION
+    assert resize([0, 1, 2], [0, 0, 7]) == 0  # the others leave in the same call
+    p.fork([2], [1], [7])
+    assert resize([1], [5]) == 0  # the fork's copy
+    assert p.ref.held == [0, 2, 2, 0, 0]

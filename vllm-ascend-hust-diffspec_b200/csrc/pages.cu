@@ -331,6 +331,7 @@ template <int T> __global__ void __launch_bounds__(T)
                   int n, int alone, int ranks) {
   extern __shared__ int32_t pg_smem[];
   int32_t *want = pg_smem, *row = want + n, *has = row + n, *target = has + n;
+  int32_t *last = target + n;  // the page it has that its new length ends inside, or -1
   __shared__ int32_t warp_tot[T / 32], told[kPgCluster];
   __shared__ int lacking, granted;
   pdl_begin();
@@ -343,14 +344,17 @@ template <int T> __global__ void __launch_bounds__(T)
   __syncthreads();
   for (int i = tid; i < n; i += T) {
     const int r = row[i];
-    int have = 0, need = -1;
+    int have = 0, need = -1, ends_in = -1;
     if (r < 0 || r >= p.rows || want[i]) {
       if (s.rank == 0) flag_error(p.err, DSB_FLAG_SLOT);
     } else {
-      have = pages_held(p, r);
       need = pages_needed(p, target[i]);
+      if (need > 0 && target[i] % p.bs != 0) ends_in = p.tables[(int64_t)r * p.stride + need - 1];
+      have = pages_held(p, r);
+      if (need > have) ends_in = -1;
       if (need < 0 && s.rank == 0) flag_error(p.err, DSB_FLAG_POSITION);
     }
+    last[i] = ends_in;
     has[i] = have;
     target[i] = need;
     want[i] = max(0, need - have);
@@ -370,6 +374,11 @@ template <int T> __global__ void __launch_bounds__(T)
   }
   Free<T> free;
   free.count(p, s, warp_tot);
+  // a length inside a page that other rows hold, too: what the row writes behind
+  // it would be theirs as well
+  for (int i = tid; i < n && s.rank == 0; i += T)
+    if (last[i] >= 0 && last[i] < p.pages && __ldcg(p.refs + last[i]) > 1)
+      flag_error(p.err, DSB_FLAG_POSITION);
   int before;
   const int nfree = s.gather(free.total, before);
   scan_rows<T>(want, n, warp_tot);
@@ -744,7 +753,7 @@ extern "C" int dsb_resize_requests(int32_t *ref_counts, int64_t num_pages, int32
                   dim3(256), 0, st, p, rows, lens, (int)n);
     if (int e = check_launch("release_kernel")) return e;
   }
-  const size_t smem = (size_t)n * 4 * sizeof(int32_t);
+  const size_t smem = (size_t)n * 5 * sizeof(int32_t);
   int e = DSB_OK;
   with_planners(num_pages, n, [&](auto threads, int ranks) {
     auto kern = resize_kernel<threads()>;

@@ -100,7 +100,13 @@ def resize_requests(ref_counts: torch.Tensor, block_tables: torch.Tensor, held: 
     that does not fit, and every later one that needs pages, keeps what it
     had and is counted in ``status[0]``.  A row outside the table or named
     twice (the first counts), and a length that the table cannot hold, are
-    flagged and left alone.  Returns ``status``."""
+    flagged and left alone.
+
+    A row cut back to inside a page that other rows hold after the call keeps
+    that page, and it stays theirs: the row's next token would be written over
+    their tokens.  Such a row is flagged (``DSB_FLAG_POSITION``); to write on
+    from there, fork it at that length instead (:func:`fork_requests` gives the
+    child a copy of the started page) and free it.  Returns ``status``."""
     if block_size <= 0:
         raise ValueError("block_size must be positive")
     pool = _pool(ref_counts, block_tables, held)
