@@ -284,3 +284,19 @@ def test_a_row_cut_back_into_a_shared_page_is_flagged(dsb, cuda, pages, cols):
     p.fork([2], [1], [7])
     assert resize([1], [5]) == 0  # the fork's copy
     assert p.ref.held == [0, 2, 2, 0, 0]
+
+
+def test_needs_whose_sum_passes_32_bits(dsb, cuda):
+    """Rows that ask for more pages together than a 32-bit count holds find
+    none, and the ones in front of them are served."""
+    cols, pages = 1_100_000_000, 100
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    refs, held = torch.zeros(pages, dtype=torch.int32, device=cuda), ints(0, 0, 0)
+    tables = torch.full((3, cols), -1, dtype=torch.int32, device=cuda)
+    st = dsb.pages.resize_requests(refs, tables, held, ints(1, 0, 2), ints(60, cols, cols), block_size=1)
+    assert st.tolist() == [2, 40] and held.tolist() == [0, 60, 0]
+    assert refs.tolist() == [1] * 60 + [0] * 40 and tables[1, :61].tolist() == [*range(60), -1]
+    st = dsb.pages.resize_requests(refs, tables, held, ints(0, 2, 1), ints(cols, cols, 3), block_size=1)
+    assert st.tolist() == [2, 97] and held.tolist() == [0, 3, 0]  # the surplus goes all the same
+    assert int((tables >= 0).sum()) == 3
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0

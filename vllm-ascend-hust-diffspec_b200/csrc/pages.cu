@@ -49,8 +49,13 @@ struct Caches {
   int n;
 };
 
+// Sums of counts; with SAT they end at INT32_MAX (what rows ask for may pass it).
+template <bool SAT> __device__ __forceinline__ int add_counts(int a, int b) {
+  return SAT ? (int)min((unsigned)a + (unsigned)b, (unsigned)INT32_MAX) : a + b;
+}
+
 // Sum of the warps' values before this warp's; `total` gets the sum of all.
-template <int T> __device__ int warps_before(int mine, int32_t *warp_tot, int &total) {
+template <int T, bool SAT = false> __device__ int warps_before(int mine, int32_t *warp_tot, int &total) {
   if ((threadIdx.x & 31) == 0) warp_tot[threadIdx.x >> 5] = mine;
   __syncthreads();
   int before = 0;
@@ -58,32 +63,32 @@ template <int T> __device__ int warps_before(int mine, int32_t *warp_tot, int &t
 #pragma unroll
   for (int w = 0; w < T / 32; ++w) {
     if (w == (int)(threadIdx.x >> 5)) before = total;
-    total += warp_tot[w];
+    total = add_counts<SAT>(total, warp_tot[w]);
   }
   __syncthreads();
   return before;
 }
 
 // Inclusive prefix sum over the CTA's threads.
-template <int T> __device__ int block_scan(int v, int32_t *warp_tot, int &total) {
+template <int T, bool SAT = false> __device__ int block_scan(int v, int32_t *warp_tot, int &total) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += x;
+    if (lane >= o) v = add_counts<SAT>(v, x);
   }
-  return warps_before<T>(__shfl_sync(0xffffffffu, v, 31), warp_tot, total) + v;
+  return add_counts<SAT>(warps_before<T, SAT>(__shfl_sync(0xffffffffu, v, 31), warp_tot, total), v);
 }
 
-// a[0..n) in shared memory becomes its inclusive prefix sum.
+// a[0..n) in shared memory becomes its inclusive prefix sum, at most INT32_MAX.
 template <int T> __device__ int scan_rows(int32_t *a, int n, int32_t *warp_tot) {
   int run = 0;
   for (int base = 0; base < n; base += T) {
     const int i = base + threadIdx.x;
     int total;
-    const int s = block_scan<T>(i < n ? a[i] : 0, warp_tot, total) + run;
-    if (i < n) a[i] = s;
-    run += total;
+    const int s = block_scan<T, true>(i < n ? a[i] : 0, warp_tot, total);
+    if (i < n) a[i] = add_counts<true>(s, run);
+    run = add_counts<true>(run, total);
   }
   __syncthreads();
   return run;
@@ -384,10 +389,10 @@ template <int T> __global__ void __launch_bounds__(T)
   scan_rows<T>(want, n, warp_tot);
   // rows in order until the first that does not fit
   for (int i = tid; i < n; i += T) {
-    const int need = want[i] - (i > 0 ? want[i - 1] : 0);
-    if (want[i] <= nfree) {
-      if (need > 0) atomicMax(&granted, want[i]);
-    } else if (need > 0) {
+    const bool needs = target[i] > has[i];
+    if (want[i] <= nfree && want[i] < INT32_MAX) {
+      if (needs) atomicMax(&granted, want[i]);
+    } else if (needs) {
       atomicAdd(&lacking, 1);
       continue;
     }
