@@ -249,3 +249,14 @@ def test_scratch_is_sized_on_the_tensors_device(dsb, monkeypatch):
                                             max_prefix_len=16, max_suffix_len=16)
     kernels._shared_prefix_floats.cache_clear()
     assert asked == [(1, 3000), (0, 1000), (1, 3000), (0, 1000)]
+
+
+def test_a_tokens_bytes_go_by_the_shape(dsb):
+    """One token a page, or one page: contiguous tensors whose strides of those
+    dimensions are anything."""
+    for cache in (torch.zeros((1, 8, 2, 8)).transpose(0, 1), torch.zeros((8, 2, 8)).unsqueeze(1),
+                  torch.zeros((8, 1, 2, 8)), torch.zeros((5, 1, 2, 8)).transpose(0, 1)):
+        assert cache.is_contiguous()
+        addresses, block_size, token_bytes = dsb.pages._caches([cache], cache.shape[0])
+        assert list(addresses) == [cache.data_ptr()]
+        assert (block_size, token_bytes) == (cache.shape[1], 2 * 8 * 4)

@@ -24,6 +24,7 @@ The tables are the ``block_table`` of the paged kernels
 
 from __future__ import annotations
 
+import math
 from array import array
 from collections.abc import Sequence
 
@@ -68,7 +69,8 @@ def _caches(caches: Sequence[torch.Tensor], pages: int):
     if shape[0] != pages:
         raise ValueError("caches must have one page per reference count")
     addresses = array("Q", [t.data_ptr() for t in caches])
-    return addresses, shape[1], first.stride(1) * first.element_size()
+    # (of the shape: a stride says nothing where a dimension has one entry)
+    return addresses, shape[1], math.prod(shape[2:]) * first.element_size()
 
 
 def _row(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
