@@ -260,3 +260,20 @@ def test_a_tokens_bytes_go_by_the_shape(dsb):
         addresses, block_size, token_bytes = dsb.pages._caches([cache], cache.shape[0])
         assert list(addresses) == [cache.data_ptr()]
         assert (block_size, token_bytes) == (cache.shape[1], 2 * 8 * 4)
+
+
+def test_the_stride_of_a_single_row_is_not_read(dsb):
+    """One token, one table row, one row of cosines: transposed columns are
+    contiguous rows, too."""
+    column = lambda n, **k: torch.zeros((n, 1), **k).t()  # noqa: E731
+    bf = dict(dtype=torch.bfloat16)
+    q, kv, out, cs, w = column(512, **bf), column(512, **bf), column(512, **bf), column(128), torch.ones(128, **bf)
+    got = dsb.kernels._qk_norm_inputs(q, kv, _i(1), cs, 2, w, w, None, out)
+    assert got[5] == (q.data_ptr(), 512, out.data_ptr(), 512, 4, kv.data_ptr(), 512)
+    assert got[7][:3] == (cs.data_ptr(), 128, 1)
+    got = dsb.kernels._qk_norm_inputs(q, kv, _i(1), cs, 2, w, w, None, None)
+    assert got[5] == (q.data_ptr(), 512, q.data_ptr(), 512, 4, kv.data_ptr(), 512)
+    table = column(7, dtype=torch.int32)
+    assert dsb.pages._pool(_i(8), table, _i(1))[3:6] == (1, 7, 7)
+    assert dsb.kernels._row_stride(table) == 7 and dsb.kernels._row_stride(_i(3, 9)[:, :7]) == 9
+    assert dsb.pages._pool(_i(8), _i(1, 3).t(), _i(3))[3:6] == (3, 1, 1)

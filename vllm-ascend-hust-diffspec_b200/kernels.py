@@ -58,6 +58,12 @@ def _prep_index(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between the rows of a matrix (those of a single row may be any
+    number: its columns then)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def _batch(query, query_index):
     return query.shape[0] if query_index is None else query_index.numel()
 
@@ -667,7 +673,7 @@ def shared_prefix_attention_lse(
     _lib.call_on(
         device, "dsb_shared_prefix_attention_lse",
         query.data_ptr(), rows, hq, hk, d, key_cache.data_ptr(), value_cache.data_ptr(), num_blocks,
-        block_size, table.data_ptr(), table.stride(0), table_shape[0], table_shape[1],
+        block_size, table.data_ptr(), _row_stride(table), table_shape[0], table_shape[1],
         seq.data_ptr(), None if trows is None else trows.data_ptr(), prefix.data_ptr(),
         None if starts is None else starts.data_ptr(), groups, max_prefix_len, max_suffix_len, scale,
         _lib.dtype_code(dtype), out.data_ptr(), lse.data_ptr(), scratch.data_ptr(), floats,
@@ -700,6 +706,8 @@ def _qk_norm_inputs(query, kv, positions, cos_sin, num_kv_heads, q_weight, k_wei
     (q_stride, q_step), (kv_stride, kv_step) = query.stride(), kv.stride()
     if q_step != 1 or kv_step != 1:
         raise ValueError("query and kv must have contiguous rows")
+    if tokens == 1:  # (the stride of a single row may be anything)
+        q_stride, kv_stride = q_cols, kv_cols
     if q_weight.shape != (d,) or k_weight.shape != (d,):
         raise ValueError("q_weight and k_weight must be [head_dim]")
     dtype = query.dtype
@@ -716,6 +724,8 @@ def _qk_norm_inputs(query, kv, positions, cos_sin, num_kv_heads, q_weight, k_wei
     (cs_rows, cs_cols), (cs_stride, cs_step) = cos_sin.shape, cos_sin.stride()
     if cs_cols < rotary_dim or cs_step != 1:
         raise ValueError("cos_sin must be a [rows, cos | sin] table of rotary_dim columns")
+    if cs_rows == 1:
+        cs_stride = cs_cols
     if (positions.dtype is not torch.int32 or positions.numel() < tokens
             or not positions.is_contiguous()):
         raise ValueError("positions must be contiguous int32 with one entry per token")
@@ -727,6 +737,8 @@ def _qk_norm_inputs(query, kv, positions, cos_sin, num_kv_heads, q_weight, k_wei
         out_stride, out_step = query_out.stride()
         if out_step != 1:
             raise ValueError("query_out must be shaped like query, in contiguous rows")
+        if tokens == 1:
+            out_stride = q_cols
     # query, query_out, heads, key: the arguments both calls begin with
     key = kv.data_ptr()
     head = (query.data_ptr(), q_stride, query_out.data_ptr(), out_stride, q_cols // d, key, kv_stride)
@@ -792,7 +804,7 @@ def qk_norm_rope_write_paged(
         device, "dsb_qk_norm_rope_paged", *head, value, head[-1], hk, d, rot,
         1 if is_neox_style else 0, q_weight.data_ptr(), k_weight.data_ptr(), eps,
         positions.data_ptr(), tokens, *cos_args, key_cache.data_ptr(), value_cache.data_ptr(),
-        num_blocks, block_size, table.data_ptr(), table.stride(0), table_shape[0], table_shape[1],
+        num_blocks, block_size, table.data_ptr(), _row_stride(table), table_shape[0], table_shape[1],
         None if trows is None else trows.data_ptr(), _lib.error_flag_ptr(device),
         _lib.stream_ptr(device),
     )

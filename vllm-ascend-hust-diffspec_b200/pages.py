@@ -48,8 +48,10 @@ def _pool(ref_counts, block_tables, held):
     if not (ref_counts.dtype is _INT32 and block_tables.dtype is _INT32 and held.dtype is _INT32):
         raise ValueError("ref_counts, block_tables and held must be int32")
     stride, step = block_tables.stride()
-    if step != 1 or not (ref_counts.is_contiguous() and held.is_contiguous()):
+    if (step != 1 and cols > 1) or not (ref_counts.is_contiguous() and held.is_contiguous()):
         raise ValueError("ref_counts and held must be contiguous, block_tables in contiguous rows")
+    if rows == 1:
+        stride = cols  # (that of a single row may be anything)
     return (ref_counts.data_ptr(), ref_counts.numel(), block_tables.data_ptr(), rows, stride, cols,
             held.data_ptr())
 
