@@ -277,3 +277,10 @@ def test_the_stride_of_a_single_row_is_not_read(dsb):
     assert dsb.pages._pool(_i(8), table, _i(1))[3:6] == (1, 7, 7)
     assert dsb.kernels._row_stride(table) == 7 and dsb.kernels._row_stride(_i(3, 9)[:, :7]) == 9
     assert dsb.pages._pool(_i(8), _i(1, 3).t(), _i(3))[3:6] == (3, 1, 1)
+
+
+def test_rows_and_lengths_beyond_32_bits_stay_out_of_range(dsb):
+    """2^32 + 5 tokens are not five, and row 2^32 is not row zero."""
+    got = dsb.pages._row(torch.tensor([5, 2 ** 32 + 5, 2 ** 31, -2 ** 40, -1]), 5, "lens")
+    assert got.dtype == torch.int32 and got.tolist() == [5, 2 ** 31 - 1, 2 ** 31 - 1, -1, -1]
+    assert dsb.pages._row(torch.tensor([5, 200], dtype=torch.uint8), 2, "rows").tolist() == [5, 200]

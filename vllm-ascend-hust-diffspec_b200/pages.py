@@ -81,6 +81,8 @@ def _row(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     if t.dtype is not _INT32:
         if t.is_floating_point() or t.dtype == torch.bool:
             raise ValueError(f"{name} must be whole numbers")
+        if t.dtype is torch.int64:  # (what 32 bits do not hold stays out of range)
+            t = t.clamp(-1, 2 ** 31 - 1)
         t = t.to(_INT32)
     return t.contiguous()
 
