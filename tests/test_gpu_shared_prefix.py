@@ -504,3 +504,24 @@ def test_nan_among_what_a_row_sees(dsb, cuda, page, dtype):
         assert torch.isnan(out[r]).all() and torch.isnan(lse[r]).all(), r
     assert (out[4] == 0).all() and torch.isneginf(lse[4]).all()
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+@pytest.mark.parametrize("prefix", [0, 2 ** 31 - 1])
+def test_lengths_up_to_31_bits(dsb, cuda, prefix):
+    """A table row that names one page again and again holds 2^31 tokens and
+    more; what a row sees is cut a few tiles below that and flagged.  Logits of
+    zero and values of one: every sum is a whole number that fp32 holds until
+    the merge (a piece has 2^24 tokens a stream at most)."""
+    page = 2 ** 16
+    key, value = (torch.ones((1, page, 1, _D), dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    query = torch.zeros((1, 8, _D), dtype=torch.bfloat16, device=cuda)
+    table = torch.zeros((1, 2 ** 15 + 3), dtype=torch.int32, device=cuda)
+    out, lse = dsb.kernels.shared_prefix_attention_lse(
+        query, key, value, table, ints(2 ** 31 - 1), ints(prefix), scale=_D ** -0.5,
+        max_prefix_len=prefix, max_suffix_len=0)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == dsb._lib.DSB_FLAG_POSITION
+    assert (out == 1).all()
+    # 148 pieces joined in fp32, and the logarithm
+    np.testing.assert_allclose(lse.cpu().numpy(), np.log(2.0 ** 31 - 1 - 512), rtol=0,
+                               atol=(148 + 4 * 22) * 2.0 ** -24)

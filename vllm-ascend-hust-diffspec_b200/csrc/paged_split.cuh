@@ -101,7 +101,8 @@ __global__ void __launch_bounds__(kTaWarps * 32, 2) paged_decode_split_kernel(co
     if (threadIdx.x == 0 && split == 0 && h == 0 && (!ANY || L > 0)) flag_error(a.err, DSB_FLAG_SLOT);
     L = 0;
   }
-  const int64_t cap = a.bt_cols * a.bs;  // tokens the table row can address
+  int64_t cap = a.bt_cols * a.bs;  // tokens the table row can address
+  if (ANY) cap = min(cap, (int64_t)INT32_MAX - 512);  // (tps is a whole number of 32 bits)
   if ((int64_t)L > cap) {  // seq_lens[r] beyond its block-table row
     if (threadIdx.x == 0 && split == 0 && h == 0) flag_error(a.err, DSB_FLAG_POSITION);
     L = (int)cap;

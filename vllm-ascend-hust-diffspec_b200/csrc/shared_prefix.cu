@@ -106,6 +106,11 @@ __device__ __forceinline__ int sp_owner(int64_t u, const SpBegin &x, int ctas) {
   return b;
 }
 
+// Tokens that a table row can address; a few tiles short of 2^31, so that the
+// places of a tile that reaches behind them are whole numbers of 32 bits, too.
+__device__ __forceinline__ int64_t sp_cap(const TaArgs &a) {
+  return min(a.bt_cols * a.bs, (int64_t)INT32_MAX - 4 * kSpTok);
+}
 // Tokens that a row of L tokens on table row `trow` may see, 0 for a row
 // without a valid table row.
 __device__ __forceinline__ int sp_sees(const TaArgs &a, int L, int64_t trow, bool report) {
@@ -114,7 +119,7 @@ __device__ __forceinline__ int sp_sees(const TaArgs &a, int L, int64_t trow, boo
     if (report) flag_error(a.err, DSB_FLAG_SLOT);
     return 0;
   }
-  const int64_t cap = a.bt_cols * a.bs;
+  const int64_t cap = sp_cap(a);
   if (L > cap) {
     if (report) flag_error(a.err, DSB_FLAG_POSITION);
     return (int)cap;
@@ -165,7 +170,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
   const TaArgs &a = s.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = a.hq / a.hk, run_rows = 128 / G;
-  const int64_t cap = a.bt_cols * a.bs;  // tokens a table row can address
+  const int64_t cap = sp_cap(a);
   pdl_begin();
 
   // The rows of a turn: what each sees, and its table row (-1: none).  A run
