@@ -300,3 +300,37 @@ def test_needs_whose_sum_passes_32_bits(dsb, cuda):
     assert st.tolist() == [2, 97] and held.tolist() == [0, 3, 0]  # the surplus goes all the same
     assert int((tables >= 0).sum()) == 3
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+def test_caches_past_32_bits(dsb, cuda):
+    """Pages whose offsets pass 2^31 elements and 2^32 bytes: copied, forked
+    into and compacted."""
+    page, hk, d = 16, 4, 128
+    pages = 2 ** 31 // (page * hk * d) + 400
+    cache = torch.zeros((pages, page, hk, d), dtype=torch.bfloat16, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    cache[-60:] = torch.randn((60, page, hk, d), generator=g, device=cuda).bfloat16()
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    want = cache[-60:].clone()
+    top = pages - 60
+    dsb.pages.copy_pages([cache], ints(top, top + 1, 7), ints(top + 40, 3, top + 41))
+    want[40], want[41] = want[0], 0
+    assert torch.equal(cache[-60:], want) and torch.equal(cache[3], want[1])
+    # every page but the last twenty is someone else's
+    refs = torch.ones(pages, dtype=torch.int32, device=cuda)
+    refs[-20:] = 0
+    tables = torch.full((3, 4), -1, dtype=torch.int32, device=cuda)
+    held = torch.zeros(3, dtype=torch.int32, device=cuda)
+    dsb.pages.resize_requests(refs, tables, held, ints(0), ints(40), block_size=page)
+    st = dsb.pages.fork_requests(refs, tables, held, ints(0), ints(1), ints(40), [cache])
+    assert tables[:2].tolist() == [[pages - 20, pages - 19, pages - 18, -1],
+                                   [pages - 20, pages - 19, pages - 17, -1]]
+    want[43, :8] = want[42, :8]
+    assert st.tolist() == [0, 16] and torch.equal(cache[-60:], want)
+    # the low half becomes free: the live pages move down, those of the rows among them
+    refs[: pages - 100] = 0
+    st = dsb.pages.compact_pages(refs, tables, held, [cache])
+    live = 100 - 16
+    assert st.tolist() == [0, pages - live] and tables[1].tolist() == [live - 4, live - 3, live - 1, -1]
+    assert torch.equal(cache[live - 44: live], want[:44])
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0

@@ -269,3 +269,47 @@ def test_heads_on_both_sides_of_a_warp(dsb, cuda, hq, hk, d):
     _close(raw[0][keep, 0], ky[keep], _both(ky[keep]), d, "bf16")
     assert torch.equal(raw[1][keep, 0], v[keep])
     assert (raw[0][n] == 7.0).all() and (raw[0][:, 1] == 7.0).all()
+
+
+@pytest.mark.parametrize("d", [128, 96])
+def test_offsets_past_32_bits(dsb, cuda, d):
+    """Rows of the projection, of the raw caches and of the pages whose offsets
+    pass 2^31 elements and 2^32 bytes (both kernels)."""
+    hq, hk, n, page, rows = 32, 4, 37, 16, 64
+    width = (hq + 2 * hk) * d
+    tokens = 2 ** 31 // width + 100
+    small, w, cs, pos_n = _inputs(cuda, n, hq, hk, d, d, "bf16", torch.float32, rows, d)
+    (qy, qr), (ky, kr) = _expect(small, w, cs, pos_n, hq, hk, d, True, 1e-6)
+    qkv = torch.zeros((tokens, width), dtype=torch.bfloat16, device=cuda)
+    qkv[-n:] = small.view(n, width)
+    pos = torch.zeros(tokens, dtype=torch.int32, device=cuda)
+    pos[-n:] = pos_n
+    slots = torch.full((tokens,), -1, dtype=torch.int32, device=cuda)  # (the others: padding)
+    at = torch.zeros(tokens, dtype=torch.int64, device=cuda)
+    max_len = 2 ** 31 // (2 * hk * d) + 50
+    raw = [torch.zeros((3, max_len, hk, d), dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    slots[-n:], at[-n:] = 2, torch.arange(max_len - n, max_len, device=cuda)
+    q, k, v = dsb.draft_layer.qk_norm_rope(
+        qkv[:, : hq * d], qkv[:, hq * d:], pos, cs, hk, *w, 1e-6, raw=(*raw, slots, at))  # in place
+    _close(q[-n:].reshape(n, hq, d), qr, _both(qy), d, "bf16")
+    _close(k[-n:], kr, _both(ky), d, "bf16")
+    assert torch.equal(v[-n:], small[:, hq + hk:])
+    _close(raw[0][2, -n:], ky, _both(ky), d, "bf16")
+    assert torch.equal(raw[1][2, -n:], small[:, hq + hk:])
+    del raw, q, k, v, qkv
+    # the last pages of a cache
+    pages = 2 ** 31 // (page * hk * d) + 400
+    caches = [torch.zeros((pages, page, hk, d), dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    table = torch.arange(pages - 4, pages, device=cuda).int()[None].expand(1, 4).contiguous()
+    pos = torch.randperm(4 * page, device=cuda)[:n].int()
+    flat = small.view(n, width)
+    out = torch.empty((n, hq * d), dtype=torch.bfloat16, device=cuda)
+    dsb.kernels.qk_norm_rope_write_paged(
+        flat[:, : hq * d], flat[:, hq * d:], pos, cs, *caches, table, *w, 1e-6,
+        table_rows=torch.zeros(n, dtype=torch.int32, device=cuda), query_out=out)
+    (qy, qr), (ky, kr) = _expect(small, w, cs, pos, hq, hk, d, True, 1e-6)
+    _close(out.view(n, hq, d), qr, _both(qy), d, "bf16")
+    place = (pages - 4 + pos.long() // page, pos.long() % page)
+    _close(caches[0][place], kr, _both(ky), d, "bf16")
+    assert torch.equal(caches[1][place], small[:, hq + hk:])
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0

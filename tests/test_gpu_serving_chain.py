@@ -159,6 +159,38 @@ def test_runtime_target_attention_with_shared_prefixes(dsb, cuda, groups):
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
 
 
+def test_runtime_selects_the_same_chunks(dsb, cuda):
+    """The retrieval driven by the LSE of the shared-prefix call selects the
+    chunks that the plain call's LSE selects: chunks of one request whose scores
+    lie far apart (its keys there point along the query, more or less)."""
+    g = torch.Generator(device=cuda).manual_seed(8)
+    hq, hk, d, page, n, prefix = 16, 2, 128, 16, 3, 304
+    seq_lens, cols = [340, 420, 460], 30
+    table = torch.arange(n * cols, device=cuda, dtype=torch.int32).view(n, cols)
+    table[1:, : prefix // page] = table[0, : prefix // page].clone()
+    query = torch.randn((1, 1, d), generator=g, device=cuda)
+    keys, value = (torch.randn((n * cols, page, hk, d), generator=g, device=cuda) for _ in range(2))
+    # each 32 tokens have their own share of the query, half a nat apart and in no order
+    step = torch.randperm(n * cols // 2, generator=g, device=cuda).repeat_interleave(2) / 2
+    keys = 0.01 * keys + (step[:, None, None, None] % 8) * query / query.square().sum() * d ** 0.5
+    cache = [keys.to(_BF), value.to(_BF)]
+    query = query.expand(n, hq, d).to(_BF).contiguous()
+    meta = SimpleNamespace(actual_seq_lengths_q=[1, 2, 3], seq_lens_list=seq_lens, block_tables=table,
+                           num_prefills=0)
+    got = []
+    for kw in ({}, dict(shared_prefix=([prefix], [n]))):
+        state = dsb.runtime.DiffSpecDraftCache(
+            dsb.runtime.DiffSpecSettings(32, 160, 1, 4, 3, 0.7, False), max_num_reqs=n,
+            max_model_len=512, num_kv_heads=hk, head_dim=d, target_num_layers=2, dtype=_BF,
+            device=cuda, cos_sin_cache=torch.zeros((160, d), device=cuda).to(_BF))
+        state.begin_target_forward(["a", "b", "c"])
+        state.run_target_attention(query, *cache, meta, d ** -0.5, **kw)
+        state.accept_target_queries(torch.tensor([1, 1, 1], device=cuda), is_prefill=False)
+        got.append([sorted(row[:k]) for row, k in zip(state.sel_chunks.tolist(), state.sel_count.tolist())])
+    assert got[0] == got[1] and all(len(row) > 1 for row in got[0][:n])
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
 @pytest.mark.parametrize("query_ends", [[1, 1, 2, 3], [0, 0, 2, 2], [3, 3, 3, 3], [0, 0, 0, 0]])
 def test_runtime_groups_without_query_rows(dsb, cuda, query_ends):
     """Requests without query rows this step, each a group of its own (more

@@ -284,3 +284,11 @@ def test_rows_and_lengths_beyond_32_bits_stay_out_of_range(dsb):
     got = dsb.pages._row(torch.tensor([5, 2 ** 32 + 5, 2 ** 31, -2 ** 40, -1]), 5, "lens")
     assert got.dtype == torch.int32 and got.tolist() == [5, 2 ** 31 - 1, 2 ** 31 - 1, -1, -1]
     assert dsb.pages._row(torch.tensor([5, 200], dtype=torch.uint8), 2, "rows").tolist() == [5, 200]
+
+
+def test_scratch_of_the_page_calls(dsb):
+    """The sizes that the Python calls work out themselves are the C side's."""
+    L = dsb._lib.load()
+    for n in (1, 7, 4096):
+        assert L.dsb_fork_scratch_ints(n) == 6 * n
+        assert L.dsb_compact_scratch_ints(n) == 1 + 3 * n
