@@ -105,6 +105,12 @@ struct Stretch {
     const int64_t per = (pages + ranks - 1) / ranks;
     from = min(pages, rank * per);
     till = min(pages, from + per);
+    if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  }
+  // Every CTA of the cluster has begun (its shared memory may not be written
+  // before): once, in front of the first sync or gather.
+  __device__ void begun() const {
+    if (ranks > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
   }
   __device__ void sync() const {
     __syncthreads();
@@ -365,6 +371,7 @@ template <int T> __global__ void __launch_bounds__(T)
     want[i] = max(0, need - have);
   }
   __syncthreads();
+  s.begun();
   // releases first, a warp a row (unless release_kernel has let them go)
   if (alone) {
     for (int i = tid >> 5; i < n && s.rank == 0; i += T / 32) {
@@ -475,6 +482,7 @@ template <int T> __global__ void __launch_bounds__(T)
     }
   }
   __syncthreads();
+  s.begun();
   int before;
   const int nfree = s.gather(free.total, before);
   scan_rows<T>(want, n, warp_tot);
@@ -576,6 +584,7 @@ template <int T> __global__ void __launch_bounds__(T)
   const unsigned below = (1u << lane) - 1;
   Free<T> free;
   free.count(p, s, warp_tot);
+  s.begun();
   int before;
   const int nfree = s.gather(free.total, before);
   const int64_t live = p.pages - nfree;
