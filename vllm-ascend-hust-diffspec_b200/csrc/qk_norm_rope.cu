@@ -242,10 +242,12 @@ __device__ __forceinline__ void qk_turn(const QkTurn &f, float inv, const float 
 // heads.  Bound by memory, by way of the loads in flight and of how soon a
 // finished warp's place is taken: 65536 tokens of 32/4 heads of 128 into
 // pages (1.35 GB) take 281 us with 16 warps of 123 registers an SM in CTAs of
-// 256 threads, 247 with 24 warps of 80 (a few spills), 235 with stores that
-// do not stay in the way in L2, 227 (5.9 TB/s, 0.90 of the measured copy) in
-// CTAs of 64.  Two or six heads a thread are slower (268 and 286), and so is
-// asking later rows into L2 ahead of their warps (243 for 235).
+// 256 threads, 247 with 24 warps of 80 (every instance then spills, 116 to 200
+// bytes stored and 360 to 532 read again a thread), 235 with stores that do not
+// stay in the way in L2, 227 in CTAs of 64 (one launch by itself, 5.9 TB/s; 242
+// in a run of calls, 5.6 TB/s, 0.85 of the measured copy).  Two or six heads a
+// thread are slower (268 and 286), and so is asking later rows into L2 ahead of
+// their warps (243 for 235).
 constexpr int kQkThreads = 64;
 
 // With fewer query heads (keys and values) than half of what a warp takes, it
