@@ -334,3 +334,23 @@ def test_caches_past_32_bits(dsb, cuda):
     assert st.tolist() == [0, pages - live] and tables[1].tolist() == [live - 4, live - 3, live - 1, -1]
     assert torch.equal(cache[live - 44: live], want[:44])
     assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+
+
+@pytest.mark.parametrize("pages", [3000, 20000])
+def test_the_most_rows_that_a_call_takes(dsb, cuda, pages):
+    """4096 rows a call, one CTA's pool and a cluster's; one more is refused."""
+    rows = 9000
+    p = _Pool(dsb, cuda, pages, rows, 5, 4)
+    rng = random.Random(pages)
+    who = rng.sample(range(rows), 4096)
+    p.resize(who, [rng.randint(0, 12) for _ in who])
+    kids = [r for r in range(rows) if not p.ref.held[r]][:4096]
+    ups = [rng.choice(who) for _ in kids]
+    p.fork(ups, kids, [rng.randint(0, p.ref.held[u] * 4) for u in ups])
+    p.resize(kids, [rng.choice([0, 3, 20]) for _ in kids])
+    p.compact()
+    many = p.ints([0] * 4097)
+    for call in (lambda: dsb.pages.resize_requests(*p.state, many, many, block_size=4),
+                 lambda: dsb.pages.fork_requests(*p.state, many, many, many, p.caches)):
+        with pytest.raises(ValueError, match="4096"):
+            call()

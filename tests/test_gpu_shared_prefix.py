@@ -525,3 +525,43 @@ def test_lengths_up_to_31_bits(dsb, cuda, prefix):
     # 148 pieces joined in fp32, and the logarithm
     np.testing.assert_allclose(lse.cpu().numpy(), np.log(2.0 ** 31 - 1 - 512), rtol=0,
                                atol=(148 + 4 * 22) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("rows,groups,hq,hk", [(5000, 3000, 8, 2), (5000, 1, 8, 1), (700, 300, 32, 2),
+                                               (65535, 1500, 1, 1)])
+def test_many_rows_and_groups(dsb, cuda, rows, groups, hq, hk):
+    """More rows, groups and segments than the plan keeps beside it, against the
+    attention of every row by itself (the module's bounds on both sides, with
+    sum |q k| at most |q| |k|, and two roundings of the output)."""
+    g = torch.Generator(device=cuda).manual_seed(rows)
+    page, prefix, requests = 16, 35, 12
+    cols = 8
+    table = torch.arange(requests * cols, device=cuda, dtype=torch.int32).view(requests, cols)
+    key, value = (torch.randn((requests * cols, page, hk, _D), generator=g, device=cuda).bfloat16()
+                  for _ in range(2))
+    table[:, :2] = table[0, :2].clone()
+    for c in (key, value):
+        c[table[1:, 2].long(), : prefix % page] = c[table[0, 2].long(), : prefix % page]
+    seq = torch.randint(0, cols * page + 1, (rows,), generator=g, device=cuda).int()
+    trow = torch.sort(torch.randint(0, requests, (rows,), generator=g, device=cuda))[0].int()
+    cuts = torch.sort(torch.randint(0, rows + 1, (groups - 1,), generator=g, device=cuda))[0].int()
+    starts = torch.cat((torch.zeros_like(seq[:1]), cuts, torch.full_like(seq[:1], rows)))
+    lens = torch.randint(0, prefix + 1, (groups,), generator=g, device=cuda).int()
+    query = torch.randn((rows, hq, _D), generator=g, device=cuda).bfloat16()
+    out, lse = dsb.kernels.shared_prefix_attention_lse(
+        query, key, value, table, seq, lens, scale=_D ** -0.5, max_prefix_len=prefix,
+        max_suffix_len=cols * page, group_starts=starts, table_rows=trow)
+    ref, ref_lse = dsb.kernels.paged_decode_attention_lse(
+        query, key, value, table, seq, scale=_D ** -0.5, max_seq_len=cols * page, table_rows=trow)
+    assert dsb._lib.read_and_clear_error_flag(cuda) == 0
+    u = 2.0 ** -24
+    ds = 128 * u * _D ** -0.5 * float(query.double().norm(dim=-1).max() * key.double().norm(dim=-1).max())
+    chain = (cols * page / 32 + 256) * u
+    e = 2 * (2 * ds + 2.0 ** -17 + 2.0 ** -22 + chain) * float(value.abs().max())
+    off = (out.double() - ref.double()).abs()
+    step = torch.finfo(torch.bfloat16).eps / 2
+    assert bool((off <= 2 * step * (ref.double().abs() + e) + e).all()), float(off.max())
+    assert torch.equal(torch.isneginf(lse), torch.isneginf(ref_lse))
+    seen = seq > 0
+    tol = 2 * (ds + 2.0 ** -22 + chain + 2 * u * ref_lse[seen].double().abs())
+    assert bool(((lse - ref_lse)[seen].double().abs() <= tol).all())
