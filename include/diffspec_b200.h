@@ -595,14 +595,14 @@ int dsb_qk_norm_rope_paged(
  * [group_starts[i], group_starts[i + 1]) (num_groups + 1 entries, ascending,
  * at most query_rows groups; null: one group of every row) hold the same
  * tokens at positions [0, prefix_lens[i]), which are read once for the group,
- * through the table
- * row of a row that sees as much of them as any; the tokens behind it, up to
- * seq_lens[r], through the row's own, once for consecutive rows on one table
- * row.  Groups that do not ascend within the rows are flagged
- * (DSB_FLAG_SLOT) and share nothing.  max_prefix_len and max_suffix_len size
- * the launches alone.  Block sizes that are no multiple of 8 share nothing.
- * Any group of up to 16 query heads per kv head, head_dim 128; scratch is
- * 32-byte aligned, of the size for the device that is current, the call's. */
+ * through the table row of a row that sees as much of them as any; the tokens
+ * behind it, up to seq_lens[r], through the row's own, once for consecutive
+ * rows on one table row.  Groups that do not ascend within the rows are
+ * flagged (DSB_FLAG_SLOT) and share nothing.  max_prefix_len and
+ * max_suffix_len size the launches alone.  Block sizes that are no multiple of
+ * 8 share nothing.  Any group of up to 16 query heads per kv head, head_dim
+ * 128; out and lse begin at any element; scratch is 32-byte aligned, of the
+ * size for the device that is current, the call's. */
 int64_t dsb_shared_prefix_scratch_floats(int32_t query_rows, int32_t num_query_heads,
                                          int32_t num_kv_heads, int32_t num_groups,
                                          int32_t block_size, int32_t max_prefix_len,
