@@ -265,8 +265,9 @@ def qk_norm_rope(query: torch.Tensor, kv: torch.Tensor, positions: torch.Tensor,
     ``[S, max_model_len, Hk, D]`` at ``[slots[t], abs_positions[t]]`` (int32,
     int64; a negative slot is padding), what
     :func:`kernels.qkv_projection_write_raw` writes for keys without a norm.
-    Two tokens of a call must not share a place.  A position outside the table is flagged and leaves the rows normed but
-    unrotated.  Returns ``(query_out, key_out, value_out)``."""
+    Two tokens of a call must not share a place.  A position outside the table
+    is flagged and leaves the rows normed but unrotated.  Returns
+    ``(query_out, key_out, value_out)``."""
     d, rot, query_out, q_weight, k_weight, head, value, table = _qk_norm_inputs(
         query, kv, positions, cos_sin, num_kv_heads, q_weight, k_weight, rotary_dim, query_out)
     tokens, dtype = query.shape[0], query.dtype
